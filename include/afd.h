@@ -34,6 +34,14 @@
  *                                (computed at P/srt/batch_overlap/operations_strategy.py:94,
  *                                255 by SGLang's DeepseekV2MLP: SiluAndMul between its
  *                                gate_up and down projections)
+ *   afd_topk ................... the router's choice that the reference leaves to SGLang's TopK
+ *                                (its StandardTopKOutput is what P/srt/managers/scheduler.py
+ *                                :410-412 and P/srt/layers/moe/token_dispatcher/asap.py:48-73
+ *                                take)
+ *   afd_expert_counts / ........ no counterpart: where the tokens go, the balance loss of a
+ *   afd_balance / ..............  router in training, and the gradient of both by its logits
+ *   afd_topk_balance /
+ *   afd_router_grad
  *   afd_pack_mxfp4 / _fp8_block  the quant methods' weight repack at load time
  *                                (FlashInfer layout, mxfp4_flashinfer_trtllm_moe.py:11-13)
  *   afd_repack_mxfp4 / ......... the checkpoint expert load (P/srt/model_loader/weight_utils.py
@@ -392,6 +400,64 @@ int afd_combine(const uint16_t* const* parts, int32_t num_parts, const uint16_t*
  * 16-byte aligned, n * inter / 8 < 2^31. */
 int afd_silu_mul(const uint16_t* gate_up, int64_t n, int32_t inter, uint16_t* out,
                  afd_stream_t stream);
+
+/* ---- the router ---------------------------------------------------------------------------
+ * Scores of a row of logits l: softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts
+ * as -inf, +inf as the largest float; a row of -inf alone has scores 0 (and weights 0).
+ * Limits: num_experts <= 1024, topk <= 32, num_groups <= 64 and a divisor of num_experts, topk
+ * experts in the groups kept; n <= 2^26, n * topk < 2^31. */
+enum afd_scoring { AFD_SCORE_SOFTMAX = 0, AFD_SCORE_SIGMOID = 1, AFD_SCORE_SQRTSOFTPLUS = 2 };
+enum afd_logits_fmt { AFD_LOGITS_F32 = 0, AFD_LOGITS_BF16 = 1 };
+
+typedef struct afd_router_cfg {
+  int32_t num_experts;
+  int32_t topk;
+  int32_t scoring;     /* enum afd_scoring */
+  int32_t num_groups;  /* 0 or 1: none */
+  int32_t topk_groups; /* groups whose experts may be chosen */
+  int32_t renormalize; /* the chosen weights add up to scale */
+  float scale;         /* routed scaling factor */
+  int32_t logits_fmt;  /* enum afd_logits_fmt */
+} afd_router_cfg;
+
+/* ids i32 [n][topk], w f32 [n][topk], best first: the topk experts with the largest choice value,
+ * equal values in index order, and w = scale * score (/ the sum of the chosen scores). The choice
+ * value is the logit, or with bias (f32 [num_experts]) score + bias in 64 bits (NaN: -inf). With
+ * groups only the experts of the topk_groups best groups are chosen; a group's value is its
+ * largest choice value, with bias the sum of its two largest. logits: rows of ld >= num_experts
+ * elements. valid: NULL, or u8 [n]: rows of 0 get ids -1 (which the expert call skips) and weights 0. */
+int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t ld, const float* bias,
+             const uint8_t* valid, int32_t n, int32_t* ids, float* w, afd_stream_t stream);
+
+/* Sequences: cu_seqlens i32 [num_seqs + 1], not decreasing: sequence s is rows [cu[s], cu[s + 1]);
+ * NULL with num_seqs 1: all rows. Rows outside them, and rows of valid 0, are not counted. The
+ * workspace (16-byte aligned) holds partial sums of one call. All results are the same bits from call to call.
+ * afd_expert_counts: counts i32 [num_seqs][num_experts], ids outside [0, num_experts) skipped. */
+int afd_balance_workspace(int32_t n, int32_t num_experts, int32_t num_seqs, uint64_t* bytes);
+int afd_expert_counts(const int32_t* ids, int32_t n, int32_t topk, int32_t num_experts,
+                      const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs,
+                      int32_t* counts, void* ws, uint64_t ws_bytes, afd_stream_t stream);
+
+/* loss = alpha * mean over sequences with T > 0 rows of
+ *          num_experts / (topk T^2) * sum_e counts_e * sum_t score_te / sum_j score_tj,
+ * with counts as above, and coef f32 [num_seqs], which the gradient takes beside counts: the factor of
+ * counts_e in d loss / d (normalized score). afd_topk_balance is afd_topk and afd_balance in one pass. */
+int afd_balance(const afd_router_cfg* cfg, const void* logits, int64_t ld, const int32_t* ids,
+                const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs, int32_t n,
+                float alpha, int32_t* counts, float* coef, float* loss, void* ws, uint64_t ws_bytes,
+                afd_stream_t stream);
+int afd_topk_balance(const afd_router_cfg* cfg, const void* logits, int64_t ld, const float* bias,
+                     const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs, int32_t n,
+                     float alpha, int32_t* ids, float* w, int32_t* counts, float* coef, float* loss,
+                     void* ws, uint64_t ws_bytes, afd_stream_t stream);
+
+/* dlogits [n][num_experts] in the logits' format: the gradient of the weights (gw f32 [n][topk]
+ * by afd_topk's w; NULL: none) plus that of the loss (gloss, one device float; coef NULL: none).
+ * The choice of experts, the counts and the bias have no gradient; rows of valid 0 get 0. */
+int afd_router_grad(const afd_router_cfg* cfg, const void* logits, int64_t ld, const int32_t* ids,
+                    const uint8_t* valid, int32_t n, const float* gw, const int32_t* cu_seqlens,
+                    int32_t num_seqs, const int32_t* counts, const float* coef, const float* gloss,
+                    void* dlogits, afd_stream_t stream);
 
 /* ---- transport (one GPU: producer and consumer streams) ---------------------------------
  * Done flags are 64-bit message counters that only grow (a message's counter is the count of

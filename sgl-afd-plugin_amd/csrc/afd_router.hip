@@ -1,0 +1,968 @@
+// The router of a MoE layer on gfx950: which experts a token goes to and with what weight, how the
+// tokens spread over the experts (counts and balance loss), and the gradient of both by the logits.
+//
+// Scores of a row's logits l: s = softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts as
+// -inf and +inf as the largest float, so every score is a finite number; a row of -inf alone scores 0.
+//
+// Selection: the choice value c is the logit itself without a correction bias (every score grows
+// with its logit) and s + bias in 64 bits with one: which of two experts wins a close race then is
+// a matter of the formula and not of a 32-bit exponential's last bit. Equal values go to the lower index.
+//
+// Balance loss of a sequence with T rows: L_s = E / (k T) sum_e cnt_e P_e, P_e = 1/T sum_t s'_te,
+// s' = s / sum_e s; L = alpha times the mean of L_s over the sequences that have rows.
+//   dL/dl_te = s'_te r(l_te) (c_e - sum_j c_j s'_tj),  c_e = gloss coef cnt_e,
+//   coef = alpha E / (S' k T^2),  r = 1, 1 - sigmoid(l), sigmoid(l) / (2 softplus(l)).
+//
+// Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
+// and a lane's first V bytes are one wide load: 16 lanes (4 rows a wavefront) up to 64 experts, 32
+// up to 128, else 64 lanes with V = 4, 8 or 16. Reductions over a row are DPP and permlane-swap butterflies; the k-th
+// winner is a max butterfly and one ballot.
+//
+// Sums over rows: a workgroup takes R consecutive rows, cut where sequences begin and end; each piece
+// writes its sums and counts to a slot of its own (slot = workgroup + sequence: from one piece to the
+// next one of the two grows), and a second launch adds a sequence's slots in their order. No sum
+// depends on which workgroup ends first.
+#include "afd_common.h"
+#include "afd_internal.h"
+
+namespace afd {
+namespace router {
+
+constexpr int kThreads = 256;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopk = 32;
+constexpr int kMaxGroups = 64;
+constexpr int kMaxSeqs = 1 << 20;
+constexpr int kMaxRows = 1 << 26;
+// rows a workgroup's slot sums at most: the sums are fp32, their error grows with the terms
+constexpr int kMaxBlockRows = 1024;
+
+struct Args {
+  const void* logits;
+  int64_t ld;
+  const float* bias;
+  const uint8_t* valid;
+  int32_t n;
+  int32_t experts, topk, scoring, groups, keep, renorm;
+  float scale;
+  int32_t* ids;  // selection: written; balance and gradient: read
+  float* w;
+  // balance
+  const int32_t* cu;  // [seqs + 1], or nullptr: one sequence of all rows
+  int32_t seqs;
+  int32_t block_rows, blocks;
+  float alpha;
+  float* slots;  // [blocks + seqs] of slot_words(experts)
+  int32_t* counts;
+  float* coef;
+  double* part;      // [seqs] unscaled losses
+  int32_t* rows;     // [seqs] rows
+  uint32_t* ticket;  // workgroups of the second launch that are done
+  float* loss;
+  // gradient
+  const float* gw;
+  const float* gloss;
+  void* dlogits;
+};
+
+// sums f32 [E], counts i32 [E], rows i32 (and 3 words of padding)
+__host__ __device__ inline int64_t slot_words(int experts) { return 2 * int64_t(experts) + 4; }
+
+// ---------------------------------------------------------------- reductions over W lanes
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+
+// f(own, partner) over the lanes of a row; every lane gets the same bits (f commutes). After the
+// quads agree, a mirrored half row is the exchange with the other quad, and so on.
+template <int W, typename F>
+__device__ __forceinline__ uint32_t reduce32(uint32_t v, F f) {
+  v = f(v, dpp<kXor1>(v));
+  v = f(v, dpp<kXor2>(v));
+  v = f(v, dpp<kHalfMirror>(v));
+  v = f(v, dpp<kMirror>(v));
+  if constexpr (W >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  if constexpr (W >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  return v;
+}
+template <int W>
+__device__ __forceinline__ uint32_t max_u32(uint32_t v) {
+  return reduce32<W>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int W>
+__device__ __forceinline__ float max_f32(float v) {
+  return __uint_as_float(reduce32<W>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+template <int W>
+__device__ __forceinline__ float sum_f32(float v) {
+  return __uint_as_float(reduce32<W>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = dpp<CTRL>(static_cast<uint32_t>(u)), hi = dpp<CTRL>(static_cast<uint32_t>(u >> 32));
+  return __builtin_bit_cast(double, lo | hi << 32);
+}
+template <int W>
+__device__ __forceinline__ double sum_f64(double v) {
+  v += dpp_f64<kXor1>(v);
+  v += dpp_f64<kXor2>(v);
+  v += dpp_f64<kHalfMirror>(v);
+  v += dpp_f64<kMirror>(v);
+  auto halves = [](uint64_t u, auto swap) {
+    const auto l = swap(static_cast<uint32_t>(u)), h = swap(static_cast<uint32_t>(u >> 32));
+    return __builtin_bit_cast(double, uint64_t(l[0]) | uint64_t(h[0]) << 32) +
+           __builtin_bit_cast(double, uint64_t(l[1]) | uint64_t(h[1]) << 32);
+  };
+  if constexpr (W >= 32)
+    v = halves(__builtin_bit_cast(uint64_t, v),
+               [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  if constexpr (W >= 64)
+    v = halves(__builtin_bit_cast(uint64_t, v),
+               [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+  return v;
+}
+
+// ---------------------------------------------------------------- keys: unsigned order = value order
+// key 0 is below every number's: an expert that is not there, already taken, or in a dropped group
+__device__ __forceinline__ uint32_t key32(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and +0 are equal
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+  return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
+}
+
+// ---------------------------------------------------------------- scores
+constexpr float kLowest = -__builtin_huge_valf();
+__device__ __forceinline__ float logit_f32(const float* p) { return *p; }
+__device__ __forceinline__ float logit_f32(const uint16_t* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ float canon(float v) {
+  return v != v ? kLowest : fminf(v, 3.402823466e38f);
+}
+__device__ __forceinline__ float softplus_f32(float v) { return log1pf(expf(-fabsf(v))) + fmaxf(v, 0.0f); }
+// sigmoid or sqrt(softplus)
+__device__ __forceinline__ float score_f32(float v, int scoring) {
+  return scoring == AFD_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : sqrtf(softplus_f32(v));
+}
+__device__ __forceinline__ double score_f64(double v, int scoring) {
+  return scoring == AFD_SCORE_SIGMOID ? 1.0 / (1.0 + exp(-v)) : sqrt(log1p(exp(-fabs(v))) + fmax(v, 0.0));
+}
+// d score / dl over the score: 1 - sigmoid, or sigmoid / (2 softplus), which tends to 1/2 where
+// softplus(l) -> e^l leaves the floats
+__device__ __forceinline__ float slope_f32(float v, int scoring) {
+  if (scoring == AFD_SCORE_SOFTMAX) return 1.0f;
+  if (scoring == AFD_SCORE_SIGMOID) return 1.0f / (1.0f + expf(v));
+  if (v < -17.0f) return 0.5f;
+  return 1.0f / ((1.0f + expf(-v)) * 2.0f * softplus_f32(v));
+}
+
+template <typename T, int W, int V>
+struct Row {
+  float l[V];  // canonical logits of the lane's experts, -inf past the last one
+  int e0;      // the lane's first expert
+
+  __device__ __forceinline__ void load(const Args& a, int64_t t, int li) {
+    e0 = li * V;
+    const T* p = static_cast<const T*>(a.logits) + t * a.ld + e0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) l[j] = e0 + j < a.experts ? canon(logit_f32(p + j)) : kLowest;
+  }
+  // The row's scores in fp32: s[j] (0 past the last expert), and their sum
+  __device__ __forceinline__ float scores(const Args& a, float (&s)[V]) const {
+    float sum = 0.0f;
+    if (a.scoring == AFD_SCORE_SOFTMAX) {
+      float m = l[0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
+      m = max_f32<W>(m);
+      const float at = m == kLowest ? 0.0f : m;  // a row of -inf: all scores 0
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s[j] = expf(l[j] - at);
+        sum += s[j];
+      }
+      return sum_f32<W>(sum);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s[j] = e0 + j < a.experts ? score_f32(l[j], a.scoring) : 0.0f;
+      sum += s[j];
+    }
+    return sum_f32<W>(sum);
+  }
+};
+
+// The lanes of this row in a ballot
+template <int W>
+__device__ __forceinline__ uint64_t row_bits(uint64_t ballot, int lane) {
+  if constexpr (W == 64) return ballot;
+  return (ballot >> (lane & ~(W - 1))) & ((uint64_t(1) << W) - 1);
+}
+
+// Takes the row's largest key (lowest index of equals): its expert, the same in every lane; the key becomes 0.
+template <int W, int V>
+__device__ __forceinline__ int take(uint32_t (&key)[V], int lane, int e0) {
+  uint32_t best = key[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
+  const uint32_t m = max_u32<W>(best);
+  const int win = __builtin_ctzll(row_bits<W>(__ballot(best == m), lane));
+  int j_win = V - 1;
+#pragma unroll
+  for (int j = V - 2; j >= 0; --j) j_win = key[j] == m ? j : j_win;
+  const bool mine = (lane & (W - 1)) == win;
+#pragma unroll
+  for (int j = 0; j < V; ++j) key[j] = mine && j == j_win ? 0u : key[j];
+  return __shfl(e0 + j_win, win, W);
+}
+template <int W, int V>
+__device__ __forceinline__ int take(uint64_t (&key)[V], int lane, int e0) {
+  uint64_t best = key[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
+  const uint32_t hi = static_cast<uint32_t>(best >> 32), m_hi = max_u32<W>(hi);
+  const uint32_t lo = hi == m_hi ? static_cast<uint32_t>(best) : 0u, m_lo = max_u32<W>(lo);
+  const uint64_t m = uint64_t(m_hi) << 32 | m_lo;
+  const int win = __builtin_ctzll(row_bits<W>(__ballot(best == m), lane));
+  int j_win = V - 1;
+#pragma unroll
+  for (int j = V - 2; j >= 0; --j) j_win = key[j] == m ? j : j_win;
+  const bool mine = (lane & (W - 1)) == win;
+#pragma unroll
+  for (int j = 0; j < V; ++j) key[j] = mine && j == j_win ? 0ull : key[j];
+  return __shfl(e0 + j_win, win, W);
+}
+
+// LDS of a wavefront's rows for the groups' values: expert e of group g at e + g
+__host__ __device__ constexpr int group_words(int W, int V) { return W * V + kMaxGroups; }
+
+// Which groups stay: the value of a group is its largest key's value (no bias) or the sum of its two
+// largest choice values (bias). A lane takes whole groups, from the row's copy in LDS.
+template <int W, int V, bool BIAS, typename K>
+__device__ __forceinline__ void drop_groups(const Args& a, K (&key)[V], const double (&c)[V], int lane, int e0,
+                                            double* lds_row) {
+  const int size = a.experts / a.groups, li = lane & (W - 1);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (e0 + j < a.experts) lds_row[e0 + j + (e0 + j) / size] = c[j];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  // lane g < groups (groups <= W) holds group g's value
+  uint64_t gkey[1] = {0};
+  if (li < a.groups) {
+    double first = -__builtin_huge_val(), second = first;
+    for (int i = 0; i < size; ++i) {
+      const double v = lds_row[li * (size + 1) + i];
+      second = fmax(second, fmin(first, v));
+      first = fmax(first, v);
+    }
+    double value = BIAS && size > 1 ? first + second : first;
+    if (value != value) value = -__builtin_huge_val();
+    gkey[0] = key64(value);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  uint64_t kept = 0;
+  for (int i = 0; i < a.keep; ++i) kept |= uint64_t(1) << take<W, 1>(gkey, lane, li);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (e0 + j < a.experts && !(kept >> ((e0 + j) / size) & 1)) key[j] = 0;
+}
+
+// Selection of one row: lane kk < topk gets the kk-th expert and its weight.
+template <typename T, int W, int V, bool BIAS>
+__device__ __forceinline__ void select_row(const Args& a, const Row<T, W, V>& row, int64_t t, int lane,
+                                           double* lds_row, int& id, float& weight) {
+  const int li = lane & (W - 1), e0 = row.e0;
+  double c[V] = {};
+  float m = row.l[0];
+  if constexpr (BIAS) {
+    double sum = 1.0;
+    if (a.scoring == AFD_SCORE_SOFTMAX) {
+#pragma unroll
+      for (int j = 1; j < V; ++j) m = fmaxf(m, row.l[j]);
+      m = max_f32<W>(m);
+      const double at = m == kLowest ? 0.0 : static_cast<double>(m);
+      sum = 0.0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        c[j] = exp(static_cast<double>(row.l[j]) - at);
+        sum += c[j];
+      }
+      sum = sum_f64<W>(sum);
+      if (sum == 0.0) sum = 1.0;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (e0 + j >= a.experts) continue;
+      if (a.scoring == AFD_SCORE_SOFTMAX)
+        c[j] /= sum;
+      else
+        c[j] = score_f64(row.l[j], a.scoring);
+      c[j] += a.bias[e0 + j];
+      if (c[j] != c[j]) c[j] = -__builtin_huge_val();
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = row.l[j];
+  }
+  using K = std::conditional_t<BIAS, uint64_t, uint32_t>;
+  K key[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if constexpr (BIAS)
+      key[j] = e0 + j < a.experts ? key64(c[j]) : 0;
+    else
+      key[j] = e0 + j < a.experts ? key32(row.l[j]) : 0;
+  }
+  if (a.groups > 1) drop_groups<W, V, BIAS>(a, key, c, lane, e0, lds_row);
+  id = 0;
+  for (int kk = 0; kk < a.topk; ++kk) {
+    const int e = take<W, V>(key, lane, e0);
+    id = li == kk ? e : id;
+  }
+  // weights, in lanes kk < topk, from the chosen logits alone where nothing else is needed
+  const bool live = li < a.topk;
+  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
+  const float l = live ? canon(logit_f32(p + id)) : kLowest;
+  float s;
+  if (a.scoring == AFD_SCORE_SOFTMAX) {
+    // renormalized, the largest chosen logit is the reference: the others' ratios to it survive
+    // however small the scores are
+    m = l;
+    if (!a.renorm) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = fmaxf(m, row.l[j]);
+    }
+    m = max_f32<W>(m);
+    const float at = m == kLowest ? 0.0f : m;
+    s = expf(l - at);  // 0 in lanes without a pick
+    float sum = s;
+    if (!a.renorm) {
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += expf(row.l[j] - at);
+    }
+    sum = sum_f32<W>(sum);
+    weight = sum > 0.0f ? s / sum * a.scale : 0.0f;
+    return;
+  }
+  s = live ? score_f32(l, a.scoring) : 0.0f;
+  if (a.renorm) {
+    const float sum = sum_f32<W>(s);
+    s = sum > 0.0f ? s / sum : 0.0f;
+  }
+  weight = s * a.scale;
+}
+
+// ---------------------------------------------------------------- selection
+template <typename T, int W, int V, bool BIAS>
+__global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
+  constexpr int kRows = kThreads / W;  // rows in flight of a workgroup
+  __shared__ double lds[kRows * group_words(W, V)];
+  const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < a.n; r0 += int64_t(gridDim.x) * kRows) {
+    const int64_t r = r0 + sub;
+    const int64_t rr = r < a.n ? r : a.n - 1;  // the lanes of a wavefront stay together
+    Row<T, W, V> row;
+    row.load(a, rr, li);
+    int id;
+    float w;
+    select_row<T, W, V, BIAS>(a, row, rr, lane, lds + sub * group_words(W, V), id, w);
+    if (a.valid != nullptr && !a.valid[rr]) id = -1, w = 0.0f;
+    if (r < a.n && li < a.topk) {
+      a.ids[r * a.topk + li] = id;
+      a.w[r * a.topk + li] = w;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- pieces of a block of rows
+// The piece of rows that starts at r: up to `end` within one sequence (`seq`), or between sequences (-1).
+// Whatever cu holds, end > r and seq < seqs.
+struct Piece {
+  int32_t end, seq;
+};
+__device__ __forceinline__ Piece next_piece(const Args& a, int32_t r, int32_t r1) {
+  if (a.cu == nullptr) return {r1, 0};
+  int lo = 0, hi = a.seqs;  // first sequence that ends behind r
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.cu[mid + 1] > r)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  if (lo == a.seqs) return {r1, -1};
+  const int32_t from = a.cu[lo];
+  if (from > r) return {min(from, r1), -1};
+  return {min(a.cu[lo + 1], r1), lo};
+}
+
+// ---------------------------------------------------------------- a sequence's slots together
+// One workgroup: counts[s], rows[s] and the unscaled loss of sequence s.
+__device__ void finish_sequence(const Args& a, int s, double* red) {
+  const int t = threadIdx.x;
+  int32_t lo = 0, hi = a.n;
+  if (a.cu != nullptr) {
+    lo = min(max(a.cu[s], 0), a.n);
+    hi = min(max(a.cu[s + 1], 0), a.n);
+  }
+  const int b0 = lo / a.block_rows, b1 = hi > lo ? (hi - 1) / a.block_rows + 1 : b0;
+  const int64_t words = slot_words(a.experts);
+  const float* first = a.slots + (int64_t(b0) + s) * words;
+  int rows = 0;
+  for (int b = 0; b < b1 - b0; ++b) rows += reinterpret_cast<const int32_t*>(first + b * words)[2 * a.experts];
+  double loss = 0.0;
+  for (int e = t; e < a.experts; e += blockDim.x) {
+    double p = 0.0;
+    int cnt = 0;
+    for (int b = 0; b < b1 - b0; ++b) {
+      p += first[b * words + e];
+      cnt += reinterpret_cast<const int32_t*>(first + b * words)[a.experts + e];
+    }
+    a.counts[int64_t(s) * a.experts + e] = cnt;
+    loss += p * cnt;
+  }
+  if (a.loss == nullptr) return;
+  red[t] = loss;
+  __syncthreads();
+  for (int h = blockDim.x / 2; h > 0; h /= 2) {
+    if (t < h) red[t] += red[t + h];
+    __syncthreads();
+  }
+  if (t == 0) {
+    a.part[s] = rows > 0 ? red[0] * a.experts / (double(a.topk) * rows * rows) : 0.0;
+    a.rows[s] = rows;
+  }
+  __syncthreads();
+}
+
+// One workgroup, after every sequence: the loss and the sequences' coefficients.
+__device__ void finish_loss(const Args& a, double* red) {
+  const int t = threadIdx.x;
+  double sum = 0.0, used = 0.0;
+  for (int s = t; s < a.seqs; s += blockDim.x) {
+    sum += a.part[s];
+    used += a.rows[s] > 0 ? 1.0 : 0.0;
+  }
+  red[t] = sum;
+  __syncthreads();
+  for (int h = blockDim.x / 2; h > 0; h /= 2) {
+    if (t < h) red[t] += red[t + h];
+    __syncthreads();
+  }
+  sum = red[0];
+  __syncthreads();
+  red[t] = used;
+  __syncthreads();
+  for (int h = blockDim.x / 2; h > 0; h /= 2) {
+    if (t < h) red[t] += red[t + h];
+    __syncthreads();
+  }
+  used = red[0];
+  if (t == 0) *a.loss = used > 0.0 ? static_cast<float>(a.alpha * sum / used) : 0.0f;
+  for (int s = t; s < a.seqs; s += blockDim.x) {
+    const double rows = a.rows[s];
+    a.coef[s] = rows > 0 ? static_cast<float>(double(a.alpha) * a.experts / (used * a.topk * rows * rows)) : 0.0f;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void finish_kernel(Args a) {
+  __shared__ double red[kThreads];
+  __shared__ uint32_t done;
+  for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) finish_sequence(a, s, red);
+  if (a.loss == nullptr) return;
+  // the last workgroup adds the sequences up
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) done = atomicAdd(a.ticket, 1u);
+  __syncthreads();
+  if (done != gridDim.x - 1) return;
+  __threadfence();
+  finish_loss(a, red);
+}
+
+// ---------------------------------------------------------------- selection, counts and balance sums
+// SELECT: choose the experts (else read a.ids). SCORES: sums of s' (else counts alone).
+template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES>
+__global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
+  constexpr int kRows = kThreads / W;
+  __shared__ double lds[SELECT ? kRows * group_words(W, V) : 1];
+  __shared__ float sums[SCORES ? kRows * W * V : 1];
+  __shared__ int32_t cnt[kMaxExperts];
+  __shared__ int32_t live_rows;
+  const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  if (blockIdx.x == 0 && t == 0 && a.ticket != nullptr) *a.ticket = 0;  // for the second launch
+  const int32_t r0 = blockIdx.x * a.block_rows;
+  const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
+  for (int32_t at = r0; at < r1;) {
+    const Piece piece = next_piece(a, at, r1);
+    const bool counted = piece.seq >= 0;
+    for (int e = t; e < a.experts; e += kThreads) cnt[e] = 0;
+    if (t == 0) live_rows = 0;
+    __syncthreads();
+    float p[V] = {};
+    int mine = 0;
+    for (int32_t base = at; base < piece.end; base += kRows) {
+      const int32_t r = base + sub;
+      const bool in = r < piece.end;
+      const int32_t rr = in ? r : piece.end - 1;
+      const bool live = in && (a.valid == nullptr || a.valid[rr]);
+      Row<T, W, V> row;
+      if constexpr (SELECT || SCORES) row.load(a, rr, li);
+      if constexpr (SELECT) {
+        int id;
+        float w;
+        select_row<T, W, V, BIAS>(a, row, rr, lane, lds + sub * group_words(W, V), id, w);
+        if (in && li < a.topk) {
+          a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
+          a.w[int64_t(r) * a.topk + li] = live ? w : 0.0f;
+          if (live && counted) atomicAdd(&cnt[id], 1);
+        }
+      } else if (live && counted) {
+        for (int kk = li; kk < a.topk; kk += W) {
+          const int id = a.ids[int64_t(r) * a.topk + kk];
+          if (id >= 0 && id < a.experts) atomicAdd(&cnt[id], 1);
+        }
+      }
+      if constexpr (SCORES) {
+        float s[V];
+        const float sum = row.scores(a, s);
+        const float inv = live && sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
+      }
+      mine += live ? 1 : 0;
+    }
+    if (counted) {
+      if (li == 0) atomicAdd(&live_rows, mine);
+      if constexpr (SCORES) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sums[sub * (W * V) + li * V + j] = p[j];
+      }
+      __syncthreads();
+      float* slot = a.slots + (int64_t(blockIdx.x) + piece.seq) * slot_words(a.experts);
+      int32_t* slot_i = reinterpret_cast<int32_t*>(slot);
+      for (int e = t; e < a.experts; e += kThreads) {
+        if constexpr (SCORES) {
+          float s = 0.0f;
+          for (int i = 0; i < kRows; ++i) s += sums[i * (W * V) + e];
+          slot[e] = s;
+        } else {
+          slot[e] = 0.0f;
+        }
+        slot_i[a.experts + e] = cnt[e];
+      }
+      if (t == 0) slot_i[2 * a.experts] = live_rows;
+    }
+    __syncthreads();
+    at = piece.end;
+  }
+}
+
+// ---------------------------------------------------------------- gradient by the logits
+template <typename T>
+__device__ __forceinline__ void store_logit(T* p, float v);
+template <>
+__device__ __forceinline__ void store_logit<float>(float* p, float v) { *p = v; }
+template <>
+__device__ __forceinline__ void store_logit<uint16_t>(uint16_t* p, float v) { *p = f32_to_bf16(v); }
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
+  constexpr int kRows = kThreads / W;
+  const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  const float gloss = a.coef != nullptr ? *a.gloss : 0.0f;
+  const int32_t r0 = blockIdx.x * a.block_rows;
+  const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
+  for (int32_t at = r0; at < r1;) {
+    Piece piece = {r1, -1};
+    if (a.coef != nullptr) piece = next_piece(a, at, r1);
+    const bool balanced = piece.seq >= 0;
+    float c[V] = {};
+    if (balanced) {
+      const float f = gloss * a.coef[piece.seq];
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (li * V + j < a.experts) c[j] = f * a.counts[int64_t(piece.seq) * a.experts + li * V + j];
+    }
+    for (int32_t base = at; base < piece.end; base += kRows) {
+      const int32_t r = base + sub;
+      const bool in = r < piece.end;
+      const int32_t rr = in ? r : piece.end - 1;
+      const bool live = a.valid == nullptr || a.valid[rr];
+      Row<T, W, V> row;
+      row.load(a, rr, li);
+      float s[V], d[V];
+      const float total = row.scores(a, s);
+      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = 0.0f;
+      if (balanced) {
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) dot += c[j] * (s[j] * inv);
+        dot = sum_f32<W>(dot);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = s[j] * inv * (c[j] - dot);
+      }
+      if (a.gw != nullptr) {
+        // lane kk < topk: the kk-th chosen expert's share of the weights' scores, and its gradient
+        const T* p = static_cast<const T*>(a.logits) + int64_t(rr) * a.ld;
+        int id = li < a.topk ? a.ids[int64_t(rr) * a.topk + li] : -1;
+        if (id >= a.experts) id = -1;
+        const float g = id >= 0 ? a.gw[int64_t(rr) * a.topk + li] * a.scale : 0.0f;
+        const float l = id >= 0 ? canon(logit_f32(p + id)) : kLowest;
+        // share: of the chosen (renormalized) or of all (softmax), or the score itself
+        float share;
+        if (a.scoring == AFD_SCORE_SOFTMAX) {
+          float m = l;
+          if (!a.renorm) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = fmaxf(m, row.l[j]);
+          }
+          m = max_f32<W>(m);
+          share = id >= 0 ? expf(l - (m == kLowest ? 0.0f : m)) : 0.0f;
+        } else {
+          share = id >= 0 ? score_f32(l, a.scoring) : 0.0f;
+        }
+        const float chosen = sum_f32<W>(share);
+        if (a.renorm)
+          share = chosen > 0.0f ? share / chosen : 0.0f;
+        else if (a.scoring == AFD_SCORE_SOFTMAX)
+          share *= inv;
+        // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something
+        float mean = 0.0f;
+        if (a.renorm || a.scoring == AFD_SCORE_SOFTMAX) mean = sum_f32<W>(g * share);
+        const float u = share * (g - (a.renorm ? mean : 0.0f));
+        for (int kk = 0; kk < a.topk; ++kk) {
+          const int e = __shfl(id, kk, W);
+          const float v = __shfl(u, kk, W);
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] += e == row.e0 + j ? v : 0.0f;
+        }
+        if (!a.renorm && a.scoring == AFD_SCORE_SOFTMAX) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] -= s[j] * inv * mean;
+        }
+      }
+      if (in) {
+        T* out = static_cast<T*>(a.dlogits) + int64_t(r) * a.experts + row.e0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (row.e0 + j >= a.experts) continue;
+          const float v = live ? d[j] * slope_f32(row.l[j], a.scoring) : 0.0f;
+          store_logit<T>(out + j, v);
+        }
+      }
+    }
+    at = piece.end;
+  }
+}
+
+// ---------------------------------------------------------------- host
+// f(W, V) for a row of `experts` whose first `lanes` lanes hold picks or groups
+template <typename F>
+int with_shape(int experts, int lanes, F&& f) {
+  using std::integral_constant;
+  if (experts <= 64 && lanes <= 16) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  if (experts <= 128 && lanes <= 32) return f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  if (experts <= 256) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  if (experts <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+}
+template <typename F>
+int with_logits(int fmt, F&& f) {
+  return fmt == AFD_LOGITS_F32 ? f(float{}) : f(uint16_t{});
+}
+
+static int check_cfg(const afd_router_cfg* c) {
+  if (!c) return AFD_ERR_ARG;
+  if (c->num_experts < 1 || c->num_experts > kMaxExperts) return AFD_ERR_SHAPE;
+  if (c->topk < 1 || c->topk > kMaxTopk || c->topk > c->num_experts) return AFD_ERR_SHAPE;
+  if (c->scoring < AFD_SCORE_SOFTMAX || c->scoring > AFD_SCORE_SQRTSOFTPLUS) return AFD_ERR_UNSUPPORTED;
+  if (c->logits_fmt != AFD_LOGITS_F32 && c->logits_fmt != AFD_LOGITS_BF16) return AFD_ERR_UNSUPPORTED;
+  if (c->num_groups < 0 || c->num_groups > kMaxGroups) return AFD_ERR_SHAPE;
+  if (c->num_groups > 1) {
+    if (c->num_experts % c->num_groups) return AFD_ERR_SHAPE;
+    if (c->topk_groups < 1 || c->topk_groups > c->num_groups) return AFD_ERR_SHAPE;
+    if (c->topk > c->topk_groups * (c->num_experts / c->num_groups)) return AFD_ERR_SHAPE;
+  }
+  return AFD_OK;
+}
+static int check_rows(int32_t n, int32_t topk) {
+  if (n < 0 || n > kMaxRows || int64_t(n) * topk > 0x7fffffffll) return AFD_ERR_ARG;
+  return AFD_OK;
+}
+static int check_logits(const afd_router_cfg& c, const void* logits, int64_t ld, int32_t n) {
+  if (n > 0 && !logits) return AFD_ERR_ARG;
+  if (ld < c.num_experts) return AFD_ERR_SHAPE;
+  return AFD_OK;
+}
+static int check_seqs(const int32_t* cu, int32_t seqs) {
+  if (seqs < 1 || seqs > kMaxSeqs || (!cu && seqs != 1)) return AFD_ERR_ARG;
+  return AFD_OK;
+}
+
+static Args base_args(const afd_router_cfg& c, const void* logits, int64_t ld, int32_t n) {
+  Args a = {};
+  a.logits = logits;
+  a.ld = ld;
+  a.n = n;
+  a.experts = c.num_experts;
+  a.topk = c.topk;
+  a.scoring = c.scoring;
+  a.groups = c.num_groups > 1 ? c.num_groups : 1;
+  a.keep = c.topk_groups;
+  a.renorm = c.renormalize != 0;
+  a.scale = c.scale;
+  return a;
+}
+static int lanes_needed(const Args& a, bool select) {
+  return select && a.groups > a.topk ? a.groups : a.topk;
+}
+
+// rows of a workgroup: four workgroups a CU, whole passes of its wavefronts, at most kMaxBlockRows
+static int block_rows_for(int32_t n, int lanes_per_row) {
+  const int pass = kThreads / lanes_per_row;
+  int64_t rows = (int64_t(n) + 1023) / 1024;
+  rows = (rows + pass - 1) / pass * pass;
+  return static_cast<int>(rows < pass ? pass : rows > kMaxBlockRows ? kMaxBlockRows : rows);
+}
+static int blocks_for(int32_t n, int block_rows) { return static_cast<int>((int64_t(n) + block_rows - 1) / block_rows); }
+
+// The workspace: slots, part f64, rows i32, ticket. Slots are counted for the smallest block of rows.
+struct WsPlan {
+  uint64_t slots, part, rows, ticket, total;
+};
+static WsPlan plan(int32_t n, int32_t experts, int32_t seqs) {
+  WsPlan p = {};
+  const int rows = block_rows_for(n, 64);
+  const uint64_t count = uint64_t(blocks_for(n, rows)) + seqs;
+  auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
+  p.slots = 0;
+  p.part = round(count * slot_words(experts) * 4);
+  p.rows = p.part + round(uint64_t(seqs) * 8);
+  p.ticket = p.rows + round(uint64_t(seqs) * 4);
+  p.total = p.ticket + 256;
+  return p;
+}
+static void place(Args& a, void* ws, const WsPlan& p) {
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  a.slots = reinterpret_cast<float*>(b + p.slots);
+  a.part = reinterpret_cast<double*>(b + p.part);
+  a.rows = reinterpret_cast<int32_t*>(b + p.rows);
+  a.ticket = reinterpret_cast<uint32_t*>(b + p.ticket);
+}
+
+__global__ __launch_bounds__(kThreads) void no_rows_kernel(Args a) {
+  for (int64_t i = blockIdx.x * int64_t(kThreads) + threadIdx.x; i < int64_t(a.seqs) * a.experts;
+       i += int64_t(gridDim.x) * kThreads)
+    a.counts[i] = 0;
+  if (a.loss == nullptr) return;
+  for (int64_t s = blockIdx.x * int64_t(kThreads) + threadIdx.x; s < a.seqs; s += int64_t(gridDim.x) * kThreads)
+    a.coef[s] = 0.0f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.loss = 0.0f;
+}
+
+// select: a.ids / a.w are written; scores: with the balance sums
+static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t s) {
+  if (a.n == 0) {
+    hipLaunchKernelGGL(no_rows_kernel, dim3(64), dim3(kThreads), 0, s, a);
+    AFD_CHECK_LAUNCH();
+    return AFD_OK;
+  }
+  const int st = with_logits(fmt, [&](auto tag) {
+    using T = decltype(tag);
+    return with_shape(a.experts, lanes_needed(a, select), [&](auto wc, auto vc) {
+      constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
+      a.block_rows = block_rows_for(a.n, W);
+      a.blocks = blocks_for(a.n, a.block_rows);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), 0, s, a);
+        AFD_CHECK_LAUNCH();
+        return int(AFD_OK);
+      };
+      if (!scores) return go(balance_kernel<T, W, V, false, false, false>);
+      if (!select) return go(balance_kernel<T, W, V, false, false, true>);
+      return a.bias ? go(balance_kernel<T, W, V, true, true, true>) : go(balance_kernel<T, W, V, true, false, true>);
+    });
+  });
+  if (st != AFD_OK) return st;
+  const int grid = a.seqs < 1024 ? a.seqs : 1024;
+  hipLaunchKernelGGL(finish_kernel, dim3(grid), dim3(kThreads), 0, s, a);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
+}
+
+}  // namespace router
+}  // namespace afd
+
+using namespace afd;
+
+extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t ld, const float* bias,
+                        const uint8_t* valid, int32_t n, int32_t* ids, float* w, afd_stream_t stream) {
+  int st = router::check_cfg(cfg);
+  if (st == AFD_OK) st = router::check_rows(n, cfg->topk);
+  if (st == AFD_OK) st = router::check_logits(*cfg, logits, ld, n);
+  if (st != AFD_OK) return st;
+  if (n == 0) return AFD_OK;
+  if (!ids || !w) return AFD_ERR_ARG;
+  router::Args a = router::base_args(*cfg, logits, ld, n);
+  a.bias = bias;
+  a.valid = valid;
+  a.ids = ids;
+  a.w = w;
+  return router::with_logits(cfg->logits_fmt, [&](auto tag) {
+    using T = decltype(tag);
+    return router::with_shape(a.experts, router::lanes_needed(a, true), [&](auto wc, auto vc) {
+      constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
+      int64_t grid = (int64_t(n) + kRows - 1) / kRows;
+      if (grid > int64_t(16) * device_cu_count()) grid = int64_t(16) * device_cu_count();
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(router::kThreads), 0,
+                           static_cast<hipStream_t>(stream), a);
+        AFD_CHECK_LAUNCH();
+        return int(AFD_OK);
+      };
+      return bias ? go(router::topk_kernel<T, W, V, true>) : go(router::topk_kernel<T, W, V, false>);
+    });
+  });
+}
+
+extern "C" int afd_balance_workspace(int32_t n, int32_t num_experts, int32_t num_seqs, uint64_t* bytes) {
+  if (!bytes || n < 0 || n > router::kMaxRows || num_seqs < 1 || num_seqs > router::kMaxSeqs) return AFD_ERR_ARG;
+  if (num_experts < 1 || num_experts > router::kMaxExperts) return AFD_ERR_SHAPE;
+  *bytes = router::plan(n, num_experts, num_seqs).total;
+  return AFD_OK;
+}
+
+extern "C" int afd_topk_balance(const afd_router_cfg* cfg, const void* logits, int64_t ld, const float* bias,
+                                const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs, int32_t n,
+                                float alpha, int32_t* ids, float* w, int32_t* counts, float* coef, float* loss,
+                                void* ws, uint64_t ws_bytes, afd_stream_t stream) {
+  int st = router::check_cfg(cfg);
+  if (st == AFD_OK) st = router::check_rows(n, cfg->topk);
+  if (st == AFD_OK) st = router::check_logits(*cfg, logits, ld, n);
+  if (st == AFD_OK) st = router::check_seqs(cu_seqlens, num_seqs);
+  if (st != AFD_OK) return st;
+  if (!counts || !coef || !loss || !ws || (n > 0 && (!ids || !w))) return AFD_ERR_ARG;
+  const router::WsPlan p = router::plan(n, cfg->num_experts, num_seqs);
+  if (ws_bytes < p.total || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
+  router::Args a = router::base_args(*cfg, logits, ld, n);
+  a.bias = bias;
+  a.valid = valid;
+  a.ids = ids;
+  a.w = w;
+  a.cu = cu_seqlens;
+  a.seqs = num_seqs;
+  a.alpha = alpha;
+  a.counts = counts;
+  a.coef = coef;
+  a.loss = loss;
+  router::place(a, ws, p);
+  return router::launch_balance(a, cfg->logits_fmt, true, true, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int afd_balance(const afd_router_cfg* cfg, const void* logits, int64_t ld, const int32_t* ids,
+                           const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs, int32_t n, float alpha,
+                           int32_t* counts, float* coef, float* loss, void* ws, uint64_t ws_bytes,
+                           afd_stream_t stream) {
+  int st = router::check_cfg(cfg);
+  if (st == AFD_OK) st = router::check_rows(n, cfg->topk);
+  if (st == AFD_OK) st = router::check_logits(*cfg, logits, ld, n);
+  if (st == AFD_OK) st = router::check_seqs(cu_seqlens, num_seqs);
+  if (st != AFD_OK) return st;
+  if (!counts || !coef || !loss || !ws || (n > 0 && !ids)) return AFD_ERR_ARG;
+  const router::WsPlan p = router::plan(n, cfg->num_experts, num_seqs);
+  if (ws_bytes < p.total || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
+  router::Args a = router::base_args(*cfg, logits, ld, n);
+  a.groups = 1;  // the choice is made
+  a.valid = valid;
+  a.ids = const_cast<int32_t*>(ids);
+  a.cu = cu_seqlens;
+  a.seqs = num_seqs;
+  a.alpha = alpha;
+  a.counts = counts;
+  a.coef = coef;
+  a.loss = loss;
+  router::place(a, ws, p);
+  return router::launch_balance(a, cfg->logits_fmt, false, true, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int afd_expert_counts(const int32_t* ids, int32_t n, int32_t topk, int32_t num_experts,
+                                 const uint8_t* valid, const int32_t* cu_seqlens, int32_t num_seqs, int32_t* counts,
+                                 void* ws, uint64_t ws_bytes, afd_stream_t stream) {
+  if (num_experts < 1 || num_experts > router::kMaxExperts || topk < 1 || topk > router::kMaxTopk)
+    return AFD_ERR_SHAPE;
+  int st = router::check_rows(n, topk);
+  if (st == AFD_OK) st = router::check_seqs(cu_seqlens, num_seqs);
+  if (st != AFD_OK) return st;
+  if (!counts || !ws || (n > 0 && !ids)) return AFD_ERR_ARG;
+  const router::WsPlan p = router::plan(n, num_experts, num_seqs);
+  if (ws_bytes < p.total || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
+  router::Args a = {};
+  a.ids = const_cast<int32_t*>(ids);
+  a.n = n;
+  a.topk = topk;
+  a.experts = num_experts;
+  a.groups = 1;
+  a.valid = valid;
+  a.cu = cu_seqlens;
+  a.seqs = num_seqs;
+  a.counts = counts;
+  router::place(a, ws, p);
+  return router::launch_balance(a, AFD_LOGITS_F32, false, false, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int afd_router_grad(const afd_router_cfg* cfg, const void* logits, int64_t ld, const int32_t* ids,
+                               const uint8_t* valid, int32_t n, const float* gw, const int32_t* cu_seqlens,
+                               int32_t num_seqs, const int32_t* counts, const float* coef, const float* gloss,
+                               void* dlogits, afd_stream_t stream) {
+  int st = router::check_cfg(cfg);
+  if (st == AFD_OK) st = router::check_rows(n, cfg->topk);
+  if (st == AFD_OK) st = router::check_logits(*cfg, logits, ld, n);
+  if (st == AFD_OK && coef) st = router::check_seqs(cu_seqlens, num_seqs);
+  if (st != AFD_OK) return st;
+  if (coef && (!counts || !gloss)) return AFD_ERR_ARG;
+  if (n == 0) return AFD_OK;
+  if (!dlogits || (gw && !ids)) return AFD_ERR_ARG;
+  router::Args a = router::base_args(*cfg, logits, ld, n);
+  a.groups = 1;
+  a.valid = valid;
+  a.ids = const_cast<int32_t*>(ids);
+  a.gw = gw;
+  a.cu = cu_seqlens;
+  a.seqs = num_seqs;
+  a.counts = const_cast<int32_t*>(counts);
+  a.coef = const_cast<float*>(coef);
+  a.gloss = gloss;
+  a.dlogits = dlogits;
+  return router::with_logits(cfg->logits_fmt, [&](auto tag) {
+    using T = decltype(tag);
+    return router::with_shape(a.experts, router::lanes_needed(a, false), [&](auto wc, auto vc) {
+      constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
+      a.block_rows = router::block_rows_for(n, W);
+      a.blocks = router::blocks_for(n, a.block_rows);
+      hipLaunchKernelGGL((router::grad_kernel<T, W, V>), dim3(a.blocks), dim3(router::kThreads), 0,
+                         static_cast<hipStream_t>(stream), a);
+      AFD_CHECK_LAUNCH();
+      return int(AFD_OK);
+    });
+  });
+}

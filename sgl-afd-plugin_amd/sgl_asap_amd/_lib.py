@@ -31,6 +31,9 @@ AFD_ACT_SWIGLU = 0
 AFD_ACT_SITU = 1
 AFD_ACT_SWIGLU_LIMIT = 2
 
+AFD_SCORE_SOFTMAX, AFD_SCORE_SIGMOID, AFD_SCORE_SQRTSOFTPLUS = 0, 1, 2
+AFD_LOGITS_F32, AFD_LOGITS_BF16 = 0, 1
+
 AFD_WAIT_GEQ, AFD_WAIT_EQ, AFD_WAIT_AND, AFD_WAIT_NOR = 0, 1, 2, 3
 
 AFD_WALK_STATIC, AFD_WALK_DYNAMIC = 0, 1
@@ -65,6 +68,12 @@ EXPORTED = (
     "afd_finalize",
     "afd_combine",
     "afd_silu_mul",
+    "afd_topk",
+    "afd_balance_workspace",
+    "afd_expert_counts",
+    "afd_balance",
+    "afd_topk_balance",
+    "afd_router_grad",
     "afd_host_alloc",
     "afd_host_free",
     "afd_copy_async",
@@ -109,6 +118,21 @@ class AfdExpertWeights(ctypes.Structure):
         ("s13", ctypes.c_void_p),
         ("w2", ctypes.c_void_p),
         ("s2", ctypes.c_void_p),
+    ]
+
+
+class AfdRouterCfg(ctypes.Structure):
+    """afd_router_cfg: a router's choice of experts (afd_topk and the balance loss)."""
+
+    _fields_ = [
+        ("num_experts", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("scoring", ctypes.c_int32),
+        ("num_groups", ctypes.c_int32),
+        ("topk_groups", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("logits_fmt", ctypes.c_int32),
     ]
 
 
@@ -206,6 +230,7 @@ class AfdReplyDesc(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I32, _I64, _U64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
+_ROUTER, _F32 = ctypes.POINTER(AfdRouterCfg), ctypes.c_float
 _SIGS = {
     "afd_abi_version": ([], _I32),
     "afd_status_string": ([_I32], ctypes.c_char_p),
@@ -251,6 +276,15 @@ _SIGS = {
     "afd_finalize": ([_P, _P, _P, _I32, _I32, _I32, _P, _P], _I32),
     "afd_combine": ([ctypes.POINTER(ctypes.c_void_p), _I32, _P, _P, _I64, _P], _I32),
     "afd_silu_mul": ([_P, _I64, _I32, _P, _P], _I32),
+    "afd_topk": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _P], _I32),
+    "afd_balance_workspace": ([_I32, _I32, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_expert_counts": ([_P, _I32, _I32, _I32, _P, _P, _I32, _P, _P, _U64, _P], _I32),
+    "afd_balance": ([_ROUTER, _P, _I64, _P, _P, _P, _I32, _I32, _F32, _P, _P, _P, _P, _U64, _P], _I32),
+    "afd_topk_balance": (
+        [_ROUTER, _P, _I64, _P, _P, _P, _I32, _I32, _F32, _P, _P, _P, _P, _P, _P, _U64, _P],
+        _I32,
+    ),
+    "afd_router_grad": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _I32, _P, _P, _P, _P, _P], _I32),
     "afd_host_alloc": ([ctypes.POINTER(ctypes.c_void_p), _U64], _I32),
     "afd_host_free": ([_P], _I32),
     "afd_copy_async": ([_P, _P, _U64, _P], _I32),

@@ -1,0 +1,360 @@
+"""GPU parity of the router: the choice of experts (exact, ties and borders included), its weights,
+counts, the balance loss, and the gradients, against 64-bit definitions and against differences.
+
+Tolerances. A score's relative error in fp32: the exponent's argument |x| <= 32 is rounded to
+|x| 2^-24, the exponential and the logarithm add 2 ulps each, a sum of up to 1024 terms as a tree of
+depth 10 ten half ulps, the quotient one: below 64 * 2^-24 = 2^-18. The weights carry that. A gradient is a
+difference of such terms, no larger than twice the largest incoming gradient times the scale:
+2^-16 of that bound, absolute, plus half a step of bf16 (eps / 2 = 2^-8, relative) where the logits
+are bf16. The loss sums shares with error 2^-18 in fp32 blocks: 2^-16."""
+
+import math
+
+import pytest
+import torch
+
+import router_ref as R
+from gpu_util import dev, say
+from sgl_asap_amd.moe import balance as B
+from sgl_asap_amd.moe import topk as T
+
+pytestmark = pytest.mark.gpu
+
+REL = 2.0**-18
+
+
+def make(n, experts, seed, dtype=torch.float32, bias=False):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(n, experts, generator=g) * 2).to(dtype)
+    b = torch.randn(experts, generator=g) * 0.05 if bias else None
+    return logits, b
+
+
+def check_choice(logits, top_k, out, scoring, bias=None, renorm=True, scale=1.0, groups=0, keep=0, valid=None):
+    z = R.canon(logits)
+    ids = R.choose(z, top_k, scoring, bias, groups, keep)
+    w = R.weights(z, ids, scoring, renorm, scale)
+    if valid is not None:
+        ids = ids.masked_fill(~valid[:, None], -1)
+        w = w.masked_fill(~valid[:, None], 0.0)
+    assert out.topk_ids.dtype == torch.int32 and out.topk_weights.dtype == torch.float32
+    assert torch.equal(out.topk_ids.cpu().long(), ids)
+    got = out.topk_weights.cpu().double()
+    assert torch.isfinite(got).all()
+    assert ((got - w).abs() <= REL * w.abs() + 1e-37).all(), ((got - w).abs() / w.abs().clamp_min(1e-37)).max()
+    return ids
+
+
+def select(logits, top_k, bias=None, valid=None, groups=0, keep=0, scale=1.0, **more):
+    return T.select_experts(logits.to(dev()), top_k, correction_bias=None if bias is None else bias.to(dev()),
+                            valid=None if valid is None else valid.to(dev()), num_expert_group=groups or None,
+                            topk_group=keep or None, routed_scaling_factor=scale, **more)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n,experts,top_k,groups,keep", [
+    (1, 1, 1, 0, 0), (5, 8, 2, 0, 0), (33, 60, 4, 0, 0), (17, 64, 16, 0, 0), (9, 64, 20, 0, 0), (130, 128, 6, 8, 3),
+    (67, 129, 8, 3, 1), (257, 256, 8, 8, 4), (12, 256, 32, 1, 1), (19, 384, 8, 64, 5), (31, 512, 8, 0, 0),
+    (7, 1000, 32, 40, 39), (3, 1024, 32, 16, 2), (6, 32, 32, 0, 0), (4, 48, 3, 48, 3), (5, 63, 9, 9, 2),
+])
+def test_choice(n, experts, top_k, groups, keep, bias, scoring):
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, b = make(n, experts, n + experts, dtype, bias)
+        for renorm, scale in ((True, 2.5), (False, 1.0)):
+            say(f"choice n={n} E={experts} k={top_k} groups={groups}/{keep} {scoring} bias={bias} {dtype} renorm={renorm}")
+            out = select(logits, top_k, b, scoring=scoring, renormalize=renorm, groups=groups, keep=keep, scale=scale)
+            check_choice(logits, top_k, out, scoring, b, renorm, scale, groups, keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_choice_ties_go_to_the_lower_index(bias, scoring):
+    """Few distinct values, both zeros among them, and a bias of few steps."""
+    g = torch.Generator().manual_seed(3)
+    logits = torch.randint(-2, 2, (200, 72), generator=g).float() * torch.where(torch.rand(200, 72, generator=g) < 0.5, -1.0, 1.0)
+    b = torch.randint(-1, 2, (72,), generator=g).float() * 0.25 if bias else None
+    for groups, keep in ((0, 0), (8, 3)):
+        say(f"ties {scoring} bias={bias} groups={groups}")
+        check_choice(logits, 8, select(logits, 8, b, scoring=scoring, groups=groups, keep=keep), scoring, b, groups=groups, keep=keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+def test_choice_between_close_scores(scoring):
+    """Biases that make pairs of choice values differ by 1e-12: beyond 32 bits, within 64."""
+    g = torch.Generator().manual_seed(5)
+    n, experts = 64, 128
+    logits = torch.randn(n, experts, generator=g)
+    logits[:, 64:] = logits[:, :64]
+    bias = torch.zeros(experts)
+    # fp32 steps near 2^-40 on top of 0: the sums' 52 bits hold them, 24 bits do not
+    bias[:64] = torch.where(torch.rand(64, generator=g) < 0.5, 0.0, 2.0**-40)
+    bias[64:] = torch.where(torch.rand(64, generator=g) < 0.5, 0.0, 2.0**-40)
+    say(f"close scores {scoring}")
+    check_choice(logits, 16, select(logits, 16, bias, scoring=scoring), scoring, bias)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_choice_of_infinite_and_masked_logits(dtype, bias, scoring):
+    logits, b = make(12, 40, 11, dtype, bias)
+    low, inf = torch.finfo(dtype).min, math.inf
+    logits[0] = -inf
+    logits[1] = low
+    logits[2, 3:] = -inf
+    logits[3, 5:] = low
+    logits[4, 7] = math.nan
+    logits[5] = math.nan
+    logits[6, 9] = inf
+    logits[7, [4, 30]] = inf
+    logits[8] = inf
+    logits[9, ::2] = low
+    logits[10] = 0.0
+    if bias:
+        b[6], b[7], b[8] = math.nan, inf, -inf
+    for renorm in (True, False):
+        for groups, keep in ((0, 0), (10, 2)):
+            say(f"masked {dtype} {scoring} bias={bias} renorm={renorm} groups={groups}")
+            out = select(logits, 6, b, scoring=scoring, renormalize=renorm, groups=groups, keep=keep)
+            check_choice(logits, 6, out, scoring, b, renorm, groups=groups, keep=keep)
+
+
+def test_choice_of_padded_rows_and_strided_logits():
+    logits, b = make(50, 96, 21, torch.float32, True)
+    valid = torch.rand(50, generator=torch.Generator().manual_seed(1)) < 0.6
+    wide = torch.full((50, 131), 99.0)
+    wide[:, 17:113] = logits
+    on = wide.to(dev())
+    say("padded rows, rows with a stride, rows off alignment")
+    out = T.select_experts(on[:, 17:113], 6, correction_bias=b.to(dev()), valid=valid.to(dev()), scoring="sigmoid")
+    check_choice(logits, 6, out, "sigmoid", b, valid=valid)
+    say("columns with a stride, one row repeated")
+    check_choice(logits, 6, T.select_experts(on.t().contiguous().t()[:, 17:113], 6), "softmax")
+    row = logits[:1].expand(9, 96)
+    check_choice(row, 6, T.select_experts(row[:1].to(dev()).expand(9, 96), 6), "softmax")
+    say("no rows")
+    none = T.select_experts(on[:0, :96], 6)
+    assert none.topk_ids.shape == (0, 6) and none.topk_weights.shape == (0, 6)
+
+
+CU = {"all": None, "one": [0, 41], "parts": [0, 7, 7, 30, 41], "inner": [3, 9, 10, 38], "none": [5, 5, 5]}
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("spans", sorted(CU))
+@pytest.mark.parametrize("experts,top_k", [(8, 2), (60, 4), (100, 17), (256, 8), (500, 8), (1024, 32)])
+def test_balance_loss_counts_and_gradient(experts, top_k, spans, scoring):
+    n, cu, alpha = 41, CU[spans], 0.01
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, _ = make(n, experts, experts + top_k, dtype)
+        g = torch.Generator().manual_seed(experts)
+        ids = torch.randint(-1, experts + 1, (n, top_k), generator=g, dtype=torch.int32)  # repeated and foreign ones
+        valid = torch.rand(n, generator=g) < 0.8 if spans != "one" else None
+        say(f"balance E={experts} k={top_k} {spans} {scoring} {dtype}")
+        leaf = logits.to(dev()).requires_grad_()
+        loss, cnt = B.balance_loss(leaf, ids.to(dev()), alpha=alpha, scoring=scoring,
+                                   cu_seqlens=None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev()),
+                                   valid=None if valid is None else valid.to(dev()))
+        (3.0 * loss).backward()
+        z = R.canon(logits)
+        want_cnt = R.counts(ids, experts, cu, valid)
+        assert torch.equal(cnt.cpu().long().view(-1, experts), want_cnt)
+        only = B.expert_counts(ids.to(dev()), experts, None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev()),
+                               None if valid is None else valid.to(dev()))
+        assert torch.equal(only, cnt)
+        want = float(R.balance(z, ids, scoring, alpha, cu, valid))
+        assert abs(float(loss.detach()) - want) <= 2.0**-16 * abs(want)
+        grad = R.grads(logits, ids, scoring, gl=3.0, alpha=alpha, cu=cu, valid=valid)
+        # the largest c_e: 3 alpha E cnt / (S' k T^2)
+        most = 0.0
+        used = sum(hi > lo for lo, hi in R.sequences(n, cu))
+        for i, (lo, hi) in enumerate(R.sequences(n, cu)):
+            rows = hi - lo if valid is None else int(valid[lo:hi].sum())
+            if rows:
+                most = max(most, 3 * alpha * experts * float(want_cnt[i].max()) / (used * top_k * rows * rows) * 2)
+        tol = 2.0**-16 * most + (2.0**-8 * grad.abs() if dtype == torch.bfloat16 else 0.0)
+        assert leaf.grad.dtype == dtype
+        assert ((leaf.grad.cpu().double() - grad).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("experts,top_k,bias", [(6, 1, False), (60, 4, True), (128, 17, False), (256, 8, True), (900, 32, True)])
+def test_gradients_of_weights_and_loss_together(experts, top_k, bias, renorm, scoring):
+    n, scale, alpha, cu = 37, 1.5, 0.02, [2, 12, 12, 35]
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, b = make(n, experts, experts + 7, dtype, bias)
+        g = torch.Generator().manual_seed(experts + 1)
+        gw = torch.randn(n, top_k, generator=g)
+        valid = torch.rand(n, generator=g) < 0.8
+        args = dict(scoring=scoring, renormalize=renorm, correction_bias=None if b is None else b.to(dev()),
+                    routed_scaling_factor=scale, valid=valid.to(dev()))
+        say(f"gradients E={experts} k={top_k} bias={bias} renorm={renorm} {scoring} {dtype}")
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, cnt = B.select_and_balance(leaf, top_k, alpha=alpha, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev()), **args)
+        ids = check_choice(logits, top_k, out, scoring, b, renorm, scale, valid=valid)
+        assert torch.equal(cnt.cpu().long(), R.counts(ids, experts, cu, valid))
+        want = float(R.balance(R.canon(logits), ids, scoring, alpha, cu, valid))
+        assert abs(float(loss.detach()) - want) <= 2.0**-16 * abs(want)
+        picked = ids.clamp_min(0)
+        bound = 2.0**-16 * scale * float(gw.abs().max())
+        for parts in ("both", "weights", "loss"):
+            lo, hi = parts != "loss", parts != "weights"
+            outs, gs = [], []
+            if lo:
+                outs.append(out.topk_weights), gs.append(gw.to(dev()))
+            if hi:
+                outs.append(loss), gs.append(torch.tensor(2.0, device=dev()))
+            (got,) = torch.autograd.grad(outs, (leaf,), gs, retain_graph=True)
+            ref = R.grads(logits, picked, scoring, renorm, scale, gw if lo else None, 2.0 if hi else None, alpha, cu, valid)
+            tol = (bound if lo else 0.0) + (2.0**-16 * 2 * alpha * experts if hi else 0.0)
+            tol = tol + (2.0**-8 * ref.abs() if dtype == torch.bfloat16 else 0.0)
+            assert ((got.cpu().double() - ref).abs() <= tol).all(), parts
+            assert (got[~valid.to(dev())] == 0).all()
+        # the selection alone has the same gradient
+        alone = T.select_experts(leaf, top_k, **args)
+        assert torch.equal(alone.topk_ids, out.topk_ids) and torch.equal(alone.topk_weights, out.topk_weights)
+        (g1,) = torch.autograd.grad(alone.topk_weights, leaf, gw.to(dev()))
+        (g2,) = torch.autograd.grad(out.topk_weights, leaf, gw.to(dev()))
+        assert torch.equal(g1, g2)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("renorm", [True, False])
+def test_gradient_against_differences(renorm, scoring):
+    """The kernel's gradient against central differences of the 64-bit loss (step h = 1e-4: truncation
+    below h^2 = 1e-8 of the derivatives' size, far below the gradient's own tolerance)."""
+    n, experts, top_k, alpha = 5, 12, 3, 0.5
+    logits, _ = make(n, experts, 40, torch.float32)
+    g = torch.Generator().manual_seed(2)
+    gw = torch.randn(n, top_k, generator=g)
+    say(f"differences {scoring} renorm={renorm}")
+    leaf = logits.to(dev()).requires_grad_()
+    out, loss, _ = B.select_and_balance(leaf, top_k, alpha=alpha, scoring=scoring, renormalize=renorm)
+    (got,) = torch.autograd.grad((out.topk_weights, loss), (leaf,), (gw.to(dev()), torch.ones((), device=dev())))
+    z, ids, h = logits.double(), out.topk_ids.cpu().long(), 1e-4
+
+    def value(at):
+        w = R.weights(at, ids, scoring, renorm, 1.0)
+        return float((w * gw.double()).sum() + R.balance(at, ids, scoring, alpha))
+
+    for t in range(n):
+        for e in range(experts):
+            up, down = z.clone(), z.clone()
+            up[t, e] += h
+            down[t, e] -= h
+            d = (value(up) - value(down)) / (2 * h)
+            assert abs(float(got[t, e]) - d) <= 2.0**-16 * float(gw.abs().max()) + 1e-6, (t, e)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+def test_gradients_of_masked_logits_are_finite(scoring):
+    logits, _ = make(8, 40, 9)
+    low = torch.finfo(torch.float32).min
+    logits[0] = -math.inf
+    logits[1] = low
+    logits[2, 6:] = -math.inf
+    logits[3, 6:] = low
+    logits[4, 5] = math.nan
+    logits[5, 5] = math.inf
+    logits[6] = -200.0
+    for renorm in (True, False):
+        say(f"masked gradients {scoring} renorm={renorm}")
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, _ = B.select_and_balance(leaf, 4, alpha=0.1, scoring=scoring, renormalize=renorm)
+        (g,) = torch.autograd.grad((out.topk_weights, loss), (leaf,), (torch.ones(8, 4, device=dev()), torch.ones((), device=dev())))
+        assert torch.isfinite(g).all() and math.isfinite(float(loss.detach()))
+        assert (g[0] == 0).all() and (g[2, 6:] == 0).all() and float(g[4, 5]) == 0.0
+
+
+def test_many_rows_sequences_and_repeated_calls():
+    """Workgroups that hold several sequences and sequences over many workgroups; the same bits each time."""
+    n, experts, top_k = 5000, 256, 8
+    logits, _ = make(n, experts, 77, torch.bfloat16)
+    g = torch.Generator().manual_seed(4)
+    cu = torch.cat([torch.randint(0, n + 1, (59,), generator=g), torch.tensor([0, 3, 3, 3, n])]).sort().values.tolist()
+    cu_dev = torch.tensor(cu, dtype=torch.int32, device=dev())
+    say("5000 rows in 63 sequences")
+    first = None
+    for _ in range(3):
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, cnt = B.select_and_balance(leaf, top_k, alpha=1.0, scoring="sigmoid", cu_seqlens=cu_dev)
+        (g1,) = torch.autograd.grad(loss, leaf)
+        now = (out.topk_ids, out.topk_weights, loss.detach(), cnt, g1)
+        if first is None:
+            first = now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+    ids = first[0].cpu().long()
+    assert torch.equal(ids, R.choose(R.canon(logits), top_k, "sigmoid"))
+    assert torch.equal(first[3].cpu().long(), R.counts(ids, experts, cu))
+    want = float(R.balance(R.canon(logits), ids, "sigmoid", 1.0, cu))
+    assert abs(float(first[2]) - want) <= 2.0**-16 * want
+    ref = R.grads(logits, ids, "sigmoid", gl=1.0, alpha=1.0, cu=cu)
+    assert ((g1.cpu().double() - ref).abs() <= 2.0**-8 * ref.abs() + 2.0**-16 * experts).all()
+
+
+def test_captured_and_replayed_with_other_inputs():
+    """Forward and backward in one graph, two graphs in turn, other inputs copied in, eager calls between."""
+    n, experts, top_k = 300, 128, 6
+    make_one = lambda seed: make(n, experts, seed)[0].to(dev())
+    cu = torch.tensor([0, 100, 300], dtype=torch.int32, device=dev())
+    gw = torch.randn(n, top_k, device=dev())
+    one = torch.ones((), device=dev())
+
+    def step(leaf):
+        out, loss, cnt = B.select_and_balance(leaf, top_k, alpha=0.1, cu_seqlens=cu)
+        (g,) = torch.autograd.grad((out.topk_weights, loss), (leaf,), (gw, one))
+        return out.topk_ids, out.topk_weights, loss, cnt, B.expert_counts(out.topk_ids, experts), g
+
+    say("capture")
+    graphs = []
+    for seed in (1, 2):
+        leaf = make_one(seed).requires_grad_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(leaf)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(leaf)
+        graphs.append((graph, leaf, outs))
+    for round_ in range(3):
+        for i, (graph, leaf, outs) in enumerate(graphs):
+            with torch.no_grad():
+                leaf.copy_(make_one(10 * round_ + i))
+            graph.replay()
+            want = step(leaf.detach().clone().requires_grad_())
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), (round_, i)
+
+
+def test_on_another_stream():
+    logits, b = make(700, 256, 31, bias=True)
+    on, bias = logits.to(dev()), b.to(dev())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    say("another stream")
+    with torch.cuda.stream(side):
+        out = T.select_experts(on, 8, scoring="sigmoid", correction_bias=bias)
+        cnt = B.expert_counts(out.topk_ids, 256)
+    side.synchronize()
+    ids = check_choice(logits, 8, out, "sigmoid", b)
+    assert torch.equal(cnt.cpu().long(), R.counts(ids, 256)[0])
+
+
+def test_more_logits_than_32_bits_count():
+    """2^31 + logits: offsets and the slots' sums past one workgroup's limit; sampled rows against the definition."""
+    n, experts, top_k = 9_000_000, 256, 2
+    say("2.3e9 logits")
+    g = torch.Generator(device=dev()).manual_seed(0)
+    logits = torch.randn(n, experts, generator=g, device=dev(), dtype=torch.bfloat16)
+    out, loss, cnt = B.select_and_balance(logits, top_k, alpha=1.0)
+    rows = torch.cat([torch.arange(0, 50), torch.arange(8_388_600, 8_388_650), torch.arange(n - 50, n)]).to(dev())
+    part = T.StandardTopKOutput(out.topk_weights[rows], out.topk_ids[rows])
+    check_choice(logits[rows].cpu(), top_k, part, "softmax")
+    assert torch.equal(cnt.long(), torch.bincount(out.topk_ids.reshape(-1).long(), minlength=experts))
+    share = sum(torch.softmax(p.double(), 1).sum(0) for p in logits.split(1_000_000))
+    want = experts / (top_k * n * n) * float((share * cnt.double()).sum())
+    assert abs(float(loss) - want) <= 2.0**-12 * want  # blocks of 1024 rows: 256 fp32 sums in a row each

@@ -38,6 +38,9 @@
  *                                (its StandardTopKOutput is what P/srt/managers/scheduler.py
  *                                :410-412 and P/srt/layers/moe/token_dispatcher/asap.py:48-73
  *                                take)
+ *   afd_linear / ............... the block-FP8 linear layers of the shared expert, SGLang's in the
+ *   afd_linear_pack              reference (the MLP called at P/srt/batch_overlap/
+ *                                operations_strategy.py:94, 255)
  *   afd_expert_counts / ........ no counterpart: where the tokens go, the balance loss of a
  *   afd_balance / ..............  router in training, and the gradient of both by its logits
  *   afd_topk_balance /
@@ -400,6 +403,28 @@ int afd_combine(const uint16_t* const* parts, int32_t num_parts, const uint16_t*
  * 16-byte aligned, n * inter / 8 < 2^31. */
 int afd_silu_mul(const uint16_t* gate_up, int64_t n, int32_t inter, uint16_t* out,
                  afd_stream_t stream);
+
+/* ---- dense FP8 block product -----------------------------------------------------------------
+ * y[t, o] = bf16(sum over K blocks of sx[t, kb] * scales[o / 128][kb] * sum of the block's qx * qw), with x bf16
+ * quantized as afd_quant_fp8_1x128 does (sx = max(amax, 1e-10) / 448, qx = e4m3(x / sx), the last
+ * block may be shorter); a row of x that holds an infinity or a NaN gives a row of NaN. Any n_out
+ * and k_in up to 65536, n <= 2^22. afd_linear_pack lays checkpoint codes e4m3 [n_out][ld] out once
+ * (image: afd_linear_layout's bytes, 16-byte aligned); scales f32 [ceil(n_out / 128)][ceil(k_in / 128)] are used
+ * as they are. x: rows of ldx >= k_in elements, y: rows of ldy >= n_out; the elements between
+ * rows stay as they are. The workspace (16-byte aligned) holds the quantized rows of one call. */
+typedef struct afd_linear_weights {
+  int32_t n_out;
+  int32_t k_in;
+  const void* image;
+  const float* scales;
+} afd_linear_weights;
+
+int afd_linear_layout(int32_t n_out, int32_t k_in, uint64_t* image_bytes);
+int afd_linear_pack(const uint8_t* codes, int64_t ld, int32_t n_out, int32_t k_in, uint8_t* image,
+                    afd_stream_t stream);
+int afd_linear_workspace(int32_t n, int32_t k_in, uint64_t* bytes);
+int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n,
+               void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream);
 
 /* ---- the router ---------------------------------------------------------------------------
  * Scores of a row of logits l: softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts

@@ -1,0 +1,431 @@
+// A dense product with FP8-e4m3 weights that carry one fp32 scale per 128x128 block, on activations
+// quantized to e4m3 with one fp32 scale per 1x128 (the block-FP8 format of the experts), on gfx950 MFMA:
+//
+//   y[t, o] = bf16( sum_kb  sx[t, kb] sw[o / 128, kb]  sum_{k in block kb} qx[t, k] qw[o, k] )
+//   sx = max(amax_kb |x|, 1e-10) / 448,  qx = e4m3(x / sx)  (both quotients in fp32)
+//
+// Any n_out and k_in: both operands live in fragment images padded to 16 rows and 128 columns,
+// [rows / 16][K / 64] pieces of 1 KiB, a piece's 16-byte chunk c (of 4) of row r at byte 256 c + 16 r. A
+// piece is one contiguous wide load, whether a wavefront takes it straight into registers (lane l
+// then holds chunk l / 16 of row l % 16: an operand of the 16-row MFMA) or copies it to LDS, where 16 consecutive
+// rows of a chunk are 256 bytes, all banks once. Which K a lane's bytes stand for does not matter as
+// long as both operands agree. Padding codes are 0; padding rows are never stored.
+//
+// Every block's MFMA sum starts from 0 and is folded into the result with its scale by one fp32
+// fused multiply-add, so scales may be 0, tiny or huge. A row of x with an infinity or a NaN in a block gets
+// the scale NaN, which makes that row of y NaN and no other.
+#include "afd_common.h"
+#include "afd_gemm_dev.h"
+#include "afd_internal.h"
+
+namespace afd {
+namespace linear {
+
+constexpr int kPiece = 1024;  // 16 rows x 64 columns of e4m3
+constexpr int kMaxDim = 65536;
+constexpr int kMaxRows = 1 << 22;
+// the activation scales are [K / 128][rows rounded up to kScaleRows]
+constexpr int kScaleRows = 256;
+
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Args {
+  const uint8_t* a;  // activation image [rows16][kt]
+  const float* as;   // [kb][a_rows]
+  const uint8_t* b;  // weight image [n_out / 16][kt]
+  const float* bs;   // [n_out / 128][kb]
+  uint16_t* y;
+  int64_t ldy;
+  int32_t n, n_out, kb;  // kb: K blocks of 128
+  int32_t a_rows;
+  bool wide;  // rows of y take 16-byte stores
+};
+
+__device__ __forceinline__ v8i join(v4i lo, v4i hi) {
+  return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// ---------------------------------------------------------------- activations
+// A wavefront quantizes 16 rows x one K block: lane l chunks l / 16 of both 64-column pieces of row
+// l % 16. vec: 16-byte loads of whole chunks.
+__global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
+                                                    uint8_t* __restrict__ q, float* __restrict__ s, int kb,
+                                                    int a_rows, bool vec) {
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= ((int64_t(n) + 15) / 16) * kb) return;
+  const int64_t r16 = item / kb;
+  const int b = static_cast<int>(item % kb);
+  const int lane = threadIdx.x & 63, c = lane >> 4;
+  const int64_t row = r16 * 16 + (lane & 15);
+  float v[2][16];
+  uint32_t top = 0;  // bits of the largest magnitude: infinities and NaN above every number
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k0 = b * 128 + h * 64 + c * 16;
+    const uint16_t* p = x + row * ldx + k0;
+    if (vec && row < n && k0 + 16 <= k_in) {
+      const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = static_cast<uint32_t>(i < 4 ? lo[i & 3] : hi[i & 3]);
+        v[h][2 * i] = __uint_as_float(w << 16);
+        v[h][2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[h][i] = row < n && k0 + i < k_in ? bf16_to_f32(p[i]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[h][i]) & 0x7fffffffu);
+  }
+  const auto r0 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = max(r0[0], r0[1]);
+  const auto r1 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+  top = max(r1[0], r1[1]);
+  const bool finite = top < 0x7f800000u;
+  const float sc = fmaxf(__uint_as_float(top), kFp8Eps) / kE4m3Max;
+  const float rsc = 1.0f / sc;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v4i out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      out[i] = finite ? static_cast<int>(pk4_e4m3(div_by(v[h][4 * i], sc, rsc), div_by(v[h][4 * i + 1], sc, rsc),
+                                                  div_by(v[h][4 * i + 2], sc, rsc), div_by(v[h][4 * i + 3], sc, rsc)))
+                      : 0;
+    *reinterpret_cast<v4i*>(q + (r16 * (2 * kb) + 2 * b + h) * kPiece + lane * 16) = out;
+  }
+  if (c == 0 && row < n) s[int64_t(b) * a_rows + row] = finite ? sc : __builtin_nanf("");
+}
+
+// ---------------------------------------------------------------- weights (load time)
+__global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ w, int64_t ld, int n_out, int k_in,
+                                                   int kb, uint8_t* __restrict__ out, int64_t pieces) {
+  for (int64_t at = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); at < pieces; at += int64_t(gridDim.x) * 4) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = at / (2 * kb) * 16 + (lane & 15);
+    const int k0 = static_cast<int>(at % (2 * kb)) * 64 + (lane >> 4) * 16;
+    uint32_t d[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t byte = row < n_out && k0 + i < k_in ? w[row * ld + k0 + i] : 0u;
+      d[i / 4] |= byte << (8 * (i % 4));
+    }
+    *reinterpret_cast<v4i*>(out + at * kPiece + lane * 16) =
+        v4i{static_cast<int>(d[0]), static_cast<int>(d[1]), static_cast<int>(d[2]), static_cast<int>(d[3])};
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// Up to 16 MT rows of x: a call is bound by reading the weights once. A workgroup owns 16 outputs over the
+// whole K, its wavefronts a share of the K blocks each, weights and activations straight into
+// registers; the wavefronts' sums meet in LDS, in their order.
+constexpr int kRowWaves = 8;
+
+template <int MT>
+__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p) {
+  __shared__ v4f part[kRowWaves][MT][64];
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int o16 = blockIdx.x;
+  const int kt = 2 * p.kb;
+  const int r16s = (p.n + 15) / 16;
+  v4f acc[MT] = {};
+  const uint8_t* bw = p.b + int64_t(o16) * kt * kPiece + lane * 16;
+  const float* sw = p.bs + int64_t(o16 / 8) * p.kb;
+  for (int b = w; b < p.kb; b += kRowWaves) {
+    const v4i lo = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * b) * kPiece));
+    const v4i hi = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * b + 1) * kPiece));
+    const v8i fw = join(lo, hi);
+    const float s_w = load_uniform(sw + b);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r16 = min(m, r16s - 1);
+      const uint8_t* ax = p.a + (int64_t(r16) * kt + 2 * b) * kPiece + lane * 16;
+      const v8i fx = join(*reinterpret_cast<const v4i*>(ax), *reinterpret_cast<const v4i*>(ax + kPiece));
+      const float s = p.as[int64_t(b) * p.a_rows + r16 * 16 + (lane & 15)] * s_w;
+      const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0,
+                                                                     127, 0, 127);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[m][q] = __builtin_fmaf(sum[q], s, acc[m][q]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) part[w][m][lane] = acc[m];
+  __syncthreads();
+  // lane l: row l % 16 of x, outputs 4 (l / 16) .. + 3
+  if (w >= MT) return;
+  for (int m = w; m < MT; m += kRowWaves) {
+    v4f y = part[0][m][lane];
+    for (int i = 1; i < kRowWaves; ++i) y += part[i][m][lane];
+    const int row = m * 16 + (lane & 15), o = o16 * 16 + 4 * (lane >> 4);
+    if (row >= p.n) continue;
+    uint16_t* out = p.y + row * p.ldy + o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (o + q < p.n_out) out[q] = f32_to_bf16(y[q]);
+  }
+}
+
+// ---------------------------------------------------------------- tiles
+// BM rows of x by BN outputs, WM x WN wavefronts of TI x TJ MFMA tiles of 32x32 each. A stage is one K
+// block of both operands and the rows' scales, copied HBM -> LDS in pieces, S stages in a ring, one
+// barrier a stage: at stage b a wavefront has waited for its own copies of it, the barrier says that
+// all have and that nobody reads stage b - 1 any more, whose slot then takes stage b + S - 1.
+template <int BM_, int BN_, int WM_, int WN_, int S_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
+  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int TI = BM / WM / 32, TJ = BN / WN / 32;
+  static constexpr int kAPieces = BM / 16 * 2, kBPieces = BN / 16 * 2;
+  static constexpr int kAQ = kAPieces / kWaves, kBQ = kBPieces / kWaves;
+  static constexpr int kBOff = kAPieces * kPiece, kSOff = kBOff + kBPieces * kPiece;
+  static constexpr int kStage = kSOff + BM * 4;
+  static constexpr int kYBytes = BM * BN * 2;
+  static constexpr int kLds = S * kStage > kYBytes ? S * kStage : kYBytes;
+  static constexpr int kScaleWaves = BM / 64;  // each copies 64 rows' scales
+  static_assert(TI * 32 * WM == BM && TJ * 32 * WN == BN && kAQ * kWaves == kAPieces && kBQ * kWaves == kBPieces, "tile");
+  static_assert(BN / WN <= 128 && 128 % (BN / WN) == 0, "one weight scale per wavefront and K block");
+  static_assert(kScaleWaves <= kWaves && BM <= kScaleRows && kLds <= 160 * 1024, "LDS");
+  static_assert((S - 1) * (kAQ + kBQ + 1) < 64, "vmcnt is a 6-bit counter");
+};
+
+template <typename T>
+__global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
+  constexpr int TI = T::TI, TJ = T::TJ, S = T::S;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wm = w / T::WN, wn = w % T::WN, lr = lane & 31, lk = lane >> 5;
+  const int mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
+  // workgroup b runs on XCD b % 8: an XCD takes whole rows of tiles where there are many (each reads
+  // all the weights, x is read once), else whole columns (the weights are read by one XCD's L2)
+  int mt, nt;
+  {
+    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    if (mts >= 16) {
+      mt = j / nts * 8 + xcd;
+      nt = j % nts;
+    } else {
+      nt = j / mts * 8 + xcd;
+      mt = j % mts;
+    }
+    if (mt >= mts || nt >= nts) return;
+  }
+  const int kt = 2 * p.kb;
+  const int m0 = mt * T::BM, n0 = nt * T::BN;
+  const int r16_last = (p.n + 15) / 16 - 1, o16_last = (p.n_out + 15) / 16 - 1;
+  const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_offset(lds));
+  const uint32_t voff = static_cast<uint32_t>(lane) * 16;
+
+  // this wavefront's pieces of a stage: piece q of an operand is row group q / 2, 64-column half q % 2.
+  // Row groups past the end re-read the last one; their results are not stored.
+  auto issue = [&](int b) {
+    const uint32_t st = lds_base + static_cast<uint32_t>((b % S) * T::kStage);
+    if (w < T::kScaleWaves)
+      lds_dma4(st + T::kSOff + w * 256, p.as + int64_t(b) * p.a_rows + m0 + 64 * w, lane * 4u);
+    static_for<T::kAQ>([&](auto qc) {
+      const int q = w * T::kAQ + decltype(qc)::value;
+      const int r16 = min(m0 / 16 + q / 2, r16_last);
+      lds_dma16(st + q * kPiece, p.a + (int64_t(r16) * kt + 2 * b + q % 2) * kPiece, voff);
+    });
+    static_for<T::kBQ>([&](auto qc) {
+      const int q = w * T::kBQ + decltype(qc)::value;
+      const int o16 = min(n0 / 16 + q / 2, o16_last);
+      lds_dma16(st + T::kBOff + q * kPiece, p.b + (int64_t(o16) * kt + 2 * b + q % 2) * kPiece, voff);
+    });
+  };
+
+  v16f acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+
+  const int sw_row = min((n0 + wn * (T::BN / T::WN)) / 128, (p.n_out - 1) / 128);
+  const float* sw = p.bs + int64_t(sw_row) * p.kb;
+  const int last = p.kb - 1;
+  // a fragment: rows r, 16-byte chunks lk and lk + 2 of a 64-column half
+  const int frag = (lr >> 4) * 2 * kPiece + (lr & 15) * 16 + lk * 256;
+  static_for<S - 1>([&](auto sc) { issue(min(static_cast<int>(decltype(sc)::value), last)); });
+  for (int b = 0; b <= last; ++b) {
+    wait_vmcnt<(S - 2) * (T::kAQ + T::kBQ)>();
+    __syncthreads();
+    issue(min(b + S - 1, last));
+    const uint8_t* st = lds + (b % S) * T::kStage;
+    const float s_w = load_uniform(sw + b);
+    float s[TI];
+    v8i fa[TI][2];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      s[i] = reinterpret_cast<const float*>(st + T::kSOff)[wm * TI * 32 + i * 32 + lr] * s_w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* f = st + (wm * TI * 2 + i * 2) * 2 * kPiece + h * kPiece + frag;
+        fa[i][h] = join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + 512));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      v8i fb[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* f = st + T::kBOff + (wn * TJ * 2 + j * 2) * 2 * kPiece + h * kPiece + frag;
+        fb[h] = join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + 512));
+      }
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        v16f sum = {};
+        sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[0], fa[i][0], sum, 0, 0, 0, 127, 0, 127);
+        sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[1], fa[i][1], sum, 0, 0, 0, 127, 0, 127);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(sum[q], s[i], acc[i][j][q]);
+      }
+    }
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+
+  // bf16 rows through LDS (16-byte chunk c of row r at c ^ (r % 16)), so the stores write whole rows
+  constexpr int kChunks = T::BN / 8;
+  auto y_at = [](int r, int c) { return (r * kChunks + (c ^ (r & 15))) * 16; };
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      v4i chunk[2];
+      bf16_chunks(acc[i][j], chunk);
+      const int row = wm * TI * 32 + i * 32 + lr;
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr)
+        *reinterpret_cast<v4i*>(lds + y_at(row, (wn * TJ * 32 + j * 32) / 8 + 2 * pr + lk)) = chunk[pr];
+    }
+  __syncthreads();
+  for (int at = t; at < T::BM * kChunks; at += T::kThreads) {
+    const int r = at / kChunks, c = at % kChunks;
+    const int row = m0 + r, o = n0 + c * 8;
+    if (row >= p.n || o >= p.n_out) continue;
+    const v4i chunk = *reinterpret_cast<const v4i*>(lds + y_at(r, c));
+    uint16_t* out = p.y + row * p.ldy + o;
+    if (p.wide && o + 8 <= p.n_out) {
+      *reinterpret_cast<v4i*>(out) = chunk;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (o + i < p.n_out)
+          out[i] = static_cast<uint16_t>(static_cast<uint32_t>(chunk[i / 2]) >> (16 * (i % 2)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+using Large = Shape<256, 256, 4, 2, 2>;
+using Mid = Shape<128, 128, 2, 2, 2>;
+
+struct Plan {
+  int kb, a_rows;
+  int64_t q_bytes, total;
+};
+static Plan plan(int32_t n, int32_t k_in) {
+  Plan p;
+  p.kb = (k_in + 127) / 128;
+  p.a_rows = static_cast<int>(round_up(n, kScaleRows));
+  p.q_bytes = round_up(n, 16) * p.kb * 128;
+  p.total = p.q_bytes + int64_t(p.kb) * p.a_rows * 4;
+  return p;
+}
+static int check_dims(int32_t n_out, int32_t k_in) {
+  return n_out < 1 || n_out > kMaxDim || k_in < 1 || k_in > kMaxDim ? AFD_ERR_SHAPE : AFD_OK;
+}
+
+template <typename T>
+static int launch_tiles(const Args& p, hipStream_t s) {
+  const int64_t mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
+  const int64_t grid = mts >= 16 ? round_up(mts, 8) * nts : round_up(nts, 8) * mts;
+  hipLaunchKernelGGL(tile_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s, p);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
+}
+template <int MT>
+static int launch_rows(const Args& p, hipStream_t s) {
+  hipLaunchKernelGGL(rows_kernel<MT>, dim3((p.n_out + 15) / 16), dim3(64 * kRowWaves), 0, s, p);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
+}
+
+}  // namespace linear
+}  // namespace afd
+
+using namespace afd;
+
+extern "C" int afd_linear_layout(int32_t n_out, int32_t k_in, uint64_t* image_bytes) {
+  if (!image_bytes) return AFD_ERR_ARG;
+  const int st = linear::check_dims(n_out, k_in);
+  if (st != AFD_OK) return st;
+  *image_bytes = static_cast<uint64_t>(linear::round_up(n_out, 16) * linear::round_up(k_in, 128));
+  return AFD_OK;
+}
+
+extern "C" int afd_linear_pack(const uint8_t* codes, int64_t ld, int32_t n_out, int32_t k_in, uint8_t* image,
+                               afd_stream_t stream) {
+  if (!codes || !image) return AFD_ERR_ARG;
+  const int st = linear::check_dims(n_out, k_in);
+  if (st != AFD_OK) return st;
+  if (ld < k_in || reinterpret_cast<uintptr_t>(image) % 16) return AFD_ERR_SHAPE;
+  const int kb = (k_in + 127) / 128;
+  const int64_t pieces = linear::round_up(n_out, 16) / 16 * 2 * kb;
+  const int64_t grid = (pieces + 3) / 4;
+  hipLaunchKernelGGL(linear::pack_kernel, dim3(static_cast<unsigned>(grid < 8192 ? grid : 8192)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), codes, ld, n_out, k_in, kb, image, pieces);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
+}
+
+extern "C" int afd_linear_workspace(int32_t n, int32_t k_in, uint64_t* bytes) {
+  if (!bytes || n < 0 || n > linear::kMaxRows) return AFD_ERR_ARG;
+  const int st = linear::check_dims(1, k_in);
+  if (st != AFD_OK) return st;
+  *bytes = static_cast<uint64_t>(linear::plan(n, k_in).total);
+  return AFD_OK;
+}
+
+extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n, void* ws,
+                          uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream) {
+  if (!weights || n < 0 || n > linear::kMaxRows) return AFD_ERR_ARG;
+  const int st = linear::check_dims(weights->n_out, weights->k_in);
+  if (st != AFD_OK) return st;
+  if (ldx < weights->k_in || ldy < weights->n_out) return AFD_ERR_SHAPE;
+  if (n == 0) return AFD_OK;
+  if (!weights->image || !weights->scales || !x || !ws || !y) return AFD_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(weights->image) % 16) return AFD_ERR_SHAPE;
+  const linear::Plan pl = linear::plan(n, weights->k_in);
+  if (ws_bytes < static_cast<uint64_t>(pl.total) || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* q = static_cast<uint8_t*>(ws);
+  float* sx = reinterpret_cast<float*>(q + pl.q_bytes);
+  const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+  hipLaunchKernelGGL(linear::quant_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, s, x, ldx, n,
+                     weights->k_in, q, sx, pl.kb, pl.a_rows, vec);
+  AFD_CHECK_LAUNCH();
+  linear::Args p = {};
+  p.a = q;
+  p.as = sx;
+  p.b = static_cast<const uint8_t*>(weights->image);
+  p.bs = weights->scales;
+  p.y = y;
+  p.ldy = ldy;
+  p.n = n;
+  p.n_out = weights->n_out;
+  p.kb = pl.kb;
+  p.a_rows = pl.a_rows;
+  p.wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy % 8 == 0;
+  if (n <= 16) return linear::launch_rows<1>(p, s);
+  if (n <= 32) return linear::launch_rows<2>(p, s);
+  if (n <= 64) return linear::launch_rows<4>(p, s);
+  const int64_t large = ((int64_t(n) + 255) / 256) * ((int64_t(p.n_out) + 255) / 256);
+  if (large >= device_cu_count()) return linear::launch_tiles<linear::Large>(p, s);
+  return linear::launch_tiles<linear::Mid>(p, s);
+}

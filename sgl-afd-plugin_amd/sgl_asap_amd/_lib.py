@@ -68,6 +68,10 @@ EXPORTED = (
     "afd_finalize",
     "afd_combine",
     "afd_silu_mul",
+    "afd_linear_layout",
+    "afd_linear_pack",
+    "afd_linear_workspace",
+    "afd_linear",
     "afd_topk",
     "afd_balance_workspace",
     "afd_expert_counts",
@@ -118,6 +122,17 @@ class AfdExpertWeights(ctypes.Structure):
         ("s13", ctypes.c_void_p),
         ("w2", ctypes.c_void_p),
         ("s2", ctypes.c_void_p),
+    ]
+
+
+class AfdLinearWeights(ctypes.Structure):
+    """afd_linear_weights: a dense layer's FP8 block weights (afd_linear)."""
+
+    _fields_ = [
+        ("n_out", ctypes.c_int32),
+        ("k_in", ctypes.c_int32),
+        ("image", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
     ]
 
 
@@ -276,6 +291,10 @@ _SIGS = {
     "afd_finalize": ([_P, _P, _P, _I32, _I32, _I32, _P, _P], _I32),
     "afd_combine": ([ctypes.POINTER(ctypes.c_void_p), _I32, _P, _P, _I64, _P], _I32),
     "afd_silu_mul": ([_P, _I64, _I32, _P, _P], _I32),
+    "afd_linear_layout": ([_I32, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_linear_pack": ([_P, _I64, _I32, _I32, _P, _P], _I32),
+    "afd_linear_workspace": ([_I32, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_linear": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
     "afd_topk": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _P], _I32),
     "afd_balance_workspace": ([_I32, _I32, _I32, ctypes.POINTER(_U64)], _I32),
     "afd_expert_counts": ([_P, _I32, _I32, _I32, _P, _P, _I32, _P, _P, _U64, _P], _I32),

@@ -12,6 +12,10 @@ torch kernels on the strided gate half took 164 us of a loop layer).
     out = W_down . bf16(silu(W_gate . x) * (W_up . x))
 
 The add itself is fused into the combine kernel (``afd_combine``'s ``shared`` argument).
+
+``Fp8SharedExpertMLP`` is the same MLP on the block-FP8 weights that FP8 checkpoints hold
+(``Fp8BlockLinear``): half the weight bytes, which is what a decode step waits for, and the FP8
+matrix rate in prefill.
 """
 
 from __future__ import annotations
@@ -19,6 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from .linear import Fp8BlockLinear
 
 
 class SharedExpertMLP(torch.nn.Module):
@@ -56,6 +61,30 @@ class SharedExpertMLP(torch.nn.Module):
             raise TypeError(f"expected bf16 [n, {self.hidden_size}], got {x.dtype} {tuple(x.shape)}")
         gate_up = torch.mm(x, self.w_gate_up.t())
         return torch.mm(silu_mul(gate_up), self.w_down.t())
+
+
+class Fp8SharedExpertMLP(torch.nn.Module):
+    """The shared expert on block-FP8 weights: e4m3 codes ``w_gate_up`` [2I, H] = [gate; up] rows and
+    ``w_down`` [H, I], each with its fp32 scales per 128x128 block. x and the activation (rounded
+    to bf16, as the bf16 MLP rounds it) are quantized per 1x128 before their products."""
+
+    def __init__(self, w_gate_up: torch.Tensor, s_gate_up: torch.Tensor, w_down: torch.Tensor, s_down: torch.Tensor,
+                 device=None):
+        super().__init__()
+        two_i, hidden = w_gate_up.shape
+        if two_i % 2 or tuple(w_down.shape) != (hidden, two_i // 2):
+            raise ValueError(f"w_gate_up {tuple(w_gate_up.shape)} and w_down {tuple(w_down.shape)} "
+                             "do not form one SwiGLU MLP")
+        if two_i % 16:
+            raise ValueError(f"the intermediate size must be a multiple of 8, got {two_i // 2}")
+        self.hidden_size, self.intermediate_size = hidden, two_i // 2
+        self.gate_up = Fp8BlockLinear(w_gate_up, s_gate_up, device)
+        self.down = Fp8BlockLinear(w_down, s_down, device)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden_size:
+            raise TypeError(f"expected bf16 [n, {self.hidden_size}], got {x.dtype} {tuple(x.shape)}")
+        return self.down(silu_mul(self.gate_up(x)))
 
 
 def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:

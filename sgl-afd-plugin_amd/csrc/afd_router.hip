@@ -7,6 +7,9 @@
 // Selection: the choice value c is the logit itself without a correction bias (every score grows
 // with its logit) and s + bias in 64 bits with one: which of two experts wins a close race then is
 // a matter of the formula and not of a 32-bit exponential's last bit. Equal values go to the lower index.
+// With a bias the choice is first made in fp32 and its margins are compared with twice the fp32
+// error's bound; only rows with a margin inside it (about one in a thousand; rows with equal values)
+// are chosen again in 64 bits.
 //
 // Balance loss of a sequence with T rows: L_s = E / (k T) sum_e cnt_e P_e, P_e = 1/T sum_t s'_te,
 // s' = s / sum_e s; L = alpha times the mean of L_s over the sequences that have rows.
@@ -44,6 +47,8 @@ struct Args {
   const uint8_t* valid;
   int32_t n;
   int32_t experts, topk, scoring, groups, keep, renorm;
+  int32_t group_lanes;  // lanes of a group where it is 1, 2, 4, .. whole lanes of V experts, else 0
+  bool wide;            // rows take 4-element loads and stores
   float scale;
   int32_t* ids;  // selection: written; balance and gradient: read
   float* w;
@@ -55,7 +60,7 @@ struct Args {
   float* slots;  // [blocks + seqs] of slot_words(experts)
   int32_t* counts;
   float* coef;
-  double* part;      // [seqs] unscaled losses
+  double* part;      // [seqs][64-expert chunks] unscaled losses
   int32_t* rows;     // [seqs] rows
   uint32_t* ticket;  // workgroups of the second launch that are done
   float* loss;
@@ -141,6 +146,9 @@ __device__ __forceinline__ uint32_t key32(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and +0 are equal
   return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key ^ (~static_cast<uint32_t>(static_cast<int32_t>(key) >> 31) | 0x80000000u));
+}
 __device__ __forceinline__ uint64_t key64(double v) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
   return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
@@ -153,21 +161,48 @@ __device__ __forceinline__ float logit_f32(const uint16_t* p) { return bf16_to_f
 __device__ __forceinline__ float canon(float v) {
   return v != v ? kLowest : fminf(v, 3.402823466e38f);
 }
-__device__ __forceinline__ float softplus_f32(float v) { return log1pf(expf(-fabsf(v))) + fmaxf(v, 0.0f); }
+// e^x from the hardware's 2^x: the product x log2(e) in two parts, the small one to first order, which
+// keeps the relative error at two ulps for every x (0 below 2^-126)
+__device__ __forceinline__ float exp_f32(float x) {
+  constexpr float kLog2e = 1.44269502f, kLog2eLo = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float t = x * kLog2e;
+  float rest = __builtin_fmaf(x, kLog2e, -t);
+  rest = __builtin_fmaf(x, kLog2eLo, rest);
+  const float y = __builtin_amdgcn_exp2f(t);
+  // no correction where t has left the floats
+  return fabsf(t) < 126.0f ? __builtin_fmaf(y, rest * kLn2, y) : y;
+}
+// log(1 + e) for e in [0, 1]: 2 atanh(z), z = e / (2 + e) <= 1/3, by its series up to z^15 (the
+// first term left out is (1/9)^8 / 17 of the sum, below 2^-29)
+__device__ __forceinline__ float log1p_f32(float e) {
+  const float z = e * __builtin_amdgcn_rcpf(2.0f + e), q = z * z;
+  float p = 1.0f / 15.0f;
+  p = __builtin_fmaf(p, q, 1.0f / 13.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 11.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 9.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 7.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 5.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 3.0f);
+  const float h = z + z;
+  return __builtin_fmaf(h * q, p, h);
+}
+__device__ __forceinline__ float softplus_f32(float v) { return log1p_f32(exp_f32(-fabsf(v))) + fmaxf(v, 0.0f); }
+__device__ __forceinline__ float sigmoid_f32(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v)); }
 // sigmoid or sqrt(softplus)
 __device__ __forceinline__ float score_f32(float v, int scoring) {
-  return scoring == AFD_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : sqrtf(softplus_f32(v));
+  return scoring == AFD_SCORE_SIGMOID ? sigmoid_f32(v) : __builtin_amdgcn_sqrtf(softplus_f32(v));
 }
 __device__ __forceinline__ double score_f64(double v, int scoring) {
   return scoring == AFD_SCORE_SIGMOID ? 1.0 / (1.0 + exp(-v)) : sqrt(log1p(exp(-fabs(v))) + fmax(v, 0.0));
 }
 // d score / dl over the score: 1 - sigmoid, or sigmoid / (2 softplus), which tends to 1/2 where
 // softplus(l) -> e^l leaves the floats
-__device__ __forceinline__ float slope_f32(float v, int scoring) {
+// (taken from the score where it is at hand)
+__device__ __forceinline__ float slope_f32(float v, float score, int scoring) {
   if (scoring == AFD_SCORE_SOFTMAX) return 1.0f;
-  if (scoring == AFD_SCORE_SIGMOID) return 1.0f / (1.0f + expf(v));
+  if (scoring == AFD_SCORE_SIGMOID) return sigmoid_f32(-v);
   if (v < -17.0f) return 0.5f;
-  return 1.0f / ((1.0f + expf(-v)) * 2.0f * softplus_f32(v));
+  return sigmoid_f32(v) * 0.5f * __builtin_amdgcn_rcpf(score * score);
 }
 
 template <typename T, int W, int V>
@@ -178,6 +213,24 @@ struct Row {
   __device__ __forceinline__ void load(const Args& a, int64_t t, int li) {
     e0 = li * V;
     const T* p = static_cast<const T*>(a.logits) + t * a.ld + e0;
+    if (a.wide) {  // E, the stride and the address are multiples of 4 elements
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const bool in = e0 + j < a.experts;
+        if constexpr (sizeof(T) == 4) {
+          const v4f q = in ? *reinterpret_cast<const v4f*>(p + j) : v4f{kLowest, kLowest, kLowest, kLowest};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l[j + i] = canon(q[i]);
+        } else {
+          const uint2 q = in ? *reinterpret_cast<const uint2*>(p + j) : uint2{0xff80ff80u, 0xff80ff80u};
+          l[j] = canon(__uint_as_float(q.x << 16));
+          l[j + 1] = canon(__uint_as_float(q.x & 0xffff0000u));
+          l[j + 2] = canon(__uint_as_float(q.y << 16));
+          l[j + 3] = canon(__uint_as_float(q.y & 0xffff0000u));
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) l[j] = e0 + j < a.experts ? canon(logit_f32(p + j)) : kLowest;
   }
@@ -192,14 +245,14 @@ struct Row {
       const float at = m == kLowest ? 0.0f : m;  // a row of -inf: all scores 0
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = expf(l[j] - at);
+        s[j] = exp_f32(l[j] - at);
         sum += s[j];
       }
       return sum_f32<W>(sum);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      s[j] = e0 + j < a.experts ? score_f32(l[j], a.scoring) : 0.0f;
+      s[j] = score_f32(l[j], a.scoring);  // 0 of -inf, past the last expert
       sum += s[j];
     }
     return sum_f32<W>(sum);
@@ -213,22 +266,67 @@ __device__ __forceinline__ uint64_t row_bits(uint64_t ballot, int lane) {
   return (ballot >> (lane & ~(W - 1))) & ((uint64_t(1) << W) - 1);
 }
 
-// Takes the row's largest key (lowest index of equals): its expert, the same in every lane; the key becomes 0.
-template <int W, int V>
-__device__ __forceinline__ int take(uint32_t (&key)[V], int lane, int e0) {
-  uint32_t best = key[0];
-#pragma unroll
-  for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
-  const uint32_t m = max_u32<W>(best);
-  const int win = __builtin_ctzll(row_bits<W>(__ballot(best == m), lane));
-  int j_win = V - 1;
-#pragma unroll
-  for (int j = V - 2; j >= 0; --j) j_win = key[j] == m ? j : j_win;
-  const bool mine = (lane & (W - 1)) == win;
-#pragma unroll
-  for (int j = 0; j < V; ++j) key[j] = mine && j == j_win ? 0u : key[j];
-  return __shfl(e0 + j_win, win, W);
+// The lane of this row that holds the first of the set bits
+template <int W>
+__device__ __forceinline__ int first_lane(bool bit, int lane) {
+  return __builtin_ctzll(row_bits<W>(__ballot(bit), lane));
 }
+
+// The row's keys, taken largest first (lowest index of equals). With 4 experts a lane sorts its own
+// keys first (adjacent exchanges, so equals keep their order) and only its head takes part in a
+// round: 8 picks of 256 experts cost 8 butterflies. Lanes with more search theirs every round.
+template <int W, int V>
+struct Keys {
+  static constexpr bool kSorted = V == 4;
+  uint32_t key[V];
+  uint32_t order;  // sorted: byte i is the place of the i-th largest
+
+  __device__ __forceinline__ void start() {
+    if constexpr (kSorted) {
+      uint32_t at[4] = {0, 1, 2, 3};
+#pragma unroll
+      for (int end = 3; end > 0; --end)
+#pragma unroll
+        for (int i = 0; i < end; ++i) {
+          const bool swap = key[i + 1] > key[i];
+          const uint32_t k = key[i], x = at[i];
+          key[i] = swap ? key[i + 1] : k;
+          key[i + 1] = swap ? k : key[i + 1];
+          at[i] = swap ? at[i + 1] : x;
+          at[i + 1] = swap ? x : at[i + 1];
+        }
+      order = at[0] | at[1] << 8 | at[2] << 16 | at[3] << 24;
+    }
+  }
+  // m: the largest key; lane: where it is; e: the winner lane's expert (its own in other lanes). Takes it.
+  __device__ __forceinline__ void next(int lane_id, uint32_t& m, int& win, int& e, int e0) {
+    uint32_t best = key[0];
+    if constexpr (!kSorted) {
+#pragma unroll
+      for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
+    }
+    m = max_u32<W>(best);
+    win = first_lane<W>(best == m, lane_id);
+    const bool mine = (lane_id & (W - 1)) == win;
+    if constexpr (kSorted) {
+      e = e0 + static_cast<int>(order & 0xff);
+      key[0] = mine ? key[1] : key[0];
+      key[1] = mine ? key[2] : key[1];
+      key[2] = mine ? key[3] : key[2];
+      key[3] = mine ? 0u : key[3];
+      order = mine ? order >> 8 : order;
+    } else {
+      int at = V - 1;
+#pragma unroll
+      for (int j = V - 2; j >= 0; --j) at = key[j] == m ? j : at;
+      e = e0 + at;
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[j] = mine && j == at ? 0u : key[j];
+    }
+  }
+};
+
+// Takes the row's largest 64-bit key (lowest index of equals): its expert, the same in every lane.
 template <int W, int V>
 __device__ __forceinline__ int take(uint64_t (&key)[V], int lane, int e0) {
   uint64_t best = key[0];
@@ -237,7 +335,7 @@ __device__ __forceinline__ int take(uint64_t (&key)[V], int lane, int e0) {
   const uint32_t hi = static_cast<uint32_t>(best >> 32), m_hi = max_u32<W>(hi);
   const uint32_t lo = hi == m_hi ? static_cast<uint32_t>(best) : 0u, m_lo = max_u32<W>(lo);
   const uint64_t m = uint64_t(m_hi) << 32 | m_lo;
-  const int win = __builtin_ctzll(row_bits<W>(__ballot(best == m), lane));
+  const int win = first_lane<W>(best == m, lane);
   int j_win = V - 1;
 #pragma unroll
   for (int j = V - 2; j >= 0; --j) j_win = key[j] == m ? j : j_win;
@@ -247,20 +345,24 @@ __device__ __forceinline__ int take(uint64_t (&key)[V], int lane, int e0) {
   return __shfl(e0 + j_win, win, W);
 }
 
-// LDS of a wavefront's rows for the groups' values: expert e of group g at e + g
-__host__ __device__ constexpr int group_words(int W, int V) { return W * V + kMaxGroups; }
+// LDS of a row: the groups' values (64-bit form: expert e of group g at e + g), or the picks
+__host__ __device__ constexpr int row_words(int W, int V) { return W * V + kMaxGroups; }
 
-// Which groups stay: the value of a group is its largest key's value (no bias) or the sum of its two
-// largest choice values (bias). A lane takes whole groups, from the row's copy in LDS.
+__device__ __forceinline__ void lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Which groups stay, any group size: the value of a group is its largest choice value (no bias) or the
+// sum of its two largest. A lane takes a whole group, from the row's copy in LDS.
 template <int W, int V, bool BIAS, typename K>
 __device__ __forceinline__ void drop_groups(const Args& a, K (&key)[V], const double (&c)[V], int lane, int e0,
-                                            double* lds_row) {
+                                         double* lds_row) {
   const int size = a.experts / a.groups, li = lane & (W - 1);
 #pragma unroll
   for (int j = 0; j < V; ++j)
     if (e0 + j < a.experts) lds_row[e0 + j + (e0 + j) / size] = c[j];
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+  lds_fence();
   // lane g < groups (groups <= W) holds group g's value
   uint64_t gkey[1] = {0};
   if (li < a.groups) {
@@ -274,8 +376,7 @@ __device__ __forceinline__ void drop_groups(const Args& a, K (&key)[V], const do
     if (value != value) value = -__builtin_huge_val();
     gkey[0] = key64(value);
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
+  lds_fence();
   uint64_t kept = 0;
   for (int i = 0; i < a.keep; ++i) kept |= uint64_t(1) << take<W, 1>(gkey, lane, li);
 #pragma unroll
@@ -283,106 +384,252 @@ __device__ __forceinline__ void drop_groups(const Args& a, K (&key)[V], const do
     if (e0 + j < a.experts && !(kept >> ((e0 + j) / size) & 1)) key[j] = 0;
 }
 
-// Selection of one row: lane kk < topk gets the kk-th expert and its weight.
-template <typename T, int W, int V, bool BIAS>
-__device__ __forceinline__ void select_row(const Args& a, const Row<T, W, V>& row, int64_t t, int lane,
-                                           double* lds_row, int& id, float& weight) {
+// A butterfly step of lane distance D (1, 2, .. 32) inside a row, for values that agree within D lanes
+template <int D>
+__device__ __forceinline__ float step_f32(float v, int lane) {
+  const uint32_t u = __float_as_uint(v);
+  if constexpr (D == 1) return __uint_as_float(dpp<kXor1>(u));
+  if constexpr (D == 2) return __uint_as_float(dpp<kXor2>(u));
+  if constexpr (D == 4) return __uint_as_float(dpp<kHalfMirror>(u));
+  if constexpr (D == 8) return __uint_as_float(dpp<kMirror>(u));
+  if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(lane & 16 ? r[0] : r[1]);
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(lane & 32 ? r[0] : r[1]);
+}
+
+// Which groups stay, groups of whole lanes (a.group_lanes, a power of two), choice values in fp32: true
+// if the lane's group stays. sure: false if the worst kept and the best dropped are within `margin`.
+template <int W, int V, bool BIAS>
+__device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], int lane, float margin, bool& sure) {
+  float first = c[0], second = kLowest;
+#pragma unroll
+  for (int j = 1; j < V; ++j) {
+    second = fmaxf(second, fminf(first, c[j]));
+    first = fmaxf(first, c[j]);
+  }
+  auto merge = [&](float f, float s) {
+    second = fmaxf(fmaxf(second, s), fminf(first, f));
+    first = fmaxf(first, f);
+  };
+  const int gl = a.group_lanes;
+  if (gl > 1) merge(step_f32<1>(first, lane), step_f32<1>(second, lane));
+  if (gl > 2) merge(step_f32<2>(first, lane), step_f32<2>(second, lane));
+  if (gl > 4) merge(step_f32<4>(first, lane), step_f32<4>(second, lane));
+  if (gl > 8) merge(step_f32<8>(first, lane), step_f32<8>(second, lane));
+  if constexpr (W > 16)
+    if (gl > 16) merge(step_f32<16>(first, lane), step_f32<16>(second, lane));
+  if constexpr (W > 32)
+    if (gl > 32) merge(step_f32<32>(first, lane), step_f32<32>(second, lane));
+  const float value = BIAS ? first + second : first;
+  const int li = lane & (W - 1);
+  // the first lane of a group stands for it
+  uint32_t key = (li & (gl - 1)) == 0 && li < a.groups * gl ? key32(value) : 0u;
+  bool kept = false;
+  float worst = 0.0f;
+  for (int i = 0; i < a.keep; ++i) {
+    const uint32_t m = max_u32<W>(key);
+    const int win = first_lane<W>(key == m, lane);
+    if (li == win) key = 0;
+    kept |= (li & ~(gl - 1)) == win;
+    worst = value_of(m);
+  }
+  if constexpr (BIAS) {
+    const uint32_t m = max_u32<W>(key);
+    sure = sure && (m == 0 || worst - value_of(m) > margin);
+  }
+  return kept;
+}
+
+// Selection in 64 bits: lane kk < topk gets the kk-th expert.
+template <typename T, int W, int V>
+__device__ __forceinline__ int choose_f64(const Args& a, const Row<T, W, V>& row, int lane, double* lds_row) {
   const int li = lane & (W - 1), e0 = row.e0;
   double c[V] = {};
-  float m = row.l[0];
-  if constexpr (BIAS) {
-    double sum = 1.0;
-    if (a.scoring == AFD_SCORE_SOFTMAX) {
+  double sum = 1.0;
+  if (a.scoring == AFD_SCORE_SOFTMAX) {
+    float m = row.l[0];
 #pragma unroll
-      for (int j = 1; j < V; ++j) m = fmaxf(m, row.l[j]);
-      m = max_f32<W>(m);
-      const double at = m == kLowest ? 0.0 : static_cast<double>(m);
-      sum = 0.0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        c[j] = exp(static_cast<double>(row.l[j]) - at);
-        sum += c[j];
-      }
-      sum = sum_f64<W>(sum);
-      if (sum == 0.0) sum = 1.0;
-    }
+    for (int j = 1; j < V; ++j) m = fmaxf(m, row.l[j]);
+    m = max_f32<W>(m);
+    const double at = m == kLowest ? 0.0 : static_cast<double>(m);
+    sum = 0.0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (e0 + j >= a.experts) continue;
-      if (a.scoring == AFD_SCORE_SOFTMAX)
-        c[j] /= sum;
-      else
-        c[j] = score_f64(row.l[j], a.scoring);
-      c[j] += a.bias[e0 + j];
-      if (c[j] != c[j]) c[j] = -__builtin_huge_val();
+      c[j] = exp(static_cast<double>(row.l[j]) - at);
+      sum += c[j];
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) c[j] = row.l[j];
+    sum = sum_f64<W>(sum);
+    if (sum == 0.0) sum = 1.0;
   }
-  using K = std::conditional_t<BIAS, uint64_t, uint32_t>;
-  K key[V];
+  uint64_t key[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    if constexpr (BIAS)
-      key[j] = e0 + j < a.experts ? key64(c[j]) : 0;
+    key[j] = 0;
+    if (e0 + j >= a.experts) continue;
+    if (a.scoring == AFD_SCORE_SOFTMAX)
+      c[j] /= sum;
     else
-      key[j] = e0 + j < a.experts ? key32(row.l[j]) : 0;
+      c[j] = score_f64(row.l[j], a.scoring);
+    c[j] += a.bias[e0 + j];
+    if (c[j] != c[j]) c[j] = -__builtin_huge_val();
+    key[j] = key64(c[j]);
   }
-  if (a.groups > 1) drop_groups<W, V, BIAS>(a, key, c, lane, e0, lds_row);
-  id = 0;
+  if (a.groups > 1) drop_groups<W, V, true>(a, key, c, lane, e0, lds_row);
+  int id = 0;
   for (int kk = 0; kk < a.topk; ++kk) {
     const int e = take<W, V>(key, lane, e0);
     id = li == kk ? e : id;
   }
-  // weights, in lanes kk < topk, from the chosen logits alone where nothing else is needed
+  return id;
+}
+
+// Selection of one row: lane kk < topk gets the kk-th expert. bias: the lane's experts' (BIAS);
+// s, sum: the row's scores (BIAS).
+template <typename T, int W, int V, bool BIAS>
+__device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int lane, double* lds_row,
+                                      const float (&bias)[V], const float (&s)[V], float sum) {
+  const int li = lane & (W - 1), e0 = row.e0;
+  float c[V], margin = 0.0f;
+  bool sure = true;
+  if constexpr (BIAS) {
+    // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal and
+    // root are within one ulp of 2^-23, every other step within 2^-24, which adds up to 9 of these; a
+    // softmax's sum over up to 16 values a lane and 6 butterflies brings it to 32, so 2^-18 there.
+    // Two values stand apart if they differ by twice the row's largest such bound.
+    const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float score = s[j] * inv;
+      c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
+      most = fmaxf(most, score + fabsf(bias[j]));
+    }
+    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX ? 0x1p-17f : 0x1p-19f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = row.l[j];
+  }
+  Keys<W, V> keys;
+#pragma unroll
+  for (int j = 0; j < V; ++j) keys.key[j] = e0 + j < a.experts ? key32(c[j]) : 0;
+  if (a.groups > 1) {
+    if (a.group_lanes) {
+      // a group's value is the sum of two choice values: twice the margin
+      const bool kept = keep_group<W, V, BIAS>(a, c, lane, 2.0f * margin, sure);
+#pragma unroll
+      for (int j = 0; j < V; ++j) keys.key[j] = kept ? keys.key[j] : 0;
+    } else if constexpr (BIAS) {
+      sure = false;
+    } else {
+      double wide[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) wide[j] = c[j];
+      drop_groups<W, V, false>(a, keys.key, wide, lane, e0, lds_row);
+    }
+  }
+  keys.start();
+  int id = 0;
+  float last = __builtin_huge_valf();
+  int* picks = reinterpret_cast<int*>(lds_row);
+  for (int kk = 0; kk < a.topk; ++kk) {
+    uint32_t m;
+    int win, e;
+    keys.next(lane, m, win, e, e0);
+    if constexpr (W == 64) {
+      const int got = __builtin_amdgcn_readlane(e, win);  // by all lanes: the winner's e is made in them
+      id = li == kk ? got : id;
+    } else if (li == win) {
+      picks[kk] = e;
+    }
+    if constexpr (BIAS) {
+      const float v = value_of(m);
+      sure = sure && last - v > margin;
+      last = v;
+    }
+  }
+  if constexpr (W < 64) {
+    lds_fence();
+    id = li < a.topk ? picks[li] : 0;
+    lds_fence();
+  }
+  if constexpr (BIAS) {
+    // the best one left
+    uint32_t best = keys.key[0];
+    if constexpr (!Keys<W, V>::kSorted) {
+#pragma unroll
+      for (int j = 1; j < V; ++j) best = keys.key[j] > best ? keys.key[j] : best;
+    }
+    best = max_u32<W>(best);
+    sure = sure && (best == 0 || last - value_of(best) > margin);
+    if (__ballot(!sure)) {
+      const int again = choose_f64<T, W, V>(a, row, lane, lds_row);
+      id = sure ? id : again;
+    }
+  }
+  return id;
+}
+
+// The weight of lane kk's expert, from the chosen logits alone where nothing else is needed.
+template <typename T, int W, int V>
+__device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, int id) {
+  const int li = lane & (W - 1);
   const bool live = li < a.topk;
-  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
-  const float l = live ? canon(logit_f32(p + id)) : kLowest;
+  const float l = live ? canon(logit_f32(static_cast<const T*>(a.logits) + t * a.ld + id)) : kLowest;
   float s;
   if (a.scoring == AFD_SCORE_SOFTMAX) {
     // renormalized, the largest chosen logit is the reference: the others' ratios to it survive
     // however small the scores are
-    m = l;
+    float m = l;
     if (!a.renorm) {
 #pragma unroll
       for (int j = 0; j < V; ++j) m = fmaxf(m, row.l[j]);
     }
     m = max_f32<W>(m);
     const float at = m == kLowest ? 0.0f : m;
-    s = expf(l - at);  // 0 in lanes without a pick
+    s = exp_f32(l - at);  // 0 in lanes without a pick
     float sum = s;
     if (!a.renorm) {
       sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += expf(row.l[j] - at);
+      for (int j = 0; j < V; ++j) sum += exp_f32(row.l[j] - at);
     }
     sum = sum_f32<W>(sum);
-    weight = sum > 0.0f ? s / sum * a.scale : 0.0f;
-    return;
+    return sum > 0.0f ? s / sum * a.scale : 0.0f;
   }
   s = live ? score_f32(l, a.scoring) : 0.0f;
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
     s = sum > 0.0f ? s / sum : 0.0f;
   }
-  weight = s * a.scale;
+  return s * a.scale;
+}
+
+template <int V>
+__device__ __forceinline__ void load_bias(const Args& a, int e0, float (&bias)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) bias[j] = a.bias != nullptr && e0 + j < a.experts ? a.bias[e0 + j] : 0.0f;
 }
 
 // ---------------------------------------------------------------- selection
 template <typename T, int W, int V, bool BIAS>
 __global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
   constexpr int kRows = kThreads / W;  // rows in flight of a workgroup
-  __shared__ double lds[kRows * group_words(W, V)];
+  __shared__ double lds[kRows * row_words(W, V)];
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  float bias[V];
+  load_bias<V>(a, li * V, bias);
   for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < a.n; r0 += int64_t(gridDim.x) * kRows) {
     const int64_t r = r0 + sub;
     const int64_t rr = r < a.n ? r : a.n - 1;  // the lanes of a wavefront stay together
     Row<T, W, V> row;
     row.load(a, rr, li);
-    int id;
-    float w;
-    select_row<T, W, V, BIAS>(a, row, rr, lane, lds + sub * group_words(W, V), id, w);
+    float s[V] = {}, sum = 0.0f;
+    if constexpr (BIAS) sum = row.scores(a, s);
+    int id = choose<T, W, V, BIAS>(a, row, lane, lds + sub * row_words(W, V), bias, s, sum);
+    float w = weigh(a, row, rr, lane, id);
     if (a.valid != nullptr && !a.valid[rr]) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
       a.ids[r * a.topk + li] = id;
@@ -414,78 +661,105 @@ __device__ __forceinline__ Piece next_piece(const Args& a, int32_t r, int32_t r1
 }
 
 // ---------------------------------------------------------------- a sequence's slots together
-// One workgroup: counts[s], rows[s] and the unscaled loss of sequence s.
-__device__ void finish_sequence(const Args& a, int s, double* red) {
+// A workgroup takes 64 experts of a sequence, its 16 wavefronts every 16th slot each; the wavefronts'
+// sums are added in their order. Loads of one wavefront follow each other, those of 16 overlap.
+constexpr int kFinishWaves = 16;
+constexpr int kFinishThreads = 64 * kFinishWaves;
+
+__device__ __forceinline__ int chunks_of(int experts) { return (experts + 63) / 64; }
+
+// The sum over a workgroup's threads, the same in all (one order); red: kFinishThreads words.
+__device__ double block_sum(double v, double* red) {
   const int t = threadIdx.x;
+  red[t] = v;
+  __syncthreads();
+  for (int h = kFinishThreads / 2; h > 0; h /= 2) {
+    if (t < h) red[t] += red[t + h];
+    __syncthreads();
+  }
+  v = red[0];
+  __syncthreads();
+  return v;
+}
+
+// counts of experts [64 c, + 64) of sequence s, their part of the unscaled loss, and (c = 0) the rows
+__device__ void finish_chunk(const Args& a, int s, int c, double* red) {
+  __shared__ double p_red[kFinishWaves][64];
+  __shared__ int32_t c_red[kFinishWaves][64];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   int32_t lo = 0, hi = a.n;
   if (a.cu != nullptr) {
     lo = min(max(a.cu[s], 0), a.n);
     hi = min(max(a.cu[s + 1], 0), a.n);
   }
-  const int b0 = lo / a.block_rows, b1 = hi > lo ? (hi - 1) / a.block_rows + 1 : b0;
+  const int b0 = lo / a.block_rows, slots = hi > lo ? (hi - 1) / a.block_rows + 1 - b0 : 0;
   const int64_t words = slot_words(a.experts);
   const float* first = a.slots + (int64_t(b0) + s) * words;
-  int rows = 0;
-  for (int b = 0; b < b1 - b0; ++b) rows += reinterpret_cast<const int32_t*>(first + b * words)[2 * a.experts];
-  double loss = 0.0;
-  for (int e = t; e < a.experts; e += blockDim.x) {
-    double p = 0.0;
-    int cnt = 0;
-    for (int b = 0; b < b1 - b0; ++b) {
-      p += first[b * words + e];
-      cnt += reinterpret_cast<const int32_t*>(first + b * words)[a.experts + e];
+  const int e = c * 64 + lane;
+  const bool in = e < a.experts;
+  double p = 0.0;
+  int cnt = 0;
+#pragma unroll 4
+  for (int b = w; b < slots; b += kFinishWaves) {
+    const float* slot = first + b * words;
+    if (in) {
+      p += slot[e];
+      cnt += reinterpret_cast<const int32_t*>(slot)[a.experts + e];
     }
-    a.counts[int64_t(s) * a.experts + e] = cnt;
-    loss += p * cnt;
   }
+  p_red[w][lane] = p;
+  c_red[w][lane] = cnt;
+  __syncthreads();
+  double loss = 0.0;
+  if (w == 0) {
+    p = 0.0;
+    cnt = 0;
+    for (int i = 0; i < kFinishWaves; ++i) {
+      p += p_red[i][lane];
+      cnt += c_red[i][lane];
+    }
+    if (in) a.counts[int64_t(s) * a.experts + e] = cnt;
+    loss = in ? p * cnt : 0.0;
+  }
+  __syncthreads();
   if (a.loss == nullptr) return;
-  red[t] = loss;
-  __syncthreads();
-  for (int h = blockDim.x / 2; h > 0; h /= 2) {
-    if (t < h) red[t] += red[t + h];
-    __syncthreads();
-  }
-  if (t == 0) {
-    a.part[s] = rows > 0 ? red[0] * a.experts / (double(a.topk) * rows * rows) : 0.0;
-    a.rows[s] = rows;
-  }
-  __syncthreads();
+  loss = block_sum(loss, red);
+  if (t == 0) a.part[int64_t(s) * chunks_of(a.experts) + c] = loss;
+  if (c != 0) return;
+  double rows = 0.0;
+  for (int b = t; b < slots; b += kFinishThreads)
+    rows += reinterpret_cast<const int32_t*>(first + b * words)[2 * a.experts];
+  rows = block_sum(rows, red);
+  if (t == 0) a.rows[s] = static_cast<int32_t>(rows);
 }
 
 // One workgroup, after every sequence: the loss and the sequences' coefficients.
 __device__ void finish_loss(const Args& a, double* red) {
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, chunks = chunks_of(a.experts);
   double sum = 0.0, used = 0.0;
-  for (int s = t; s < a.seqs; s += blockDim.x) {
-    sum += a.part[s];
-    used += a.rows[s] > 0 ? 1.0 : 0.0;
+  for (int s = t; s < a.seqs; s += kFinishThreads) {
+    const double rows = a.rows[s];
+    if (rows == 0.0) continue;
+    double loss = 0.0;
+    for (int c = 0; c < chunks; ++c) loss += a.part[int64_t(s) * chunks + c];
+    sum += loss * a.experts / (a.topk * rows * rows);
+    used += 1.0;
   }
-  red[t] = sum;
-  __syncthreads();
-  for (int h = blockDim.x / 2; h > 0; h /= 2) {
-    if (t < h) red[t] += red[t + h];
-    __syncthreads();
-  }
-  sum = red[0];
-  __syncthreads();
-  red[t] = used;
-  __syncthreads();
-  for (int h = blockDim.x / 2; h > 0; h /= 2) {
-    if (t < h) red[t] += red[t + h];
-    __syncthreads();
-  }
-  used = red[0];
+  sum = block_sum(sum, red);
+  used = block_sum(used, red);
   if (t == 0) *a.loss = used > 0.0 ? static_cast<float>(a.alpha * sum / used) : 0.0f;
-  for (int s = t; s < a.seqs; s += blockDim.x) {
+  for (int s = t; s < a.seqs; s += kFinishThreads) {
     const double rows = a.rows[s];
     a.coef[s] = rows > 0 ? static_cast<float>(double(a.alpha) * a.experts / (used * a.topk * rows * rows)) : 0.0f;
   }
 }
 
-__global__ __launch_bounds__(kThreads) void finish_kernel(Args a) {
-  __shared__ double red[kThreads];
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
+  __shared__ double red[kFinishThreads];
   __shared__ uint32_t done;
-  for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) finish_sequence(a, s, red);
+  const int chunks = chunks_of(a.experts);
+  for (int64_t i = blockIdx.x; i < int64_t(a.seqs) * chunks; i += gridDim.x)
+    finish_chunk(a, static_cast<int>(i / chunks), static_cast<int>(i % chunks), red);
   if (a.loss == nullptr) return;
   // the last workgroup adds the sequences up
   __threadfence();
@@ -502,12 +776,14 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(Args a) {
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES>
 __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
   constexpr int kRows = kThreads / W;
-  __shared__ double lds[SELECT ? kRows * group_words(W, V) : 1];
+  __shared__ double lds[SELECT ? kRows * row_words(W, V) : 1];
   __shared__ float sums[SCORES ? kRows * W * V : 1];
   __shared__ int32_t cnt[kMaxExperts];
   __shared__ int32_t live_rows;
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   if (blockIdx.x == 0 && t == 0 && a.ticket != nullptr) *a.ticket = 0;  // for the second launch
+  float bias[V];
+  if constexpr (SELECT) load_bias<V>(a, li * V, bias);
   const int32_t r0 = blockIdx.x * a.block_rows;
   const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
   for (int32_t at = r0; at < r1;) {
@@ -524,11 +800,12 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
       const int32_t rr = in ? r : piece.end - 1;
       const bool live = in && (a.valid == nullptr || a.valid[rr]);
       Row<T, W, V> row;
+      float s[V] = {}, sum = 0.0f;
       if constexpr (SELECT || SCORES) row.load(a, rr, li);
+      if constexpr (SCORES) sum = row.scores(a, s);
       if constexpr (SELECT) {
-        int id;
-        float w;
-        select_row<T, W, V, BIAS>(a, row, rr, lane, lds + sub * group_words(W, V), id, w);
+        const int id = choose<T, W, V, BIAS>(a, row, lane, lds + sub * row_words(W, V), bias, s, sum);
+        const float w = weigh(a, row, rr, lane, id);
         if (in && li < a.topk) {
           a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
           a.w[int64_t(r) * a.topk + li] = live ? w : 0.0f;
@@ -541,8 +818,6 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
         }
       }
       if constexpr (SCORES) {
-        float s[V];
-        const float sum = row.scores(a, s);
         const float inv = live && sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
@@ -587,6 +862,7 @@ template <typename T, int W, int V>
 __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
   constexpr int kRows = kThreads / W;
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  __shared__ __attribute__((aligned(16))) float spread[kRows * W * V];
   const float gloss = a.coef != nullptr ? *a.gloss : 0.0f;
   const int32_t r0 = blockIdx.x * a.block_rows;
   const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
@@ -637,7 +913,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
             for (int j = 0; j < V; ++j) m = fmaxf(m, row.l[j]);
           }
           m = max_f32<W>(m);
-          share = id >= 0 ? expf(l - (m == kLowest ? 0.0f : m)) : 0.0f;
+          share = id >= 0 ? exp_f32(l - (m == kLowest ? 0.0f : m)) : 0.0f;
         } else {
           share = id >= 0 ? score_f32(l, a.scoring) : 0.0f;
         }
@@ -650,12 +926,15 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
         float mean = 0.0f;
         if (a.renorm || a.scoring == AFD_SCORE_SOFTMAX) mean = sum_f32<W>(g * share);
         const float u = share * (g - (a.renorm ? mean : 0.0f));
-        for (int kk = 0; kk < a.topk; ++kk) {
-          const int e = __shfl(id, kk, W);
-          const float v = __shfl(u, kk, W);
+        // to the lanes that hold the experts, through LDS (an id that comes twice is added up)
+        float* mine = spread + sub * (W * V) + row.e0;
 #pragma unroll
-          for (int j = 0; j < V; ++j) d[j] += e == row.e0 + j ? v : 0.0f;
-        }
+        for (int j = 0; j < V; ++j) mine[j] = 0.0f;
+        lds_fence();
+        if (id >= 0) atomicAdd(spread + sub * (W * V) + id, u);
+        lds_fence();
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] += mine[j];
         if (!a.renorm && a.scoring == AFD_SCORE_SOFTMAX) {
 #pragma unroll
           for (int j = 0; j < V; ++j) d[j] -= s[j] * inv * mean;
@@ -664,10 +943,20 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
       if (in) {
         T* out = static_cast<T*>(a.dlogits) + int64_t(r) * a.experts + row.e0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (row.e0 + j >= a.experts) continue;
-          const float v = live ? d[j] * slope_f32(row.l[j], a.scoring) : 0.0f;
-          store_logit<T>(out + j, v);
+        for (int j = 0; j < V; ++j) d[j] = live ? d[j] * slope_f32(row.l[j], s[j], a.scoring) : 0.0f;
+        if (a.wide) {
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            if (row.e0 + j >= a.experts) continue;
+            if constexpr (sizeof(T) == 4)
+              *reinterpret_cast<v4f*>(out + j) = v4f{d[j], d[j + 1], d[j + 2], d[j + 3]};
+            else
+              *reinterpret_cast<uint2*>(out + j) = uint2{pk_bf16(d[j], d[j + 1]), pk_bf16(d[j + 2], d[j + 3])};
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (row.e0 + j < a.experts) store_logit<T>(out + j, d[j]);
         }
       }
     }
@@ -733,14 +1022,21 @@ static Args base_args(const afd_router_cfg& c, const void* logits, int64_t ld, i
   a.scale = c.scale;
   return a;
 }
+// what depends on the lanes' share V of a row
+static void set_shape(Args& a, int W, int V, size_t logit_bytes) {
+  a.wide = a.experts % 4 == 0 && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % (4 * logit_bytes) == 0 &&
+           reinterpret_cast<uintptr_t>(a.dlogits) % (4 * logit_bytes) == 0;
+  const int size = a.experts / a.groups, lanes = size / V;
+  a.group_lanes = a.groups > 1 && size % V == 0 && (lanes & (lanes - 1)) == 0 && lanes <= W ? lanes : 0;
+}
 static int lanes_needed(const Args& a, bool select) {
   return select && a.groups > a.topk ? a.groups : a.topk;
 }
 
-// rows of a workgroup: four workgroups a CU, whole passes of its wavefronts, at most kMaxBlockRows
+// rows of a workgroup: two workgroups a CU, whole passes of its wavefronts, at most kMaxBlockRows
 static int block_rows_for(int32_t n, int lanes_per_row) {
   const int pass = kThreads / lanes_per_row;
-  int64_t rows = (int64_t(n) + 1023) / 1024;
+  int64_t rows = (int64_t(n) + 511) / 512;
   rows = (rows + pass - 1) / pass * pass;
   return static_cast<int>(rows < pass ? pass : rows > kMaxBlockRows ? kMaxBlockRows : rows);
 }
@@ -757,7 +1053,7 @@ static WsPlan plan(int32_t n, int32_t experts, int32_t seqs) {
   auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
   p.slots = 0;
   p.part = round(count * slot_words(experts) * 4);
-  p.rows = p.part + round(uint64_t(seqs) * 8);
+  p.rows = p.part + round(uint64_t(seqs) * ((experts + 63) / 64) * 8);
   p.ticket = p.rows + round(uint64_t(seqs) * 4);
   p.total = p.ticket + 256;
   return p;
@@ -793,6 +1089,7 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
       a.block_rows = block_rows_for(a.n, W);
       a.blocks = blocks_for(a.n, a.block_rows);
+      set_shape(a, W, V, sizeof(T));
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), 0, s, a);
         AFD_CHECK_LAUNCH();
@@ -804,8 +1101,9 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
     });
   });
   if (st != AFD_OK) return st;
-  const int grid = a.seqs < 1024 ? a.seqs : 1024;
-  hipLaunchKernelGGL(finish_kernel, dim3(grid), dim3(kThreads), 0, s, a);
+  const int64_t items = int64_t(a.seqs) * ((a.experts + 63) / 64);
+  hipLaunchKernelGGL(finish_kernel, dim3(static_cast<unsigned>(items < 2048 ? items : 2048)), dim3(kFinishThreads), 0,
+                     s, a);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
@@ -832,6 +1130,7 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
     using T = decltype(tag);
     return router::with_shape(a.experts, router::lanes_needed(a, true), [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
+      router::set_shape(a, W, V, sizeof(T));
       int64_t grid = (int64_t(n) + kRows - 1) / kRows;
       if (grid > int64_t(16) * device_cu_count()) grid = int64_t(16) * device_cu_count();
       auto go = [&](auto kernel) {
@@ -959,6 +1258,7 @@ extern "C" int afd_router_grad(const afd_router_cfg* cfg, const void* logits, in
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
       a.block_rows = router::block_rows_for(n, W);
       a.blocks = router::blocks_for(n, a.block_rows);
+      router::set_shape(a, W, V, sizeof(T));
       hipLaunchKernelGGL((router::grad_kernel<T, W, V>), dim3(a.blocks), dim3(router::kThreads), 0,
                          static_cast<hipStream_t>(stream), a);
       AFD_CHECK_LAUNCH();

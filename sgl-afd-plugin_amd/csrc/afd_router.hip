@@ -32,6 +32,7 @@ namespace afd {
 namespace router {
 
 constexpr int kThreads = 256;
+constexpr int kBalanceThreads = 512;  // more wavefronts for the same number of slots
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 32;
 constexpr int kMaxGroups = 64;
@@ -60,7 +61,7 @@ struct Args {
   float* slots;  // [blocks + seqs] of slot_words(experts)
   int32_t* counts;
   float* coef;
-  double* part;      // [seqs][64-expert chunks] unscaled losses
+  double* part;      // [seqs][chunks of experts] unscaled losses
   int32_t* rows;     // [seqs] rows
   uint32_t* ticket;  // workgroups of the second launch that are done
   float* loss;
@@ -149,6 +150,9 @@ __device__ __forceinline__ uint32_t key32(float v) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key ^ (~static_cast<uint32_t>(static_cast<int32_t>(key) >> 31) | 0x80000000u));
 }
+__device__ __forceinline__ double value_of(uint64_t key) {
+  return __builtin_bit_cast(double, key ^ (~static_cast<uint64_t>(static_cast<int64_t>(key) >> 63) | 0x8000000000000000ull));
+}
 __device__ __forceinline__ uint64_t key64(double v) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
   return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
@@ -192,8 +196,12 @@ __device__ __forceinline__ float sigmoid_f32(float v) { return __builtin_amdgcn_
 __device__ __forceinline__ float score_f32(float v, int scoring) {
   return scoring == AFD_SCORE_SIGMOID ? sigmoid_f32(v) : __builtin_amdgcn_sqrtf(softplus_f32(v));
 }
-__device__ __forceinline__ double score_f64(double v, int scoring) {
-  return scoring == AFD_SCORE_SIGMOID ? 1.0 / (1.0 + exp(-v)) : sqrt(log1p(exp(-fabs(v))) + fmax(v, 0.0));
+// e^v (softmax, v relative to the row's largest), sigmoid or sqrt(softplus) in 64 bits: called, not inlined, so
+// its registers are not the callers'
+__device__ __attribute__((noinline)) double score_f64(double v, int scoring) {
+  const double e = exp(scoring == AFD_SCORE_SOFTMAX ? v : scoring == AFD_SCORE_SIGMOID ? -v : -fabs(v));
+  if (scoring == AFD_SCORE_SOFTMAX) return e;
+  return scoring == AFD_SCORE_SIGMOID ? 1.0 / (1.0 + e) : sqrt(log1p(e) + fmax(v, 0.0));
 }
 // d score / dl over the score: 1 - sigmoid, or sigmoid / (2 softplus), which tends to 1/2 where
 // softplus(l) -> e^l leaves the floats
@@ -326,62 +334,114 @@ struct Keys {
   }
 };
 
-// Takes the row's largest 64-bit key (lowest index of equals): its expert, the same in every lane.
-template <int W, int V>
-__device__ __forceinline__ int take(uint64_t (&key)[V], int lane, int e0) {
-  uint64_t best = key[0];
-#pragma unroll
-  for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
-  const uint32_t hi = static_cast<uint32_t>(best >> 32), m_hi = max_u32<W>(hi);
-  const uint32_t lo = hi == m_hi ? static_cast<uint32_t>(best) : 0u, m_lo = max_u32<W>(lo);
-  const uint64_t m = uint64_t(m_hi) << 32 | m_lo;
-  const int win = first_lane<W>(best == m, lane);
-  int j_win = V - 1;
-#pragma unroll
-  for (int j = V - 2; j >= 0; --j) j_win = key[j] == m ? j : j_win;
-  const bool mine = (lane & (W - 1)) == win;
-#pragma unroll
-  for (int j = 0; j < V; ++j) key[j] = mine && j == j_win ? 0ull : key[j];
-  return __shfl(e0 + j_win, win, W);
-}
-
-// LDS of a row: the groups' values (64-bit form: expert e of group g at e + g), or the picks
-__host__ __device__ constexpr int row_words(int W, int V) { return W * V + kMaxGroups; }
+// LDS of a row: the keys of the 64-bit choice, or the picks
+__host__ __device__ constexpr int row_words(int W, int V) { return W * V; }
 
 __device__ __forceinline__ void lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
 
-// Which groups stay, any group size: the value of a group is its largest choice value (no bias) or the
-// sum of its two largest. A lane takes a whole group, from the row's copy in LDS.
-template <int W, int V, bool BIAS, typename K>
-__device__ __forceinline__ void drop_groups(const Args& a, K (&key)[V], const double (&c)[V], int lane, int e0,
-                                         double* lds_row) {
-  const int size = a.experts / a.groups, li = lane & (W - 1);
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (e0 + j < a.experts) lds_row[e0 + j + (e0 + j) / size] = c[j];
-  lds_fence();
-  // lane g < groups (groups <= W) holds group g's value
-  uint64_t gkey[1] = {0};
-  if (li < a.groups) {
-    double first = -__builtin_huge_val(), second = first;
-    for (int i = 0; i < size; ++i) {
-      const double v = lds_row[li * (size + 1) + i];
-      second = fmax(second, fmin(first, v));
-      first = fmax(first, v);
+// The lane with the row's largest 64-bit key (the first of equals)
+template <int W>
+__device__ __forceinline__ int best_lane(uint64_t key, int lane) {
+  const uint32_t hi = static_cast<uint32_t>(key >> 32), m_hi = max_u32<W>(hi);
+  const uint32_t lo = hi == m_hi ? static_cast<uint32_t>(key) : 0u, m_lo = max_u32<W>(lo);
+  return first_lane<W>(hi == m_hi && static_cast<uint32_t>(key) == m_lo, lane);
+}
+
+// The choice in 64 bits, and with groups of any size: lane kk < topk gets the kk-th expert. Rare, so
+// its values live in LDS and its loops stay loops: it must not cost the usual case its registers.
+template <typename T, int W, int V, bool BIAS>
+__device__ __forceinline__ int choose_f64(const Args& a, int64_t t, int lane, uint64_t* keys) {
+  const int li = lane & (W - 1), e0 = li * V;
+  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
+  double at = 0.0, sum = 1.0;
+  if (BIAS && a.scoring == AFD_SCORE_SOFTMAX) {
+    float m = kLowest;
+#pragma unroll 1
+    for (int j = 0; j < V; ++j) m = fmaxf(m, e0 + j < a.experts ? canon(logit_f32(p + e0 + j)) : kLowest);
+    m = max_f32<W>(m);
+    at = m == kLowest ? 0.0 : static_cast<double>(m);
+  }
+  sum = 0.0;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    uint64_t key = 0;
+    if (e0 + j < a.experts) {
+      double c = canon(logit_f32(p + e0 + j));
+      if constexpr (BIAS) {
+        c = score_f64(c - at, a.scoring);  // at is 0 but for softmax
+        sum += c;
+      }
+      key = __builtin_bit_cast(uint64_t, c);
     }
-    double value = BIAS && size > 1 ? first + second : first;
-    if (value != value) value = -__builtin_huge_val();
-    gkey[0] = key64(value);
+    keys[e0 + j] = key;
+  }
+  if (BIAS && a.scoring == AFD_SCORE_SOFTMAX) {
+    sum = sum_f64<W>(sum);
+    if (sum == 0.0) sum = 1.0;
+  }
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    if (e0 + j >= a.experts) break;
+    double c = __builtin_bit_cast(double, keys[e0 + j]);
+    if constexpr (BIAS) {
+      if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
+      c += a.bias[e0 + j];
+      if (c != c) c = -__builtin_huge_val();
+    }
+    keys[e0 + j] = key64(c);
   }
   lds_fence();
-  uint64_t kept = 0;
-  for (int i = 0; i < a.keep; ++i) kept |= uint64_t(1) << take<W, 1>(gkey, lane, li);
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (e0 + j < a.experts && !(kept >> ((e0 + j) / size) & 1)) key[j] = 0;
+  if (a.groups > 1) {
+    // lane g < groups (groups <= W) makes group g's value: its largest choice value (no bias) or the
+    // sum of its two largest
+    const int size = a.experts / a.groups;
+    uint64_t gkey = 0;
+    if (li < a.groups) {
+      uint64_t first = 0, second = 0;
+#pragma unroll 1
+      for (int i = 0; i < size; ++i) {
+        const uint64_t k = keys[li * size + i];
+        second = k > first ? first : k > second ? k : second;
+        first = k > first ? k : first;
+      }
+      double value = value_of(first);
+      if (BIAS && size > 1) value += value_of(second);
+      if (value != value) value = -__builtin_huge_val();
+      gkey = key64(value);
+    }
+    uint64_t kept = 0;
+    for (int i = 0; i < a.keep; ++i) {
+      const int g = best_lane<W>(gkey, lane);
+      if (li == g) gkey = 0;
+      kept |= uint64_t(1) << g;
+    }
+    lds_fence();
+#pragma unroll 1
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < a.experts && !(kept >> ((e0 + j) / size) & 1)) keys[e0 + j] = 0;
+    lds_fence();
+  }
+  int id = 0;
+#pragma unroll 1
+  for (int kk = 0; kk < a.topk; ++kk) {
+    uint64_t best = 0;
+    int e = e0;
+#pragma unroll 1
+    for (int j = 0; j < V; ++j) {
+      const uint64_t k = keys[e0 + j];
+      e = k > best ? e0 + j : e;
+      best = k > best ? k : best;
+    }
+    const int win = best_lane<W>(best, lane);
+    if (li == win) keys[e] = 0;
+    const int got = __shfl(e, win, W);
+    id = li == kk ? got : id;
+    lds_fence();
+  }
+  return id;
 }
 
 // A butterfly step of lane distance D (1, 2, .. 32) inside a row, for values that agree within D lanes
@@ -443,53 +503,10 @@ __device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], i
   return kept;
 }
 
-// Selection in 64 bits: lane kk < topk gets the kk-th expert.
-template <typename T, int W, int V>
-__device__ __forceinline__ int choose_f64(const Args& a, const Row<T, W, V>& row, int lane, double* lds_row) {
-  const int li = lane & (W - 1), e0 = row.e0;
-  double c[V] = {};
-  double sum = 1.0;
-  if (a.scoring == AFD_SCORE_SOFTMAX) {
-    float m = row.l[0];
-#pragma unroll
-    for (int j = 1; j < V; ++j) m = fmaxf(m, row.l[j]);
-    m = max_f32<W>(m);
-    const double at = m == kLowest ? 0.0 : static_cast<double>(m);
-    sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      c[j] = exp(static_cast<double>(row.l[j]) - at);
-      sum += c[j];
-    }
-    sum = sum_f64<W>(sum);
-    if (sum == 0.0) sum = 1.0;
-  }
-  uint64_t key[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    key[j] = 0;
-    if (e0 + j >= a.experts) continue;
-    if (a.scoring == AFD_SCORE_SOFTMAX)
-      c[j] /= sum;
-    else
-      c[j] = score_f64(row.l[j], a.scoring);
-    c[j] += a.bias[e0 + j];
-    if (c[j] != c[j]) c[j] = -__builtin_huge_val();
-    key[j] = key64(c[j]);
-  }
-  if (a.groups > 1) drop_groups<W, V, true>(a, key, c, lane, e0, lds_row);
-  int id = 0;
-  for (int kk = 0; kk < a.topk; ++kk) {
-    const int e = take<W, V>(key, lane, e0);
-    id = li == kk ? e : id;
-  }
-  return id;
-}
-
 // Selection of one row: lane kk < topk gets the kk-th expert. bias: the lane's experts' (BIAS);
 // s, sum: the row's scores (BIAS).
 template <typename T, int W, int V, bool BIAS>
-__device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int lane, double* lds_row,
+__device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, uint64_t* lds_row,
                                       const float (&bias)[V], const float (&s)[V], float sum) {
   const int li = lane & (W - 1), e0 = row.e0;
   float c[V], margin = 0.0f;
@@ -521,13 +538,8 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       const bool kept = keep_group<W, V, BIAS>(a, c, lane, 2.0f * margin, sure);
 #pragma unroll
       for (int j = 0; j < V; ++j) keys.key[j] = kept ? keys.key[j] : 0;
-    } else if constexpr (BIAS) {
-      sure = false;
     } else {
-      double wide[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) wide[j] = c[j];
-      drop_groups<W, V, false>(a, keys.key, wide, lane, e0, lds_row);
+      sure = false;
     }
   }
   keys.start();
@@ -564,10 +576,10 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     }
     best = max_u32<W>(best);
     sure = sure && (best == 0 || last - value_of(best) > margin);
-    if (__ballot(!sure)) {
-      const int again = choose_f64<T, W, V>(a, row, lane, lds_row);
-      id = sure ? id : again;
-    }
+  }
+  if (__ballot(!sure)) {
+    const int again = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
+    id = sure ? id : again;
   }
   return id;
 }
@@ -617,7 +629,7 @@ __device__ __forceinline__ void load_bias(const Args& a, int e0, float (&bias)[V
 template <typename T, int W, int V, bool BIAS>
 __global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
   constexpr int kRows = kThreads / W;  // rows in flight of a workgroup
-  __shared__ double lds[kRows * row_words(W, V)];
+  __shared__ uint64_t lds[kRows * row_words(W, V)];
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   float bias[V];
   load_bias<V>(a, li * V, bias);
@@ -628,7 +640,7 @@ __global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
     row.load(a, rr, li);
     float s[V] = {}, sum = 0.0f;
     if constexpr (BIAS) sum = row.scores(a, s);
-    int id = choose<T, W, V, BIAS>(a, row, lane, lds + sub * row_words(W, V), bias, s, sum);
+    int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum);
     float w = weigh(a, row, rr, lane, id);
     if (a.valid != nullptr && !a.valid[rr]) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
@@ -661,31 +673,18 @@ __device__ __forceinline__ Piece next_piece(const Args& a, int32_t r, int32_t r1
 }
 
 // ---------------------------------------------------------------- a sequence's slots together
-// A workgroup takes 64 experts of a sequence, its 16 wavefronts every 16th slot each; the wavefronts'
-// sums are added in their order. Loads of one wavefront follow each other, those of 16 overlap.
+// A workgroup takes 16 experts (one 64-byte line of a slot) of a sequence: 64 slots side by side, 4 a
+// wavefront, so that a long sequence's slots are in flight together; their sums are added in one order.
 constexpr int kFinishWaves = 16;
 constexpr int kFinishThreads = 64 * kFinishWaves;
+constexpr int kChunk = 16;
 
-__device__ __forceinline__ int chunks_of(int experts) { return (experts + 63) / 64; }
+__host__ __device__ inline int chunks_of(int experts) { return (experts + kChunk - 1) / kChunk; }
 
-// The sum over a workgroup's threads, the same in all (one order); red: kFinishThreads words.
-__device__ double block_sum(double v, double* red) {
-  const int t = threadIdx.x;
-  red[t] = v;
-  __syncthreads();
-  for (int h = kFinishThreads / 2; h > 0; h /= 2) {
-    if (t < h) red[t] += red[t + h];
-    __syncthreads();
-  }
-  v = red[0];
-  __syncthreads();
-  return v;
-}
-
-// counts of experts [64 c, + 64) of sequence s, their part of the unscaled loss, and (c = 0) the rows
-__device__ void finish_chunk(const Args& a, int s, int c, double* red) {
-  __shared__ double p_red[kFinishWaves][64];
-  __shared__ int32_t c_red[kFinishWaves][64];
+// counts of experts [16 c, + 16) of sequence s, their part of the unscaled loss, and (c = 0) the rows
+__device__ __forceinline__ void finish_chunk(const Args& a, int s, int c) {
+  __shared__ double p_red[kFinishWaves][kChunk];
+  __shared__ int32_t c_red[kFinishWaves][kChunk];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   int32_t lo = 0, hi = a.n;
   if (a.cu != nullptr) {
@@ -695,55 +694,77 @@ __device__ void finish_chunk(const Args& a, int s, int c, double* red) {
   const int b0 = lo / a.block_rows, slots = hi > lo ? (hi - 1) / a.block_rows + 1 - b0 : 0;
   const int64_t words = slot_words(a.experts);
   const float* first = a.slots + (int64_t(b0) + s) * words;
-  const int e = c * 64 + lane;
-  const bool in = e < a.experts;
+  const int e = c * kChunk + (lane & 15);
   double p = 0.0;
   int cnt = 0;
-#pragma unroll 4
-  for (int b = w; b < slots; b += kFinishWaves) {
-    const float* slot = first + b * words;
-    if (in) {
+  if (e < a.experts) {
+#pragma unroll 8
+    for (int b = t >> 4; b < slots; b += 4 * kFinishWaves) {
+      const float* slot = first + b * words;
       p += slot[e];
       cnt += reinterpret_cast<const int32_t*>(slot)[a.experts + e];
     }
   }
-  p_red[w][lane] = p;
-  c_red[w][lane] = cnt;
+  // the wavefront's four slots, then the wavefronts
+  p += __shfl_xor(p, 16);
+  p += __shfl_xor(p, 32);
+  cnt += __shfl_xor(cnt, 16);
+  cnt += __shfl_xor(cnt, 32);
+  if (lane < kChunk) {
+    p_red[w][lane] = p;
+    c_red[w][lane] = cnt;
+  }
+  if (w == 1 && c == 0 && a.loss != nullptr) {
+    double rows = 0.0;
+    for (int b = lane; b < slots; b += 64) rows += reinterpret_cast<const int32_t*>(first + b * words)[2 * a.experts];
+    rows = sum_f64<64>(rows);
+    if (lane == 0) a.rows[s] = static_cast<int32_t>(rows);
+  }
   __syncthreads();
-  double loss = 0.0;
   if (w == 0) {
     p = 0.0;
     cnt = 0;
-    for (int i = 0; i < kFinishWaves; ++i) {
-      p += p_red[i][lane];
-      cnt += c_red[i][lane];
+    if (lane < kChunk) {
+      for (int i = 0; i < kFinishWaves; ++i) {
+        p += p_red[i][lane];
+        cnt += c_red[i][lane];
+      }
+      if (e < a.experts) a.counts[int64_t(s) * a.experts + e] = cnt;
     }
-    if (in) a.counts[int64_t(s) * a.experts + e] = cnt;
-    loss = in ? p * cnt : 0.0;
+    if (a.loss != nullptr) {
+      const double loss = sum_f64<64>(p * cnt);
+      if (lane == 0) a.part[int64_t(s) * chunks_of(a.experts) + c] = loss;
+    }
   }
   __syncthreads();
-  if (a.loss == nullptr) return;
-  loss = block_sum(loss, red);
-  if (t == 0) a.part[int64_t(s) * chunks_of(a.experts) + c] = loss;
-  if (c != 0) return;
-  double rows = 0.0;
-  for (int b = t; b < slots; b += kFinishThreads)
-    rows += reinterpret_cast<const int32_t*>(first + b * words)[2 * a.experts];
-  rows = block_sum(rows, red);
-  if (t == 0) a.rows[s] = static_cast<int32_t>(rows);
+}
+
+// The sum over the workgroup, in one order, the same in every thread
+__device__ __forceinline__ double block_sum(double v, double* red) {
+  const int t = threadIdx.x;
+  v = sum_f64<64>(v);
+  if ((t & 63) == 0) red[t >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < kFinishWaves; ++i) v += red[i];
+  __syncthreads();
+  return v;
 }
 
 // One workgroup, after every sequence: the loss and the sequences' coefficients.
-__device__ void finish_loss(const Args& a, double* red) {
+__device__ __forceinline__ void finish_loss(const Args& a) {
+  __shared__ double red[kFinishWaves];
   const int t = threadIdx.x, chunks = chunks_of(a.experts);
   double sum = 0.0, used = 0.0;
-  for (int s = t; s < a.seqs; s += kFinishThreads) {
+  // 16 threads a sequence, its chunks dealt to them
+  for (int64_t s = t >> 4; s < a.seqs; s += kFinishThreads / 16) {
     const double rows = a.rows[s];
-    if (rows == 0.0) continue;
     double loss = 0.0;
-    for (int c = 0; c < chunks; ++c) loss += a.part[int64_t(s) * chunks + c];
-    sum += loss * a.experts / (a.topk * rows * rows);
-    used += 1.0;
+    for (int c = t & 15; c < chunks; c += 16) loss += a.part[s * chunks + c];
+    if (rows > 0.0) {
+      sum += loss * a.experts / (a.topk * rows * rows);
+      used += (t & 15) == 0 ? 1.0 : 0.0;
+    }
   }
   sum = block_sum(sum, red);
   used = block_sum(used, red);
@@ -755,28 +776,28 @@ __device__ void finish_loss(const Args& a, double* red) {
 }
 
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
-  __shared__ double red[kFinishThreads];
   __shared__ uint32_t done;
   const int chunks = chunks_of(a.experts);
   for (int64_t i = blockIdx.x; i < int64_t(a.seqs) * chunks; i += gridDim.x)
-    finish_chunk(a, static_cast<int>(i / chunks), static_cast<int>(i % chunks), red);
+    finish_chunk(a, static_cast<int>(i / chunks), static_cast<int>(i % chunks));
   if (a.loss == nullptr) return;
-  // the last workgroup adds the sequences up
-  __threadfence();
+  // the last workgroup adds the sequences up: what it reads (part and rows) was written by the first two
+  // wavefronts, which order their writes device-wide before the first one's count
+  if (threadIdx.x < 128) __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) done = atomicAdd(a.ticket, 1u);
   __syncthreads();
   if (done != gridDim.x - 1) return;
   __threadfence();
-  finish_loss(a, red);
+  finish_loss(a);
 }
 
 // ---------------------------------------------------------------- selection, counts and balance sums
 // SELECT: choose the experts (else read a.ids). SCORES: sums of s' (else counts alone).
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES>
-__global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
-  constexpr int kRows = kThreads / W;
-  __shared__ double lds[SELECT ? kRows * row_words(W, V) : 1];
+__global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
+  constexpr int kRows = kBalanceThreads / W;
+  __shared__ uint64_t lds[SELECT ? kRows * row_words(W, V) : 1];
   __shared__ float sums[SCORES ? kRows * W * V : 1];
   __shared__ int32_t cnt[kMaxExperts];
   __shared__ int32_t live_rows;
@@ -789,7 +810,7 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
   for (int32_t at = r0; at < r1;) {
     const Piece piece = next_piece(a, at, r1);
     const bool counted = piece.seq >= 0;
-    for (int e = t; e < a.experts; e += kThreads) cnt[e] = 0;
+    for (int e = t; e < a.experts; e += kBalanceThreads) cnt[e] = 0;
     if (t == 0) live_rows = 0;
     __syncthreads();
     float p[V] = {};
@@ -804,7 +825,7 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
       if constexpr (SELECT || SCORES) row.load(a, rr, li);
       if constexpr (SCORES) sum = row.scores(a, s);
       if constexpr (SELECT) {
-        const int id = choose<T, W, V, BIAS>(a, row, lane, lds + sub * row_words(W, V), bias, s, sum);
+        const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum);
         const float w = weigh(a, row, rr, lane, id);
         if (in && li < a.topk) {
           a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
@@ -833,7 +854,7 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(Args a) {
       __syncthreads();
       float* slot = a.slots + (int64_t(blockIdx.x) + piece.seq) * slot_words(a.experts);
       int32_t* slot_i = reinterpret_cast<int32_t*>(slot);
-      for (int e = t; e < a.experts; e += kThreads) {
+      for (int e = t; e < a.experts; e += kBalanceThreads) {
         if constexpr (SCORES) {
           float s = 0.0f;
           for (int i = 0; i < kRows; ++i) s += sums[i * (W * V) + e];
@@ -1033,10 +1054,10 @@ static int lanes_needed(const Args& a, bool select) {
   return select && a.groups > a.topk ? a.groups : a.topk;
 }
 
-// rows of a workgroup: two workgroups a CU, whole passes of its wavefronts, at most kMaxBlockRows
-static int block_rows_for(int32_t n, int lanes_per_row) {
-  const int pass = kThreads / lanes_per_row;
-  int64_t rows = (int64_t(n) + 511) / 512;
+// rows of a workgroup: `groups` workgroups of `threads`, whole passes of their wavefronts, at most kMaxBlockRows
+static int block_rows_for(int32_t n, int lanes_per_row, int threads = kBalanceThreads, int groups = 512) {
+  const int pass = threads / lanes_per_row;
+  int64_t rows = (int64_t(n) + groups - 1) / groups;
   rows = (rows + pass - 1) / pass * pass;
   return static_cast<int>(rows < pass ? pass : rows > kMaxBlockRows ? kMaxBlockRows : rows);
 }
@@ -1053,7 +1074,7 @@ static WsPlan plan(int32_t n, int32_t experts, int32_t seqs) {
   auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
   p.slots = 0;
   p.part = round(count * slot_words(experts) * 4);
-  p.rows = p.part + round(uint64_t(seqs) * ((experts + 63) / 64) * 8);
+  p.rows = p.part + round(uint64_t(seqs) * chunks_of(experts) * 8);
   p.ticket = p.rows + round(uint64_t(seqs) * 4);
   p.total = p.ticket + 256;
   return p;
@@ -1091,7 +1112,7 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
       a.blocks = blocks_for(a.n, a.block_rows);
       set_shape(a, W, V, sizeof(T));
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kBalanceThreads), 0, s, a);
         AFD_CHECK_LAUNCH();
         return int(AFD_OK);
       };
@@ -1101,7 +1122,7 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
     });
   });
   if (st != AFD_OK) return st;
-  const int64_t items = int64_t(a.seqs) * ((a.experts + 63) / 64);
+  const int64_t items = int64_t(a.seqs) * chunks_of(a.experts);
   hipLaunchKernelGGL(finish_kernel, dim3(static_cast<unsigned>(items < 2048 ? items : 2048)), dim3(kFinishThreads), 0,
                      s, a);
   AFD_CHECK_LAUNCH();
@@ -1256,7 +1277,7 @@ extern "C" int afd_router_grad(const afd_router_cfg* cfg, const void* logits, in
     using T = decltype(tag);
     return router::with_shape(a.experts, router::lanes_needed(a, false), [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
-      a.block_rows = router::block_rows_for(n, W);
+      a.block_rows = router::block_rows_for(n, W, router::kThreads, 2048);
       a.blocks = router::blocks_for(n, a.block_rows);
       router::set_shape(a, W, V, sizeof(T));
       hipLaunchKernelGGL((router::grad_kernel<T, W, V>), dim3(a.blocks), dim3(router::kThreads), 0,

@@ -79,23 +79,28 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
 }
+constexpr int kBcast15 = 0x142, kBcast31 = 0x143;
 constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
 
 // f(own, partner) over the lanes of a row; every lane gets the same bits (f commutes). After the
-// quads agree, a mirrored half row is the exchange with the other quad, and so on.
+// quads agree, a mirrored half row is the exchange with the other quad, and so on. Over a whole
+// wavefront the last two steps only gather towards lane 63, whose value is read into a scalar: every
+// step is then one instruction with its DPP operand.
 template <int W, typename F>
 __device__ __forceinline__ uint32_t reduce32(uint32_t v, F f) {
   v = f(v, dpp<kXor1>(v));
   v = f(v, dpp<kXor2>(v));
   v = f(v, dpp<kHalfMirror>(v));
   v = f(v, dpp<kMirror>(v));
-  if constexpr (W >= 32) {
+  if constexpr (W == 32) {
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = f(r[0], r[1]);
   }
-  if constexpr (W >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = f(r[0], r[1]);
+  if constexpr (W == 64) {
+    // row 0's lane 15 into row 1 (and row 2's into row 3), then lane 31 into rows 2 and 3: lane 63 has all
+    v = f(v, dpp<kBcast15>(v));
+    v = f(v, dpp<kBcast31>(v));
+    v = __builtin_amdgcn_readlane(v, 63);
   }
   return v;
 }
@@ -176,6 +181,8 @@ __device__ __forceinline__ float exp_f32(float x) {
   // no correction where t has left the floats
   return fabsf(t) < 126.0f ? __builtin_fmaf(y, rest * kLn2, y) : y;
 }
+// e^x to |x| 2^-24 relative: for terms of a row's sum and shares, of which the large ones have a small x
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 // log(1 + e) for e in [0, 1]: 2 atanh(z), z = e / (2 + e) <= 1/3, by its series up to z^15 (the
 // first term left out is (1/9)^8 / 17 of the sum, below 2^-29)
 __device__ __forceinline__ float log1p_f32(float e) {
@@ -190,11 +197,14 @@ __device__ __forceinline__ float log1p_f32(float e) {
   const float h = z + z;
   return __builtin_fmaf(h * q, p, h);
 }
-__device__ __forceinline__ float softplus_f32(float v) { return log1p_f32(exp_f32(-fabsf(v))) + fmaxf(v, 0.0f); }
-__device__ __forceinline__ float sigmoid_f32(float v) { return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v)); }
 // sigmoid or sqrt(softplus)
 __device__ __forceinline__ float score_f32(float v, int scoring) {
-  return scoring == AFD_SCORE_SIGMOID ? sigmoid_f32(v) : __builtin_amdgcn_sqrtf(softplus_f32(v));
+  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v));
+  return __builtin_amdgcn_sqrtf(log1p_f32(exp_f32(-fabsf(v))) + fmaxf(v, 0.0f));
+}
+__device__ __forceinline__ float score_fast(float v, int scoring) {
+  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_fast(-v));
+  return __builtin_amdgcn_sqrtf(log1p_f32(exp_fast(-fabsf(v))) + fmaxf(v, 0.0f));
 }
 // e^v (softmax, v relative to the row's largest), sigmoid or sqrt(softplus) in 64 bits: called, not inlined, so
 // its registers are not the callers'
@@ -208,9 +218,9 @@ __device__ __attribute__((noinline)) double score_f64(double v, int scoring) {
 // (taken from the score where it is at hand)
 __device__ __forceinline__ float slope_f32(float v, float score, int scoring) {
   if (scoring == AFD_SCORE_SOFTMAX) return 1.0f;
-  if (scoring == AFD_SCORE_SIGMOID) return sigmoid_f32(-v);
+  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_fast(v));
   if (v < -17.0f) return 0.5f;
-  return sigmoid_f32(v) * 0.5f * __builtin_amdgcn_rcpf(score * score);
+  return 0.5f * __builtin_amdgcn_rcpf((1.0f + exp_fast(-v)) * (score * score));
 }
 
 template <typename T, int W, int V>
@@ -253,14 +263,14 @@ struct Row {
       const float at = m == kLowest ? 0.0f : m;  // a row of -inf: all scores 0
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = exp_f32(l[j] - at);
+        s[j] = exp_fast(l[j] - at);
         sum += s[j];
       }
       return sum_f32<W>(sum);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      s[j] = score_f32(l[j], a.scoring);  // 0 of -inf, past the last expert
+      s[j] = score_fast(l[j], a.scoring);  // 0 of -inf, past the last expert
       sum += s[j];
     }
     return sum_f32<W>(sum);
@@ -281,60 +291,110 @@ __device__ __forceinline__ int first_lane(bool bit, int lane) {
 }
 
 // The row's keys, taken largest first (lowest index of equals). With 4 experts a lane sorts its own
-// keys first (adjacent exchanges, so equals keep their order) and only its head takes part in a
-// round: 8 picks of 256 experts cost 8 butterflies. Lanes with more search theirs every round.
-template <int W, int V>
+// keys first and only its head takes part in a round: 8 picks of 256 experts cost 8 butterflies. Lanes
+// with more experts search theirs every round. Spare low bits of a key say which expert it is:
+// kIndexed (bf16 logits, 16 spare bits): kMaxExperts - 1 - e, so that no two are equal, the winning key
+//   names the winner and equal logits are already in index order;
+// kPlaced (choice values that carry a margin; equal ones are chosen again): 3 - the place in the lane;
+// kBare (fp32 logits, none): the places are sorted along, by adjacent exchanges (equals keep their order).
+enum KeyKind { kBare, kPlaced, kIndexed };
+
+template <int W, int V, KeyKind KIND>
 struct Keys {
   static constexpr bool kSorted = V == 4;
   uint32_t key[V];
-  uint32_t order;  // sorted: byte i is the place of the i-th largest
+  uint32_t order;  // sorted bare keys: byte i is the place of the i-th largest
 
-  __device__ __forceinline__ void start() {
-    if constexpr (kSorted) {
+  __device__ __forceinline__ void start(int e0) {
+    if constexpr (KIND == kIndexed) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & 0xffff0000u) | (kMaxExperts - 1 - e0 - j) : 0u;
+    } else if constexpr (KIND == kPlaced && kSorted) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & ~3u) | (3 - j) : 0u;
+    }
+    if constexpr (kSorted && KIND != kBare) {
+      auto sort = [&](int i, int j) {
+        const uint32_t x = key[i], y = key[j];
+        key[i] = max(x, y);
+        key[j] = min(x, y);
+      };
+      sort(0, 1);
+      sort(2, 3);
+      sort(0, 2);
+      sort(1, 3);
+      sort(1, 2);
+    } else if constexpr (kSorted) {
       uint32_t at[4] = {0, 1, 2, 3};
 #pragma unroll
       for (int end = 3; end > 0; --end)
 #pragma unroll
         for (int i = 0; i < end; ++i) {
           const bool swap = key[i + 1] > key[i];
-          const uint32_t k = key[i], x = at[i];
-          key[i] = swap ? key[i + 1] : k;
-          key[i + 1] = swap ? k : key[i + 1];
+          const uint32_t x = at[i], lo = min(key[i], key[i + 1]);
+          key[i] = max(key[i], key[i + 1]);
+          key[i + 1] = lo;
           at[i] = swap ? at[i + 1] : x;
           at[i + 1] = swap ? x : at[i + 1];
         }
       order = at[0] | at[1] << 8 | at[2] << 16 | at[3] << 24;
     }
   }
-  // m: the largest key; lane: where it is; e: the winner lane's expert (its own in other lanes). Takes it.
-  __device__ __forceinline__ void next(int lane_id, uint32_t& m, int& win, int& e, int e0) {
+  __device__ __forceinline__ uint32_t head() const {
     uint32_t best = key[0];
     if constexpr (!kSorted) {
 #pragma unroll
-      for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
+      for (int j = 1; j < V; ++j) best = max(best, key[j]);
     }
+    return best;
+  }
+  __device__ __forceinline__ void pop(bool mine) {
+    key[0] = mine ? key[1] : key[0];
+    key[1] = mine ? key[2] : key[1];
+    key[2] = mine ? key[3] : key[2];
+    key[3] = mine ? 0u : key[3];
+  }
+  // Takes the largest key m and returns its expert, the same in every lane of the row.
+  __device__ __forceinline__ int next(int lane, int e0, uint32_t& m) {
+    const uint32_t best = head();
     m = max_u32<W>(best);
-    win = first_lane<W>(best == m, lane_id);
-    const bool mine = (lane_id & (W - 1)) == win;
-    if constexpr (kSorted) {
-      e = e0 + static_cast<int>(order & 0xff);
-      key[0] = mine ? key[1] : key[0];
-      key[1] = mine ? key[2] : key[1];
-      key[2] = mine ? key[3] : key[2];
-      key[3] = mine ? 0u : key[3];
-      order = mine ? order >> 8 : order;
+    if constexpr (KIND == kIndexed) {
+      if constexpr (kSorted) {
+        pop(key[0] == m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) key[j] = key[j] == m ? 0u : key[j];
+      }
+      return kMaxExperts - 1 - static_cast<int>(m & (kMaxExperts - 1));
     } else {
-      int at = V - 1;
+      const int win = first_lane<W>(best == m, lane);
+      const bool mine = (lane & (W - 1)) == win;
+      if constexpr (kSorted && KIND == kPlaced) {
+        pop(mine);
+        return win * 4 + 3 - static_cast<int>(m & 3);
+      } else {
+        int e;
+        if constexpr (kSorted) {
+          e = e0 + static_cast<int>(order & 0xff);
+          order = mine ? order >> 8 : order;
+          pop(mine);
+        } else {
+          int at = V - 1;
 #pragma unroll
-      for (int j = V - 2; j >= 0; --j) at = key[j] == m ? j : at;
-      e = e0 + at;
+          for (int j = V - 2; j >= 0; --j) at = key[j] == m ? j : at;
+          e = e0 + at;
 #pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = mine && j == at ? 0u : key[j];
+          for (int j = 0; j < V; ++j) key[j] = mine && j == at ? 0u : key[j];
+        }
+        // read by all lanes: the winner's e is made in them
+        if constexpr (W == 64) return __builtin_amdgcn_readlane(e, win);
+        return __shfl(e, win, W);
+      }
     }
   }
 };
 
-// LDS of a row: the keys of the 64-bit choice, or the picks
+// LDS of a row: the keys of the 64-bit choice
 __host__ __device__ constexpr int row_words(int W, int V) { return W * V; }
 
 __device__ __forceinline__ void lds_fence() {
@@ -512,10 +572,12 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
   float c[V], margin = 0.0f;
   bool sure = true;
   if constexpr (BIAS) {
-    // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal and
-    // root are within one ulp of 2^-23, every other step within 2^-24, which adds up to 9 of these; a
-    // softmax's sum over up to 16 values a lane and 6 butterflies brings it to 32, so 2^-18 there.
-    // Two values stand apart if they differ by twice the row's largest such bound.
+    // An fp32 choice value is off by less than 2^-18 (s + |bias|): the exponential by (|x| + 2) 2^-24 of
+    // itself, which is below 2^-22 of the score for every x (a score's slope falls as e^-|x|), the
+    // hardware's reciprocal, root and exponential by one ulp of 2^-23, the other steps by 2^-24, a
+    // softmax's sum over 16 values a lane and 6 butterflies by 22 of these, and the two bits that
+    // hold the place by 2^-21: together below 52 * 2^-24. Two values stand apart if they differ by
+    // twice the row's largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
@@ -524,12 +586,12 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
       most = fmaxf(most, score + fabsf(bias[j]));
     }
-    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX ? 0x1p-17f : 0x1p-19f);
+    margin = max_f32<W>(most) * 0x1p-17f;
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
   }
-  Keys<W, V> keys;
+  Keys<W, V, BIAS ? kPlaced : sizeof(T) == 2 ? kIndexed : kBare> keys;
 #pragma unroll
   for (int j = 0; j < V; ++j) keys.key[j] = e0 + j < a.experts ? key32(c[j]) : 0;
   if (a.groups > 1) {
@@ -542,40 +604,22 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       sure = false;
     }
   }
-  keys.start();
+  keys.start(e0);
   int id = 0;
-  float last = __builtin_huge_valf();
-  int* picks = reinterpret_cast<int*>(lds_row);
+  uint32_t taken = 0;  // lane kk: the kk-th key
   for (int kk = 0; kk < a.topk; ++kk) {
     uint32_t m;
-    int win, e;
-    keys.next(lane, m, win, e, e0);
-    if constexpr (W == 64) {
-      const int got = __builtin_amdgcn_readlane(e, win);  // by all lanes: the winner's e is made in them
-      id = li == kk ? got : id;
-    } else if (li == win) {
-      picks[kk] = e;
-    }
-    if constexpr (BIAS) {
-      const float v = value_of(m);
-      sure = sure && last - v > margin;
-      last = v;
-    }
-  }
-  if constexpr (W < 64) {
-    lds_fence();
-    id = li < a.topk ? picks[li] : 0;
-    lds_fence();
+    const int e = keys.next(lane, e0, m);
+    id = li == kk ? e : id;
+    if constexpr (BIAS) taken = li == kk ? m : taken;
   }
   if constexpr (BIAS) {
-    // the best one left
-    uint32_t best = keys.key[0];
-    if constexpr (!Keys<W, V>::kSorted) {
-#pragma unroll
-      for (int j = 1; j < V; ++j) best = keys.key[j] > best ? keys.key[j] : best;
-    }
-    best = max_u32<W>(best);
-    sure = sure && (best == 0 || last - value_of(best) > margin);
+    // lane kk compares the kk-th with the next one, the last with the best that is left
+    const uint32_t left = max_u32<W>(keys.head());
+    const uint32_t after = __shfl_down(taken, 1, W);
+    const uint32_t below = li == a.topk - 1 ? left : after;
+    if (li < a.topk && below != 0 && !(value_of(taken) - value_of(below) > margin)) sure = false;
+    sure = row_bits<W>(__ballot(!sure), lane) == 0;
   }
   if (__ballot(!sure)) {
     const int again = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
@@ -606,15 +650,15 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, i
     if (!a.renorm) {
       sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += exp_f32(row.l[j] - at);
+      for (int j = 0; j < V; ++j) sum += exp_fast(row.l[j] - at);
     }
     sum = sum_f32<W>(sum);
-    return sum > 0.0f ? s / sum * a.scale : 0.0f;
+    return sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
   }
   s = live ? score_f32(l, a.scoring) : 0.0f;
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
-    s = sum > 0.0f ? s / sum : 0.0f;
+    s = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
   }
   return s * a.scale;
 }
@@ -839,7 +883,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
         }
       }
       if constexpr (SCORES) {
-        const float inv = live && sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
       }
@@ -907,7 +951,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
       row.load(a, rr, li);
       float s[V], d[V];
       const float total = row.scores(a, s);
-      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+      const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) d[j] = 0.0f;
       if (balanced) {
@@ -940,7 +984,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
         }
         const float chosen = sum_f32<W>(share);
         if (a.renorm)
-          share = chosen > 0.0f ? share / chosen : 0.0f;
+          share = chosen > 0.0f ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
         else if (a.scoring == AFD_SCORE_SOFTMAX)
           share *= inv;
         // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something

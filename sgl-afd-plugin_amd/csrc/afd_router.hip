@@ -8,8 +8,8 @@
 // with its logit) and s + bias in 64 bits with one: which of two experts wins a close race then is
 // a matter of the formula and not of a 32-bit exponential's last bit. Equal values go to the lower index.
 // With a bias the choice is first made in fp32 and its margins are compared with twice the fp32
-// error's bound; only rows with a margin inside it (about one in a thousand; rows with equal values)
-// are chosen again in 64 bits.
+// error's bound; only rows with a margin inside it (a few in a thousand; rows with equal values) are
+// settled in 64 bits.
 //
 // Balance loss of a sequence with T rows: L_s = E / (k T) sum_e cnt_e P_e, P_e = 1/T sum_t s'_te,
 // s' = s / sum_e s; L = alpha times the mean of L_s over the sequences that have rows.
@@ -228,31 +228,56 @@ struct Row {
   float l[V];  // canonical logits of the lane's experts, -inf past the last one
   int e0;      // the lane's first expert
 
-  __device__ __forceinline__ void load(const Args& a, int64_t t, int li) {
-    e0 = li * V;
-    const T* p = static_cast<const T*>(a.logits) + t * a.ld + e0;
-    if (a.wide) {  // E, the stride and the address are multiples of 4 elements
+  // A row's logits as they lie in memory, so that a row can be on its way while another is worked on
+  struct Raw {
+    static constexpr int kWords = V * sizeof(T) / 4;
+    uint32_t u[kWords];
+  };
+  // WIDE: E, the stride and the address are multiples of 4 elements. No branches: lanes past the last
+  // expert read it again (set() drops them), and a load that is not branched around is waited for only
+  // where its row is used.
+  template <bool WIDE>
+  static __device__ __forceinline__ Raw fetch(const Args& a, int64_t t, int li) {
+    Raw r;
+    const T* p = static_cast<const T*>(a.logits) + t * a.ld;
+    if constexpr (WIDE) {
 #pragma unroll
       for (int j = 0; j < V; j += 4) {
-        const bool in = e0 + j < a.experts;
+        const T* q = p + min(li * V + j, a.experts - 4);
         if constexpr (sizeof(T) == 4) {
-          const v4f q = in ? *reinterpret_cast<const v4f*>(p + j) : v4f{kLowest, kLowest, kLowest, kLowest};
+          const v4i x = *reinterpret_cast<const v4i*>(q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) l[j + i] = canon(q[i]);
+          for (int i = 0; i < 4; ++i) r.u[j + i] = x[i];
         } else {
-          const uint2 q = in ? *reinterpret_cast<const uint2*>(p + j) : uint2{0xff80ff80u, 0xff80ff80u};
-          l[j] = canon(__uint_as_float(q.x << 16));
-          l[j + 1] = canon(__uint_as_float(q.x & 0xffff0000u));
-          l[j + 2] = canon(__uint_as_float(q.y << 16));
-          l[j + 3] = canon(__uint_as_float(q.y & 0xffff0000u));
+          const uint2 x = *reinterpret_cast<const uint2*>(q);
+          r.u[j / 2] = x.x;
+          r.u[j / 2 + 1] = x.y;
         }
       }
-      return;
-    }
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) l[j] = e0 + j < a.experts ? canon(logit_f32(p + j)) : kLowest;
+      for (int j = 0; j < V; ++j) r.u[j] = __float_as_uint(p[min(li * V + j, a.experts - 1)]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j += 2)
+        r.u[j / 2] = p[min(li * V + j, a.experts - 1)] | uint32_t(p[min(li * V + j + 1, a.experts - 1)]) << 16;
+    }
+    return r;
   }
-  // The row's scores in fp32: s[j] (0 past the last expert), and their sum
+  __device__ __forceinline__ void set(const Args& a, const Raw& r, int li) {
+    e0 = li * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float v;
+      if constexpr (sizeof(T) == 4)
+        v = __uint_as_float(r.u[j]);
+      else
+        v = __uint_as_float(j & 1 ? r.u[j / 2] & 0xffff0000u : r.u[j / 2] << 16);
+      l[j] = e0 + j < a.experts ? canon(v) : kLowest;
+    }
+  }
+  // The row's scores in fp32: s[j] (0 past the last expert), and their sum. EXACT: to a few ulps, for choosing.
+  template <bool EXACT>
   __device__ __forceinline__ float scores(const Args& a, float (&s)[V]) const {
     float sum = 0.0f;
     if (a.scoring == AFD_SCORE_SOFTMAX) {
@@ -263,16 +288,20 @@ struct Row {
       const float at = m == kLowest ? 0.0f : m;  // a row of -inf: all scores 0
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        s[j] = exp_fast(l[j] - at);
+        s[j] = EXACT ? exp_f32(l[j] - at) : exp_fast(l[j] - at);
         sum += s[j];
       }
       return sum_f32<W>(sum);
     }
+    if (a.scoring == AFD_SCORE_SIGMOID) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      s[j] = score_fast(l[j], a.scoring);  // 0 of -inf, past the last expert
-      sum += s[j];
+      for (int j = 0; j < V; ++j) s[j] = EXACT ? score_f32(l[j], AFD_SCORE_SIGMOID) : score_fast(l[j], AFD_SCORE_SIGMOID);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] = EXACT ? score_f32(l[j], AFD_SCORE_SQRTSOFTPLUS) : score_fast(l[j], AFD_SCORE_SQRTSOFTPLUS);
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum += s[j];  // 0 of -inf, past the last expert
     return sum_f32<W>(sum);
   }
 };
@@ -299,6 +328,14 @@ __device__ __forceinline__ int first_lane(bool bit, int lane) {
 // kBare (fp32 logits, none): the places are sorted along, by adjacent exchanges (equals keep their order).
 enum KeyKind { kBare, kPlaced, kIndexed };
 
+// A bf16 logit's key with its low half free: the low half is 0 of a positive number and all ones of a
+// negative one or of the largest float (+inf), which rounds to the next key, unused by any other.
+__device__ __forceinline__ uint32_t index_key(uint32_t key) { return (key + 0x8000u) & 0xffff0000u; }
+__device__ __forceinline__ float index_value(uint32_t key) {
+  key &= 0xffff0000u;
+  return canon(value_of(key >> 31 ? key : key - 1));
+}
+
 template <int W, int V, KeyKind KIND>
 struct Keys {
   static constexpr bool kSorted = V == 4;
@@ -308,7 +345,7 @@ struct Keys {
   __device__ __forceinline__ void start(int e0) {
     if constexpr (KIND == kIndexed) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & 0xffff0000u) | (kMaxExperts - 1 - e0 - j) : 0u;
+      for (int j = 0; j < V; ++j) key[j] = key[j] ? index_key(key[j]) | (kMaxExperts - 1 - e0 - j) : 0u;
     } else if constexpr (KIND == kPlaced && kSorted) {
 #pragma unroll
       for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & ~3u) | (3 - j) : 0u;
@@ -563,21 +600,77 @@ __device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], i
   return kept;
 }
 
-// Selection of one row: lane kk < topk gets the kk-th expert. bias: the lane's experts' (BIAS);
-// s, sum: the row's scores (BIAS).
+// Close choice values in 64 bits. The fp32 choice is right but for experts within `margin` of each
+// other, so the chosen ones and every other within it of the last (taken on from `keys`) are ranked
+// by their 64-bit values, one a lane. False if they are more than the row's lanes.
+template <typename T, int W, int V>
+__device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint64_t* lds_row,
+                                       Keys<W, V, kPlaced>& keys, float margin, uint32_t taken, int& id) {
+  const int li = lane & (W - 1), e0 = li * V;
+  const float bar = value_of(__shfl(taken, a.topk - 1, W)) - margin;
+  int count = a.topk;
+  while (true) {
+    const uint32_t top = max_u32<W>(keys.head());
+    const bool more = top != 0 && !(value_of(top) < bar);
+    if (__ballot(more && count == W)) return false;
+    if (!__ballot(more)) break;
+    const Keys<W, V, kPlaced> before = keys;
+    uint32_t m;
+    const int e = keys.next(lane, e0, m);
+    if (!more) keys = before;  // another row of the wavefront goes on
+    if (more && li == count) id = e;
+    count += more ? 1 : 0;
+  }
+  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
+  double at = 0.0, sum = 1.0;
+  if (a.scoring == AFD_SCORE_SOFTMAX) {
+    float m = kLowest;
+#pragma unroll 1
+    for (int j = 0; j < V; ++j) m = fmaxf(m, e0 + j < a.experts ? canon(logit_f32(p + e0 + j)) : kLowest);
+    m = max_f32<W>(m);
+    at = m == kLowest ? 0.0 : static_cast<double>(m);
+    sum = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < V; ++j)
+      if (e0 + j < a.experts) sum += score_f64(canon(logit_f32(p + e0 + j)) - at, a.scoring);
+    sum = sum_f64<W>(sum);
+    if (sum == 0.0) sum = 1.0;
+  }
+  double c = score_f64(canon(logit_f32(p + (li < count ? id : 0))) - at, a.scoring);
+  if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
+  c += a.bias[li < count ? id : 0];
+  if (c != c) c = -__builtin_huge_val();
+  const uint64_t key = key64(c);
+  const uint32_t lo = static_cast<uint32_t>(key), hi = static_cast<uint32_t>(key >> 32);
+  int rank = 0;
+  const int most = W == 64 ? count : static_cast<int>(max_u32<64>(count));
+  for (int i = 0; i < most; ++i) {
+    const uint64_t other = uint64_t(__shfl(hi, i, W)) << 32 | __shfl(lo, i, W);
+    const int e = __shfl(id, i, W);
+    rank += i < count && (other > key || (other == key && e < id)) ? 1 : 0;
+  }
+  int* picks = reinterpret_cast<int*>(lds_row);
+  if (li < count && rank < a.topk) picks[rank] = id;
+  lds_fence();
+  id = li < a.topk ? picks[li] : 0;
+  lds_fence();
+  return true;
+}
+
+// Selection of one row: lane kk < topk gets the kk-th expert and its logit (`chosen`; -inf in other lanes).
+// bias: the lane's experts' (BIAS); s, sum: the row's scores (BIAS).
 template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, uint64_t* lds_row,
-                                      const float (&bias)[V], const float (&s)[V], float sum) {
+                                      const float (&bias)[V], const float (&s)[V], float sum, float& chosen) {
   const int li = lane & (W - 1), e0 = row.e0;
   float c[V], margin = 0.0f;
   bool sure = true;
   if constexpr (BIAS) {
-    // An fp32 choice value is off by less than 2^-18 (s + |bias|): the exponential by (|x| + 2) 2^-24 of
-    // itself, which is below 2^-22 of the score for every x (a score's slope falls as e^-|x|), the
-    // hardware's reciprocal, root and exponential by one ulp of 2^-23, the other steps by 2^-24, a
-    // softmax's sum over 16 values a lane and 6 butterflies by 22 of these, and the two bits that
-    // hold the place by 2^-21: together below 52 * 2^-24. Two values stand apart if they differ by
-    // twice the row's largest such bound.
+    // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal
+    // and root are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together,
+    // and the two bits that hold the place take 6; a softmax's sum over 16 values a lane and 6
+    // butterflies brings it to 40, so 2^-18 there. Two values stand apart if they differ by twice
+    // the row's largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
@@ -586,7 +679,7 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
       most = fmaxf(most, score + fabsf(bias[j]));
     }
-    margin = max_f32<W>(most) * 0x1p-17f;
+    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX ? 0x1p-17f : 0x1p-19f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
@@ -611,29 +704,38 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     uint32_t m;
     const int e = keys.next(lane, e0, m);
     id = li == kk ? e : id;
-    if constexpr (BIAS) taken = li == kk ? m : taken;
+    taken = li == kk ? m : taken;
   }
+  const bool live = li < a.topk;
+  bool all = __ballot(!sure) != 0;  // groups not settled (or not of whole lanes): the whole choice in 64 bits
   if constexpr (BIAS) {
-    // lane kk compares the kk-th with the next one, the last with the best that is left
-    const uint32_t left = max_u32<W>(keys.head());
-    const uint32_t after = __shfl_down(taken, 1, W);
-    const uint32_t below = li == a.topk - 1 ? left : after;
-    if (li < a.topk && below != 0 && !(value_of(taken) - value_of(below) > margin)) sure = false;
-    sure = row_bits<W>(__ballot(!sure), lane) == 0;
+    if (!all) {
+      // lane kk compares the kk-th with the next one, the last with the best that is left
+      const uint32_t left = max_u32<W>(keys.head());
+      const uint32_t after = __shfl_down(taken, 1, W);
+      const uint32_t below = li == a.topk - 1 ? left : after;
+      const bool close = live && below != 0 && !(value_of(taken) - value_of(below) > margin);
+      if (__ballot(close)) all = !settle<T, W, V>(a, t, lane, lds_row, keys, margin, taken, id);
+    }
   }
-  if (__ballot(!sure)) {
-    const int again = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
-    id = sure ? id : again;
+  if (all) id = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
+  if (all || BIAS) {
+    // the row's logits by way of LDS
+    float* mine = reinterpret_cast<float*>(lds_row);
+#pragma unroll
+    for (int j = 0; j < V; ++j) mine[e0 + j] = row.l[j];
+    lds_fence();
+    chosen = live ? mine[id] : kLowest;
+    lds_fence();
+  } else {
+    chosen = live ? sizeof(T) == 2 ? index_value(taken) : value_of(taken) : kLowest;  // the key is the logit
   }
   return id;
 }
 
-// The weight of lane kk's expert, from the chosen logits alone where nothing else is needed.
+// The weight of lane kk's expert, whose logit is l, from the chosen logits alone where nothing else is needed.
 template <typename T, int W, int V>
-__device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, int id) {
-  const int li = lane & (W - 1);
-  const bool live = li < a.topk;
-  const float l = live ? canon(logit_f32(static_cast<const T*>(a.logits) + t * a.ld + id)) : kLowest;
+__device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, float l) {
   float s;
   if (a.scoring == AFD_SCORE_SOFTMAX) {
     // renormalized, the largest chosen logit is the reference: the others' ratios to it survive
@@ -655,7 +757,7 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, i
     sum = sum_f32<W>(sum);
     return sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
   }
-  s = live ? score_f32(l, a.scoring) : 0.0f;
+  s = score_f32(l, a.scoring);
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
     s = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
@@ -666,32 +768,50 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, i
 template <int V>
 __device__ __forceinline__ void load_bias(const Args& a, int e0, float (&bias)[V]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) bias[j] = a.bias != nullptr && e0 + j < a.experts ? a.bias[e0 + j] : 0.0f;
+  for (int j = 0; j < V; ++j) {
+    const float b = a.bias != nullptr && e0 + j < a.experts ? a.bias[e0 + j] : 0.0f;
+    bias[j] = b != b ? kLowest : b;
+  }
 }
 
 // ---------------------------------------------------------------- selection
-template <typename T, int W, int V, bool BIAS>
-__global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
+template <typename T, int W, int V, bool BIAS, bool WIDE>
+__device__ __forceinline__ void topk_rows(const Args& a, uint64_t* lds) {
   constexpr int kRows = kThreads / W;  // rows in flight of a workgroup
-  __shared__ uint64_t lds[kRows * row_words(W, V)];
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   float bias[V];
   load_bias<V>(a, li * V, bias);
-  for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < a.n; r0 += int64_t(gridDim.x) * kRows) {
-    const int64_t r = r0 + sub;
-    const int64_t rr = r < a.n ? r : a.n - 1;  // the lanes of a wavefront stay together
-    Row<T, W, V> row;
-    row.load(a, rr, li);
-    float s[V] = {}, sum = 0.0f;
-    if constexpr (BIAS) sum = row.scores(a, s);
-    int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum);
-    float w = weigh(a, row, rr, lane, id);
+  using R = Row<T, W, V>;
+  const int64_t step = int64_t(gridDim.x) * kRows;
+  // the lanes of a wavefront stay together: rows past the end are the last one again
+  auto clamp_row = [&](int64_t r) { return r < a.n ? r : int64_t(a.n) - 1; };
+  int64_t r0 = int64_t(blockIdx.x) * kRows;
+  typename R::Raw next = R::template fetch<WIDE>(a, clamp_row(r0 + sub), li);
+  for (; r0 < a.n; r0 += step) {
+    const int64_t r = r0 + sub, rr = clamp_row(r);
+    const typename R::Raw raw = next;
+    next = R::template fetch<WIDE>(a, clamp_row(r + step), li);
+    R row;
+    row.set(a, raw, li);
+    float s[V] = {}, sum = 0.0f, l;
+    if constexpr (BIAS) sum = row.template scores<true>(a, s);
+    int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
+    float w = weigh(a, row, l);
     if (a.valid != nullptr && !a.valid[rr]) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
       a.ids[r * a.topk + li] = id;
       a.w[r * a.topk + li] = w;
     }
   }
+}
+
+template <typename T, int W, int V, bool BIAS>
+__global__ __launch_bounds__(kThreads) void topk_kernel(Args a) {
+  __shared__ uint64_t lds[kThreads / W * row_words(W, V)];
+  if (a.wide)
+    topk_rows<T, W, V, BIAS, true>(a, lds);
+  else
+    topk_rows<T, W, V, BIAS, false>(a, lds);
 }
 
 // ---------------------------------------------------------------- pieces of a block of rows
@@ -837,6 +957,54 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- selection, counts and balance sums
+// The rows of one piece: p, the lane's sums of s' over its rows; mine, their number; cnt, the counts (LDS).
+template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES, bool WIDE>
+__device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Piece& piece, const float (&bias)[V],
+                                             float (&p)[V], int& mine, int32_t* cnt, uint64_t* lds) {
+  constexpr int kRows = kBalanceThreads / W;
+  const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
+  const bool counted = piece.seq >= 0;
+  using R = Row<T, W, V>;
+  auto clamp_row = [&](int32_t r) { return min(r, piece.end - 1); };
+  typename R::Raw next = {};
+  if constexpr (SELECT || SCORES) next = R::template fetch<WIDE>(a, clamp_row(at + sub), li);
+  for (int32_t base = at; base < piece.end; base += kRows) {
+    const int32_t r = base + sub;
+    const bool in = r < piece.end;
+    const int32_t rr = in ? r : piece.end - 1;
+    const bool live = in && (a.valid == nullptr || a.valid[rr]);
+    R row;
+    float s[V] = {}, sum = 0.0f;
+    if constexpr (SELECT || SCORES) {
+      const typename R::Raw raw = next;
+      next = R::template fetch<WIDE>(a, clamp_row(r + kRows), li);
+      row.set(a, raw, li);
+    }
+    if constexpr (SCORES) sum = row.template scores<BIAS>(a, s);
+    if constexpr (SELECT) {
+      float l;
+      const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
+      const float w = weigh(a, row, l);
+      if (in && li < a.topk) {
+        a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
+        a.w[int64_t(r) * a.topk + li] = live ? w : 0.0f;
+        if (live && counted) atomicAdd(&cnt[id], 1);
+      }
+    } else if (live && counted) {
+      for (int kk = li; kk < a.topk; kk += W) {
+        const int id = a.ids[int64_t(r) * a.topk + kk];
+        if (id >= 0 && id < a.experts) atomicAdd(&cnt[id], 1);
+      }
+    }
+    if constexpr (SCORES) {
+      const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
+    }
+    mine += live ? 1 : 0;
+  }
+}
+
 // SELECT: choose the experts (else read a.ids). SCORES: sums of s' (else counts alone).
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES>
 __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
@@ -859,36 +1027,10 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
     __syncthreads();
     float p[V] = {};
     int mine = 0;
-    for (int32_t base = at; base < piece.end; base += kRows) {
-      const int32_t r = base + sub;
-      const bool in = r < piece.end;
-      const int32_t rr = in ? r : piece.end - 1;
-      const bool live = in && (a.valid == nullptr || a.valid[rr]);
-      Row<T, W, V> row;
-      float s[V] = {}, sum = 0.0f;
-      if constexpr (SELECT || SCORES) row.load(a, rr, li);
-      if constexpr (SCORES) sum = row.scores(a, s);
-      if constexpr (SELECT) {
-        const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum);
-        const float w = weigh(a, row, rr, lane, id);
-        if (in && li < a.topk) {
-          a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
-          a.w[int64_t(r) * a.topk + li] = live ? w : 0.0f;
-          if (live && counted) atomicAdd(&cnt[id], 1);
-        }
-      } else if (live && counted) {
-        for (int kk = li; kk < a.topk; kk += W) {
-          const int id = a.ids[int64_t(r) * a.topk + kk];
-          if (id >= 0 && id < a.experts) atomicAdd(&cnt[id], 1);
-        }
-      }
-      if constexpr (SCORES) {
-        const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
-      }
-      mine += live ? 1 : 0;
-    }
+    if (a.wide)
+      balance_rows<T, W, V, SELECT, BIAS, SCORES, true>(a, at, piece, bias, p, mine, cnt, lds);
+    else
+      balance_rows<T, W, V, SELECT, BIAS, SCORES, false>(a, at, piece, bias, p, mine, cnt, lds);
     if (counted) {
       if (li == 0) atomicAdd(&live_rows, mine);
       if constexpr (SCORES) {
@@ -923,11 +1065,10 @@ __device__ __forceinline__ void store_logit<float>(float* p, float v) { *p = v; 
 template <>
 __device__ __forceinline__ void store_logit<uint16_t>(uint16_t* p, float v) { *p = f32_to_bf16(v); }
 
-template <typename T, int W, int V>
-__global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
+template <typename T, int W, int V, bool WIDE>
+__device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
   constexpr int kRows = kThreads / W;
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
-  __shared__ __attribute__((aligned(16))) float spread[kRows * W * V];
   const float gloss = a.coef != nullptr ? *a.gloss : 0.0f;
   const int32_t r0 = blockIdx.x * a.block_rows;
   const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
@@ -942,15 +1083,20 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
       for (int j = 0; j < V; ++j)
         if (li * V + j < a.experts) c[j] = f * a.counts[int64_t(piece.seq) * a.experts + li * V + j];
     }
+    using R = Row<T, W, V>;
+    auto clamp_row = [&](int32_t r) { return min(r, piece.end - 1); };
+    typename R::Raw next = R::template fetch<WIDE>(a, clamp_row(at + sub), li);
     for (int32_t base = at; base < piece.end; base += kRows) {
       const int32_t r = base + sub;
       const bool in = r < piece.end;
-      const int32_t rr = in ? r : piece.end - 1;
+      const int32_t rr = clamp_row(r);
       const bool live = a.valid == nullptr || a.valid[rr];
-      Row<T, W, V> row;
-      row.load(a, rr, li);
+      R row;
+      const typename R::Raw raw = next;
+      next = R::template fetch<WIDE>(a, clamp_row(r + kRows), li);
+      row.set(a, raw, li);
       float s[V], d[V];
-      const float total = row.scores(a, s);
+      const float total = row.template scores<false>(a, s);
       const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) d[j] = 0.0f;
@@ -1009,7 +1155,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
         T* out = static_cast<T*>(a.dlogits) + int64_t(r) * a.experts + row.e0;
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] = live ? d[j] * slope_f32(row.l[j], s[j], a.scoring) : 0.0f;
-        if (a.wide) {
+        if constexpr (WIDE) {
 #pragma unroll
           for (int j = 0; j < V; j += 4) {
             if (row.e0 + j >= a.experts) continue;
@@ -1027,6 +1173,15 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
     }
     at = piece.end;
   }
+}
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(kThreads) void grad_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) float spread[kThreads * V];
+  if (a.wide)
+    grad_rows<T, W, V, true>(a, spread);
+  else
+    grad_rows<T, W, V, false>(a, spread);
 }
 
 // ---------------------------------------------------------------- host
@@ -1197,7 +1352,7 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
       router::set_shape(a, W, V, sizeof(T));
       int64_t grid = (int64_t(n) + kRows - 1) / kRows;
-      if (grid > int64_t(16) * device_cu_count()) grid = int64_t(16) * device_cu_count();
+      if (grid > int64_t(4) * device_cu_count()) grid = int64_t(4) * device_cu_count();
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(router::kThreads), 0,
                            static_cast<hipStream_t>(stream), a);

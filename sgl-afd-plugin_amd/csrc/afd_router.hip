@@ -768,8 +768,8 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, f
 template <int V>
 __device__ __forceinline__ void load_bias(const Args& a, int e0, float (&bias)[V]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float b = a.bias != nullptr && e0 + j < a.experts ? a.bias[e0 + j] : 0.0f;
+  for (int j = 0; j < V; ++j) {  // no branches: the loads travel together
+    const float b = a.bias != nullptr ? a.bias[min(e0 + j, a.experts - 1)] : 0.0f;
     bias[j] = b != b ? kLowest : b;
   }
 }
@@ -791,13 +791,14 @@ __device__ __forceinline__ void topk_rows(const Args& a, uint64_t* lds) {
     const int64_t r = r0 + sub, rr = clamp_row(r);
     const typename R::Raw raw = next;
     next = R::template fetch<WIDE>(a, clamp_row(r + step), li);
+    const bool valid = a.valid == nullptr || a.valid[rr] != 0;
     R row;
     row.set(a, raw, li);
     float s[V] = {}, sum = 0.0f, l;
     if constexpr (BIAS) sum = row.template scores<true>(a, s);
     int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
     float w = weigh(a, row, l);
-    if (a.valid != nullptr && !a.valid[rr]) id = -1, w = 0.0f;
+    if (!valid) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
       a.ids[r * a.topk + li] = id;
       a.w[r * a.topk + li] = w;
@@ -1079,22 +1080,40 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
     float c[V] = {};
     if (balanced) {
       const float f = gloss * a.coef[piece.seq];
+      int32_t cnt[V];
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (li * V + j < a.experts) c[j] = f * a.counts[int64_t(piece.seq) * a.experts + li * V + j];
+        cnt[j] = a.counts[int64_t(piece.seq) * a.experts + min(li * V + j, a.experts - 1)];
+#pragma unroll
+      for (int j = 0; j < V; ++j) c[j] = f * cnt[j];
     }
     using R = Row<T, W, V>;
     auto clamp_row = [&](int32_t r) { return min(r, piece.end - 1); };
-    typename R::Raw next = R::template fetch<WIDE>(a, clamp_row(at + sub), li);
+    // what a row needs is fetched a row ahead
+    struct Ahead {
+      typename R::Raw raw;
+      int id;
+      float gw;
+      bool live;
+    };
+    const int pick = min(li, a.topk - 1);
+    auto fetch = [&](int32_t r) {
+      Ahead x;
+      x.raw = R::template fetch<WIDE>(a, r, li);
+      x.id = a.gw != nullptr ? a.ids[int64_t(r) * a.topk + pick] : -1;
+      x.gw = a.gw != nullptr ? a.gw[int64_t(r) * a.topk + pick] : 0.0f;
+      x.live = a.valid == nullptr || a.valid[r] != 0;
+      return x;
+    };
+    Ahead next = fetch(clamp_row(at + sub));
     for (int32_t base = at; base < piece.end; base += kRows) {
       const int32_t r = base + sub;
       const bool in = r < piece.end;
-      const int32_t rr = clamp_row(r);
-      const bool live = a.valid == nullptr || a.valid[rr];
+      const Ahead now = next;
+      next = fetch(clamp_row(r + kRows));
+      const bool live = now.live;
       R row;
-      const typename R::Raw raw = next;
-      next = R::template fetch<WIDE>(a, clamp_row(r + kRows), li);
-      row.set(a, raw, li);
+      row.set(a, now.raw, li);
       float s[V], d[V];
       const float total = row.template scores<false>(a, s);
       const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
@@ -1110,11 +1129,14 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
       }
       if (a.gw != nullptr) {
         // lane kk < topk: the kk-th chosen expert's share of the weights' scores, and its gradient
-        const T* p = static_cast<const T*>(a.logits) + int64_t(rr) * a.ld;
-        int id = li < a.topk ? a.ids[int64_t(rr) * a.topk + li] : -1;
-        if (id >= a.experts) id = -1;
-        const float g = id >= 0 ? a.gw[int64_t(rr) * a.topk + li] * a.scale : 0.0f;
-        const float l = id >= 0 ? canon(logit_f32(p + id)) : kLowest;
+        const int id = li < a.topk && static_cast<uint32_t>(now.id) < static_cast<uint32_t>(a.experts) ? now.id : -1;
+        const float g = id >= 0 ? now.gw * a.scale : 0.0f;
+        float* mine = spread + sub * (W * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) mine[row.e0 + j] = row.l[j];
+        lds_fence();
+        const float l = id >= 0 ? mine[id] : kLowest;
+        lds_fence();
         // share: of the chosen (renormalized) or of all (softmax), or the score itself
         float share;
         if (a.scoring == AFD_SCORE_SOFTMAX) {
@@ -1138,14 +1160,14 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
         if (a.renorm || a.scoring == AFD_SCORE_SOFTMAX) mean = sum_f32<W>(g * share);
         const float u = share * (g - (a.renorm ? mean : 0.0f));
         // to the lanes that hold the experts, through LDS (an id that comes twice is added up)
-        float* mine = spread + sub * (W * V) + row.e0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) mine[j] = 0.0f;
+        for (int j = 0; j < V; ++j) mine[row.e0 + j] = 0.0f;
         lds_fence();
-        if (id >= 0) atomicAdd(spread + sub * (W * V) + id, u);
+        if (id >= 0) atomicAdd(mine + id, u);
         lds_fence();
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] += mine[j];
+        for (int j = 0; j < V; ++j) d[j] += mine[row.e0 + j];
+        lds_fence();
         if (!a.renorm && a.scoring == AFD_SCORE_SOFTMAX) {
 #pragma unroll
           for (int j = 0; j < V; ++j) d[j] -= s[j] * inv * mean;

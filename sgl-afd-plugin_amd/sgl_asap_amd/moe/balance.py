@@ -21,10 +21,9 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .topk import StandardTopKOutput, choice_cfg, launch, logit_rows, need_gpu, on_device, router_cfg, router_grad
+from .topk import StandardTopKOutput, choice_cfg, launch, logit_rows, need_gpu, on_device, once, router_cfg, router_grad
 
 
 @lru_cache(maxsize=1024)
@@ -106,8 +105,11 @@ class _Balance(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
+        return once(_Balance._backward, ctx, *grads)
+
+    @staticmethod
+    def _backward(ctx, *grads):
         logits, ids, cu, valid, counts, coef = ctx.saved_tensors
         gw, gloss = (grads[0], grads[2]) if ids is not None else (None, grads[0])
         grad = None

@@ -144,6 +144,15 @@ def router_grad(cfg, logits, ids, valid, gw, cu=None, counts=None, coef=None, gl
     return out
 
 
+_once_differentiable = once_differentiable(lambda ctx, run, *grads: run(ctx, *grads))
+
+
+def once(run, ctx, *grads):
+    """``run(ctx, *grads)``, a backward without a backward of its own. Torch's guard against a second
+    derivative costs as much host time as a launch, so it is put up only where one could be asked for."""
+    return _once_differentiable(ctx, run, *grads) if torch.is_grad_enabled() else run(ctx, *grads)
+
+
 class _Select(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, cfg, top_k, bias, valid):
@@ -155,8 +164,11 @@ class _Select(torch.autograd.Function):
         return weights, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gw, _):
+        return once(_Select._backward, ctx, gw)
+
+    @staticmethod
+    def _backward(ctx, gw):
         if gw is None:
             return None, None, None, None, None
         logits, ids, valid = ctx.saved_tensors

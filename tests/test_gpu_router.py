@@ -358,3 +358,25 @@ def test_more_logits_than_32_bits_count():
     share = sum(torch.softmax(p.double(), 1).sum(0) for p in logits.split(1_000_000))
     want = experts / (top_k * n * n) * float((share * cnt.double()).sum())
     assert abs(float(loss) - want) <= 2.0**-12 * want  # blocks of 1024 rows: 256 fp32 sums in a row each
+
+
+@pytest.mark.parametrize("which", ["select", "balance", "both"])
+def test_no_second_derivative(which):
+    """create_graph gives the gradient and an error where it is differentiated again."""
+    logits, _ = make(4, 16, 50)
+    leaf = logits.to(dev()).requires_grad_()
+    say(f"second derivative {which}")
+
+    def value(x):
+        if which == "select":
+            return (T.select_experts(x, 3).topk_weights ** 2).sum()
+        if which == "balance":
+            return B.balance_loss(x, torch.zeros(4, 3, dtype=torch.int32, device=dev()), alpha=1.0)[0]
+        out, loss, _ = B.select_and_balance(x, 3, alpha=1.0)
+        return (out.topk_weights ** 2).sum() + loss
+
+    (plain,) = torch.autograd.grad(value(leaf), leaf)
+    (graph,) = torch.autograd.grad(value(leaf), leaf, create_graph=True)
+    assert torch.equal(plain, graph.detach())
+    with pytest.raises(RuntimeError):
+        graph.sum().backward()

@@ -168,35 +168,38 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p) {
 }
 
 // ---------------------------------------------------------------- tiles
-// BM rows of x by BN outputs, WM x WN wavefronts of TI x TJ MFMA tiles of 32x32 each. A stage is one K
-// block of both operands and the rows' scales, copied HBM -> LDS in pieces, S stages in a ring, one
-// barrier a stage: at stage b a wavefront has waited for its own copies of it, the barrier says that
-// all have and that nobody reads stage b - 1 any more, whose slot then takes stage b + S - 1.
-template <int BM_, int BN_, int WM_, int WN_, int S_>
+// BM rows of x by BN outputs, WM x WN wavefronts of TI x TJ MFMA tiles of 16x16 each (K 128 in one
+// instruction, so a block's sum is one MFMA from 0 and its 4 values a lane are folded at once). A stage
+// is one K block of both operands and the rows' scales, copied HBM -> LDS in 1 KiB pieces into two slots.
+//
+// A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments,
+// read two ahead. When the last two are in registers (all of its reads of the stage done) it waits for
+// its copies of the next stage and meets the others at the stage's one barrier: the next stage
+// is there for all, and this one's slot is free for the copies of the stage after. The MFMAs of the
+// last two weight fragments run while the next stage's first fragments are read.
+template <int BM_, int BN_, int WM_, int WN_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int TI = BM / WM / 32, TJ = BN / WN / 32;
+  static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
   static constexpr int kAPieces = BM / 16 * 2, kBPieces = BN / 16 * 2;
   static constexpr int kAQ = kAPieces / kWaves, kBQ = kBPieces / kWaves;
   static constexpr int kBOff = kAPieces * kPiece, kSOff = kBOff + kBPieces * kPiece;
   static constexpr int kStage = kSOff + BM * 4;
-  static constexpr int kYBytes = BM * BN * 2;
-  static constexpr int kLds = S * kStage > kYBytes ? S * kStage : kYBytes;
+  static constexpr int kLds = 2 * kStage;
   static constexpr int kScaleWaves = BM / 64;  // each copies 64 rows' scales
-  static_assert(TI * 32 * WM == BM && TJ * 32 * WN == BN && kAQ * kWaves == kAPieces && kBQ * kWaves == kBPieces, "tile");
-  static_assert(BN / WN <= 128 && 128 % (BN / WN) == 0, "one weight scale per wavefront and K block");
+  static_assert(TI * 16 * WM == BM && TJ * 16 * WN == BN && kAQ * kWaves == kAPieces && kBQ * kWaves == kBPieces, "tile");
+  static_assert(TJ % 4 == 0 && BN / WN <= 128 && 128 % (BN / WN) == 0, "one weight scale per wavefront and K block");
   static_assert(kScaleWaves <= kWaves && BM <= kScaleRows && kLds <= 160 * 1024, "LDS");
-  static_assert((S - 1) * (kAQ + kBQ + 1) < 64, "vmcnt is a 6-bit counter");
 };
 
 template <typename T>
 __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
-  constexpr int TI = T::TI, TJ = T::TJ, S = T::S;
+  constexpr int TI = T::TI, TJ = T::TJ;
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wm = w / T::WN, wn = w % T::WN, lr = lane & 31, lk = lane >> 5;
+  const int wm = w / T::WN, wn = w % T::WN;
   const int mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
   // workgroup b runs on XCD b % 8: an XCD takes whole rows of tiles where there are many (each reads
   // all the weights, x is read once), else whole columns (the weights are read by one XCD's L2)
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
     }
     if (mt >= mts || nt >= nts) return;
   }
-  const int kt = 2 * p.kb;
+  const int kt = 2 * p.kb, last = p.kb - 1;
   const int m0 = mt * T::BM, n0 = nt * T::BN;
   const int r16_last = (p.n + 15) / 16 - 1, o16_last = (p.n_out + 15) / 16 - 1;
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_offset(lds));
@@ -220,109 +223,125 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 
   // this wavefront's pieces of a stage: piece q of an operand is row group q / 2, 64-column half q % 2.
   // Row groups past the end re-read the last one; their results are not stored.
+  const uint8_t* a_src[T::kAQ];
+  const uint8_t* b_src[T::kBQ];
+#pragma unroll
+  for (int i = 0; i < T::kAQ; ++i) {
+    const int q = w * T::kAQ + i;
+    a_src[i] = p.a + (int64_t(min(m0 / 16 + q / 2, r16_last)) * kt + q % 2) * kPiece;
+  }
+#pragma unroll
+  for (int i = 0; i < T::kBQ; ++i) {
+    const int q = w * T::kBQ + i;
+    b_src[i] = p.b + (int64_t(min(n0 / 16 + q / 2, o16_last)) * kt + q % 2) * kPiece;
+  }
   auto issue = [&](int b) {
-    const uint32_t st = lds_base + static_cast<uint32_t>((b % S) * T::kStage);
+    const uint32_t st = lds_base + static_cast<uint32_t>((b & 1) * T::kStage);
     if (w < T::kScaleWaves)
       lds_dma4(st + T::kSOff + w * 256, p.as + int64_t(b) * p.a_rows + m0 + 64 * w, lane * 4u);
-    static_for<T::kAQ>([&](auto qc) {
-      const int q = w * T::kAQ + decltype(qc)::value;
-      const int r16 = min(m0 / 16 + q / 2, r16_last);
-      lds_dma16(st + q * kPiece, p.a + (int64_t(r16) * kt + 2 * b + q % 2) * kPiece, voff);
-    });
-    static_for<T::kBQ>([&](auto qc) {
-      const int q = w * T::kBQ + decltype(qc)::value;
-      const int o16 = min(n0 / 16 + q / 2, o16_last);
-      lds_dma16(st + T::kBOff + q * kPiece, p.b + (int64_t(o16) * kt + 2 * b + q % 2) * kPiece, voff);
-    });
+#pragma unroll
+    for (int i = 0; i < T::kAQ; ++i)
+      lds_dma16(st + (w * T::kAQ + i) * kPiece, a_src[i] + int64_t(b) * 2 * kPiece, voff);
+#pragma unroll
+    for (int i = 0; i < T::kBQ; ++i)
+      lds_dma16(st + T::kBOff + (w * T::kBQ + i) * kPiece, b_src[i] + int64_t(b) * 2 * kPiece, voff);
   };
 
-  v16f acc[TI][TJ];
+  v4f acc[TI][TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+    for (int j = 0; j < TJ; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int sw_row = min((n0 + wn * (T::BN / T::WN)) / 128, (p.n_out - 1) / 128);
   const float* sw = p.bs + int64_t(sw_row) * p.kb;
-  const int last = p.kb - 1;
-  // a fragment: rows r, 16-byte chunks lk and lk + 2 of a 64-column half
-  const int frag = (lr >> 4) * 2 * kPiece + (lr & 15) * 16 + lk * 256;
-  static_for<S - 1>([&](auto sc) { issue(min(static_cast<int>(decltype(sc)::value), last)); });
-  for (int b = 0; b <= last; ++b) {
-    wait_vmcnt<(S - 2) * (T::kAQ + T::kBQ)>();
-    __syncthreads();
-    issue(min(b + S - 1, last));
-    const uint8_t* st = lds + (b % S) * T::kStage;
-    const float s_w = load_uniform(sw + b);
-    float s[TI];
-    v8i fa[TI][2];
-#pragma unroll
-    for (int i = 0; i < TI; ++i) {
-      s[i] = reinterpret_cast<const float*>(st + T::kSOff)[wm * TI * 32 + i * 32 + lr] * s_w;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* f = st + (wm * TI * 2 + i * 2) * 2 * kPiece + h * kPiece + frag;
-        fa[i][h] = join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + 512));
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      v8i fb[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* f = st + T::kBOff + (wn * TJ * 2 + j * 2) * 2 * kPiece + h * kPiece + frag;
-        fb[h] = join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + 512));
-      }
-#pragma unroll
-      for (int i = 0; i < TI; ++i) {
-        v16f sum = {};
-        sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[0], fa[i][0], sum, 0, 0, 0, 127, 0, 127);
-        sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[1], fa[i][1], sum, 0, 0, 0, 127, 0, 127);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(sum[q], s[i], acc[i][j][q]);
-      }
-    }
-  }
+  float sw64 = 0.0f;  // lane l: the weight scale of K block 64 c + l
+  const uint8_t* a_lds = lds + wm * TI * 2 * kPiece + lane * 16;
+  const uint8_t* b_lds = lds + T::kBOff + wn * TJ * 2 * kPiece + lane * 16;
+  const uint8_t* s_lds = lds + T::kSOff + (wm * TI * 16 + (lane & 15)) * 4;
+  v8i fa[TI], fb[4];
+  float sx[TI];
+  auto read = [&](const uint8_t* f) {
+    return join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + kPiece));
+  };
+  auto read_a = [&](int b, int i) {
+    fa[i] = read(a_lds + (b & 1) * T::kStage + i * 2 * kPiece);
+    sx[i] = *reinterpret_cast<const float*>(s_lds + (b & 1) * T::kStage + i * 64);
+  };
+  auto read_b = [&](int b, int j) { return read(b_lds + (b & 1) * T::kStage + j * 2 * kPiece); };
+
+  sw64 = sw[min(lane, last)];
+  issue(0);
   wait_vmcnt<0>();
   __syncthreads();
+  issue(min(1, last));
+#pragma unroll
+  for (int i = 0; i < TI; ++i) read_a(0, i);
+  fb[0] = read_b(0, 0);
+  fb[1] = read_b(0, 1);
+  for (int b = 0; b <= last; ++b) {
+    if (b != 0 && (b & 63) == 0) sw64 = sw[min(b + lane, last)];
+    const float s_w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sw64), b & 63));
+    float s[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) s[i] = sx[i] * s_w;
+    static_for<TJ>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      if constexpr (j == TJ - 2) {
+        wait_vmcnt_lds<0>();
+        __syncthreads();
+        issue(min(b + 2, last));  // past the end: the last stage over itself, the same bytes
+      }
+      if constexpr (j < TJ - 2)
+        fb[(j + 2) % 4] = read_b(b, j + 2);
+      else
+        fb[(j + 2) % 4] = read_b(b + 1, j + 2 - TJ);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fb[j % 4], fa[i], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0 /*e4m3*/, 0 /*e4m3*/, 0, 127 /*x1*/, 0, 127 /*x1*/);
+        if constexpr (j == TJ - 1) read_a(b + 1, i);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(sum[q], s[i], acc[i][j][q]);
+      }
+    });
+  }
+  wait_vmcnt<0>();
 
-  // bf16 rows through LDS (16-byte chunk c of row r at c ^ (r % 16)), so the stores write whole rows
-  constexpr int kChunks = T::BN / 8;
-  auto y_at = [](int r, int c) { return (r * kChunks + (c ^ (r & 15))) * 16; };
+  // lane l holds, of row l % 16 of an activation tile, outputs 4 (l / 16) .. + 3 of each weight tile. Two
+  // neighbouring weight tiles trade halves so that a lane holds 8 outputs: lane groups 0 and 2 those of tile
+  // j, 1 and 3 of tile j + 1, 64 contiguous bytes of a row from its four lanes.
+  const int lg = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < TI; ++i)
+  for (int i = 0; i < TI; ++i) {
+    const int row = m0 + (wm * TI + i) * 16 + (lane & 15);
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      v4i chunk[2];
-      bf16_chunks(acc[i][j], chunk);
-      const int row = wm * TI * 32 + i * 32 + lr;
+    for (int j = 0; j < TJ; j += 2) {
+      const uint32_t x0 = pk_bf16(acc[i][j][0], acc[i][j][1]), x1 = pk_bf16(acc[i][j][2], acc[i][j][3]);
+      const uint32_t y0 = pk_bf16(acc[i][j + 1][0], acc[i][j + 1][1]);
+      const uint32_t y1 = pk_bf16(acc[i][j + 1][2], acc[i][j + 1][3]);
+      const auto d0 = __builtin_amdgcn_permlane16_swap(x0, y0, false, false);
+      const auto d1 = __builtin_amdgcn_permlane16_swap(x1, y1, false, false);
+      const v4i chunk = {static_cast<int>(d0[0]), static_cast<int>(d1[0]), static_cast<int>(d0[1]),
+                         static_cast<int>(d1[1])};
+      const int o = n0 + (wn * TJ + j + (lg & 1)) * 16 + (lg >> 1) * 8;
+      if (row >= p.n) continue;
+      uint16_t* out = p.y + row * p.ldy + o;
+      if (p.wide && o + 8 <= p.n_out) {
+        *reinterpret_cast<v4i*>(out) = chunk;
+      } else {
 #pragma unroll
-      for (int pr = 0; pr < 2; ++pr)
-        *reinterpret_cast<v4i*>(lds + y_at(row, (wn * TJ * 32 + j * 32) / 8 + 2 * pr + lk)) = chunk[pr];
-    }
-  __syncthreads();
-  for (int at = t; at < T::BM * kChunks; at += T::kThreads) {
-    const int r = at / kChunks, c = at % kChunks;
-    const int row = m0 + r, o = n0 + c * 8;
-    if (row >= p.n || o >= p.n_out) continue;
-    const v4i chunk = *reinterpret_cast<const v4i*>(lds + y_at(r, c));
-    uint16_t* out = p.y + row * p.ldy + o;
-    if (p.wide && o + 8 <= p.n_out) {
-      *reinterpret_cast<v4i*>(out) = chunk;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (o + i < p.n_out)
-          out[i] = static_cast<uint16_t>(static_cast<uint32_t>(chunk[i / 2]) >> (16 * (i % 2)));
+        for (int q = 0; q < 8; ++q)
+          if (o + q < p.n_out)
+            out[q] = static_cast<uint16_t>(static_cast<uint32_t>(chunk[q / 2]) >> (16 * (q % 2)));
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------- host
-using Large = Shape<256, 256, 4, 2, 2>;
-using Mid = Shape<128, 128, 2, 2, 2>;
+using Large = Shape<256, 256, 4, 2>;
+using Mid = Shape<128, 128, 2, 2>;
 
 struct Plan {
   int kb, a_rows;

@@ -173,7 +173,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p) {
 // is one K block of both operands and the rows' scales, copied HBM -> LDS in 1 KiB pieces into two slots.
 //
 // A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments,
-// read two ahead. When the last two are in registers (all of its reads of the stage done) it waits for
+// read two ahead, in an order kept as written (left alone, the compiler reads all of a stage first and then
+// waits out every MFMA in turn: 322 us for 16384 x 4096 x 4096). When the last two are in registers (all of its reads of the stage done) it waits for
 // its copies of the next stage and meets the others at the stage's one barrier: the next stage
 // is there for all, and this one's slot is free for the copies of the stage after. The MFMAs of the
 // last two weight fragments run while the next stage's first fragments are read.
@@ -193,6 +194,36 @@ struct Shape {
   static_assert(kScaleWaves <= kWaves && BM <= kScaleRows && kLds <= 160 * 1024, "LDS");
 };
 
+// Workgroup b runs on XCD b % 8, each with its own L2. Where there are many row tiles an XCD takes a
+// contiguous eighth of them with all the columns, so that x is read by one L2 and the weights by all; else an eighth
+// of the columns with all the rows. Inside, 8 tiles of the long side at a time, the other side
+// running behind it: the 32 workgroups of an XCD work on about 8 x 4 tiles and share their operands 4 and 8 ways.
+constexpr int kSplitRows = 16;
+struct TileAt {
+  int mt, nt;
+};
+__host__ __device__ inline TileAt tile_at(unsigned block, int mts, int nts) {
+  const bool rows = mts >= kSplitRows;
+  const int major = rows ? mts : nts, minor = rows ? nts : mts;
+  const int xcd = block & 7, lo = static_cast<int>(int64_t(major) * xcd / 8);
+  const int here = static_cast<int>(int64_t(major) * (xcd + 1) / 8) - lo;
+  const int64_t i = block >> 3;
+  if (i >= int64_t(here) * minor) return {-1, -1};
+  const int full = here / 8;
+  int rb = static_cast<int>(i / (8 * minor)), wide = 8;
+  if (rb >= full) {
+    rb = full;
+    wide = here - 8 * full;
+  }
+  const int j = static_cast<int>(i - int64_t(rb) * 8 * minor);
+  const int a = lo + rb * 8 + j % wide, b = j / wide;
+  return rows ? TileAt{a, b} : TileAt{b, a};
+}
+// workgroups that cover every tile
+inline int64_t tile_grid(int64_t mts, int64_t nts) {
+  return mts >= kSplitRows ? round_up(mts, 8) * nts : round_up(nts, 8) * mts;
+}
+
 template <typename T>
 __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   constexpr int TI = T::TI, TJ = T::TJ;
@@ -201,20 +232,10 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = w / T::WN, wn = w % T::WN;
   const int mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
-  // workgroup b runs on XCD b % 8: an XCD takes whole rows of tiles where there are many (each reads
-  // all the weights, x is read once), else whole columns (the weights are read by one XCD's L2)
-  int mt, nt;
-  {
-    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
-    if (mts >= 16) {
-      mt = j / nts * 8 + xcd;
-      nt = j % nts;
-    } else {
-      nt = j / mts * 8 + xcd;
-      mt = j % mts;
-    }
-    if (mt >= mts || nt >= nts) return;
-  }
+  const TileAt at = tile_at(blockIdx.x, mts, nts);
+  if (at.mt < 0) return;
+  // (the divisions run in vector registers; what follows from the tile is scalar)
+  const int mt = __builtin_amdgcn_readfirstlane(at.mt), nt = __builtin_amdgcn_readfirstlane(at.nt);
   const int kt = 2 * p.kb, last = p.kb - 1;
   const int m0 = mt * T::BM, n0 = nt * T::BN;
   const int r16_last = (p.n + 15) / 16 - 1, o16_last = (p.n_out + 15) / 16 - 1;
@@ -235,17 +256,24 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
     const int q = w * T::kBQ + i;
     b_src[i] = p.b + (int64_t(min(n0 / 16 + q / 2, o16_last)) * kt + q % 2) * kPiece;
   }
-  auto issue = [&](int b) {
+  // copy number c of a stage: the scales, then the activation pieces, then the weight pieces
+  constexpr int kCopies = 1 + T::kAQ + T::kBQ;
+  const int ws = w % T::kScaleWaves;
+  auto copy = [&](int b, auto c_c) {
+    constexpr int c = decltype(c_c)::value;
     const uint32_t st = lds_base + static_cast<uint32_t>((b & 1) * T::kStage);
-    if (w < T::kScaleWaves)
-      lds_dma4(st + T::kSOff + w * 256, p.as + int64_t(b) * p.a_rows + m0 + 64 * w, lane * 4u);
-#pragma unroll
-    for (int i = 0; i < T::kAQ; ++i)
-      lds_dma16(st + (w * T::kAQ + i) * kPiece, a_src[i] + int64_t(b) * 2 * kPiece, voff);
-#pragma unroll
-    for (int i = 0; i < T::kBQ; ++i)
-      lds_dma16(st + T::kBOff + (w * T::kBQ + i) * kPiece, b_src[i] + int64_t(b) * 2 * kPiece, voff);
+    const uint32_t off = voff + static_cast<uint32_t>(b) * (2 * kPiece);
+    if constexpr (c == 0) {
+      // (every wavefront: two may write the same bytes, and the steps stay one block of code)
+      lds_dma4(st + T::kSOff + ws * 256, p.as + int64_t(b) * p.a_rows + m0 + 64 * ws, lane * 4u);
+    } else if constexpr (c <= T::kAQ) {
+      lds_dma16(st + (w * T::kAQ + c - 1) * kPiece, a_src[c - 1], off);
+    } else {
+      constexpr int i = c - 1 - T::kAQ;
+      lds_dma16(st + T::kBOff + (w * T::kBQ + i) * kPiece, b_src[i], off);
+    }
   };
+  auto issue = [&](int b) { static_for<kCopies>([&](auto c) { copy(b, c); }); };
 
   v4f acc[TI][TJ];
 #pragma unroll
@@ -255,12 +283,12 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 
   const int sw_row = min((n0 + wn * (T::BN / T::WN)) / 128, (p.n_out - 1) / 128);
   const float* sw = p.bs + int64_t(sw_row) * p.kb;
-  float sw64 = 0.0f;  // lane l: the weight scale of K block 64 c + l
+  float s_w = load_uniform(sw);  // of the stage; the next one's is read where no LDS read is in flight
   const uint8_t* a_lds = lds + wm * TI * 2 * kPiece + lane * 16;
   const uint8_t* b_lds = lds + T::kBOff + wn * TJ * 2 * kPiece + lane * 16;
   const uint8_t* s_lds = lds + T::kSOff + (wm * TI * 16 + (lane & 15)) * 4;
   v8i fa[TI], fb[4];
-  float sx[TI];
+  float sx[TI], s[TI];
   auto read = [&](const uint8_t* f) {
     return join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + kPiece));
   };
@@ -270,7 +298,21 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   };
   auto read_b = [&](int b, int j) { return read(b_lds + (b & 1) * T::kStage + j * 2 * kPiece); };
 
-  sw64 = sw[min(lane, last)];
+  // An MFMA's result is folded kLate steps after it was issued (its latency is one step of its own and
+  // one of the other wavefront's); the last ones of a stage in the next stage's first steps.
+  constexpr int kSteps = TI * TJ, kLate = 3, kSums = 4;
+  static_assert(kSteps % kSums == 0 && kLate < kSums, "a sum is folded before its registers take another");
+  v4f sum[kSums];
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) sum[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < TI; ++i) s[i] = 0.0f;
+  auto fold = [&](auto m_c) {
+    constexpr int m = decltype(m_c)::value, i = m % TI, j = m / TI;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(sum[m % kSums][q], s[i], acc[i][j][q]);
+  };
+
   issue(0);
   wait_vmcnt<0>();
   __syncthreads();
@@ -280,32 +322,41 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   fb[0] = read_b(0, 0);
   fb[1] = read_b(0, 1);
   for (int b = 0; b <= last; ++b) {
-    if (b != 0 && (b & 63) == 0) sw64 = sw[min(b + lane, last)];
-    const float s_w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sw64), b & 63));
-    float s[TI];
-#pragma unroll
-    for (int i = 0; i < TI; ++i) s[i] = sx[i] * s_w;
-    static_for<TJ>([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      if constexpr (j == TJ - 2) {
+    const int ahead = min(b + 2, last);  // past the end: the last stage over itself, the same bytes
+    static_for<kSteps>([&](auto mc) {
+      constexpr int m = decltype(mc)::value, i = m % TI, j = m / TI;
+      constexpr int kFree = (TJ - 2) * TI;  // the first step at which the stage's slot is free
+      if constexpr (m == kFree) {
         wait_vmcnt_lds<0>();
         __syncthreads();
-        issue(min(b + 2, last));  // past the end: the last stage over itself, the same bytes
+        s_w = load_uniform(sw + min(b + 1, last));
       }
-      if constexpr (j < TJ - 2)
-        fb[(j + 2) % 4] = read_b(b, j + 2);
+      if constexpr (i == 0) {
+        if constexpr (j < TJ - 2)
+          fb[(j + 2) % 4] = read_b(b, j + 2);
+        else
+          fb[(j + 2) % 4] = read_b(b + 1, j + 2 - TJ);
+      }
+      sum[m % kSums] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          fb[j % 4], fa[i], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0 /*e4m3*/, 0 /*e4m3*/, 0, 0, 0, 0);
+      if constexpr (m >= kLate)
+        fold(std::integral_constant<int, m - kLate>{});
       else
-        fb[(j + 2) % 4] = read_b(b + 1, j + 2 - TJ);
+        fold(std::integral_constant<int, kSteps + m - kLate>{});
+      if constexpr (m == kLate - 1) {
 #pragma unroll
-      for (int i = 0; i < TI; ++i) {
-        const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            fb[j % 4], fa[i], v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0 /*e4m3*/, 0 /*e4m3*/, 0, 127 /*x1*/, 0, 127 /*x1*/);
-        if constexpr (j == TJ - 1) read_a(b + 1, i);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(sum[q], s[i], acc[i][j][q]);
+        for (int x = 0; x < TI; ++x) s[x] = sx[x] * s_w;
       }
+      if constexpr (m >= kFree) {  // the copies of the stage after next, dealt to the steps that are left
+        constexpr int kLeft = kSteps - kFree, at = m - kFree;
+        constexpr int c0 = kCopies * at / kLeft, c1 = kCopies * (at + 1) / kLeft;
+        static_for<c1 - c0>([&](auto c) { copy(ahead, std::integral_constant<int, c0 + decltype(c)::value>{}); });
+      }
+      if constexpr (j == TJ - 1) read_a(b + 1, i);
+      __builtin_amdgcn_sched_barrier(0);
     });
   }
+  static_for<kLate>([&](auto c) { fold(std::integral_constant<int, kSteps - kLate + decltype(c)::value>{}); });
   wait_vmcnt<0>();
 
   // lane l holds, of row l % 16 of an activation tile, outputs 4 (l / 16) .. + 3 of each weight tile. Two
@@ -362,8 +413,7 @@ static int check_dims(int32_t n_out, int32_t k_in) {
 template <typename T>
 static int launch_tiles(const Args& p, hipStream_t s) {
   const int64_t mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
-  const int64_t grid = mts >= 16 ? round_up(mts, 8) * nts : round_up(nts, 8) * mts;
-  hipLaunchKernelGGL(tile_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s, p);
+  hipLaunchKernelGGL(tile_kernel<T>, dim3(static_cast<unsigned>(tile_grid(mts, nts))), dim3(T::kThreads), 0, s, p);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }

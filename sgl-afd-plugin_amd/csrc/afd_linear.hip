@@ -46,56 +46,88 @@ __device__ __forceinline__ v8i join(v4i lo, v4i hi) {
 }
 
 // ---------------------------------------------------------------- activations
-// A wavefront quantizes 16 rows x one K block: lane l chunks l / 16 of both 64-column pieces of row
-// l % 16. vec: 16-byte loads of whole chunks.
-__global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
-                                                    uint8_t* __restrict__ q, float* __restrict__ s, int kb,
-                                                    int a_rows, bool vec) {
-  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= ((int64_t(n) + 15) / 16) * kb) return;
-  const int64_t r16 = item / kb;
-  const int b = static_cast<int>(item % kb);
-  const int lane = threadIdx.x & 63, c = lane >> 4;
-  const int64_t row = r16 * 16 + (lane & 15);
-  float v[2][16];
-  uint32_t top = 0;  // bits of the largest magnitude: infinities and NaN above every number
+// A wavefront's share of an activation image: 16 rows x one K block, lane l chunks l / 16 of both
+// 64-column pieces of row l % 16. Raw: those 2 x 16 bf16 values, two a word.
+struct Raw {
+  uint32_t u[2][8];
+};
+// VEC: rows take 16-byte loads and k_in is a multiple of 16 (then a chunk is whole or missing). p: the
+// row; c: the lane's chunk. What lies past k_in reads as 0.
+template <bool VEC>
+__device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int c) {
+  Raw r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int k0 = b * 128 + h * 64 + c * 16;
-    const uint16_t* p = x + row * ldx + k0;
-    if (vec && row < n && k0 + 16 <= k_in) {
-      const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 8);
+    if constexpr (VEC) {
+      const v4i* src = reinterpret_cast<const v4i*>(p + min(k0, k_in - 16));
+      const v4i lo = src[0], hi = src[1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t w = static_cast<uint32_t>(i < 4 ? lo[i & 3] : hi[i & 3]);
-        v[h][2 * i] = __uint_as_float(w << 16);
-        v[h][2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      for (int i = 0; i < 4; ++i) {
+        r.u[h][i] = k0 < k_in ? lo[i] : 0;
+        r.u[h][4 + i] = k0 < k_in ? hi[i] : 0;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[h][i] = row < n && k0 + i < k_in ? bf16_to_f32(p[i]) : 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + 2 * i;
+        const uint32_t lo = p[min(k, k_in - 1)], hi = p[min(k + 1, k_in - 1)];
+        r.u[h][i] = (k < k_in ? lo : 0u) | (k + 1 < k_in ? hi << 16 : 0u);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[h][i]) & 0x7fffffffu);
   }
+  return r;
+}
+// e4m3 codes of both pieces' chunks, and the row's scale of the K block (NaN of a row that is not finite)
+__device__ __forceinline__ float quantize(const Raw& r, v4i (&q)[2]) {
+  // the largest magnitude's bits, two columns at a time: infinities and NaN above every number
+  typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+  v2u most = {0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, r.u[h][i] & 0x7fff7fffu));
+  uint32_t top = uint32_t(max(most[0], most[1])) << 16;
   const auto r0 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
   top = max(r0[0], r0[1]);
   const auto r1 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
   top = max(r1[0], r1[1]);
   const bool finite = top < 0x7f800000u;
-  const float sc = fmaxf(__uint_as_float(top), kFp8Eps) / kE4m3Max;
+  const float sc = fmaxf(__uint_as_float(finite ? top : 0u), kFp8Eps) / kE4m3Max;
   const float rsc = 1.0f / sc;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    v4i out;
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      out[i] = finite ? static_cast<int>(pk4_e4m3(div_by(v[h][4 * i], sc, rsc), div_by(v[h][4 * i + 1], sc, rsc),
-                                                  div_by(v[h][4 * i + 2], sc, rsc), div_by(v[h][4 * i + 3], sc, rsc)))
-                      : 0;
-    *reinterpret_cast<v4i*>(q + (r16 * (2 * kb) + 2 * b + h) * kPiece + lane * 16) = out;
-  }
-  if (c == 0 && row < n) s[int64_t(b) * a_rows + row] = finite ? sc : __builtin_nanf("");
+    for (int i = 0; i < 4; ++i) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t w = finite ? r.u[h][2 * i + j] : 0u;
+        v[2 * j] = div_by(__uint_as_float(w << 16), sc, rsc);
+        v[2 * j + 1] = div_by(__uint_as_float(w & 0xffff0000u), sc, rsc);
+      }
+      // quotients of a row's block stay below 448 (1 + 2^-23)
+      q[h][i] = static_cast<int>(pk4_e4m3_near(v[0], v[1], v[2], v[3]));
+    }
+  return finite ? sc : __builtin_nanf("");
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
+                                                    uint8_t* __restrict__ q, float* __restrict__ s, int kb,
+                                                    int a_rows) {
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (item >= ((int64_t(n) + 15) / 16) * kb) return;
+  const int64_t r16 = item / kb;
+  const int b = static_cast<int>(item % kb), lane = threadIdx.x & 63;
+  const int64_t row = min(r16 * 16 + (lane & 15), int64_t(n) - 1);  // past the end: the last again
+  v4i code[2];
+  const float sc = quantize(load_raw<VEC>(x + row * ldx, k_in, b, lane >> 4), code);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    *reinterpret_cast<v4i*>(q + (r16 * (2 * kb) + 2 * b + h) * kPiece + lane * 16) = code[h];
+  if (lane < 16) s[int64_t(b) * a_rows + r16 * 16 + lane] = sc;
 }
 
 // ---------------------------------------------------------------- weights (load time)
@@ -117,81 +149,174 @@ __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ w
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 16 MT rows of x: a call is bound by reading the weights once. A workgroup owns 16 outputs over the
-// whole K, its wavefronts a share of the K blocks each, weights and activations straight into
-// registers; the wavefronts' sums meet in LDS, in their order.
+// Calls of few rows are bound by reading the weights once and by latency. A workgroup owns 16 outputs over
+// the whole K and 16 MT rows, its wavefronts every kRowWaves-th K block each: the weights straight into registers
+// (non-temporal, DEPTH blocks ahead), the activations from the image likewise; the wavefronts' sums
+// meet in LDS, in their order.
+// FUSED: no launch before it. The workgroup quantizes its rows into LDS while its first weights are on
+// their way (16 rows' K blocks a wavefront at a time, whichever rows they are of): n K elements, which every
+// workgroup does again, so only where they are few and fit kFusedBytes.
 constexpr int kRowWaves = 8;
+constexpr int kFusedBytes = 32768;
 
-template <int MT>
-__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p) {
-  __shared__ v4f part[kRowWaves][MT][64];
+struct RowsIn {
+  const uint16_t* x;  // FUSED
+  int64_t ldx;
+  int k_in;
+};
+
+template <int MT, bool FUSED, bool VEC>
+__global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in) {
+  constexpr int kDepth = FUSED || MT <= 2 ? 4 : 2;
+  constexpr int kPart = kRowWaves * MT * 64 * 16;
+  constexpr int kCodes = FUSED ? kFusedBytes : 0;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kCodes > kPart ? kCodes : kPart];
+  __shared__ float scales[FUSED ? kFusedBytes / 128 : 1];
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int o16 = blockIdx.x;
-  const int kt = 2 * p.kb;
-  const int r16s = (p.n + 15) / 16;
-  v4f acc[MT] = {};
+  const int o16 = blockIdx.x, g0 = blockIdx.y * MT;
+  const int kt = 2 * p.kb, last = p.kb - 1;
+  const int r16_last = (p.n + 15) / 16 - 1;
+  v4f acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const uint8_t* bw = p.b + int64_t(o16) * kt * kPiece + lane * 16;
   const float* sw = p.bs + int64_t(o16 / 8) * p.kb;
-  for (int b = w; b < p.kb; b += kRowWaves) {
-    const v4i lo = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * b) * kPiece));
-    const v4i hi = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * b + 1) * kPiece));
-    const v8i fw = join(lo, hi);
-    const float s_w = load_uniform(sw + b);
+  // what a K block needs; blocks past the end read the last one and are not added
+  struct Block {
+    v4i w[2];
+    float s_w;
+    v4i x[FUSED ? 1 : MT][2];
+    float s_x[FUSED ? 1 : MT];
+  };
+  auto fetch = [&](int b) {
+    Block k;
+    const int c = min(b, last);
+    k.w[0] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * c) * kPiece));
+    k.w[1] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(bw + int64_t(2 * c + 1) * kPiece));
+    k.s_w = sw[c];
+    if constexpr (!FUSED) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int r16 = min(m, r16s - 1);
-      const uint8_t* ax = p.a + (int64_t(r16) * kt + 2 * b) * kPiece + lane * 16;
-      const v8i fx = join(*reinterpret_cast<const v4i*>(ax), *reinterpret_cast<const v4i*>(ax + kPiece));
-      const float s = p.as[int64_t(b) * p.a_rows + r16 * 16 + (lane & 15)] * s_w;
-      const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0,
-                                                                     127, 0, 127);
+      for (int m = 0; m < MT; ++m) {
+        const int64_t r16 = min(g0 + m, r16_last);
+        const uint8_t* ax = p.a + (r16 * kt + 2 * c) * kPiece + lane * 16;
+        k.x[m][0] = *reinterpret_cast<const v4i*>(ax);
+        k.x[m][1] = *reinterpret_cast<const v4i*>(ax + kPiece);
+        k.s_x[m] = p.as[int64_t(c) * p.a_rows + r16 * 16 + (lane & 15)];
+      }
+    }
+    return k;
+  };
+  Block ring[kDepth];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) acc[m][q] = __builtin_fmaf(sum[q], s, acc[m][q]);
+  for (int d = 0; d < kDepth; ++d) ring[d] = fetch(w + d * kRowWaves);
+  // FUSED: chunk c of half h of K block b of row r at ((2 b + h) 4 + c) 16 n + 16 r
+  if constexpr (FUSED) {
+    constexpr int kUp = 4;  // items on their way at once
+    const int items = p.n * p.kb, c = lane >> 4;
+    for (int at = w * 16; at < items; at += kUp * kRowWaves * 16) {
+      Raw raw[kUp];
+      int r[kUp], b[kUp];
+#pragma unroll
+      for (int u = 0; u < kUp; ++u) {
+        const int it = min(at + u * kRowWaves * 16 + (lane & 15), items - 1);
+        r[u] = it / p.kb;
+        b[u] = it - r[u] * p.kb;
+        raw[u] = load_raw<VEC>(in.x + r[u] * in.ldx, in.k_in, b[u], c);
+      }
+#pragma unroll
+      for (int u = 0; u < kUp; ++u) {
+        if (u > 0 && at + u * kRowWaves * 16 >= items) break;
+        v4i q[2];
+        const float sc = quantize(raw[u], q);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<v4i*>(lds + (((2 * b[u] + h) * 4 + c) * p.n + r[u]) * 16) = q[h];
+        scales[b[u] * p.n + r[u]] = sc;
+      }
+    }
+    __syncthreads();
+  }
+  for (int b0 = w; b0 <= last; b0 += kDepth * kRowWaves) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int b = b0 + d * kRowWaves;
+      if (b > last) break;
+      const Block k = ring[d];
+      ring[d] = fetch(b + kDepth * kRowWaves);
+      const v8i fw = join(k.w[0], k.w[1]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        v4i q[2];
+        float s;
+        if constexpr (FUSED) {
+          const int r = min(m * 16 + (lane & 15), p.n - 1);
+          q[0] = *reinterpret_cast<const v4i*>(lds + ((8 * b + (lane >> 4)) * p.n + r) * 16);
+          q[1] = *reinterpret_cast<const v4i*>(lds + ((8 * b + 4 + (lane >> 4)) * p.n + r) * 16);
+          s = scales[b * p.n + r];
+        } else {
+          q[0] = k.x[m][0];
+          q[1] = k.x[m][1];
+          s = k.s_x[m];
+        }
+        s *= k.s_w;
+        const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fw, join(q[0], q[1]), v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0 /*e4m3*/, 0 /*e4m3*/, 0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][i] = __builtin_fmaf(sum[i], s, acc[m][i]);
+      }
     }
   }
+  if constexpr (FUSED) __syncthreads();  // the codes are read: the sums take their place
+  v4f* part = reinterpret_cast<v4f*>(lds);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) part[w][m][lane] = acc[m];
+  for (int m = 0; m < MT; ++m) part[(w * MT + m) * 64 + lane] = acc[m];
   __syncthreads();
   // lane l: row l % 16 of x, outputs 4 (l / 16) .. + 3
-  if (w >= MT) return;
   for (int m = w; m < MT; m += kRowWaves) {
-    v4f y = part[0][m][lane];
-    for (int i = 1; i < kRowWaves; ++i) y += part[i][m][lane];
-    const int row = m * 16 + (lane & 15), o = o16 * 16 + 4 * (lane >> 4);
+    v4f y = part[m * 64 + lane];
+    for (int i = 1; i < kRowWaves; ++i) y += part[(i * MT + m) * 64 + lane];
+    const int64_t row = int64_t(g0 + m) * 16 + (lane & 15);
+    const int o = o16 * 16 + 4 * (lane >> 4);
     if (row >= p.n) continue;
     uint16_t* out = p.y + row * p.ldy + o;
+    if (p.wide && o + 4 <= p.n_out) {
+      *reinterpret_cast<uint2*>(out) = uint2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+    } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (o + q < p.n_out) out[q] = f32_to_bf16(y[q]);
+      for (int q = 0; q < 4; ++q)
+        if (o + q < p.n_out) out[q] = f32_to_bf16(y[q]);
+    }
   }
 }
 
 // ---------------------------------------------------------------- tiles
 // BM rows of x by BN outputs, WM x WN wavefronts of TI x TJ MFMA tiles of 16x16 each (K 128 in one
 // instruction, so a block's sum is one MFMA from 0 and its 4 values a lane are folded at once). A stage
-// is one K block of both operands and the rows' scales, copied HBM -> LDS in 1 KiB pieces into two slots.
+// is one K block of both operands and the rows' scales, copied HBM -> LDS in 1 KiB pieces into S slots.
 //
 // A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments,
 // read two ahead, in an order kept as written (left alone, the compiler reads all of a stage first and then
 // waits out every MFMA in turn: 322 us for 16384 x 4096 x 4096). When the last two are in registers (all of its reads of the stage done) it waits for
 // its copies of the next stage and meets the others at the stage's one barrier: the next stage
-// is there for all, and this one's slot is free for the copies of the stage after. The MFMAs of the
+// is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the
 // last two weight fragments run while the next stage's first fragments are read.
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int S_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
   static constexpr int kAPieces = BM / 16 * 2, kBPieces = BN / 16 * 2;
   static constexpr int kAQ = kAPieces / kWaves, kBQ = kBPieces / kWaves;
   static constexpr int kBOff = kAPieces * kPiece, kSOff = kBOff + kBPieces * kPiece;
   static constexpr int kStage = kSOff + BM * 4;
-  static constexpr int kLds = 2 * kStage;
+  static constexpr int kLds = S * kStage;
+  static constexpr int kCopies = 1 + kAQ + kBQ;  // a wavefront's copies of a stage
   static constexpr int kScaleWaves = BM / 64;  // each copies 64 rows' scales
   static_assert(TI * 16 * WM == BM && TJ * 16 * WN == BN && kAQ * kWaves == kAPieces && kBQ * kWaves == kBPieces, "tile");
   static_assert(TJ % 4 == 0 && BN / WN <= 128 && 128 % (BN / WN) == 0, "one weight scale per wavefront and K block");
   static_assert(kScaleWaves <= kWaves && BM <= kScaleRows && kLds <= 160 * 1024, "LDS");
+  static_assert((S & (S - 1)) == 0 && (S - 1) * kCopies < 64, "slots by a mask; vmcnt is a 6-bit counter");
 };
 
 // Workgroup b runs on XCD b % 8, each with its own L2. Where there are many row tiles an XCD takes a
@@ -257,11 +382,11 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
     b_src[i] = p.b + (int64_t(min(n0 / 16 + q / 2, o16_last)) * kt + q % 2) * kPiece;
   }
   // copy number c of a stage: the scales, then the activation pieces, then the weight pieces
-  constexpr int kCopies = 1 + T::kAQ + T::kBQ;
+  constexpr int kCopies = T::kCopies, S = T::S;
   const int ws = w % T::kScaleWaves;
   auto copy = [&](int b, auto c_c) {
     constexpr int c = decltype(c_c)::value;
-    const uint32_t st = lds_base + static_cast<uint32_t>((b & 1) * T::kStage);
+    const uint32_t st = lds_base + static_cast<uint32_t>((b & (S - 1)) * T::kStage);
     const uint32_t off = voff + static_cast<uint32_t>(b) * (2 * kPiece);
     if constexpr (c == 0) {
       // (every wavefront: two may write the same bytes, and the steps stay one block of code)
@@ -293,15 +418,15 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
     return join(*reinterpret_cast<const v4i*>(f), *reinterpret_cast<const v4i*>(f + kPiece));
   };
   auto read_a = [&](int b, int i) {
-    fa[i] = read(a_lds + (b & 1) * T::kStage + i * 2 * kPiece);
-    sx[i] = *reinterpret_cast<const float*>(s_lds + (b & 1) * T::kStage + i * 64);
+    fa[i] = read(a_lds + (b & (S - 1)) * T::kStage + i * 2 * kPiece);
+    sx[i] = *reinterpret_cast<const float*>(s_lds + (b & (S - 1)) * T::kStage + i * 64);
   };
-  auto read_b = [&](int b, int j) { return read(b_lds + (b & 1) * T::kStage + j * 2 * kPiece); };
+  auto read_b = [&](int b, int j) { return read(b_lds + (b & (S - 1)) * T::kStage + j * 2 * kPiece); };
 
   // An MFMA's result is folded kLate steps after it was issued (its latency is one step of its own and
   // one of the other wavefront's); the last ones of a stage in the next stage's first steps.
   constexpr int kSteps = TI * TJ, kLate = 3, kSums = 4;
-  static_assert(kSteps % kSums == 0 && kLate < kSums, "a sum is folded before its registers take another");
+  static_assert(kLate <= kSteps && kSteps % kSums == 0 && kLate < kSums, "a sum is folded before its registers take another");
   v4f sum[kSums];
 #pragma unroll
   for (int i = 0; i < kSums; ++i) sum[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -313,23 +438,23 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
     for (int q = 0; q < 4; ++q) acc[i][j][q] = __builtin_fmaf(sum[m % kSums][q], s[i], acc[i][j][q]);
   };
 
-  issue(0);
-  wait_vmcnt<0>();
+  static_for<S>([&](auto c) { issue(min(static_cast<int>(decltype(c)::value), last)); });
+  wait_vmcnt<(S - 1) * kCopies>();
   __syncthreads();
-  issue(min(1, last));
 #pragma unroll
   for (int i = 0; i < TI; ++i) read_a(0, i);
   fb[0] = read_b(0, 0);
   fb[1] = read_b(0, 1);
   for (int b = 0; b <= last; ++b) {
-    const int ahead = min(b + 2, last);  // past the end: the last stage over itself, the same bytes
+    float s_w_next = 0.0f;
+    const int ahead = min(b + S, last);  // past the end: the last stage over itself, the same bytes
     static_for<kSteps>([&](auto mc) {
       constexpr int m = decltype(mc)::value, i = m % TI, j = m / TI;
       constexpr int kFree = (TJ - 2) * TI;  // the first step at which the stage's slot is free
       if constexpr (m == kFree) {
-        wait_vmcnt_lds<0>();
+        wait_vmcnt_lds<(S - 2) * kCopies>();  // copies land in the order they were issued in
         __syncthreads();
-        s_w = load_uniform(sw + min(b + 1, last));
+        s_w_next = load_uniform(sw + min(b + 1, last));
       }
       if constexpr (i == 0) {
         if constexpr (j < TJ - 2)
@@ -355,6 +480,7 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
       if constexpr (j == TJ - 1) read_a(b + 1, i);
       __builtin_amdgcn_sched_barrier(0);
     });
+    s_w = s_w_next;
   }
   static_for<kLate>([&](auto c) { fold(std::integral_constant<int, kSteps - kLate + decltype(c)::value>{}); });
   wait_vmcnt<0>();
@@ -391,8 +517,15 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 }
 
 // ---------------------------------------------------------------- host
-using Large = Shape<256, 256, 4, 2>;
-using Mid = Shape<128, 128, 2, 2>;
+// Tile shapes. With a tile on each of 256 CUs a K block takes 0.35, 0.49, 0.72, 1.16 and 1.86 us (4096 inputs),
+// that is 0.35, 0.25, 0.18, 0.15 and 0.12 for every 64 x 64 outputs: the larger the tile, the less of its
+// time goes into moving operands, and the fewer of them there are to fill the CUs. The ring is as deep as the
+// LDS allows with the fragments' order in mind: small tiles wait for latency, large ones do not.
+using T64 = Shape<64, 64, 4, 1, 4>;
+using T64x128 = Shape<64, 128, 2, 2, 4>;
+using T128 = Shape<128, 128, 2, 2, 4>;
+using T256x128 = Shape<256, 128, 4, 2, 2>;
+using T256 = Shape<256, 256, 4, 2, 2>;
 
 struct Plan {
   int kb, a_rows;
@@ -417,11 +550,35 @@ static int launch_tiles(const Args& p, hipStream_t s) {
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
-template <int MT>
-static int launch_rows(const Args& p, hipStream_t s) {
-  hipLaunchKernelGGL(rows_kernel<MT>, dim3((p.n_out + 15) / 16), dim3(64 * kRowWaves), 0, s, p);
+template <int MT, bool FUSED>
+static int launch_rows(const Args& p, const RowsIn& in, bool vec, hipStream_t s) {
+  const dim3 grid((p.n_out + 15) / 16, (p.n + 16 * MT - 1) / (16 * MT)), block(64 * kRowWaves);
+  if (!FUSED || vec)
+    hipLaunchKernelGGL((rows_kernel<MT, FUSED, true>), grid, block, 0, s, p, in);
+  else
+    hipLaunchKernelGGL((rows_kernel<MT, FUSED, !FUSED>), grid, block, 0, s, p, in);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
+}
+
+// The shape whose rounds over the CUs take least: rounds x the measured time of one K block (T64 .. T256
+// above). At 4096 x 4096, measured best and chosen: 512 rows T64x128 (20.7 us, T128 25.6), 1024 T128 (28.9, T256x128
+// 40), 1500 T256x128 (41.7, T128 46.4), 2900 T256 (59.7, T256x128 70.7).
+enum { kT64, kT64x128, kT128, kT256x128, kT256, kShapes };
+static int best_shape(int64_t n, int64_t n_out, int cus) {
+  static const int bm[kShapes] = {64, 64, 128, 256, 256}, bn[kShapes] = {64, 128, 128, 128, 256};
+  static const int cost[kShapes] = {35, 49, 72, 116, 186};
+  int best = 0;
+  int64_t least = 0;
+  for (int i = 0; i < kShapes; ++i) {
+    const int64_t tiles = ((n + bm[i] - 1) / bm[i]) * ((n_out + bn[i] - 1) / bn[i]);
+    const int64_t time = (tiles + cus - 1) / cus * cost[i];
+    if (i == 0 || time < least) {
+      best = i;
+      least = time;
+    }
+  }
+  return best;
 }
 
 }  // namespace linear
@@ -474,11 +631,7 @@ extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, 
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* q = static_cast<uint8_t*>(ws);
   float* sx = reinterpret_cast<float*>(q + pl.q_bytes);
-  const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
-  hipLaunchKernelGGL(linear::quant_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, s, x, ldx, n,
-                     weights->k_in, q, sx, pl.kb, pl.a_rows, vec);
-  AFD_CHECK_LAUNCH();
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && weights->k_in % 16 == 0;
   linear::Args p = {};
   p.a = q;
   p.as = sx;
@@ -491,10 +644,33 @@ extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, 
   p.kb = pl.kb;
   p.a_rows = pl.a_rows;
   p.wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy % 8 == 0;
-  if (n <= 16) return linear::launch_rows<1>(p, s);
-  if (n <= 32) return linear::launch_rows<2>(p, s);
-  if (n <= 64) return linear::launch_rows<4>(p, s);
-  const int64_t large = ((int64_t(n) + 255) / 256) * ((int64_t(p.n_out) + 255) / 256);
-  if (large >= device_cu_count()) return linear::launch_tiles<linear::Large>(p, s);
-  return linear::launch_tiles<linear::Mid>(p, s);
+  const linear::RowsIn in = {x, ldx, weights->k_in};
+  // the rows kernel's own quantization is faster up to 32 K elements (4096 x 4096: 4 rows 6.7 against 8.8 us,
+  // 16 rows 10.8 against 9.0; 1024 x 1000: 32 rows 6.4 against 7.1, 64 rows 9.5 against 7.4), a third
+  // of that where the rows do not take wide loads (300 x 3000: 32 rows 6.7 against 7.3, 64 rows 10.0 against 7.5)
+  const int64_t elements = int64_t(n) * pl.kb * 128;
+  if (n <= 64 && elements <= (vec ? linear::kFusedBytes : linear::kFusedBytes / 3)) {
+    if (n <= 16) return linear::launch_rows<1, true>(p, in, vec, s);
+    if (n <= 32) return linear::launch_rows<2, true>(p, in, vec, s);
+    return linear::launch_rows<4, true>(p, in, vec, s);
+  }
+  const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
+  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+  if (vec)
+    hipLaunchKernelGGL(linear::quant_kernel<true>, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+  else
+    hipLaunchKernelGGL(linear::quant_kernel<false>, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+  AFD_CHECK_LAUNCH();
+  // up to 64 rows the weights are read once; above, tiles (4096 x 4096: 64 rows 12.8 against 13.5 us, 128
+  // rows 14.7 against 13.9)
+  if (n <= 16) return linear::launch_rows<1, false>(p, in, vec, s);
+  if (n <= 32) return linear::launch_rows<2, false>(p, in, vec, s);
+  if (n <= 64) return linear::launch_rows<4, false>(p, in, vec, s);
+  switch (linear::best_shape(n, p.n_out, device_cu_count())) {
+    case linear::kT64: return linear::launch_tiles<linear::T64>(p, s);
+    case linear::kT64x128: return linear::launch_tiles<linear::T64x128>(p, s);
+    case linear::kT128: return linear::launch_tiles<linear::T128>(p, s);
+    case linear::kT256x128: return linear::launch_tiles<linear::T256x128>(p, s);
+    default: return linear::launch_tiles<linear::T256>(p, s);
+  }
 }

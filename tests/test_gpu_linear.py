@@ -267,3 +267,14 @@ def test_shared_expert(n):
     # a code of h may be its neighbour (1/8 apart at most) where gate and up round to other bf16
     rel = float((y.cpu().double() - want).norm() / want.norm())
     assert rel <= 2.0**-5, rel
+
+
+@pytest.mark.parametrize("n,n_out", [(65, 4096), (500, 4100), (1000, 4000), (1500, 4096), (2900, 4096), (70, 65000), (5000, 300)])
+def test_exact_integers_every_tile_shape(n, n_out):
+    """Calls that take each of the tile shapes, with rows and outputs that end inside a tile."""
+    k = 700
+    x, w, s = integers(n, k, n_out, n)
+    say(f"exact, tile shapes n={n} n_out={n_out}")
+    y = Fp8BlockLinear(e4m3(w).to(dev()), s.to(dev()))(x.to(torch.bfloat16).to(dev()))
+    want = (x @ (w * widen(s, n_out, k)).t()).to(torch.bfloat16)  # exact in fp32 too
+    assert torch.equal(y.cpu(), want)

@@ -26,6 +26,8 @@ constexpr int kMaxDim = 65536;
 constexpr int kMaxRows = 1 << 22;
 // the activation scales are [K / 128][rows rounded up to kScaleRows]
 constexpr int kScaleRows = 256;
+// an x above this is read past the caches (the memory-side cache has 256 MB, shared with codes and weights)
+constexpr int64_t kCachedBytes = int64_t(64) << 20;
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -53,7 +55,7 @@ struct Raw {
 };
 // VEC: rows take 16-byte loads and k_in is a multiple of 16 (then a chunk is whole or missing). p: the
 // row; c: the lane's chunk. What lies past k_in reads as 0.
-template <bool VEC>
+template <bool VEC, bool NT = false>
 __device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int c) {
   Raw r;
 #pragma unroll
@@ -61,7 +63,7 @@ __device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int 
     const int k0 = b * 128 + h * 64 + c * 16;
     if constexpr (VEC) {
       const v4i* src = reinterpret_cast<const v4i*>(p + min(k0, k_in - 16));
-      const v4i lo = src[0], hi = src[1];
+      const v4i lo = NT ? __builtin_nontemporal_load(src) : src[0], hi = NT ? __builtin_nontemporal_load(src + 1) : src[1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         r.u[h][i] = k0 < k_in ? lo[i] : 0;
@@ -113,7 +115,8 @@ __device__ __forceinline__ float quantize(const Raw& r, v4i (&q)[2]) {
   return finite ? sc : __builtin_nanf("");
 }
 
-template <bool VEC>
+// NT: non-temporal reads, for an x that no cache holds anyway.
+template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
                                                     uint8_t* __restrict__ q, float* __restrict__ s, int kb,
                                                     int a_rows) {
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__
   const int b = static_cast<int>(item % kb), lane = threadIdx.x & 63;
   const int64_t row = min(r16 * 16 + (lane & 15), int64_t(n) - 1);  // past the end: the last again
   v4i code[2];
-  const float sc = quantize(load_raw<VEC>(x + row * ldx, k_in, b, lane >> 4), code);
+  const float sc = quantize(load_raw<VEC, NT>(x + row * ldx, k_in, b, lane >> 4), code);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     *reinterpret_cast<v4i*>(q + (r16 * (2 * kb) + 2 * b + h) * kPiece + lane * 16) = code[h];
@@ -167,7 +170,7 @@ struct RowsIn {
 
 template <int MT, bool FUSED, bool VEC>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in) {
-  constexpr int kDepth = FUSED || MT <= 2 ? 4 : 2;
+  constexpr int kDepth = FUSED || MT <= 2 ? 4 : MT == 3 ? 3 : 2;
   constexpr int kPart = kRowWaves * MT * 64 * 16;
   constexpr int kCodes = FUSED ? kFusedBytes : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kCodes > kPart ? kCodes : kPart];
@@ -656,15 +659,23 @@ extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, 
   }
   const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
   const dim3 grid(static_cast<unsigned>((items + 3) / 4));
-  if (vec)
-    hipLaunchKernelGGL(linear::quant_kernel<true>, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+  // (134 MB of x: 36 us non-temporal, 42 through the caches; 24 MB, which they hold: 9.3 against 8.0)
+  const bool nt = int64_t(n) * weights->k_in * 2 > linear::kCachedBytes;
+  auto quant = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+  };
+  if (vec && nt)
+    quant(linear::quant_kernel<true, true>);
+  else if (vec)
+    quant(linear::quant_kernel<true, false>);
   else
-    hipLaunchKernelGGL(linear::quant_kernel<false>, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+    quant(linear::quant_kernel<false, false>);
   AFD_CHECK_LAUNCH();
   // up to 64 rows the weights are read once; above, tiles (4096 x 4096: 64 rows 12.8 against 13.5 us, 128
   // rows 14.7 against 13.9)
   if (n <= 16) return linear::launch_rows<1, false>(p, in, vec, s);
   if (n <= 32) return linear::launch_rows<2, false>(p, in, vec, s);
+  if (n <= 48) return linear::launch_rows<3, false>(p, in, vec, s);
   if (n <= 64) return linear::launch_rows<4, false>(p, in, vec, s);
   switch (linear::best_shape(n, p.n_out, device_cu_count())) {
     case linear::kT64: return linear::launch_tiles<linear::T64>(p, s);

@@ -959,7 +959,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
 
 // ---------------------------------------------------------------- selection, counts and balance sums
 // The rows of one piece: p, the lane's sums of s' over its rows; mine, their number; cnt, the counts (LDS).
-template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES, bool WIDE>
+template <typename T, int W, int V, bool SELECT, bool BIAS, bool WIDE>
 __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Piece& piece, const float (&bias)[V],
                                              float (&p)[V], int& mine, int32_t* cnt, uint64_t* lds) {
   constexpr int kRows = kBalanceThreads / W;
@@ -967,21 +967,18 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
   const bool counted = piece.seq >= 0;
   using R = Row<T, W, V>;
   auto clamp_row = [&](int32_t r) { return min(r, piece.end - 1); };
-  typename R::Raw next = {};
-  if constexpr (SELECT || SCORES) next = R::template fetch<WIDE>(a, clamp_row(at + sub), li);
+  typename R::Raw next = R::template fetch<WIDE>(a, clamp_row(at + sub), li);
   for (int32_t base = at; base < piece.end; base += kRows) {
     const int32_t r = base + sub;
     const bool in = r < piece.end;
     const int32_t rr = in ? r : piece.end - 1;
     const bool live = in && (a.valid == nullptr || a.valid[rr]);
     R row;
-    float s[V] = {}, sum = 0.0f;
-    if constexpr (SELECT || SCORES) {
-      const typename R::Raw raw = next;
-      next = R::template fetch<WIDE>(a, clamp_row(r + kRows), li);
-      row.set(a, raw, li);
-    }
-    if constexpr (SCORES) sum = row.template scores<BIAS>(a, s);
+    float s[V];
+    const typename R::Raw raw = next;
+    next = R::template fetch<WIDE>(a, clamp_row(r + kRows), li);
+    row.set(a, raw, li);
+    const float sum = row.template scores<BIAS>(a, s);
     if constexpr (SELECT) {
       float l;
       const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
@@ -997,11 +994,9 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
         if (id >= 0 && id < a.experts) atomicAdd(&cnt[id], 1);
       }
     }
-    if constexpr (SCORES) {
-      const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
+    const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
-    }
+    for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
     mine += live ? 1 : 0;
   }
 }
@@ -1028,10 +1023,20 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
     __syncthreads();
     float p[V] = {};
     int mine = 0;
-    if (a.wide)
-      balance_rows<T, W, V, SELECT, BIAS, SCORES, true>(a, at, piece, bias, p, mine, cnt, lds);
-    else
-      balance_rows<T, W, V, SELECT, BIAS, SCORES, false>(a, at, piece, bias, p, mine, cnt, lds);
+    if constexpr (!SCORES) {
+      // the rows' ids are one run of memory
+      const int64_t last = counted ? int64_t(piece.end) * a.topk : 0;
+      for (int64_t i = int64_t(at) * a.topk + t; i < last; i += kBalanceThreads) {
+        const int id = a.ids[i];
+        const bool live = a.valid == nullptr || a.valid[i / a.topk] != 0;
+        if (live && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts)) atomicAdd(&cnt[id], 1);
+      }
+      __syncthreads();
+    } else if (a.wide) {
+      balance_rows<T, W, V, SELECT, BIAS, true>(a, at, piece, bias, p, mine, cnt, lds);
+    } else {
+      balance_rows<T, W, V, SELECT, BIAS, false>(a, at, piece, bias, p, mine, cnt, lds);
+    }
     if (counted) {
       if (li == 0) atomicAdd(&live_rows, mine);
       if constexpr (SCORES) {
@@ -1055,6 +1060,40 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
     }
     __syncthreads();
     at = piece.end;
+  }
+}
+
+// ---------------------------------------------------------------- counts alone, few ids
+// One launch: a workgroup counts a sequence's ids in LDS, a histogram for every two of its 16 wavefronts (popular
+// experts meet in fewer atomics).
+constexpr int kCountThreads = 1024, kHists = 8;
+constexpr int64_t kDirectIds = 16384;
+
+__global__ __launch_bounds__(kCountThreads) void count_kernel(Args a) {
+  __shared__ int32_t hist[kHists][kMaxExperts];
+  const int t = threadIdx.x;
+  for (int i = t; i < kHists * kMaxExperts; i += kCountThreads) (&hist[0][0])[i] = 0;
+  int32_t lo = 0, hi = a.n;
+  if (a.cu != nullptr) {
+    lo = min(max(a.cu[blockIdx.x], 0), a.n);
+    hi = min(max(a.cu[blockIdx.x + 1], 0), a.n);
+  }
+  __syncthreads();
+  int32_t* mine = hist[t >> 7];
+  // the rows' ids are one run of memory
+  const int64_t first = int64_t(lo) * a.topk, last = int64_t(hi) * a.topk;
+#pragma unroll 4
+  for (int64_t i = first + t; i < last; i += kCountThreads) {
+    const int id = a.ids[i];
+    const bool live = a.valid == nullptr || a.valid[i / a.topk] != 0;
+    if (live && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts)) atomicAdd(&mine[id], 1);
+  }
+  __syncthreads();
+  for (int e = t; e < a.experts; e += kCountThreads) {
+    int sum = 0;
+#pragma unroll
+    for (int h = 0; h < kHists; ++h) sum += hist[h][e];
+    a.counts[int64_t(blockIdx.x) * a.experts + e] = sum;
   }
 }
 
@@ -1329,7 +1368,8 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
     using T = decltype(tag);
     return with_shape(a.experts, lanes_needed(a, select), [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
-      a.block_rows = block_rows_for(a.n, W);
+      // counts alone are soon summed: fewer slots for the second launch to read
+      a.block_rows = block_rows_for(a.n, W, kBalanceThreads, scores ? 512 : 64);
       a.blocks = blocks_for(a.n, a.block_rows);
       set_shape(a, W, V, sizeof(T));
       auto go = [&](auto kernel) {
@@ -1337,7 +1377,7 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
         AFD_CHECK_LAUNCH();
         return int(AFD_OK);
       };
-      if (!scores) return go(balance_kernel<T, W, V, false, false, false>);
+      if (!scores) return go(balance_kernel<float, 64, 4, false, false, false>);
       if (!select) return go(balance_kernel<T, W, V, false, false, true>);
       return a.bias ? go(balance_kernel<T, W, V, true, true, true>) : go(balance_kernel<T, W, V, true, false, true>);
     });
@@ -1468,6 +1508,13 @@ extern "C" int afd_expert_counts(const int32_t* ids, int32_t n, int32_t topk, in
   a.seqs = num_seqs;
   a.counts = counts;
   router::place(a, ws, p);
+  // DIRECT
+  if (n > 0 && int64_t(n) * topk <= router::kDirectIds) {
+    hipLaunchKernelGGL(router::count_kernel, dim3(num_seqs), dim3(router::kCountThreads), 0,
+                       static_cast<hipStream_t>(stream), a);
+    AFD_CHECK_LAUNCH();
+    return AFD_OK;
+  }
   return router::launch_balance(a, AFD_LOGITS_F32, false, false, static_cast<hipStream_t>(stream));
 }
 

@@ -48,8 +48,9 @@ LOGITS_FORMATS = {torch.float32: _lib.AFD_LOGITS_F32, torch.bfloat16: _lib.AFD_L
 
 def launch(name: str, device: torch.device, *args) -> None:
     """``_lib.call`` on ``device``'s current stream, with ``device`` current."""
+    # (the plain bindings: torch.cuda's wrappers of these two cost a microsecond each)
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))

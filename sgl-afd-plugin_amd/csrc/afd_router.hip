@@ -32,7 +32,10 @@ namespace afd {
 namespace router {
 
 constexpr int kThreads = 256;
-constexpr int kBalanceThreads = 512;  // more wavefronts for the same number of slots
+// threads of a workgroup that fills a slot: many where a row takes a wavefront (16384 x 256: the second
+// launch 9.0 us with 1024 threads and 256 slots, 12.5 with 512 and 512), fewer where it takes less (8192 x
+// 64: the first launch 6.6 us with 512, 9.0 with 1024) or where lanes hold many experts (registers, LDS)
+__host__ __device__ constexpr int balance_threads(int W, int V) { return W == 64 && V == 4 ? 1024 : 512; }
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 32;
 constexpr int kMaxGroups = 64;
@@ -657,7 +660,8 @@ __device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint6
   return true;
 }
 
-// Selection of one row: lane kk < topk gets the kk-th expert and its logit (`chosen`; -inf in other lanes).
+// Selection of one row: lane kk < topk gets the kk-th expert and `chosen`, its logit, or with a bias and
+// scores of their own its score (-inf in other lanes).
 // bias: the lane's experts' (BIAS); s, sum: the row's scores (BIAS).
 template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, uint64_t* lds_row,
@@ -720,10 +724,15 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
   }
   if (all) id = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
   if (all || BIAS) {
-    // the row's logits by way of LDS
+    // the row's logits (scores) by way of LDS
     float* mine = reinterpret_cast<float*>(lds_row);
+    if (BIAS && a.scoring != AFD_SCORE_SOFTMAX) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) mine[e0 + j] = row.l[j];
+      for (int j = 0; j < V; ++j) mine[e0 + j] = s[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) mine[e0 + j] = row.l[j];
+    }
     lds_fence();
     chosen = live ? mine[id] : kLowest;
     lds_fence();
@@ -733,8 +742,8 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
   return id;
 }
 
-// The weight of lane kk's expert, whose logit is l, from the chosen logits alone where nothing else is needed.
-template <typename T, int W, int V>
+// The weight of lane kk's expert from what choose() gave, the chosen ones' alone where nothing else is needed.
+template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, float l) {
   float s;
   if (a.scoring == AFD_SCORE_SOFTMAX) {
@@ -757,7 +766,7 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, f
     sum = sum_f32<W>(sum);
     return sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
   }
-  s = score_f32(l, a.scoring);
+  s = BIAS ? fmaxf(l, 0.0f) : score_f32(l, a.scoring);
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
     s = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
@@ -797,7 +806,7 @@ __device__ __forceinline__ void topk_rows(const Args& a, uint64_t* lds) {
     float s[V] = {}, sum = 0.0f, l;
     if constexpr (BIAS) sum = row.template scores<true>(a, s);
     int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
-    float w = weigh(a, row, l);
+    float w = weigh<T, W, V, BIAS>(a, row, l);
     if (!valid) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
       a.ids[r * a.topk + li] = id;
@@ -838,18 +847,20 @@ __device__ __forceinline__ Piece next_piece(const Args& a, int32_t r, int32_t r1
 }
 
 // ---------------------------------------------------------------- a sequence's slots together
-// A workgroup takes 16 experts (one 64-byte line of a slot) of a sequence: 64 slots side by side, 4 a
-// wavefront, so that a long sequence's slots are in flight together; their sums are added in one order.
+// A workgroup takes CH experts of a sequence, its threads 1024 / CH slots side by side, so that a long
+// sequence's slots are in flight together; their sums are added in one order. 16 experts (one 64-byte line of a
+// slot) where a sequence has many slots, 64 where it has few.
 constexpr int kFinishWaves = 16;
 constexpr int kFinishThreads = 64 * kFinishWaves;
-constexpr int kChunk = 16;
+constexpr int kNarrow = 16, kBroad = 64;
 
-__host__ __device__ inline int chunks_of(int experts) { return (experts + kChunk - 1) / kChunk; }
+__host__ __device__ inline int chunks_of(int experts, int ch) { return (experts + ch - 1) / ch; }
 
-// counts of experts [16 c, + 16) of sequence s, their part of the unscaled loss, and (c = 0) the rows
+// counts of experts [CH c, + CH) of sequence s, their part of the unscaled loss, and (c = 0) the rows
+template <int CH>
 __device__ __forceinline__ void finish_chunk(const Args& a, int s, int c) {
-  __shared__ double p_red[kFinishWaves][kChunk];
-  __shared__ int32_t c_red[kFinishWaves][kChunk];
+  __shared__ double p_red[kFinishWaves][CH];
+  __shared__ int32_t c_red[kFinishWaves][CH];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   int32_t lo = 0, hi = a.n;
   if (a.cu != nullptr) {
@@ -859,23 +870,24 @@ __device__ __forceinline__ void finish_chunk(const Args& a, int s, int c) {
   const int b0 = lo / a.block_rows, slots = hi > lo ? (hi - 1) / a.block_rows + 1 - b0 : 0;
   const int64_t words = slot_words(a.experts);
   const float* first = a.slots + (int64_t(b0) + s) * words;
-  const int e = c * kChunk + (lane & 15);
+  const int e = c * CH + (lane & (CH - 1));
   double p = 0.0;
   int cnt = 0;
   if (e < a.experts) {
 #pragma unroll 8
-    for (int b = t >> 4; b < slots; b += 4 * kFinishWaves) {
+    for (int b = t / CH; b < slots; b += kFinishThreads / CH) {
       const float* slot = first + b * words;
       p += slot[e];
       cnt += reinterpret_cast<const int32_t*>(slot)[a.experts + e];
     }
   }
-  // the wavefront's four slots, then the wavefronts
-  p += __shfl_xor(p, 16);
-  p += __shfl_xor(p, 32);
-  cnt += __shfl_xor(cnt, 16);
-  cnt += __shfl_xor(cnt, 32);
-  if (lane < kChunk) {
+  // the wavefront's slots, then the wavefronts
+#pragma unroll
+  for (int d = CH; d < 64; d *= 2) {
+    p += __shfl_xor(p, d);
+    cnt += __shfl_xor(cnt, d);
+  }
+  if (lane < CH) {
     p_red[w][lane] = p;
     c_red[w][lane] = cnt;
   }
@@ -889,7 +901,8 @@ __device__ __forceinline__ void finish_chunk(const Args& a, int s, int c) {
   if (w == 0) {
     p = 0.0;
     cnt = 0;
-    if (lane < kChunk) {
+    if (lane < CH) {
+#pragma unroll
       for (int i = 0; i < kFinishWaves; ++i) {
         p += p_red[i][lane];
         cnt += c_red[i][lane];
@@ -898,7 +911,7 @@ __device__ __forceinline__ void finish_chunk(const Args& a, int s, int c) {
     }
     if (a.loss != nullptr) {
       const double loss = sum_f64<64>(p * cnt);
-      if (lane == 0) a.part[int64_t(s) * chunks_of(a.experts) + c] = loss;
+      if (lane == 0) a.part[int64_t(s) * chunks_of(a.experts, CH) + c] = loss;
     }
   }
   __syncthreads();
@@ -917,9 +930,9 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 }
 
 // One workgroup, after every sequence: the loss and the sequences' coefficients.
-__device__ __forceinline__ void finish_loss(const Args& a) {
+__device__ __forceinline__ void finish_loss(const Args& a, int chunks) {
   __shared__ double red[kFinishWaves];
-  const int t = threadIdx.x, chunks = chunks_of(a.experts);
+  const int t = threadIdx.x;
   double sum = 0.0, used = 0.0;
   // 16 threads a sequence, its chunks dealt to them
   for (int64_t s = t >> 4; s < a.seqs; s += kFinishThreads / 16) {
@@ -940,11 +953,12 @@ __device__ __forceinline__ void finish_loss(const Args& a) {
   }
 }
 
+template <int CH>
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
   __shared__ uint32_t done;
-  const int chunks = chunks_of(a.experts);
+  const int chunks = chunks_of(a.experts, CH);
   for (int64_t i = blockIdx.x; i < int64_t(a.seqs) * chunks; i += gridDim.x)
-    finish_chunk(a, static_cast<int>(i / chunks), static_cast<int>(i % chunks));
+    finish_chunk<CH>(a, static_cast<int>(i / chunks), static_cast<int>(i % chunks));
   if (a.loss == nullptr) return;
   // the last workgroup adds the sequences up: what it reads (part and rows) was written by the first two
   // wavefronts, which order their writes device-wide before the first one's count
@@ -954,7 +968,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
   __syncthreads();
   if (done != gridDim.x - 1) return;
   __threadfence();
-  finish_loss(a);
+  finish_loss(a, chunks);
 }
 
 // ---------------------------------------------------------------- selection, counts and balance sums
@@ -962,7 +976,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool WIDE>
 __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Piece& piece, const float (&bias)[V],
                                              float (&p)[V], int& mine, int32_t* cnt, uint64_t* lds) {
-  constexpr int kRows = kBalanceThreads / W;
+  constexpr int kRows = balance_threads(W, V) / W;
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   const bool counted = piece.seq >= 0;
   using R = Row<T, W, V>;
@@ -982,7 +996,7 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
     if constexpr (SELECT) {
       float l;
       const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
-      const float w = weigh(a, row, l);
+      const float w = weigh<T, W, V, BIAS>(a, row, l);
       if (in && li < a.topk) {
         a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
         a.w[int64_t(r) * a.topk + li] = live ? w : 0.0f;
@@ -1003,8 +1017,8 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
 
 // SELECT: choose the experts (else read a.ids). SCORES: sums of s' (else counts alone).
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool SCORES>
-__global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
-  constexpr int kRows = kBalanceThreads / W;
+__global__ __launch_bounds__(balance_threads(W, V)) void balance_kernel(Args a) {
+  constexpr int kRows = balance_threads(W, V) / W;
   __shared__ uint64_t lds[SELECT ? kRows * row_words(W, V) : 1];
   __shared__ float sums[SCORES ? kRows * W * V : 1];
   __shared__ int32_t cnt[kMaxExperts];
@@ -1018,7 +1032,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
   for (int32_t at = r0; at < r1;) {
     const Piece piece = next_piece(a, at, r1);
     const bool counted = piece.seq >= 0;
-    for (int e = t; e < a.experts; e += kBalanceThreads) cnt[e] = 0;
+    for (int e = t; e < a.experts; e += balance_threads(W, V)) cnt[e] = 0;
     if (t == 0) live_rows = 0;
     __syncthreads();
     float p[V] = {};
@@ -1026,7 +1040,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
     if constexpr (!SCORES) {
       // the rows' ids are one run of memory
       const int64_t last = counted ? int64_t(piece.end) * a.topk : 0;
-      for (int64_t i = int64_t(at) * a.topk + t; i < last; i += kBalanceThreads) {
+      for (int64_t i = int64_t(at) * a.topk + t; i < last; i += balance_threads(W, V)) {
         const int id = a.ids[i];
         const bool live = a.valid == nullptr || a.valid[i / a.topk] != 0;
         if (live && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts)) atomicAdd(&cnt[id], 1);
@@ -1046,7 +1060,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_kernel(Args a) {
       __syncthreads();
       float* slot = a.slots + (int64_t(blockIdx.x) + piece.seq) * slot_words(a.experts);
       int32_t* slot_i = reinterpret_cast<int32_t*>(slot);
-      for (int e = t; e < a.experts; e += kBalanceThreads) {
+      for (int e = t; e < a.experts; e += balance_threads(W, V)) {
         if constexpr (SCORES) {
           float s = 0.0f;
           for (int i = 0; i < kRows; ++i) s += sums[i * (W * V) + e];
@@ -1315,7 +1329,7 @@ static int lanes_needed(const Args& a, bool select) {
 }
 
 // rows of a workgroup: `groups` workgroups of `threads`, whole passes of their wavefronts, at most kMaxBlockRows
-static int block_rows_for(int32_t n, int lanes_per_row, int threads = kBalanceThreads, int groups = 512) {
+static int block_rows_for(int32_t n, int lanes_per_row, int threads, int groups) {
   const int pass = threads / lanes_per_row;
   int64_t rows = (int64_t(n) + groups - 1) / groups;
   rows = (rows + pass - 1) / pass * pass;
@@ -1329,12 +1343,12 @@ struct WsPlan {
 };
 static WsPlan plan(int32_t n, int32_t experts, int32_t seqs) {
   WsPlan p = {};
-  const int rows = block_rows_for(n, 64);
+  const int rows = block_rows_for(n, 64, balance_threads(64, 16), 256);
   const uint64_t count = uint64_t(blocks_for(n, rows)) + seqs;
   auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
   p.slots = 0;
   p.part = round(count * slot_words(experts) * 4);
-  p.rows = p.part + round(uint64_t(seqs) * chunks_of(experts) * 8);
+  p.rows = p.part + round(uint64_t(seqs) * chunks_of(experts, kNarrow) * 8);
   p.ticket = p.rows + round(uint64_t(seqs) * 4);
   p.total = p.ticket + 256;
   return p;
@@ -1369,11 +1383,11 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
     return with_shape(a.experts, lanes_needed(a, select), [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value;
       // counts alone are soon summed: fewer slots for the second launch to read
-      a.block_rows = block_rows_for(a.n, W, kBalanceThreads, scores ? 512 : 64);
+      a.block_rows = block_rows_for(a.n, W, balance_threads(W, V), scores ? 256 : 64);
       a.blocks = blocks_for(a.n, a.block_rows);
       set_shape(a, W, V, sizeof(T));
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(kBalanceThreads), 0, s, a);
+        hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(scores ? balance_threads(W, V) : balance_threads(64, 4)), 0, s, a);
         AFD_CHECK_LAUNCH();
         return int(AFD_OK);
       };
@@ -1383,9 +1397,14 @@ static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t
     });
   });
   if (st != AFD_OK) return st;
-  const int64_t items = int64_t(a.seqs) * chunks_of(a.experts);
-  hipLaunchKernelGGL(finish_kernel, dim3(static_cast<unsigned>(items < 2048 ? items : 2048)), dim3(kFinishThreads), 0,
-                     s, a);
+  // (8192 x 64 in 32 sequences, 8 slots each: 9.9 us with workgroups of 64 experts, 12.0 with 16)
+  const bool broad = a.blocks / a.seqs <= kFinishThreads / kBroad;
+  const int64_t items = int64_t(a.seqs) * chunks_of(a.experts, broad ? kBroad : kNarrow);
+  const dim3 grid(static_cast<unsigned>(items < 2048 ? items : 2048));
+  if (broad)
+    hipLaunchKernelGGL(finish_kernel<kBroad>, grid, dim3(kFinishThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(finish_kernel<kNarrow>, grid, dim3(kFinishThreads), 0, s, a);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
@@ -1508,7 +1527,8 @@ extern "C" int afd_expert_counts(const int32_t* ids, int32_t n, int32_t topk, in
   a.seqs = num_seqs;
   a.counts = counts;
   router::place(a, ws, p);
-  // DIRECT
+  // one workgroup a sequence up to 16384 ids, which may all be one sequence's (4096 ids 2.8 us against 5.6 in two
+  // launches, 32768 ids 6.3, popular experts 10.5, against 5.7)
   if (n > 0 && int64_t(n) * topk <= router::kDirectIds) {
     hipLaunchKernelGGL(router::count_kernel, dim3(num_seqs), dim3(router::kCountThreads), 0,
                        static_cast<hipStream_t>(stream), a);

@@ -322,13 +322,14 @@ __device__ __forceinline__ int first_lane(bool bit, int lane) {
   return __builtin_ctzll(row_bits<W>(__ballot(bit), lane));
 }
 
-// The row's keys, taken largest first (lowest index of equals). With 4 experts a lane sorts its own
-// keys first and only its head takes part in a round: 8 picks of 256 experts cost 8 butterflies. Lanes
-// with more experts search theirs every round. Spare low bits of a key say which expert it is:
+// The row's keys, taken largest first (lowest index of equals). A lane sorts its own keys once and only
+// its head takes part in a round. Low bits of a key say which expert it is:
 // kIndexed (bf16 logits, 16 spare bits): kMaxExperts - 1 - e, so that no two are equal, the winning key
 //   names the winner and equal logits are already in index order;
-// kPlaced (choice values that carry a margin; equal ones are chosen again): 3 - the place in the lane;
-// kBare (fp32 logits, none): the places are sorted along, by adjacent exchanges (equals keep their order).
+// kPlaced: V - 1 - the place in the lane, over the value's lowest bits; values that this could bring out of
+//   order are looked at again;
+// kBare (4 fp32 logits a lane, no bias): the places are sorted along, by adjacent exchanges (equals keep
+//   their order).
 enum KeyKind { kBare, kPlaced, kIndexed };
 
 // A bf16 logit's key with its low half free: the low half is 0 of a positive number and all ones of a
@@ -341,30 +342,12 @@ __device__ __forceinline__ float index_value(uint32_t key) {
 
 template <int W, int V, KeyKind KIND>
 struct Keys {
-  static constexpr bool kSorted = V == 4;
   uint32_t key[V];
-  uint32_t order;  // sorted bare keys: byte i is the place of the i-th largest
+  uint32_t order;  // bare keys: byte i is the place of the i-th largest
 
   __device__ __forceinline__ void start(int e0) {
-    if constexpr (KIND == kIndexed) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = key[j] ? index_key(key[j]) | (kMaxExperts - 1 - e0 - j) : 0u;
-    } else if constexpr (KIND == kPlaced && kSorted) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & ~3u) | (3 - j) : 0u;
-    }
-    if constexpr (kSorted && KIND != kBare) {
-      auto sort = [&](int i, int j) {
-        const uint32_t x = key[i], y = key[j];
-        key[i] = max(x, y);
-        key[j] = min(x, y);
-      };
-      sort(0, 1);
-      sort(2, 3);
-      sort(0, 2);
-      sort(1, 3);
-      sort(1, 2);
-    } else if constexpr (kSorted) {
+    if constexpr (KIND == kBare) {
+      static_assert(V == 4, "places are bytes of a word");
       uint32_t at[4] = {0, 1, 2, 3};
 #pragma unroll
       for (int end = 3; end > 0; --end)
@@ -378,61 +361,66 @@ struct Keys {
           at[i + 1] = swap ? x : at[i + 1];
         }
       order = at[0] | at[1] << 8 | at[2] << 16 | at[3] << 24;
+      return;
     }
-  }
-  __device__ __forceinline__ uint32_t head() const {
-    uint32_t best = key[0];
-    if constexpr (!kSorted) {
 #pragma unroll
-      for (int j = 1; j < V; ++j) best = max(best, key[j]);
+    for (int j = 0; j < V; ++j) {
+      if constexpr (KIND == kIndexed)
+        key[j] = key[j] ? index_key(key[j]) | (kMaxExperts - 1 - e0 - j) : 0u;
+      else
+        key[j] = key[j] ? (key[j] & ~uint32_t(V - 1)) | (V - 1 - j) : 0u;
     }
-    return best;
+    // odd-even merge sort, largest first: 5, 19 or 63 exchanges of a maximum and a minimum
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+      for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+        for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+          for (int i = 0; i < k; ++i)
+            if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+              const uint32_t x = key[i + j], y = key[i + j + k];
+              key[i + j] = max(x, y);
+              key[i + j + k] = min(x, y);
+            }
   }
-  __device__ __forceinline__ void pop(bool mine) {
-    key[0] = mine ? key[1] : key[0];
-    key[1] = mine ? key[2] : key[1];
-    key[2] = mine ? key[3] : key[2];
-    key[3] = mine ? 0u : key[3];
-  }
+  __device__ __forceinline__ uint32_t head() const { return key[0]; }
   // Takes the largest key m and returns its expert, the same in every lane of the row.
   __device__ __forceinline__ int next(int lane, int e0, uint32_t& m) {
-    const uint32_t best = head();
-    m = max_u32<W>(best);
+    m = max_u32<W>(key[0]);
+    bool mine;
+    int e = 0, win = 0;
     if constexpr (KIND == kIndexed) {
-      if constexpr (kSorted) {
-        pop(key[0] == m);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) key[j] = key[j] == m ? 0u : key[j];
-      }
-      return kMaxExperts - 1 - static_cast<int>(m & (kMaxExperts - 1));
+      mine = key[0] == m;
+      e = kMaxExperts - 1 - static_cast<int>(m & (kMaxExperts - 1));
     } else {
-      const int win = first_lane<W>(best == m, lane);
-      const bool mine = (lane & (W - 1)) == win;
-      if constexpr (kSorted && KIND == kPlaced) {
-        pop(mine);
-        return win * 4 + 3 - static_cast<int>(m & 3);
+      win = first_lane<W>(key[0] == m, lane);
+      mine = (lane & (W - 1)) == win;
+      if constexpr (KIND == kPlaced) {
+        e = win * V + V - 1 - static_cast<int>(m & (V - 1));
       } else {
-        int e;
-        if constexpr (kSorted) {
-          e = e0 + static_cast<int>(order & 0xff);
-          order = mine ? order >> 8 : order;
-          pop(mine);
-        } else {
-          int at = V - 1;
-#pragma unroll
-          for (int j = V - 2; j >= 0; --j) at = key[j] == m ? j : at;
-          e = e0 + at;
-#pragma unroll
-          for (int j = 0; j < V; ++j) key[j] = mine && j == at ? 0u : key[j];
-        }
-        // read by all lanes: the winner's e is made in them
-        if constexpr (W == 64) return __builtin_amdgcn_readlane(e, win);
-        return __shfl(e, win, W);
+        e = e0 + static_cast<int>(order & 0xff);
+        order = mine ? order >> 8 : order;
       }
     }
+#pragma unroll
+    for (int j = 0; j + 1 < V; ++j) key[j] = mine ? key[j + 1] : key[j];
+    key[V - 1] = mine ? 0u : key[V - 1];
+    if constexpr (KIND == kBare) {
+      // read by all lanes: the winner's e is made in them
+      if constexpr (W == 64) return __builtin_amdgcn_readlane(e, win);
+      return __shfl(e, win, W);
+    }
+    return e;
   }
 };
+
+// A placed key's value for comparisons (-inf, whose place bits make it a NaN, is -inf)
+__device__ __forceinline__ float placed_value(uint32_t key) {
+  const float v = value_of(key);
+  return v != v ? kLowest : v;
+}
 
 // LDS of a row: the keys of the 64-bit choice
 __host__ __device__ constexpr int row_words(int W, int V) { return W * V; }
@@ -450,6 +438,22 @@ __device__ __forceinline__ int best_lane(uint64_t key, int lane) {
   return first_lane<W>(hi == m_hi && static_cast<uint32_t>(key) == m_lo, lane);
 }
 
+// A softmax's largest logit and sum in 64 bits
+template <typename T, int W, int V>
+__device__ __forceinline__ void softmax_f64(const Args& a, const T* p, int e0, double& at, double& sum) {
+  float m = kLowest;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) m = fmaxf(m, e0 + j < a.experts ? canon(logit_f32(p + e0 + j)) : kLowest);
+  m = max_f32<W>(m);
+  at = m == kLowest ? 0.0 : static_cast<double>(m);
+  sum = 0.0;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j)
+    if (e0 + j < a.experts) sum += score_f64(canon(logit_f32(p + e0 + j)) - at, AFD_SCORE_SOFTMAX);
+  sum = sum_f64<W>(sum);
+  if (sum == 0.0) sum = 1.0;
+}
+
 // The choice in 64 bits, and with groups of any size: lane kk < topk gets the kk-th expert. Rare, so
 // its values live in LDS and its loops stay loops: it must not cost the usual case its registers.
 template <typename T, int W, int V, bool BIAS>
@@ -457,14 +461,7 @@ __device__ __forceinline__ int choose_f64(const Args& a, int64_t t, int lane, ui
   const int li = lane & (W - 1), e0 = li * V;
   const T* p = static_cast<const T*>(a.logits) + t * a.ld;
   double at = 0.0, sum = 1.0;
-  if (BIAS && a.scoring == AFD_SCORE_SOFTMAX) {
-    float m = kLowest;
-#pragma unroll 1
-    for (int j = 0; j < V; ++j) m = fmaxf(m, e0 + j < a.experts ? canon(logit_f32(p + e0 + j)) : kLowest);
-    m = max_f32<W>(m);
-    at = m == kLowest ? 0.0 : static_cast<double>(m);
-  }
-  sum = 0.0;
+  if (BIAS && a.scoring == AFD_SCORE_SOFTMAX) softmax_f64<T, W, V>(a, p, e0, at, sum);
 #pragma unroll 1
   for (int j = 0; j < V; ++j) {
     uint64_t key = 0;
@@ -472,26 +469,13 @@ __device__ __forceinline__ int choose_f64(const Args& a, int64_t t, int lane, ui
       double c = canon(logit_f32(p + e0 + j));
       if constexpr (BIAS) {
         c = score_f64(c - at, a.scoring);  // at is 0 but for softmax
-        sum += c;
+        if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
+        c += a.bias[e0 + j];
+        if (c != c) c = -__builtin_huge_val();
       }
-      key = __builtin_bit_cast(uint64_t, c);
+      key = key64(c);
     }
     keys[e0 + j] = key;
-  }
-  if (BIAS && a.scoring == AFD_SCORE_SOFTMAX) {
-    sum = sum_f64<W>(sum);
-    if (sum == 0.0) sum = 1.0;
-  }
-#pragma unroll 1
-  for (int j = 0; j < V; ++j) {
-    if (e0 + j >= a.experts) break;
-    double c = __builtin_bit_cast(double, keys[e0 + j]);
-    if constexpr (BIAS) {
-      if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
-      c += a.bias[e0 + j];
-      if (c != c) c = -__builtin_huge_val();
-    }
-    keys[e0 + j] = key64(c);
   }
   lds_fence();
   if (a.groups > 1) {
@@ -603,18 +587,58 @@ __device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], i
   return kept;
 }
 
-// Close choice values in 64 bits. The fp32 choice is right but for experts within `margin` of each
+// keep_group in 64 bits, for groups whose fp32 values are close. Rare: its loops stay loops.
+template <typename T, int W, int V>
+__device__ __forceinline__ bool keep_group_f64(const Args& a, int64_t t, int lane) {
+  const int li = lane & (W - 1), e0 = li * V, gl = a.group_lanes;
+  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
+  double at = 0.0, sum = 1.0;
+  if (a.scoring == AFD_SCORE_SOFTMAX) softmax_f64<T, W, V>(a, p, e0, at, sum);
+  double first = -__builtin_huge_val(), second = first;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    if (e0 + j >= a.experts) break;
+    double c = score_f64(canon(logit_f32(p + e0 + j)) - at, a.scoring);
+    if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
+    c += a.bias[e0 + j];
+    if (c != c) c = -__builtin_huge_val();
+    second = fmax(second, fmin(first, c));
+    first = fmax(first, c);
+  }
+#pragma unroll 1
+  for (int d = 1; d < gl; d *= 2) {
+    const double f = __shfl_xor(first, d, W), s = __shfl_xor(second, d, W);
+    second = fmax(fmax(second, s), fmin(first, f));
+    first = fmax(first, f);
+  }
+  double value = first + second;
+  if (value != value) value = -__builtin_huge_val();
+  uint64_t key = (li & (gl - 1)) == 0 && li < a.groups * gl ? key64(value) : 0u;
+  bool kept = false;
+  for (int i = 0; i < a.keep; ++i) {
+    const int win = best_lane<W>(key, lane);
+    if (li == win) key = 0;
+    kept |= (li & ~(gl - 1)) == win;
+  }
+  return kept;
+}
+
+// A placed key is off by at most 15 ulps of 2^-23 of its value, two of them by twice that.
+constexpr float kPlaceError = 0x1p-18f;
+
+// Close choice values in 64 bits (no bias: the logits themselves). The fp32 choice is right but for experts within `margin` of each
 // other, so the chosen ones and every other within it of the last (taken on from `keys`) are ranked
 // by their 64-bit values, one a lane. False if they are more than the row's lanes.
-template <typename T, int W, int V>
+template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint64_t* lds_row,
                                        Keys<W, V, kPlaced>& keys, float margin, uint32_t taken, int& id) {
   const int li = lane & (W - 1), e0 = li * V;
-  const float bar = value_of(__shfl(taken, a.topk - 1, W)) - margin;
+  const float worst = placed_value(__shfl(taken, a.topk - 1, W));
+  const float bar = worst - (BIAS ? margin : kPlaceError * 2.0f * fabsf(worst));
   int count = a.topk;
   while (true) {
     const uint32_t top = max_u32<W>(keys.head());
-    const bool more = top != 0 && !(value_of(top) < bar);
+    const bool more = top != 0 && !(placed_value(top) < bar);
     if (__ballot(more && count == W)) return false;
     if (!__ballot(more)) break;
     const Keys<W, V, kPlaced> before = keys;
@@ -625,24 +649,15 @@ __device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint6
     count += more ? 1 : 0;
   }
   const T* p = static_cast<const T*>(a.logits) + t * a.ld;
-  double at = 0.0, sum = 1.0;
-  if (a.scoring == AFD_SCORE_SOFTMAX) {
-    float m = kLowest;
-#pragma unroll 1
-    for (int j = 0; j < V; ++j) m = fmaxf(m, e0 + j < a.experts ? canon(logit_f32(p + e0 + j)) : kLowest);
-    m = max_f32<W>(m);
-    at = m == kLowest ? 0.0 : static_cast<double>(m);
-    sum = 0.0;
-#pragma unroll 1
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < a.experts) sum += score_f64(canon(logit_f32(p + e0 + j)) - at, a.scoring);
-    sum = sum_f64<W>(sum);
-    if (sum == 0.0) sum = 1.0;
+  double c = canon(logit_f32(p + (li < count ? id : 0)));
+  if constexpr (BIAS) {
+    double at = 0.0, sum = 1.0;
+    if (a.scoring == AFD_SCORE_SOFTMAX) softmax_f64<T, W, V>(a, p, e0, at, sum);
+    c = score_f64(c - at, a.scoring);
+    if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
+    c += a.bias[li < count ? id : 0];
+    if (c != c) c = -__builtin_huge_val();
   }
-  double c = score_f64(canon(logit_f32(p + (li < count ? id : 0))) - at, a.scoring);
-  if (a.scoring == AFD_SCORE_SOFTMAX) c /= sum;
-  c += a.bias[li < count ? id : 0];
-  if (c != c) c = -__builtin_huge_val();
   const uint64_t key = key64(c);
   const uint32_t lo = static_cast<uint32_t>(key), hi = static_cast<uint32_t>(key >> 32);
   int rank = 0;
@@ -672,9 +687,9 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
   if constexpr (BIAS) {
     // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal
     // and root are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together,
-    // and the two bits that hold the place take 6; a softmax's sum over 16 values a lane and 6
-    // butterflies brings it to 40, so 2^-18 there. Two values stand apart if they differ by twice
-    // the row's largest such bound.
+    // and two bits that hold the place take 6. Four such bits take 30, a softmax's sum over 16 values a lane
+    // and 6 butterflies 24: 2^-18 there. Two values stand apart if they differ by twice the row's
+    // largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
@@ -683,18 +698,23 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
       most = fmaxf(most, score + fabsf(bias[j]));
     }
-    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX ? 0x1p-17f : 0x1p-19f);
+    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX || V > 4 ? 0x1p-17f : 0x1p-19f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
   }
-  Keys<W, V, BIAS ? kPlaced : sizeof(T) == 2 ? kIndexed : kBare> keys;
+  constexpr KeyKind kKind = BIAS ? kPlaced : sizeof(T) == 2 ? kIndexed : V == 4 ? kBare : kPlaced;
+  Keys<W, V, kKind> keys;
 #pragma unroll
   for (int j = 0; j < V; ++j) keys.key[j] = e0 + j < a.experts ? key32(c[j]) : 0;
   if (a.groups > 1) {
     if (a.group_lanes) {
       // a group's value is the sum of two choice values: twice the margin
-      const bool kept = keep_group<W, V, BIAS>(a, c, lane, 2.0f * margin, sure);
+      bool kept = keep_group<W, V, BIAS>(a, c, lane, 2.0f * margin, sure);
+      if constexpr (BIAS) {
+        if (__ballot(!sure)) kept = keep_group_f64<T, W, V>(a, t, lane);
+        sure = true;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) keys.key[j] = kept ? keys.key[j] : 0;
     } else {
@@ -711,19 +731,22 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     taken = li == kk ? m : taken;
   }
   const bool live = li < a.topk;
-  bool all = __ballot(!sure) != 0;  // groups not settled (or not of whole lanes): the whole choice in 64 bits
-  if constexpr (BIAS) {
+  bool all = !sure;  // groups that are not whole lanes (for every row alike): the whole choice in 64 bits
+  if constexpr (kKind == kPlaced) {
     if (!all) {
       // lane kk compares the kk-th with the next one, the last with the best that is left
       const uint32_t left = max_u32<W>(keys.head());
       const uint32_t after = __shfl_down(taken, 1, W);
       const uint32_t below = li == a.topk - 1 ? left : after;
-      const bool close = live && below != 0 && !(value_of(taken) - value_of(below) > margin);
-      if (__ballot(close)) all = !settle<T, W, V>(a, t, lane, lds_row, keys, margin, taken, id);
+      const float x = placed_value(taken), y = placed_value(below);
+      const float apart = BIAS ? margin : kPlaceError * fmaxf(fabsf(x), fabsf(y));
+      // (-inf behind a number is far)
+      const bool close = live && below != 0 && !(x - y > apart || (y == kLowest && x != kLowest && !BIAS));
+      if (__ballot(close)) all = !settle<T, W, V, BIAS>(a, t, lane, lds_row, keys, margin, taken, id);
     }
   }
   if (all) id = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
-  if (all || BIAS) {
+  if (all || kKind == kPlaced) {
     // the row's logits (scores) by way of LDS
     float* mine = reinterpret_cast<float*>(lds_row);
     if (BIAS && a.scoring != AFD_SCORE_SOFTMAX) {
@@ -1270,6 +1293,20 @@ int with_shape(int experts, int lanes, F&& f) {
   if (experts <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
   return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
+// Choosing by the logits alone, many rows: 16 lanes a row, so that what a row costs beside its experts
+// (rounds, sums, weights) is shared by 4 rows of a wavefront. 256 experts: 4096 rows 5.4 us against 5.0 in
+// the shapes above, 8192 6.4 against 7.5, 65536 26.7 against 43.7. With a bias the scores cost more than the
+// rounds and the close rows' 64-bit work is longer with 16 experts a lane (16384 rows 19.3 against 16.2).
+constexpr int kManyRows = 6144;
+template <typename F>
+int with_choice_shape(int experts, int lanes, bool bias, int n, F&& f) {
+  using std::integral_constant;
+  if (!bias && n >= kManyRows && lanes <= 16 && experts > 64) {
+    if (experts <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    if (experts <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  }
+  return with_shape(experts, lanes, f);
+}
 template <typename F>
 int with_logits(int fmt, F&& f) {
   return fmt == AFD_LOGITS_F32 ? f(float{}) : f(uint16_t{});
@@ -1429,7 +1466,7 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
   a.w = w;
   return router::with_logits(cfg->logits_fmt, [&](auto tag) {
     using T = decltype(tag);
-    return router::with_shape(a.experts, router::lanes_needed(a, true), [&](auto wc, auto vc) {
+    return router::with_choice_shape(a.experts, router::lanes_needed(a, true), bias != nullptr, n, [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
       router::set_shape(a, W, V, sizeof(T));
       int64_t grid = (int64_t(n) + kRows - 1) / kRows;
@@ -1440,7 +1477,10 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
         AFD_CHECK_LAUNCH();
         return int(AFD_OK);
       };
-      return bias ? go(router::topk_kernel<T, W, V, true>) : go(router::topk_kernel<T, W, V, false>);
+      if constexpr (W == 16 && V > 4)
+        return go(router::topk_kernel<T, W, V, false>);
+      else
+        return bias ? go(router::topk_kernel<T, W, V, true>) : go(router::topk_kernel<T, W, V, false>);
     });
   });
 }

@@ -380,3 +380,71 @@ def test_no_second_derivative(which):
     assert torch.equal(plain, graph.detach())
     with pytest.raises(RuntimeError):
         graph.sum().backward()
+
+
+MANY = 6151  # above the rows from which 16 lanes hold a row
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("experts,top_k,groups,keep", [(64, 8, 8, 3), (100, 6, 0, 0), (128, 16, 16, 9), (129, 4, 3, 2),
+                                                       (200, 1, 0, 0), (256, 8, 8, 4), (256, 16, 16, 3)])
+def test_choice_of_many_rows(experts, top_k, groups, keep, bias, scoring):
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, b = make(MANY, experts, experts + 3, dtype, bias)
+        renorm = experts % 2 == 0
+        say(f"many rows E={experts} k={top_k} groups={groups}/{keep} {scoring} bias={bias} {dtype}")
+        out = select(logits, top_k, b, scoring=scoring, renormalize=renorm, groups=groups, keep=keep, scale=1.5)
+        check_choice(logits, top_k, out, scoring, b, renorm, 1.5, groups, keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("experts", [72, 160])
+def test_ties_close_scores_and_masks_of_many_rows(experts, bias, scoring):
+    g = torch.Generator().manual_seed(experts)
+    n = MANY
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.randn(n, experts, generator=g)
+        sign = torch.where(torch.rand(n, experts, generator=g) < 0.5, -1.0, 1.0)
+        logits[::3] = (torch.randint(-2, 2, (n, experts), generator=g).float() * sign)[::3]  # ties, both zeros
+        logits[1::3, experts // 2 :] = logits[1::3, : experts // 2] * (1 + 2.0**-22)  # next floats
+        logits[torch.rand(n, experts, generator=g) < 0.02] = -math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.005] = math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.005] = math.nan
+        logits[torch.rand(n, experts, generator=g) < 0.01] = torch.finfo(dtype).min
+        logits[5, 4:], logits[6], logits[7] = -math.inf, -math.inf, math.nan
+        logits = logits.to(dtype)
+        b = torch.randint(-1, 2, (experts,), generator=g).float() * 2.0**-40 if bias else None
+        for groups, keep in ((0, 0), (8, 3)):
+            say(f"many rows, ties and masks E={experts} {scoring} bias={bias} {dtype} groups={groups}")
+            out = select(logits, 7, b, scoring=scoring, groups=groups, keep=keep)
+            check_choice(logits, 7, out, scoring, b, groups=groups, keep=keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("experts,top_k,bias,renorm", [(60, 4, False, False), (128, 8, True, True), (160, 6, True, False), (256, 8, False, True)])
+def test_gradients_of_many_rows(experts, top_k, bias, renorm, scoring):
+    n, scale, alpha, cu = MANY, 1.5, 5.0, [2, 12, 1500, 1500, 4000]
+    for dtype in (torch.float32, torch.bfloat16):
+        logits, b = make(n, experts, experts + 9, dtype, bias)
+        g = torch.Generator().manual_seed(experts)
+        gw = torch.randn(n, top_k, generator=g)
+        valid = torch.rand(n, generator=g) < 0.9
+        say(f"many rows, gradients E={experts} bias={bias} renorm={renorm} {scoring} {dtype}")
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, cnt = B.select_and_balance(leaf, top_k, alpha=alpha, scoring=scoring, renormalize=renorm,
+                                              correction_bias=None if b is None else b.to(dev()), routed_scaling_factor=scale,
+                                              valid=valid.to(dev()), cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev()))
+        ids = check_choice(logits, top_k, out, scoring, b, renorm, scale, valid=valid)
+        assert torch.equal(cnt.cpu().long(), R.counts(ids, experts, cu, valid))
+        want = float(R.balance(R.canon(logits), ids, scoring, alpha, cu, valid))
+        assert abs(float(loss.detach()) - want) <= 2.0**-16 * abs(want)
+        for lo, hi in ((True, True), (False, True)):
+            outs = ([out.topk_weights] if lo else []) + [loss]
+            gs = ([gw.to(dev())] if lo else []) + [torch.tensor(2.0, device=dev())]
+            (got,) = torch.autograd.grad(outs, (leaf,), gs, retain_graph=True)
+            ref = R.grads(logits, ids.clamp_min(0), scoring, renorm, scale, gw if lo else None, 2.0, alpha, cu, valid)
+            tol = 2.0**-16 * (scale * float(gw.abs().max()) if lo else 0.0) + 2.0**-16 * 2 * alpha * experts / 10
+            tol = tol + (2.0**-8 * ref.abs() if dtype == torch.bfloat16 else 0.0)
+            assert ((got.cpu().double() - ref).abs() <= tol).all()

@@ -17,9 +17,9 @@
 //   coef = alpha E / (S' k T^2),  r = 1, 1 - sigmoid(l), sigmoid(l) / (2 softplus(l)).
 //
 // Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
-// and a lane's first V bytes are one wide load: 16 lanes (4 rows a wavefront) up to 64 experts, 32
-// up to 128, else 64 lanes with V = 4, 8 or 16. Reductions over a row are DPP and permlane-swap butterflies; the k-th
-// winner is a max butterfly and one ballot.
+// and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
+// else 64 lanes with V = 4, 8 or 16; where many rows choose by their logits alone, 16 lanes up to 256 experts. A
+// lane sorts its values once; a pick is then a max butterfly (DPP and permlane swaps) over the lanes' heads.
 //
 // Sums over rows: a workgroup takes R consecutive rows, cut where sequences begin and end; each piece
 // writes its sums and counts to a slot of its own (slot = workgroup + sequence: from one piece to the
@@ -51,7 +51,8 @@ struct Args {
   const uint8_t* valid;
   int32_t n;
   int32_t experts, topk, scoring, groups, keep, renorm;
-  int32_t group_lanes;  // lanes of a group where it is 1, 2, 4, .. whole lanes of V experts, else 0
+  int32_t group_lanes;  // lanes that make a group's value, a power of two
+  bool whole_lanes;     // ... and hold its experts
   bool wide;            // rows take 4-element loads and stores
   float scale;
   int32_t* ids;  // selection: written; balance and gradient: read
@@ -200,14 +201,14 @@ __device__ __forceinline__ float log1p_f32(float e) {
   const float h = z + z;
   return __builtin_fmaf(h * q, p, h);
 }
-// sigmoid or sqrt(softplus)
+// sigmoid or sqrt(softplus); the latter is e^(v/2) (1 - e^v / 4 + ..) of a small v, whose e^v may have left the floats
+constexpr float kSmall = -17.0f;
+template <bool EXACT>
 __device__ __forceinline__ float score_f32(float v, int scoring) {
-  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_f32(-v));
-  return __builtin_amdgcn_sqrtf(log1p_f32(exp_f32(-fabsf(v))) + fmaxf(v, 0.0f));
-}
-__device__ __forceinline__ float score_fast(float v, int scoring) {
-  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_fast(-v));
-  return __builtin_amdgcn_sqrtf(log1p_f32(exp_fast(-fabsf(v))) + fmaxf(v, 0.0f));
+  auto e_to = [](float x) { return EXACT ? exp_f32(x) : exp_fast(x); };
+  if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + e_to(-v));
+  const float e = e_to(v < kSmall ? 0.5f * v : -fabsf(v));
+  return v < kSmall ? e : __builtin_amdgcn_sqrtf(log1p_f32(e) + fmaxf(v, 0.0f));
 }
 // e^v (softmax, v relative to the row's largest), sigmoid or sqrt(softplus) in 64 bits: called, not inlined, so
 // its registers are not the callers'
@@ -222,7 +223,7 @@ __device__ __attribute__((noinline)) double score_f64(double v, int scoring) {
 __device__ __forceinline__ float slope_f32(float v, float score, int scoring) {
   if (scoring == AFD_SCORE_SOFTMAX) return 1.0f;
   if (scoring == AFD_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + exp_fast(v));
-  if (v < -17.0f) return 0.5f;
+  if (v < kSmall) return 0.5f;
   return 0.5f * __builtin_amdgcn_rcpf((1.0f + exp_fast(-v)) * (score * score));
 }
 
@@ -298,10 +299,10 @@ struct Row {
     }
     if (a.scoring == AFD_SCORE_SIGMOID) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[j] = EXACT ? score_f32(l[j], AFD_SCORE_SIGMOID) : score_fast(l[j], AFD_SCORE_SIGMOID);
+      for (int j = 0; j < V; ++j) s[j] = score_f32<EXACT>(l[j], AFD_SCORE_SIGMOID);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[j] = EXACT ? score_f32(l[j], AFD_SCORE_SQRTSOFTPLUS) : score_fast(l[j], AFD_SCORE_SQRTSOFTPLUS);
+      for (int j = 0; j < V; ++j) s[j] = score_f32<EXACT>(l[j], AFD_SCORE_SQRTSOFTPLUS);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) sum += s[j];  // 0 of -inf, past the last expert
@@ -454,7 +455,7 @@ __device__ __forceinline__ void softmax_f64(const Args& a, const T* p, int e0, d
   if (sum == 0.0) sum = 1.0;
 }
 
-// The choice in 64 bits, and with groups of any size: lane kk < topk gets the kk-th expert. Rare, so
+// The choice in 64 bits, groups of any size: lane kk < topk gets the kk-th expert. Rare, so
 // its values live in LDS and its loops stay loops: it must not cost the usual case its registers.
 template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ int choose_f64(const Args& a, int64_t t, int lane, uint64_t* keys) {
@@ -544,21 +545,41 @@ __device__ __forceinline__ float step_f32(float v, int lane) {
   return __uint_as_float(lane & 32 ? r[0] : r[1]);
 }
 
-// Which groups stay, groups of whole lanes (a.group_lanes, a power of two), choice values in fp32: true
-// if the lane's group stays. sure: false if the worst kept and the best dropped are within `margin`.
+// A bit for each lane of a row
+template <int W>
+using Lanes = std::conditional_t<W == 64, uint64_t, uint32_t>;
+
+// Which groups stay, by choice values in fp32, as the bits of their first lanes (lane gl g of the row stands for
+// group g, gl = a.group_lanes). sure: false if the worst kept and the best dropped are within `margin`.
+// Groups of 1, 2, 4, .. whole lanes are made from the lanes' own values; others go through LDS, where the
+// gl = 1, 2, 4, .. lanes that a group can have read its values in turn (16384 rows, 160 experts in 8
+// groups: 11.7 us, as the 64-bit choice below 47.6).
 template <int W, int V, bool BIAS>
-__device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], int lane, float margin, bool& sure) {
-  float first = c[0], second = kLowest;
-#pragma unroll
-  for (int j = 1; j < V; ++j) {
-    second = fmaxf(second, fminf(first, c[j]));
-    first = fmaxf(first, c[j]);
-  }
+__device__ __forceinline__ Lanes<W> keep_groups(const Args& a, const float (&c)[V], int lane, float* lds_row,
+                                                float margin, bool& sure) {
+  const int li = lane & (W - 1), gl = a.group_lanes;
+  float first = kLowest, second = kLowest;
+  auto add = [&](float f) {
+    second = fmaxf(second, fminf(first, f));
+    first = fmaxf(first, f);
+  };
   auto merge = [&](float f, float s) {
     second = fmaxf(fmaxf(second, s), fminf(first, f));
     first = fmaxf(first, f);
   };
-  const int gl = a.group_lanes;
+  const int size = a.experts / a.groups;
+  if (a.whole_lanes) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) add(c[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds_row[li * V + j] = c[j];
+    lds_fence();
+    // (lanes past the last group read the last one's values)
+    const int log_gl = __builtin_ctz(gl), g = min(li >> log_gl, a.groups - 1);
+    for (int i = li & (gl - 1); i < size; i += gl) add(lds_row[g * size + i]);
+    lds_fence();
+  }
   if (gl > 1) merge(step_f32<1>(first, lane), step_f32<1>(second, lane));
   if (gl > 2) merge(step_f32<2>(first, lane), step_f32<2>(second, lane));
   if (gl > 4) merge(step_f32<4>(first, lane), step_f32<4>(second, lane));
@@ -567,17 +588,15 @@ __device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], i
     if (gl > 16) merge(step_f32<16>(first, lane), step_f32<16>(second, lane));
   if constexpr (W > 32)
     if (gl > 32) merge(step_f32<32>(first, lane), step_f32<32>(second, lane));
-  const float value = BIAS ? first + second : first;
-  const int li = lane & (W - 1);
-  // the first lane of a group stands for it
+  const float value = BIAS && size > 1 ? first + second : first;
   uint32_t key = (li & (gl - 1)) == 0 && li < a.groups * gl ? key32(value) : 0u;
-  bool kept = false;
+  Lanes<W> kept = 0;
   float worst = 0.0f;
   for (int i = 0; i < a.keep; ++i) {
     const uint32_t m = max_u32<W>(key);
     const int win = first_lane<W>(key == m, lane);
     if (li == win) key = 0;
-    kept |= (li & ~(gl - 1)) == win;
+    kept |= Lanes<W>(1) << win;
     worst = value_of(m);
   }
   if constexpr (BIAS) {
@@ -587,9 +606,9 @@ __device__ __forceinline__ bool keep_group(const Args& a, const float (&c)[V], i
   return kept;
 }
 
-// keep_group in 64 bits, for groups whose fp32 values are close. Rare: its loops stay loops.
+// keep_groups in 64 bits, for groups of whole lanes whose fp32 values are close. Rare: its loops stay loops.
 template <typename T, int W, int V>
-__device__ __forceinline__ bool keep_group_f64(const Args& a, int64_t t, int lane) {
+__device__ __forceinline__ Lanes<W> keep_groups_f64(const Args& a, int64_t t, int lane) {
   const int li = lane & (W - 1), e0 = li * V, gl = a.group_lanes;
   const T* p = static_cast<const T*>(a.logits) + t * a.ld;
   double at = 0.0, sum = 1.0;
@@ -614,27 +633,27 @@ __device__ __forceinline__ bool keep_group_f64(const Args& a, int64_t t, int lan
   double value = first + second;
   if (value != value) value = -__builtin_huge_val();
   uint64_t key = (li & (gl - 1)) == 0 && li < a.groups * gl ? key64(value) : 0u;
-  bool kept = false;
+  Lanes<W> kept = 0;
   for (int i = 0; i < a.keep; ++i) {
     const int win = best_lane<W>(key, lane);
     if (li == win) key = 0;
-    kept |= (li & ~(gl - 1)) == win;
+    kept |= Lanes<W>(1) << win;
   }
   return kept;
 }
 
-// A placed key is off by at most 15 ulps of 2^-23 of its value, two of them by twice that.
-constexpr float kPlaceError = 0x1p-18f;
+// A placed key is off by at most 15 ulps of 2^-23 of its value or, near zero, of 2^-149; two of them by twice that.
+__device__ __forceinline__ float place_error(float v) { return __builtin_fmaf(fabsf(v), 0x1p-18f, 0x1p-144f); }
 
-// Close choice values in 64 bits (no bias: the logits themselves). The fp32 choice is right but for experts within `margin` of each
-// other, so the chosen ones and every other within it of the last (taken on from `keys`) are ranked
-// by their 64-bit values, one a lane. False if they are more than the row's lanes.
+// Close choice values in 64 bits (no bias: the logits themselves). The fp32 choice is right but for experts within
+// `margin` of each other, so the chosen ones and every other within it of the last (taken on from `keys`) are
+// ranked by their 64-bit values, one a lane. False if they are more than the row's lanes.
 template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint64_t* lds_row,
                                        Keys<W, V, kPlaced>& keys, float margin, uint32_t taken, int& id) {
   const int li = lane & (W - 1), e0 = li * V;
   const float worst = placed_value(__shfl(taken, a.topk - 1, W));
-  const float bar = worst - (BIAS ? margin : kPlaceError * 2.0f * fabsf(worst));
+  const float bar = worst - (BIAS ? margin : 2.0f * place_error(worst));
   int count = a.topk;
   while (true) {
     const uint32_t top = max_u32<W>(keys.head());
@@ -688,8 +707,8 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal
     // and root are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together,
     // and two bits that hold the place take 6. Four such bits take 30, a softmax's sum over 16 values a lane
-    // and 6 butterflies 24: 2^-18 there. Two values stand apart if they differ by twice the row's
-    // largest such bound.
+    // and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if they
+    // differ by twice the row's largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
@@ -698,7 +717,7 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
       most = fmaxf(most, score + fabsf(bias[j]));
     }
-    margin = max_f32<W>(most) * (a.scoring == AFD_SCORE_SOFTMAX || V > 4 ? 0x1p-17f : 0x1p-19f);
+    margin = __builtin_fmaf(max_f32<W>(most), a.scoring == AFD_SCORE_SOFTMAX || V > 4 ? 0x1p-17f : 0x1p-19f, 0x1p-124f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
@@ -708,17 +727,28 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
 #pragma unroll
   for (int j = 0; j < V; ++j) keys.key[j] = e0 + j < a.experts ? key32(c[j]) : 0;
   if (a.groups > 1) {
-    if (a.group_lanes) {
-      // a group's value is the sum of two choice values: twice the margin
-      bool kept = keep_group<W, V, BIAS>(a, c, lane, 2.0f * margin, sure);
-      if constexpr (BIAS) {
-        if (__ballot(!sure)) kept = keep_group_f64<T, W, V>(a, t, lane);
+    // a group's value is the sum of two choice values: twice the margin
+    Lanes<W> kept = keep_groups<W, V, BIAS>(a, c, lane, reinterpret_cast<float*>(lds_row), 2.0f * margin, sure);
+    if constexpr (BIAS) {
+      sure = !__ballot(!sure);
+      if (!sure && a.whole_lanes) {
+        kept = keep_groups_f64<T, W, V>(a, t, lane);
         sure = true;
       }
+    }
+    if (a.whole_lanes) {
+      const bool mine = kept >> (li & ~(a.group_lanes - 1)) & 1;
 #pragma unroll
-      for (int j = 0; j < V; ++j) keys.key[j] = kept ? keys.key[j] : 0;
+      for (int j = 0; j < V; ++j) keys.key[j] = mine ? keys.key[j] : 0;
     } else {
-      sure = false;
+      // e / size for e < 1024: the quotient of e + 1/2 is at least 1 / (2 size) from a whole number
+      const float per = 1.0f / (a.experts / a.groups);
+      const int gl = a.group_lanes;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int g = static_cast<int>((e0 + j + 0.5f) * per);
+        keys.key[j] = kept >> ((g * gl) & (W - 1)) & 1 ? keys.key[j] : 0;
+      }
     }
   }
   keys.start(e0);
@@ -731,7 +761,7 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     taken = li == kk ? m : taken;
   }
   const bool live = li < a.topk;
-  bool all = !sure;  // groups that are not whole lanes (for every row alike): the whole choice in 64 bits
+  bool all = !sure;  // close groups that are not whole lanes: the whole choice in 64 bits
   if constexpr (kKind == kPlaced) {
     if (!all) {
       // lane kk compares the kk-th with the next one, the last with the best that is left
@@ -739,14 +769,14 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       const uint32_t after = __shfl_down(taken, 1, W);
       const uint32_t below = li == a.topk - 1 ? left : after;
       const float x = placed_value(taken), y = placed_value(below);
-      const float apart = BIAS ? margin : kPlaceError * fmaxf(fabsf(x), fabsf(y));
+      const float apart = BIAS ? margin : place_error(fmaxf(fabsf(x), fabsf(y)));
       // (-inf behind a number is far)
       const bool close = live && below != 0 && !(x - y > apart || (y == kLowest && x != kLowest && !BIAS));
       if (__ballot(close)) all = !settle<T, W, V, BIAS>(a, t, lane, lds_row, keys, margin, taken, id);
     }
   }
-  if (all) id = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
-  if (all || kKind == kPlaced) {
+  if constexpr (kKind == kPlaced) {
+    if (all) id = choose_f64<T, W, V, BIAS>(a, t, lane, lds_row);
     // the row's logits (scores) by way of LDS
     float* mine = reinterpret_cast<float*>(lds_row);
     if (BIAS && a.scoring != AFD_SCORE_SOFTMAX) {
@@ -789,7 +819,7 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, f
     sum = sum_f32<W>(sum);
     return sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
   }
-  s = BIAS ? fmaxf(l, 0.0f) : score_f32(l, a.scoring);
+  s = BIAS ? fmaxf(l, 0.0f) : score_f32<true>(l, a.scoring);
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
     s = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
@@ -1224,7 +1254,7 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
           m = max_f32<W>(m);
           share = id >= 0 ? exp_f32(l - (m == kLowest ? 0.0f : m)) : 0.0f;
         } else {
-          share = id >= 0 ? score_f32(l, a.scoring) : 0.0f;
+          share = id >= 0 ? score_f32<true>(l, a.scoring) : 0.0f;
         }
         const float chosen = sum_f32<W>(share);
         if (a.renorm)
@@ -1359,7 +1389,10 @@ static void set_shape(Args& a, int W, int V, size_t logit_bytes) {
   a.wide = a.experts % 4 == 0 && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) % (4 * logit_bytes) == 0 &&
            reinterpret_cast<uintptr_t>(a.dlogits) % (4 * logit_bytes) == 0;
   const int size = a.experts / a.groups, lanes = size / V;
-  a.group_lanes = a.groups > 1 && size % V == 0 && (lanes & (lanes - 1)) == 0 && lanes <= W ? lanes : 0;
+  a.whole_lanes = size % V == 0 && (lanes & (lanes - 1)) == 0;
+  a.group_lanes = lanes;
+  if (!a.whole_lanes)
+    for (a.group_lanes = 1; 2 * a.group_lanes * a.groups <= W;) a.group_lanes *= 2;
 }
 static int lanes_needed(const Args& a, bool select) {
   return select && a.groups > a.topk ? a.groups : a.topk;

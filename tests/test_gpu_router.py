@@ -57,6 +57,7 @@ def select(logits, top_k, bias=None, valid=None, groups=0, keep=0, scale=1.0, **
     (1, 1, 1, 0, 0), (5, 8, 2, 0, 0), (33, 60, 4, 0, 0), (17, 64, 16, 0, 0), (9, 64, 20, 0, 0), (130, 128, 6, 8, 3),
     (67, 129, 8, 3, 1), (257, 256, 8, 8, 4), (12, 256, 32, 1, 1), (19, 384, 8, 64, 5), (31, 512, 8, 0, 0),
     (7, 1000, 32, 40, 39), (3, 1024, 32, 16, 2), (6, 32, 32, 0, 0), (4, 48, 3, 48, 3), (5, 63, 9, 9, 2),
+    (11, 160, 6, 8, 3), (9, 320, 8, 10, 4), (21, 96, 6, 2, 1), (6, 64, 8, 32, 7), (13, 768, 12, 6, 2), (8, 16, 4, 16, 5),
 ])
 def test_choice(n, experts, top_k, groups, keep, bias, scoring):
     for dtype in (torch.float32, torch.bfloat16):
@@ -448,3 +449,51 @@ def test_gradients_of_many_rows(experts, top_k, bias, renorm, scoring):
             tol = 2.0**-16 * (scale * float(gw.abs().max()) if lo else 0.0) + 2.0**-16 * 2 * alpha * experts / 10
             tol = tol + (2.0**-8 * ref.abs() if dtype == torch.bfloat16 else 0.0)
             assert ((got.cpu().double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("experts", [48, 72, 160, 300, 1000])
+def test_ties_at_zero_and_denormals(experts):
+    """Equal and nearly equal logits around zero, where a float's last bits are all that it has."""
+    g = torch.Generator().manual_seed(experts)
+    for n in (40, MANY):
+        logits = torch.randint(-3, 4, (n, experts), generator=g).float() * 2.0**-149
+        logits[1::4] = torch.where(torch.rand(n, experts, generator=g) < 0.5, -0.0, 0.0)[1::4]
+        logits[2::4] = (torch.randint(-9, 10, (n, experts), generator=g).float() * 2.0**-130)[2::4]
+        logits[3::4] = torch.randint(-3, 1, (n, experts), generator=g).float()[3::4]  # zeros are the best
+        for groups, keep in ((0, 0), (4, 2)):
+            say(f"around zero n={n} E={experts} groups={groups}")
+            check_choice(logits, 8, select(logits, 8, groups=groups, keep=keep), "softmax", groups=groups, keep=keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("experts", [64, 72, 256, 1000])
+def test_choice_by_scores_that_leave_the_floats(experts, scoring):
+    """No bias to speak of and scores that fp32 does not hold: the 64-bit score decides."""
+    g = torch.Generator().manual_seed(experts)
+    n = 60
+    logits = -70 - 130 * torch.rand(n, experts, generator=g)
+    logits[0::3, 5] = 0.0  # a softmax's others are below 2^-100
+    logits[1::3] = -math.inf
+    for b in (torch.zeros(experts), torch.randint(-1, 2, (experts,), generator=g).float() * 2.0**-145):
+        for groups, keep in ((0, 0), (4, 2)):
+            say(f"small scores E={experts} {scoring} groups={groups}")
+            out = select(logits, 8, b, scoring=scoring, groups=groups, keep=keep, renormalize=False)
+            ids = R.choose(R.canon(logits), 8, scoring, b, groups, keep)
+            assert torch.equal(out.topk_ids.cpu().long(), ids)
+            want = R.weights(R.canon(logits), ids, scoring, False, 1.0)
+            # a score below 2^-126 may be 0; else the bound of the other tests
+            assert ((out.topk_weights.cpu().double() - want).abs() <= 2.0**-20 * want + 2.0**-125).all()
+
+
+@pytest.mark.parametrize("renorm", [False, True])
+def test_sqrtsoftplus_of_small_logits_keeps_its_weights(renorm):
+    """e^l leaves the floats at -88, sqrt(e^l) at -175."""
+    g = torch.Generator().manual_seed(5)
+    logits = -60 - 100 * torch.rand(50, 64, generator=g)
+    say(f"small sqrtsoftplus {renorm}")
+    out = select(logits, 6, scoring="sqrtsoftplus", renormalize=renorm)
+    z = R.canon(logits)
+    ids = R.choose(z, 6, "sqrtsoftplus")
+    want = R.weights(z, ids, "sqrtsoftplus", renorm, 1.0)
+    assert torch.equal(out.topk_ids.cpu().long(), ids)
+    assert ((out.topk_weights.cpu().double() - want).abs() <= 2.0**-20 * want + 2.0**-125).all()

@@ -410,8 +410,8 @@ int afd_silu_mul(const uint16_t* gate_up, int64_t n, int32_t inter, uint16_t* ou
  * block may be shorter); a row of x that holds an infinity or a NaN gives a row of NaN. Any n_out
  * and k_in up to 65536, n <= 2^22. afd_linear_pack lays checkpoint codes e4m3 [n_out][ld] out once
  * (image: afd_linear_layout's bytes, 16-byte aligned); scales f32 [ceil(n_out / 128)][ceil(k_in / 128)] are used
- * as they are. x: rows of ldx >= k_in elements, y: rows of ldy >= n_out; the elements between
- * rows stay as they are. The workspace (16-byte aligned) holds the quantized rows of one call. */
+ * as they are. x: rows of ldx >= k_in elements, y: rows of ldy >= n_out, none of them x's; the
+ * elements between rows stay as they are. The workspace (16-byte aligned) holds the quantized rows of one call. */
 typedef struct afd_linear_weights {
   int32_t n_out;
   int32_t k_in;
@@ -428,7 +428,8 @@ int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
 
 /* ---- the router ---------------------------------------------------------------------------
  * Scores of a row of logits l: softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts
- * as -inf, +inf as the largest float; a row of -inf alone has scores 0 (and weights 0).
+ * as -inf, +inf as the largest float; a row of -inf alone has scores 0 (and weights 0). Scores are
+ * fp32 (one below 2^-126 may be 0) but where they choose, which is done as 64 bits would.
  * Limits: num_experts <= 1024, topk <= 32, num_groups <= 64 and a divisor of num_experts, topk
  * experts in the groups kept; n <= 2^26, n * topk < 2^31. */
 enum afd_scoring { AFD_SCORE_SOFTMAX = 0, AFD_SCORE_SIGMOID = 1, AFD_SCORE_SQRTSOFTPLUS = 2 };

@@ -27,6 +27,21 @@ def _workspace_bytes(n: int, k_in: int) -> int:
     return out.value
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows of a and b (of one length in bytes an element) may share an element."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    n, size = a.shape[0], a.element_size()
+    ends = [t.data_ptr() + ((n - 1) * t.stride(0) + t.shape[1]) * size for t in (a, b)]
+    if ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr():
+        return False
+    # columns of one buffer: b's begin behind a's and end before the next row's
+    if n > 1 and a.stride(0) == b.stride(0):
+        at = (b.data_ptr() - a.data_ptr()) % (a.stride(0) * size)
+        return at < a.shape[1] * size or at + b.shape[1] * size > a.stride(0) * size
+    return True
+
+
 class Fp8BlockLinear(torch.nn.Module):
     """``weight``: e4m3 codes [n_out, k_in] (float8_e4m3fn, or their bytes); ``scales``: fp32
     [ceil(n_out / 128), ceil(k_in / 128)], the weight being code x scale. Laid out once for the kernels, on ``device``
@@ -56,12 +71,12 @@ class Fp8BlockLinear(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """bf16 [..., k_in] -> bf16 [..., n_out] on the device's current stream, into ``out`` if given ([n,
-        n_out] with contiguous rows, x two-dimensional)."""
+        n_out] with contiguous rows that share no element with x, x two-dimensional)."""
         if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != self.in_features:
             raise TypeError(f"expected bf16 [..., {self.in_features}], got {x.dtype} {tuple(x.shape)}")
         if x.device != self.image.device:
             raise ValueError(f"x is on {x.device}, the weights on {self.image.device}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        if torch.is_grad_enabled() and (x.requires_grad or out is not None and out.requires_grad):
             raise NotImplementedError("Fp8BlockLinear has no gradient: call it under torch.no_grad()")
         rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
         n, k = rows.shape
@@ -75,6 +90,8 @@ class Fp8BlockLinear(torch.nn.Module):
                 raise ValueError(f"out must be bf16 [{n}, {self.out_features}] for a two-dimensional x, got {y.dtype} {tuple(y.shape)}")
             if y.device != x.device or n > 0 and y.stride(1) != 1 or n > 1 and y.stride(0) < self.out_features:
                 raise ValueError("out must have contiguous rows of its own on x's device")
+            if _overlap(rows, y):
+                raise ValueError("out shares elements with x")
         size = _workspace_bytes(n, k)
         # a call's own: calls on other streams and captured graphs each have theirs
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)

@@ -22,8 +22,8 @@ from __future__ import annotations
 
 import torch
 
-from .. import _lib
 from .linear import Fp8BlockLinear
+from .topk import launch, need_gpu
 
 
 class SharedExpertMLP(torch.nn.Module):
@@ -92,9 +92,9 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
     SGLang's SiluAndMul, as ``afd_silu_mul``."""
     if gate_up.dtype != torch.bfloat16 or gate_up.dim() != 2 or gate_up.shape[1] % 2:
         raise TypeError(f"expected bf16 [n, 2I], got {gate_up.dtype} {tuple(gate_up.shape)}")
+    need_gpu("gate_up", gate_up)
     gate_up = gate_up.contiguous()
     n, inter = gate_up.shape[0], gate_up.shape[1] // 2
     out = torch.empty(n, inter, dtype=torch.bfloat16, device=gate_up.device)
-    _lib.call("afd_silu_mul", gate_up.data_ptr(), n, inter, out.data_ptr(),
-              torch.cuda.current_stream(gate_up.device).cuda_stream)
+    launch("afd_silu_mul", gate_up.device, gate_up.data_ptr(), n, inter, out.data_ptr())
     return out

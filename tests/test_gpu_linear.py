@@ -278,3 +278,24 @@ def test_exact_integers_every_tile_shape(n, n_out):
     y = Fp8BlockLinear(e4m3(w).to(dev()), s.to(dev()))(x.to(torch.bfloat16).to(dev()))
     want = (x @ (w * widen(s, n_out, k)).t()).to(torch.bfloat16)  # exact in fp32 too
     assert torch.equal(y.cpu(), want)
+
+
+def test_out_that_shares_elements_with_x_is_refused():
+    n, k = 6, 256
+    x, w, s = integers(n, k, k, 8)
+    layer = Fp8BlockLinear(e4m3(w).to(dev()), s.to(dev()))
+    buf = torch.zeros(n + 3, 3 * k, dtype=torch.bfloat16, device=dev())
+    buf[:n, :k] = x.to(torch.bfloat16).to(dev())
+    rows = buf[:n, :k]
+    say("out over x")
+    for out in (rows, buf[1 : n + 1, :k], buf[:n, 128 : 128 + k], buf[:n, k - 1 : 2 * k - 1]):
+        with pytest.raises(ValueError, match="shares"):
+            layer(rows, out=out)
+    with pytest.raises(NotImplementedError):
+        layer(rows.clone(), out=torch.zeros(n, k, dtype=torch.bfloat16, device=dev(), requires_grad=True))
+    say("out beside x in one buffer")
+    want = layer(rows.clone())
+    for at in (k, 2 * k):
+        out = buf[:n, at : at + k]
+        assert layer(rows, out=out) is out and torch.equal(out, want)
+    assert torch.equal(buf[:n, :k].cpu(), x.to(torch.bfloat16))

@@ -84,3 +84,18 @@ def test_python_refusals_of_calls():
             layer(x, out=out)
     with pytest.raises(ValueError):
         layer(x.view(2, 2, 200), out=torch.empty(4, 130, dtype=torch.bfloat16, device="cuda"))
+
+
+def test_overlap():
+    from sgl_asap_amd.moe.linear import _overlap
+
+    buf = torch.zeros(10, 48, dtype=torch.bfloat16)
+    x = buf[2:6, 8:24]
+    apart = [buf[2:6, 24:48], buf[2:6, :8], buf[1:5, 24:40], buf[3:7, 24:30], buf[6:10, 8:24], torch.zeros(4, 16), buf[2:2, :]]
+    shared = [x, buf[2:6, 23:30], buf[2:6, :9], buf[1:5, 8:24], buf[3:7, 0:48], buf[5:9, 8:24], buf.view(5, 96)[1:3, :16]]
+    for y in apart:
+        assert not _overlap(x[: y.shape[0]], y) and not _overlap(y, x[: y.shape[0]])
+    for y in shared:
+        assert _overlap(x[: y.shape[0]], y) and _overlap(y, x[: y.shape[0]])
+    one = buf[3:4, :16]
+    assert not _overlap(one, buf[3:4, 16:40]) and _overlap(one, buf[3:4, 15:40])

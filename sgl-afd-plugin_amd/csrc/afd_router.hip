@@ -18,7 +18,7 @@
 //
 // Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
 // and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
-// else 64 lanes with V = 4, 8 or 16; where many rows choose by their logits alone, 16 lanes up to 256 experts. A
+// else 64 lanes with V = 4, 8 or 16; a choice of many rows takes 16 or 32 lanes up to 256 experts. A
 // lane sorts its values once; a pick is then a max butterfly (DPP and permlane swaps) over the lanes' heads.
 //
 // Sums over rows: a workgroup takes R consecutive rows, cut where sequences begin and end; each piece
@@ -706,8 +706,8 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
   if constexpr (BIAS) {
     // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal
     // and root are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together,
-    // and two bits that hold the place take 6. Four such bits take 30, a softmax's sum over 16 values a lane
-    // and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if they
+    // and two bits that hold the place take 6. Three such bits take 14 (2^-19 then), four 30, a softmax's sum
+    // over 16 values a lane and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if they
     // differ by twice the row's largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
@@ -717,7 +717,7 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
       most = fmaxf(most, score + fabsf(bias[j]));
     }
-    margin = __builtin_fmaf(max_f32<W>(most), a.scoring == AFD_SCORE_SOFTMAX || V > 4 ? 0x1p-17f : 0x1p-19f, 0x1p-124f);
+    margin = __builtin_fmaf(max_f32<W>(most), a.scoring == AFD_SCORE_SOFTMAX || V > 8 ? 0x1p-17f : V > 4 ? 0x1p-18f : 0x1p-19f, 0x1p-124f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
@@ -1323,11 +1323,12 @@ int with_shape(int experts, int lanes, F&& f) {
   if (experts <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
   return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
-// Choosing by the logits alone, many rows: 16 lanes a row, so that what a row costs beside its experts
-// (rounds, sums, weights) is shared by 4 rows of a wavefront. 256 experts: 4096 rows 5.4 us against 5.0 in
-// the shapes above, 8192 6.4 against 7.5, 65536 26.7 against 43.7. With a bias the scores cost more than the
-// rounds and the close rows' 64-bit work is longer with 16 experts a lane (16384 rows 19.3 against 16.2).
-constexpr int kManyRows = 6144;
+// Choosing among many rows: fewer lanes a row, so that what a row costs beside its experts (rounds, sums, weights)
+// is shared by the rows of a wavefront. By the logits alone 16 lanes (256 experts: 4096 rows 5.4 us
+// against 5.0 in the shapes above, 8192 6.4 against 7.5, 65536 26.7 against 43.7), with a bias, whose scores
+// cost more than the rounds and whose close rows take longer the more experts a lane has, 32 (8192 rows 11.9
+// against 10.4, 16384 14.5 against 16.4, 65536 41.2 against 50.8; 16 lanes: 16384 rows 19.3).
+constexpr int kManyRows = 6144, kManyBiasedRows = 12288;
 template <typename F>
 int with_choice_shape(int experts, int lanes, bool bias, int n, F&& f) {
   using std::integral_constant;
@@ -1335,6 +1336,8 @@ int with_choice_shape(int experts, int lanes, bool bias, int n, F&& f) {
     if (experts <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     if (experts <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
   }
+  if (bias && n >= kManyBiasedRows && lanes <= 32 && experts > 128 && experts <= 256)
+    return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
   return with_shape(experts, lanes, f);
 }
 template <typename F>
@@ -1441,6 +1444,20 @@ __global__ __launch_bounds__(kThreads) void no_rows_kernel(Args a) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.loss = 0.0f;
 }
 
+// As many workgroups as the CUs hold at once share the rows: those that came after would run behind them (with
+// 145 registers 3 a CU: 65536 x 256 with a bias 50.8 us in 4 a CU, 41.2 in 3).
+template <void (*KERNEL)(Args)>
+static int launch_topk(const Args& a, int rows, hipStream_t s) {
+  static const int per_cu = [] {
+    int v = 0;
+    return hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, kThreads, 0) == hipSuccess && v > 0 ? v : 1;
+  }();
+  const int64_t need = (int64_t(a.n) + rows - 1) / rows, most = int64_t(per_cu) * device_cu_count();
+  hipLaunchKernelGGL(KERNEL, dim3(static_cast<unsigned>(need < most ? need : most)), dim3(kThreads), 0, s, a);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
+}
+
 // select: a.ids / a.w are written; scores: with the balance sums
 static int launch_balance(Args a, int fmt, bool select, bool scores, hipStream_t s) {
   if (a.n == 0) {
@@ -1502,18 +1519,14 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
     return router::with_choice_shape(a.experts, router::lanes_needed(a, true), bias != nullptr, n, [&](auto wc, auto vc) {
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
       router::set_shape(a, W, V, sizeof(T));
-      int64_t grid = (int64_t(n) + kRows - 1) / kRows;
-      if (grid > int64_t(4) * device_cu_count()) grid = int64_t(4) * device_cu_count();
-      auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(router::kThreads), 0,
-                           static_cast<hipStream_t>(stream), a);
-        AFD_CHECK_LAUNCH();
-        return int(AFD_OK);
-      };
+      hipStream_t s = static_cast<hipStream_t>(stream);
       if constexpr (W == 16 && V > 4)
-        return go(router::topk_kernel<T, W, V, false>);
+        return router::launch_topk<router::topk_kernel<T, W, V, false>>(a, kRows, s);
+      else if constexpr (W == 32 && V > 4)
+        return router::launch_topk<router::topk_kernel<T, W, V, true>>(a, kRows, s);
       else
-        return bias ? go(router::topk_kernel<T, W, V, true>) : go(router::topk_kernel<T, W, V, false>);
+        return bias ? router::launch_topk<router::topk_kernel<T, W, V, true>>(a, kRows, s)
+                    : router::launch_topk<router::topk_kernel<T, W, V, false>>(a, kRows, s);
     });
   });
 }

@@ -497,3 +497,25 @@ def test_sqrtsoftplus_of_small_logits_keeps_its_weights(renorm):
     want = R.weights(z, ids, "sqrtsoftplus", renorm, 1.0)
     assert torch.equal(out.topk_ids.cpu().long(), ids)
     assert ((out.topk_weights.cpu().double() - want).abs() <= 2.0**-20 * want + 2.0**-125).all()
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("experts,top_k,groups,keep", [(129, 4, 3, 2), (160, 6, 8, 3), (200, 17, 0, 0), (256, 8, 8, 4), (256, 32, 32, 9)])
+def test_biased_choice_of_many_rows(experts, top_k, groups, keep, scoring):
+    """Above the rows from which 32 lanes hold a row with a bias: ordinary rows, ties, masks, next floats."""
+    g = torch.Generator().manual_seed(experts + top_k)
+    n = 12301
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.randn(n, experts, generator=g) * 2
+        logits[::5] = torch.randint(-2, 2, (n, experts), generator=g).float()[::5]
+        half = experts // 2
+        logits[1::5, half : 2 * half] = logits[1::5, :half] * (1 + 2.0**-22)
+        logits[torch.rand(n, experts, generator=g) < 0.01] = -math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.003] = math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.003] = math.nan
+        logits[7, 9:], logits[8], logits[9] = -math.inf, -math.inf, math.nan
+        logits = logits.to(dtype)
+        for b in (torch.randn(experts, generator=g) * 0.05, torch.zeros(experts)):
+            say(f"many biased rows E={experts} k={top_k} groups={groups}/{keep} {scoring} {dtype}")
+            out = select(logits, top_k, b, scoring=scoring, groups=groups, keep=keep, scale=1.5)
+            check_choice(logits, top_k, out, scoring, b, True, 1.5, groups, keep)

@@ -387,13 +387,14 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   // copy number c of a stage: the scales, then the activation pieces, then the weight pieces
   constexpr int kCopies = T::kCopies, S = T::S;
   const int ws = w % T::kScaleWaves;
+  const int s_row = min(m0 + 64 * ws, p.a_rows - 64);  // rows past the end take other rows' scales
   auto copy = [&](int b, auto c_c) {
     constexpr int c = decltype(c_c)::value;
     const uint32_t st = lds_base + static_cast<uint32_t>((b & (S - 1)) * T::kStage);
     const uint32_t off = voff + static_cast<uint32_t>(b) * (2 * kPiece);
     if constexpr (c == 0) {
       // (every wavefront: two may write the same bytes, and the steps stay one block of code)
-      lds_dma4(st + T::kSOff + ws * 256, p.as + int64_t(b) * p.a_rows + m0 + 64 * ws, lane * 4u);
+      lds_dma4(st + T::kSOff + ws * 256, p.as + int64_t(b) * p.a_rows + s_row, lane * 4u);
     } else if constexpr (c <= T::kAQ) {
       lds_dma16(st + (w * T::kAQ + c - 1) * kPiece, a_src[c - 1], off);
     } else {
@@ -520,14 +521,15 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 }
 
 // ---------------------------------------------------------------- host
-// Tile shapes. With a tile on each of 256 CUs a K block takes 0.35, 0.49, 0.72, 1.16 and 1.86 us (4096 inputs),
-// that is 0.35, 0.25, 0.18, 0.15 and 0.12 for every 64 x 64 outputs: the larger the tile, the less of its
+// Tile shapes. With a tile on each of 256 CUs a K block takes 0.35, 0.49, 0.72, 1.16, 1.48 and 1.86 us (4096
+// inputs), that is 0.35, 0.25, 0.18, 0.15, 0.12 and 0.12 for every 64 x 64 outputs: the larger the tile, the less of its
 // time goes into moving operands, and the fewer of them there are to fill the CUs. The ring is as deep as the
 // LDS allows with the fragments' order in mind: small tiles wait for latency, large ones do not.
 using T64 = Shape<64, 64, 4, 1, 4>;
 using T64x128 = Shape<64, 128, 2, 2, 4>;
 using T128 = Shape<128, 128, 2, 2, 4>;
 using T256x128 = Shape<256, 128, 4, 2, 2>;
+using T192x256 = Shape<192, 256, 2, 4, 2>;
 using T256 = Shape<256, 256, 4, 2, 2>;
 
 struct Plan {
@@ -566,11 +568,12 @@ static int launch_rows(const Args& p, const RowsIn& in, bool vec, hipStream_t s)
 
 // The shape whose rounds over the CUs take least: rounds x the measured time of one K block (T64 .. T256
 // above). At 4096 x 4096, measured best and chosen: 512 rows T64x128 (20.7 us, T128 25.6), 1024 T128 (28.9, T256x128
-// 40), 1500 T256x128 (41.7, T128 46.4), 2900 T256 (59.7, T256x128 70.7).
-enum { kT64, kT64x128, kT128, kT256x128, kT256, kShapes };
+// 40), 1500 T256x128 (43, T128 46), 2900 T192x256 (57.8, T256 60.3, T256x128 72), 5800 T192x256 (106, T256 114),
+// 8192 T256 (136, T192x256 152).
+enum { kT64, kT64x128, kT128, kT256x128, kT192x256, kT256, kShapes };
 static int best_shape(int64_t n, int64_t n_out, int cus) {
-  static const int bm[kShapes] = {64, 64, 128, 256, 256}, bn[kShapes] = {64, 128, 128, 128, 256};
-  static const int cost[kShapes] = {35, 49, 72, 116, 186};
+  static const int bm[kShapes] = {64, 64, 128, 256, 192, 256}, bn[kShapes] = {64, 128, 128, 128, 256, 256};
+  static const int cost[kShapes] = {35, 49, 72, 116, 148, 186};
   int best = 0;
   int64_t least = 0;
   for (int i = 0; i < kShapes; ++i) {
@@ -681,6 +684,7 @@ extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, 
     case linear::kT64: return linear::launch_tiles<linear::T64>(p, s);
     case linear::kT64x128: return linear::launch_tiles<linear::T64x128>(p, s);
     case linear::kT128: return linear::launch_tiles<linear::T128>(p, s);
+    case linear::kT192x256: return linear::launch_tiles<linear::T192x256>(p, s);
     case linear::kT256x128: return linear::launch_tiles<linear::T256x128>(p, s);
     default: return linear::launch_tiles<linear::T256>(p, s);
   }

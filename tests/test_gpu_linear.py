@@ -269,7 +269,8 @@ def test_shared_expert(n):
     assert rel <= 2.0**-5, rel
 
 
-@pytest.mark.parametrize("n,n_out", [(65, 4096), (500, 4100), (1000, 4000), (1500, 4096), (2900, 4096), (70, 65000), (5000, 300)])
+@pytest.mark.parametrize("n,n_out", [(65, 4096), (500, 4100), (1000, 4000), (1500, 4096), (2900, 4096), (70, 65000), (5000, 300),
+                                     (5800, 4096), (2885, 4091), (3900, 3100)])
 def test_exact_integers_every_tile_shape(n, n_out):
     """Calls that take each of the tile shapes, with rows and outputs that end inside a tile."""
     k = 700

@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .topk import launch, need_gpu
+from .topk import launch, matrix_rows, need_gpu
 
 FP8_BLOCK = 128
 
@@ -79,9 +79,8 @@ class Fp8BlockLinear(torch.nn.Module):
         if torch.is_grad_enabled() and (x.requires_grad or out is not None and out.requires_grad):
             raise NotImplementedError("Fp8BlockLinear has no gradient: call it under torch.no_grad()")
         rows = x if x.dim() == 2 else x.reshape(-1, self.in_features)
+        rows, ldx = matrix_rows(rows)
         n, k = rows.shape
-        if n > 1 and (rows.stride(1) != 1 and k > 1 or rows.stride(0) < k) or n == 1 and rows.stride(1) != 1:
-            rows = rows.contiguous()
         if out is None:
             y = torch.empty(n, self.out_features, dtype=torch.bfloat16, device=x.device)
         else:
@@ -95,6 +94,6 @@ class Fp8BlockLinear(torch.nn.Module):
         size = _workspace_bytes(n, k)
         # a call's own: calls on other streams and captured graphs each have theirs
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        launch("afd_linear", x.device, self._weights_ref, rows.data_ptr(), rows.stride(0) if n > 1 else k, n,
+        launch("afd_linear", x.device, self._weights_ref, rows.data_ptr(), ldx, n,
                ws.data_ptr(), size, y.data_ptr(), y.stride(0) if n > 1 else self.out_features)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)

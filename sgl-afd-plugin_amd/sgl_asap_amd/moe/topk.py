@@ -69,14 +69,20 @@ def router_cfg(num_experts: int, top_k: int, scoring: str, renormalize: bool, gr
     return ctypes.pointer(cfg)
 
 
+def matrix_rows(t: torch.Tensor):
+    """(t [n, columns] with contiguous rows, their stride in elements)."""
+    columns = t.shape[1]
+    if t.is_contiguous():
+        return t, columns
+    if t.shape[0] == 1 or t.stride(1) != 1 or t.stride(0) < columns:
+        return t.contiguous(), columns
+    return t, t.stride(0)
+
+
 def logit_rows(logits: torch.Tensor):
-    """(logits whose rows are contiguous, their row stride in elements)."""
     if logits.dim() != 2:
         raise ValueError(f"router logits must be [n, num_experts], got {tuple(logits.shape)}")
-    n, experts = logits.shape
-    if n > 1 and (logits.stride(1) != 1 and experts > 1 or logits.stride(0) < experts) or n == 1 and logits.stride(1) != 1:
-        logits = logits.contiguous()
-    return logits, logits.stride(0) if n > 1 else experts
+    return matrix_rows(logits)
 
 
 def on_device(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: tuple, device) -> int:
@@ -85,7 +91,7 @@ def on_device(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: t
         return 0
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {shape}, got {tuple(t.shape)} strides {t.stride()}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other arguments on {device}")
@@ -108,6 +114,8 @@ def _groups(num_expert_group: Optional[int], topk_group: Optional[int]):
 
 
 def choice_cfg(logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor):
+    if logits.dim() != 2:
+        raise ValueError(f"router logits must be [n, num_experts], got {tuple(logits.shape)}")
     groups, keep = _groups(num_expert_group, topk_group)
     scale = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)
     return router_cfg(logits.shape[1], top_k, scoring, bool(renormalize), groups, keep, scale, logits.dtype)

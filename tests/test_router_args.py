@@ -150,3 +150,13 @@ def test_reference_gradients_against_differences():
                     up[t, e] += 1e-5
                     down[t, e] -= 1e-5
                     assert abs((value(up) - value(down)) / 2e-5 - float(got[t, e])) < 1e-7
+
+
+def test_logits_of_other_dimensions():
+    for shape in ((8,), (2, 3, 8)):
+        with pytest.raises(ValueError):
+            T.select_experts(torch.zeros(shape), 2)
+        with pytest.raises(ValueError):
+            B.select_and_balance(torch.zeros(shape), 2, alpha=1.0)
+        with pytest.raises(ValueError):
+            B.balance_loss(torch.zeros(shape), torch.zeros(shape[0], 2, dtype=torch.int32), alpha=1.0)

@@ -519,3 +519,52 @@ def test_biased_choice_of_many_rows(experts, top_k, groups, keep, scoring):
             say(f"many biased rows E={experts} k={top_k} groups={groups}/{keep} {scoring} {dtype}")
             out = select(logits, top_k, b, scoring=scoring, groups=groups, keep=keep, scale=1.5)
             check_choice(logits, top_k, out, scoring, b, True, 1.5, groups, keep)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("experts", [64, 256, 1000])
+def test_scores_at_the_floats_lower_end_give_finite_results(experts, scoring):
+    """Scores around 2^-126, where a reciprocal of their sum can leave the floats."""
+    g = torch.Generator().manual_seed(experts)
+    n, top_k, scale = 96, 8, 1.5
+    low = -2.0 if scoring == "sqrtsoftplus" else -1.0
+    # a row's logits within a few of the border, the rows from well above it to well below
+    logits = low * torch.linspace(84, 106, n)[:, None] + torch.rand(n, experts, generator=g) * 2
+    for renorm in (True, False):
+        for b in (None, torch.zeros(experts)):
+            say(f"lower end E={experts} {scoring} renorm={renorm} bias={b is not None}")
+            leaf = logits.to(dev()).requires_grad_()
+            out, loss, _ = B.select_and_balance(leaf, top_k, alpha=1.0, scoring=scoring, renormalize=renorm,
+                                                correction_bias=None if b is None else b.to(dev()), routed_scaling_factor=scale)
+            (grad,) = torch.autograd.grad((out.topk_weights.sum(), loss), (leaf,))
+            w = out.topk_weights.detach()
+            loss = loss.detach()
+            assert torch.isfinite(w).all() and torch.isfinite(loss) and torch.isfinite(grad).all()
+            assert (w >= 0).all() and (w.sum(1) <= scale * (1 + 2.0**-20)).all()
+            # s' adds up to at most one a row, so the loss is at most experts / k * n * k / n
+            assert 0 <= float(loss) <= experts * (1 + 2.0**-12)
+            alone = select(logits, top_k, b, scoring=scoring, renormalize=renorm, scale=scale)
+            assert torch.equal(alone.topk_ids, out.topk_ids) and torch.equal(alone.topk_weights, w)
+
+
+@pytest.mark.parametrize("scoring,lo,hi", [("softmax", -60, 60), ("sigmoid", -80, 60), ("sqrtsoftplus", -160, 60)])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_gradients_of_logits_far_from_zero(scoring, lo, hi, renorm):
+    """Weights' gradient within 2^-16 of its largest factor. Balance gradient: the shares' exponentials are off by |x| 2^-24
+    relative with |x| <= 160, their sum by the same, so r s' (c - sum c s') by less than 2^-14 of the largest c,
+    alpha E / (k T)."""
+    n, experts, top_k, alpha, scale = 60, 128, 6, 3.0, 2.0
+    g = torch.Generator().manual_seed(7)
+    logits = lo + (hi - lo) * torch.rand(n, experts, generator=g)
+    logits[::3] = lo + 20 * torch.rand(n, experts, generator=g)[::3]  # rows of small scores alone
+    gw = torch.randn(n, top_k, generator=g)
+    say(f"far gradients {scoring} renorm={renorm}")
+    leaf = logits.to(dev()).requires_grad_()
+    out, loss, _ = B.select_and_balance(leaf, top_k, alpha=alpha, scoring=scoring, renormalize=renorm, routed_scaling_factor=scale)
+    ids = check_choice(logits, top_k, out, scoring, None, renorm, scale)
+    for with_w in (True, False):
+        outs, gs = ([out.topk_weights, loss], [gw.to(dev()), torch.tensor(1.0, device=dev())]) if with_w else ([loss], [torch.tensor(1.0, device=dev())])
+        (got,) = torch.autograd.grad(outs, (leaf,), gs, retain_graph=True)
+        want = R.grads(logits, ids, scoring, renorm, scale, gw if with_w else None, 1.0, alpha)
+        tol = 2.0**-14 * alpha * experts / (top_k * n) + (2.0**-16 * scale * float(gw.abs().max()) if with_w else 0.0)
+        assert ((got.cpu().double() - want).abs() <= tol).all(), float((got.cpu().double() - want).abs().max()) / tol

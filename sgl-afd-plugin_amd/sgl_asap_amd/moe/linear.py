@@ -63,7 +63,7 @@ class Fp8BlockLinear(torch.nn.Module):
         need_gpu("weight", codes)
         self.out_features, self.in_features = n_out, k_in
         self.image = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
-        self.scales = scales.to(codes.device).contiguous()
+        self.scales = scales.to(codes.device, copy=True).contiguous()
         launch("afd_linear_pack", codes.device, codes.data_ptr(), k_in, n_out, k_in, self.image.data_ptr())
         # _weights holds addresses: the tensors stay attributes, not buffers that a module move would replace
         self._weights = _lib.AfdLinearWeights(n_out, k_in, self.image.data_ptr(), self.scales.data_ptr())

@@ -27,7 +27,7 @@
 // writes its sums and counts to a slot of its own (slot = workgroup + sequence: from one piece to the
 // next one of the two grows), and a second launch adds a sequence's slots in their order. No sum
 // depends on which workgroup ends first. With the choice 16384 x 256 takes 22 us and 9.6 for the second launch (of
-// which 3.6 are any launch's), the gradient, again one pass, 15 (34 MB); given ids, 8192 x 64 6.6, 9.2 and 7.1.
+// which 3.6 are any launch's), the gradient, again one pass, 16 (34 MB); given ids, 8192 x 64 6.6, 9.2 and 7.1.
 #include "afd_common.h"
 #include "afd_internal.h"
 
@@ -1239,7 +1239,7 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
       if (a.gw != nullptr) {
         // lane kk < topk: the kk-th chosen expert's share of the weights' scores, and its gradient
         const int id = li < a.topk && static_cast<uint32_t>(now.id) < static_cast<uint32_t>(a.experts) ? now.id : -1;
-        const float g = id >= 0 ? now.gw * a.scale : 0.0f;
+        float g = id >= 0 ? now.gw : 0.0f;
         float* mine = spread + sub * (W * V);
 #pragma unroll
         for (int j = 0; j < V; ++j) mine[row.e0 + j] = row.l[j];
@@ -1264,8 +1264,12 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
           share = chosen > 0.0f ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
         else if (a.scoring == AFD_SCORE_SOFTMAX)
           share *= inv;
-        // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something
+        // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something. Renormalized ones
+        // add up to one themselves, so g counts from the largest share's: one that holds nearly all (or all, of one
+        // pick) leaves no difference of two close numbers.
         float mean = 0.0f;
+        if (a.renorm) g -= __shfl(g, first_lane<W>(share == max_f32<W>(share), lane), W);
+        g *= a.scale;
         if (a.renorm || a.scoring == AFD_SCORE_SOFTMAX) mean = sum_f32<W>(g * share);
         const float u = share * (g - (a.renorm ? mean : 0.0f));
         // to the lanes that hold the experts, through LDS (an id that comes twice is added up)

@@ -568,3 +568,33 @@ def test_gradients_of_logits_far_from_zero(scoring, lo, hi, renorm):
         want = R.grads(logits, ids, scoring, renorm, scale, gw if with_w else None, 1.0, alpha)
         tol = 2.0**-14 * alpha * experts / (top_k * n) + (2.0**-16 * scale * float(gw.abs().max()) if with_w else 0.0)
         assert ((got.cpu().double() - want).abs() <= tol).all(), float((got.cpu().double() - want).abs().max()) / tol
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("experts,top_k,bias", [(48, 1, False), (200, 1, True), (64, 4, False), (256, 8, True), (700, 3, True)])
+def test_gradient_of_a_weight_that_holds_nearly_all(experts, top_k, bias, scoring):
+    """Renormalized weights of which one is close to one: its gradient is small and still right. With g counted from
+    the largest share's, u_i = share_i ((g_i - g*) - sum_j share_j (g_j - g*)): a share is off by 2^-21 of itself (an
+    exponential of two ulps, a sum, a reciprocal), the differences by 2^-24, the slope by 2^-21."""
+    g = torch.Generator().manual_seed(experts)
+    n, scale = 40, 1.5
+    logits = torch.randn(n, experts, generator=g) - 9
+    logits[torch.arange(n), torch.randint(0, experts, (n,), generator=g)] = 5.0
+    b = torch.randn(experts, generator=g) * 1e-5 if bias else None
+    gw = torch.randn(n, top_k, generator=g)
+    say(f"one share E={experts} k={top_k} {scoring}")
+    leaf = logits.to(dev()).requires_grad_()
+    out = T.select_experts(leaf, top_k, scoring=scoring, correction_bias=None if b is None else b.to(dev()), routed_scaling_factor=scale)
+    (got,) = torch.autograd.grad(out.topk_weights, leaf, gw.to(dev()))
+    ids = check_choice(logits, top_k, out, scoring, b, True, scale)
+    want = R.grads(logits, ids, scoring, True, scale, gw)
+    if top_k == 1:
+        assert (got == 0).all() and (want.abs() < 1e-12).all()
+        return
+    share = R.weights(R.canon(logits), ids, scoring, True, 1.0)
+    d = (gw.double() - gw.double().gather(1, share.argmax(1, keepdim=True))).abs()
+    bound = torch.zeros(n, experts, dtype=torch.float64).scatter_(1, ids, scale * share * (d + (share * d).sum(1, keepdim=True)))
+    # the reference goes through the whole softmax: fewer than 8 steps, each 2^-53 of terms up to scale |gw|, also in
+    # the experts that were not chosen, whose gradient is 0
+    own = 2.0**-50 * scale * float(gw.abs().max())
+    assert ((got.cpu().double() - want).abs() <= 2.0**-18 * bound + own).all()

@@ -34,12 +34,12 @@
  *                                (computed at P/srt/batch_overlap/operations_strategy.py:94,
  *                                255 by SGLang's DeepseekV2MLP: SiluAndMul between its
  *                                gate_up and down projections)
- *   afd_topk ................... the router's choice that the reference leaves to SGLang's TopK
- *                                (its StandardTopKOutput is what P/srt/managers/scheduler.py
+ *   afd_topk ................... the router's choice, which the reference leaves to the serving
+ *                                engine (its StandardTopKOutput is what P/srt/managers/scheduler.py
  *                                :410-412 and P/srt/layers/moe/token_dispatcher/asap.py:48-73
  *                                take)
- *   afd_linear / ............... the block-FP8 linear layers of the shared expert, SGLang's in the
- *   afd_linear_pack              reference (the MLP called at P/srt/batch_overlap/
+ *   afd_linear / ............... the block-FP8 linear layers of the shared expert, the engine's in
+ *   afd_linear_pack              the reference (the MLP called at P/srt/batch_overlap/
  *                                operations_strategy.py:94, 255)
  *   afd_expert_counts / ........ no counterpart: where the tokens go, the balance loss of a
  *   afd_balance / ..............  router in training, and the gradient of both by its logits

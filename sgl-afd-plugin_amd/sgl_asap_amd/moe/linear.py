@@ -1,8 +1,8 @@
 """A dense layer with block-FP8 weights: ``y = bf16(q(x) W^T)``, W in e4m3 with one fp32 scale per 128x128 block, x
 quantized in the call to e4m3 with one fp32 scale per 1x128 (``afd_linear``).
 
-The format is the experts' (DeepSeek-style FP8 checkpoints hold their dense layers in it too, the
-shared expert's among them); the reference leaves these layers to SGLang. Any sizes, one token to prefill.
+The format is the experts' (FP8 checkpoints hold their dense layers in it too, the
+shared expert's among them); the reference leaves these layers to the serving engine. Any sizes, one token to prefill.
 For serving: the product has no gradient.
 """
 

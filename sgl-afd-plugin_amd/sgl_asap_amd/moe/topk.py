@@ -6,9 +6,9 @@ The reference passes SGLang's ``StandardTopKOutput(topk_weights, topk_ids, route
 so the same three-field tuple is defined locally; any object with ``topk_weights`` and
 ``topk_ids`` attributes is accepted where it is consumed.
 
-``select_experts`` makes that output from a router's logits (``afd_topk``: SGLang's TopK, which
-the reference's models call before the MoE layer), with its gradient; ``TopK`` is the module form,
-with SGLang's argument names:
+``select_experts`` makes that output from a router's logits (``afd_topk``; the reference
+leaves it to the serving engine), with its gradient; ``TopK`` is the module form, with the argument
+names that the engine's models use:
 
     s   = softmax(l), sigmoid(l) or sqrt(softplus(l))
     c   = l, or s + correction_bias (in 64 bits)        the choice value
@@ -212,7 +212,7 @@ def select_experts(
 
 
 class TopK(torch.nn.Module):
-    """``select_experts`` with a layer's settings, by SGLang's argument names."""
+    """``select_experts`` with a layer's settings."""
 
     def __init__(
         self,

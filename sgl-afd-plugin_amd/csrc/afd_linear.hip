@@ -301,12 +301,12 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 // instruction, so a block's sum is one MFMA from 0 and its 4 values a lane are folded at once). A stage
 // is one K block of both operands and the rows' scales, copied HBM -> LDS in 1 KiB pieces into S slots.
 //
-// A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments,
-// read two ahead, in an order kept as written (left alone, the compiler reads all of a stage first and then
-// waits out every MFMA in turn: 322 us for 16384 x 4096 x 4096). When the last two are in registers (all of its reads of the stage done) it waits for
-// its copies of the next stage and meets the others at the stage's one barrier: the next stage
-// is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the
-// last two weight fragments run while the next stage's first fragments are read.
+// A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments, read two
+// ahead, in an order kept as written (left alone, the compiler reads all of a stage first and then waits out every
+// MFMA in turn: 322 us for 16384 x 4096 x 4096). When the last two are in registers (all of its reads of the
+// stage done) it waits for its copies of the next stage and meets the others at the stage's one barrier: the
+// next stage is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the last two
+// weight fragments run while the next stage's first fragments are read.
 //
 // 16384 x 4096 x 4096 takes 232 to 280 us (1.96 to 2.37 PFLOP/s; the library's product without block scales 230), at
 // a clock of 1.4 to 1.7 GHz: power first, and within the cycles (MFMA busy in 65% of them) LDS, whose bytes for a

@@ -591,7 +591,8 @@ __device__ __forceinline__ Lanes<W> keep_groups(const Args& a, const float (&c)[
     if (gl > 16) merge(step_f32<16>(first, lane), step_f32<16>(second, lane));
   if constexpr (W > 32)
     if (gl > 32) merge(step_f32<32>(first, lane), step_f32<32>(second, lane));
-  const float value = BIAS && size > 1 ? first + second : first;
+  float value = BIAS && size > 1 ? first + second : first;
+  if constexpr (BIAS) value = value != value ? kLowest : value;  // +inf and -inf
   uint32_t key = (li & (gl - 1)) == 0 && li < a.groups * gl ? key32(value) : 0u;
   Lanes<W> kept = 0;
   float worst = 0.0f;
@@ -699,28 +700,30 @@ __device__ __forceinline__ bool settle(const Args& a, int64_t t, int lane, uint6
 
 // Selection of one row: lane kk < topk gets the kk-th expert and `chosen`, its logit, or with a bias and
 // scores of their own its score (-inf in other lanes).
-// bias: the lane's experts' (BIAS); s, sum: the row's scores (BIAS).
+// bias: the lane's experts', bias_most: the largest (BIAS); s, sum: the row's scores (BIAS).
 template <typename T, int W, int V, bool BIAS>
 __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, int64_t t, int lane, uint64_t* lds_row,
-                                      const float (&bias)[V], const float (&s)[V], float sum, float& chosen) {
+                                      const float (&bias)[V], float bias_most, const float (&s)[V], float sum,
+                                      float& chosen) {
   const int li = lane & (W - 1), e0 = row.e0;
   float c[V], margin = 0.0f;
   bool sure = true;
   if constexpr (BIAS) {
-    // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal
-    // and root are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together,
-    // and two bits that hold the place take 6. Three such bits take 14 (2^-19 then), four 30, a softmax's sum
-    // over 16 values a lane and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if they
-    // differ by twice the row's largest such bound.
+    // An fp32 choice value is off by less than 2^-20 (s + |bias|): the hardware's exponential, reciprocal and root
+    // are within one ulp of 2^-23, every other step within 2^-24, at most 9 of these together, and two bits
+    // that hold the place take 6. Three such bits take 14 (2^-19 then), four 30, a softmax's sum over 16 values a
+    // lane and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if
+    // they differ by twice the row's largest such bound.
     const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float score = s[j] * inv;
       c[j] = e0 + j < a.experts ? score + bias[j] : kLowest;
-      most = fmaxf(most, score + fabsf(bias[j]));
+      most = fmaxf(most, score);
     }
-    margin = __builtin_fmaf(max_f32<W>(most), a.scoring == AFD_SCORE_SOFTMAX || V > 8 ? 0x1p-17f : V > 4 ? 0x1p-18f : 0x1p-19f, 0x1p-124f);
+    const float part = a.scoring == AFD_SCORE_SOFTMAX || V > 8 ? 0x1p-17f : V > 4 ? 0x1p-18f : 0x1p-19f;
+    margin = __builtin_fmaf(max_f32<W>(most) + bias_most, part, 0x1p-124f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = row.l[j];
@@ -830,13 +833,18 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, f
   return s * a.scale;
 }
 
-template <int V>
-__device__ __forceinline__ void load_bias(const Args& a, int e0, float (&bias)[V]) {
+// Returns the largest |bias| of all experts (-inf, which bars an expert, aside)
+template <int W, int V>
+__device__ __forceinline__ float load_bias(const Args& a, int e0, float (&bias)[V]) {
+  float most = 0.0f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {  // no branches: the loads travel together
     const float b = a.bias != nullptr ? a.bias[min(e0 + j, a.experts - 1)] : 0.0f;
     bias[j] = b != b ? kLowest : b;
   }
+#pragma unroll
+  for (int j = 0; j < V; ++j) most = fmaxf(most, bias[j] == kLowest ? 0.0f : fabsf(bias[j]));
+  return max_f32<W>(most);
 }
 
 // ---------------------------------------------------------------- selection
@@ -845,7 +853,7 @@ __device__ __forceinline__ void topk_rows(const Args& a, uint64_t* lds) {
   constexpr int kRows = kThreads / W;  // rows in flight of a workgroup
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   float bias[V];
-  load_bias<V>(a, li * V, bias);
+  const float bias_most = load_bias<W, V>(a, li * V, bias);
   using R = Row<T, W, V>;
   const int64_t step = int64_t(gridDim.x) * kRows;
   // the lanes of a wavefront stay together: rows past the end are the last one again
@@ -861,7 +869,7 @@ __device__ __forceinline__ void topk_rows(const Args& a, uint64_t* lds) {
     row.set(a, raw, li);
     float s[V] = {}, sum = 0.0f, l;
     if constexpr (BIAS) sum = row.template scores<true>(a, s);
-    int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
+    int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, bias_most, s, sum, l);
     float w = weigh<T, W, V, BIAS>(a, row, l);
     if (!valid) id = -1, w = 0.0f;
     if (r < a.n && li < a.topk) {
@@ -1031,7 +1039,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(Args a) {
 // The rows of one piece: p, the lane's sums of s' over its rows; mine, their number; cnt, the counts (LDS).
 template <typename T, int W, int V, bool SELECT, bool BIAS, bool WIDE>
 __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Piece& piece, const float (&bias)[V],
-                                             float (&p)[V], int& mine, int32_t* cnt, uint64_t* lds) {
+                                             float bias_most, float (&p)[V], int& mine, int32_t* cnt, uint64_t* lds) {
   constexpr int kRows = balance_threads(W, V) / W;
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   const bool counted = piece.seq >= 0;
@@ -1051,7 +1059,7 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
     const float sum = row.template scores<BIAS>(a, s);
     if constexpr (SELECT) {
       float l;
-      const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, s, sum, l);
+      const int id = choose<T, W, V, BIAS>(a, row, rr, lane, lds + sub * row_words(W, V), bias, bias_most, s, sum, l);
       const float w = weigh<T, W, V, BIAS>(a, row, l);
       if (in && li < a.topk) {
         a.ids[int64_t(r) * a.topk + li] = live ? id : -1;
@@ -1082,7 +1090,8 @@ __global__ __launch_bounds__(balance_threads(W, V)) void balance_kernel(Args a) 
   const int t = threadIdx.x, lane = t & 63, li = lane & (W - 1), sub = t / W;
   if (blockIdx.x == 0 && t == 0 && a.ticket != nullptr) *a.ticket = 0;  // for the second launch
   float bias[V];
-  if constexpr (SELECT) load_bias<V>(a, li * V, bias);
+  float bias_most = 0.0f;
+  if constexpr (SELECT) bias_most = load_bias<W, V>(a, li * V, bias);
   const int32_t r0 = blockIdx.x * a.block_rows;
   const int32_t r1 = a.n - r0 < a.block_rows ? a.n : r0 + a.block_rows;
   for (int32_t at = r0; at < r1;) {
@@ -1103,9 +1112,9 @@ __global__ __launch_bounds__(balance_threads(W, V)) void balance_kernel(Args a) 
       }
       __syncthreads();
     } else if (a.wide) {
-      balance_rows<T, W, V, SELECT, BIAS, true>(a, at, piece, bias, p, mine, cnt, lds);
+      balance_rows<T, W, V, SELECT, BIAS, true>(a, at, piece, bias, bias_most, p, mine, cnt, lds);
     } else {
-      balance_rows<T, W, V, SELECT, BIAS, false>(a, at, piece, bias, p, mine, cnt, lds);
+      balance_rows<T, W, V, SELECT, BIAS, false>(a, at, piece, bias, bias_most, p, mine, cnt, lds);
     }
     if (counted) {
       if (li == 0) atomicAdd(&live_rows, mine);

@@ -86,7 +86,8 @@ class Fp8BlockLinear(torch.nn.Module):
         else:
             y = out
             if x.dim() != 2 or y.dtype != torch.bfloat16 or tuple(y.shape) != (n, self.out_features):
-                raise ValueError(f"out must be bf16 [{n}, {self.out_features}] for a two-dimensional x, got {y.dtype} {tuple(y.shape)}")
+                raise ValueError(f"out must be bf16 [{n}, {self.out_features}] for a two-dimensional x, got {y.dtype} "
+                                 f"{tuple(y.shape)}")
             if y.device != x.device or n > 0 and y.stride(1) != 1 or n > 1 and y.stride(0) < self.out_features:
                 raise ValueError("out must have contiguous rows of its own on x's device")
             if _overlap(rows, y):

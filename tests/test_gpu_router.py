@@ -598,3 +598,19 @@ def test_gradient_of_a_weight_that_holds_nearly_all(experts, top_k, bias, scorin
     # the experts that were not chosen, whose gradient is 0
     own = 2.0**-50 * scale * float(gw.abs().max())
     assert ((got.cpu().double() - want).abs() <= 2.0**-18 * bound + own).all()
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("n,experts,top_k,groups,keep", [(40, 64, 6, 0, 0), (40, 60, 6, 12, 4), (40, 256, 8, 8, 4), (33, 160, 6, 8, 3),
+                                                         (20, 700, 8, 0, 0), (20, 768, 8, 48, 7), (12301, 256, 8, 8, 4)])
+def test_bias_that_bars_or_forces_experts(n, experts, top_k, groups, keep, scoring):
+    """-inf and NaN in the bias bar an expert, +inf forces it; a group of both has no value."""
+    g = torch.Generator().manual_seed(n + experts)
+    logits = torch.randn(n, experts, generator=g) * 2
+    for kinds in ((-math.inf,), (-math.inf, math.nan), (math.inf,), (math.inf, -math.inf)):
+        b = torch.randn(experts, generator=g) * 0.05
+        for kind in kinds:
+            b[torch.rand(experts, generator=g) < (0.6 if len(kinds) == 2 and kind == -math.inf else 0.1)] = kind
+        say(f"bias of {kinds} n={n} E={experts} groups={groups}/{keep} {scoring}")
+        out = select(logits, top_k, b, scoring=scoring, groups=groups, keep=keep)
+        check_choice(logits, top_k, out, scoring, b, groups=groups, keep=keep)

@@ -39,8 +39,8 @@
  *                                :410-412 and P/srt/layers/moe/token_dispatcher/asap.py:48-73
  *                                take)
  *   afd_linear / ............... the block-FP8 linear layers of the shared expert, the engine's in
- *   afd_linear_pack              the reference (the MLP called at P/srt/batch_overlap/
- *                                operations_strategy.py:94, 255)
+ *   afd_linear_pack /            the reference (the MLP called at P/srt/batch_overlap/
+ *   afd_linear_silu_mul          operations_strategy.py:94, 255)
  *   afd_expert_counts / ........ no counterpart: where the tokens go, the balance loss of a
  *   afd_balance / ..............  router in training, and the gradient of both by its logits
  *   afd_topk_balance /
@@ -425,6 +425,11 @@ int afd_linear_pack(const uint8_t* codes, int64_t ld, int32_t n_out, int32_t k_i
 int afd_linear_workspace(int32_t n, int32_t k_in, uint64_t* bytes);
 int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n,
                void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream);
+/* afd_silu_mul's result of gate_up bf16 [n][ld >= 2 k_in] as afd_linear's x, bit for bit, which never
+ * is in memory: a SwiGLU MLP's down projection. */
+int afd_linear_silu_mul(const afd_linear_weights* weights, const uint16_t* gate_up, int64_t ld,
+                        int32_t n, void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy,
+                        afd_stream_t stream);
 
 /* ---- the router ---------------------------------------------------------------------------
  * Scores of a row of logits l: softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts

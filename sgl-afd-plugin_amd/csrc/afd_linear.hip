@@ -115,9 +115,25 @@ __device__ __forceinline__ float quantize(const Raw& r, v4i (&q)[2]) {
   return finite ? sc : __builtin_nanf("");
 }
 
+// bf16(silu(g) u) of a lane's gate and up values
+__device__ __forceinline__ Raw silu_mul(const Raw& g, const Raw& u) {
+  Raw r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = g.u[h][i], b = u.u[h][i];
+      r.u[h][i] = pk_bf16(act_swiglu(__uint_as_float(a << 16), __uint_as_float(b << 16)),
+                          act_swiglu(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)));
+    }
+  return r;
+}
+
 // One wavefront an item, one pass: bound by its bytes where x is large (16384 x 4096, 201 MB in all: 35 us, 5.7 TB/s).
 // NT: non-temporal reads, for an x that no cache holds anyway.
-template <bool VEC, bool NT>
+// SILU: x's rows are [gate | up] of 2 k_in columns and what is quantized is bf16(silu(gate) up), which then
+// never is in memory (the product of 16384 x 1536 x 4096 with it 134 us, 157 in two launches; 48 rows 9.1 against 9.9).
+template <bool VEC, bool NT, bool SILU>
 __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
                                                     uint8_t* __restrict__ q, float* __restrict__ s, int kb,
                                                     int a_rows) {
@@ -127,7 +143,10 @@ __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__
   const int b = static_cast<int>(item % kb), lane = threadIdx.x & 63;
   const int64_t row = min(r16 * 16 + (lane & 15), int64_t(n) - 1);  // past the end: the last again
   v4i code[2];
-  const float sc = quantize(load_raw<VEC, NT>(x + row * ldx, k_in, b, lane >> 4), code);
+  const uint16_t* p = x + row * ldx;
+  Raw raw = load_raw<VEC, NT>(p, k_in, b, lane >> 4);
+  if constexpr (SILU) raw = silu_mul(raw, load_raw<VEC, NT>(p + k_in, k_in, b, lane >> 4));
+  const float sc = quantize(raw, code);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     *reinterpret_cast<v4i*>(q + (r16 * (2 * kb) + 2 * b + h) * kPiece + lane * 16) = code[h];
@@ -161,7 +180,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ w
 // nothing is 3.6; 48 x 2048 x 4096 5.5 to 6.5 us after 3.2 of quantization.
 // FUSED: no launch before it. The workgroup quantizes its rows into LDS while its first weights are on
 // their way (16 rows' K blocks a wavefront at a time, whichever rows they are of): n K elements, which every
-// workgroup does again, so only where they are few and fit kFusedBytes.
+// workgroup does again, so only where they are few and fit kFusedBytes. SILU: as the quantization's.
 constexpr int kRowWaves = 8;
 constexpr int kFusedBytes = 32768;
 
@@ -171,7 +190,7 @@ struct RowsIn {
   int k_in;
 };
 
-template <int MT, bool FUSED, bool VEC>
+template <int MT, bool FUSED, bool VEC, bool SILU>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in) {
   constexpr int kDepth = FUSED || MT <= 2 ? 4 : MT == 3 ? 3 : 2;
   constexpr int kPart = kRowWaves * MT * 64 * 16;
@@ -218,22 +237,25 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
   for (int d = 0; d < kDepth; ++d) ring[d] = fetch(w + d * kRowWaves);
   // FUSED: chunk c of half h of K block b of row r at ((2 b + h) 4 + c) 16 n + 16 r
   if constexpr (FUSED) {
-    constexpr int kUp = 4;  // items on their way at once
+    constexpr int kUp = SILU ? 2 : 4;  // items on their way at once
     const int items = p.n * p.kb, c = lane >> 4;
     for (int at = w * 16; at < items; at += kUp * kRowWaves * 16) {
-      Raw raw[kUp];
+      Raw raw[kUp], up[SILU ? kUp : 1];
       int r[kUp], b[kUp];
 #pragma unroll
       for (int u = 0; u < kUp; ++u) {
         const int it = min(at + u * kRowWaves * 16 + (lane & 15), items - 1);
         r[u] = it / p.kb;
         b[u] = it - r[u] * p.kb;
-        raw[u] = load_raw<VEC>(in.x + r[u] * in.ldx, in.k_in, b[u], c);
+        const uint16_t* x = in.x + r[u] * in.ldx;
+        raw[u] = load_raw<VEC>(x, in.k_in, b[u], c);
+        if constexpr (SILU) up[u] = load_raw<VEC>(x + in.k_in, in.k_in, b[u], c);
       }
 #pragma unroll
       for (int u = 0; u < kUp; ++u) {
         if (u > 0 && at + u * kRowWaves * 16 >= items) break;
         v4i q[2];
+        if constexpr (SILU) raw[u] = silu_mul(raw[u], up[u]);
         const float sc = quantize(raw[u], q);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -563,15 +585,21 @@ static int launch_tiles(const Args& p, hipStream_t s) {
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
-template <int MT, bool FUSED>
+template <int MT, bool FUSED, bool SILU>
 static int launch_rows(const Args& p, const RowsIn& in, bool vec, hipStream_t s) {
   const dim3 grid((p.n_out + 15) / 16, (p.n + 16 * MT - 1) / (16 * MT)), block(64 * kRowWaves);
   if (!FUSED || vec)
-    hipLaunchKernelGGL((rows_kernel<MT, FUSED, true>), grid, block, 0, s, p, in);
+    hipLaunchKernelGGL((rows_kernel<MT, FUSED, true, SILU>), grid, block, 0, s, p, in);
   else
-    hipLaunchKernelGGL((rows_kernel<MT, FUSED, !FUSED>), grid, block, 0, s, p, in);
+    hipLaunchKernelGGL((rows_kernel<MT, FUSED, !FUSED, SILU>), grid, block, 0, s, p, in);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
+}
+template <bool SILU>
+static int launch_fused_rows(const Args& p, const RowsIn& in, bool vec, hipStream_t s) {
+  if (p.n <= 16) return launch_rows<1, true, SILU>(p, in, vec, s);
+  if (p.n <= 32) return launch_rows<2, true, SILU>(p, in, vec, s);
+  return launch_rows<4, true, SILU>(p, in, vec, s);
 }
 
 // The shape whose rounds over the CUs take least: rounds x the measured time of one K block (T64 .. T256
@@ -593,6 +621,77 @@ static int best_shape(int64_t n, int64_t n_out, int cus) {
     }
   }
   return best;
+}
+
+// y = q(x) W^T, or with silu of the activation of x's rows [gate | up]
+static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n, bool silu, void* ws,
+               uint64_t ws_bytes, uint16_t* y, int64_t ldy, hipStream_t s) {
+  if (!weights || n < 0 || n > kMaxRows) return AFD_ERR_ARG;
+  const int st = check_dims(weights->n_out, weights->k_in);
+  if (st != AFD_OK) return st;
+  if (ldx < int64_t(silu ? 2 : 1) * weights->k_in || ldy < weights->n_out) return AFD_ERR_SHAPE;
+  if (n == 0) return AFD_OK;
+  if (!weights->image || !weights->scales || !x || !ws || !y) return AFD_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(weights->image) % 16) return AFD_ERR_SHAPE;
+  const Plan pl = plan(n, weights->k_in);
+  if (ws_bytes < static_cast<uint64_t>(pl.total) || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
+  uint8_t* q = static_cast<uint8_t*>(ws);
+  float* sx = reinterpret_cast<float*>(q + pl.q_bytes);
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && weights->k_in % 16 == 0;
+  Args p = {};
+  p.a = q;
+  p.as = sx;
+  p.b = static_cast<const uint8_t*>(weights->image);
+  p.bs = weights->scales;
+  p.y = y;
+  p.ldy = ldy;
+  p.n = n;
+  p.n_out = weights->n_out;
+  p.kb = pl.kb;
+  p.a_rows = pl.a_rows;
+  p.wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy % 8 == 0;
+  const RowsIn in = {x, ldx, weights->k_in};
+  // the rows kernel's own quantization is faster up to 32 K elements (4096 x 4096: 4 rows 6.7 against 8.8 us,
+  // 16 rows 10.8 against 9.0; 1024 x 1000: 32 rows 6.4 against 7.1, 64 rows 9.5 against 7.4), a third
+  // of that where the rows do not take wide loads (300 x 3000: 32 rows 6.7 against 7.3, 64 rows 10.0 against 7.5)
+  const int64_t elements = int64_t(n) * pl.kb * 128;
+  if (n <= 64 && elements <= (vec ? kFusedBytes : kFusedBytes / 3))
+    return silu ? launch_fused_rows<true>(p, in, vec, s) : launch_fused_rows<false>(p, in, vec, s);
+  const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
+  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
+  // (134 MB of x: 36 us non-temporal, 42 through the caches; 24 MB, which they hold: 9.3 against 8.0)
+  const bool nt = int64_t(n) * weights->k_in * (silu ? 4 : 2) > kCachedBytes;
+  auto quant = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
+  };
+  auto quant_any = [&](auto silu_c) {
+    constexpr bool kSilu = decltype(silu_c)::value;
+    if (vec && nt)
+      quant(quant_kernel<true, true, kSilu>);
+    else if (vec)
+      quant(quant_kernel<true, false, kSilu>);
+    else
+      quant(quant_kernel<false, false, kSilu>);
+  };
+  if (silu)
+    quant_any(std::true_type{});
+  else
+    quant_any(std::false_type{});
+  AFD_CHECK_LAUNCH();
+  // up to 64 rows the weights are read once; above, tiles (4096 x 4096: 64 rows 12.8 against 13.5 us, 128
+  // rows 14.7 against 13.9)
+  if (n <= 16) return launch_rows<1, false, false>(p, in, vec, s);
+  if (n <= 32) return launch_rows<2, false, false>(p, in, vec, s);
+  if (n <= 48) return launch_rows<3, false, false>(p, in, vec, s);
+  if (n <= 64) return launch_rows<4, false, false>(p, in, vec, s);
+  switch (best_shape(n, p.n_out, device_cu_count())) {
+    case kT64: return launch_tiles<T64>(p, s);
+    case kT64x128: return launch_tiles<T64x128>(p, s);
+    case kT128: return launch_tiles<T128>(p, s);
+    case kT192x256: return launch_tiles<T192x256>(p, s);
+    case kT256x128: return launch_tiles<T256x128>(p, s);
+    default: return launch_tiles<T256>(p, s);
+  }
 }
 
 }  // namespace linear
@@ -633,67 +732,10 @@ extern "C" int afd_linear_workspace(int32_t n, int32_t k_in, uint64_t* bytes) {
 
 extern "C" int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n, void* ws,
                           uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream) {
-  if (!weights || n < 0 || n > linear::kMaxRows) return AFD_ERR_ARG;
-  const int st = linear::check_dims(weights->n_out, weights->k_in);
-  if (st != AFD_OK) return st;
-  if (ldx < weights->k_in || ldy < weights->n_out) return AFD_ERR_SHAPE;
-  if (n == 0) return AFD_OK;
-  if (!weights->image || !weights->scales || !x || !ws || !y) return AFD_ERR_ARG;
-  if (reinterpret_cast<uintptr_t>(weights->image) % 16) return AFD_ERR_SHAPE;
-  const linear::Plan pl = linear::plan(n, weights->k_in);
-  if (ws_bytes < static_cast<uint64_t>(pl.total) || reinterpret_cast<uintptr_t>(ws) % 16) return AFD_ERR_WORKSPACE;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  uint8_t* q = static_cast<uint8_t*>(ws);
-  float* sx = reinterpret_cast<float*>(q + pl.q_bytes);
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && weights->k_in % 16 == 0;
-  linear::Args p = {};
-  p.a = q;
-  p.as = sx;
-  p.b = static_cast<const uint8_t*>(weights->image);
-  p.bs = weights->scales;
-  p.y = y;
-  p.ldy = ldy;
-  p.n = n;
-  p.n_out = weights->n_out;
-  p.kb = pl.kb;
-  p.a_rows = pl.a_rows;
-  p.wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy % 8 == 0;
-  const linear::RowsIn in = {x, ldx, weights->k_in};
-  // the rows kernel's own quantization is faster up to 32 K elements (4096 x 4096: 4 rows 6.7 against 8.8 us,
-  // 16 rows 10.8 against 9.0; 1024 x 1000: 32 rows 6.4 against 7.1, 64 rows 9.5 against 7.4), a third
-  // of that where the rows do not take wide loads (300 x 3000: 32 rows 6.7 against 7.3, 64 rows 10.0 against 7.5)
-  const int64_t elements = int64_t(n) * pl.kb * 128;
-  if (n <= 64 && elements <= (vec ? linear::kFusedBytes : linear::kFusedBytes / 3)) {
-    if (n <= 16) return linear::launch_rows<1, true>(p, in, vec, s);
-    if (n <= 32) return linear::launch_rows<2, true>(p, in, vec, s);
-    return linear::launch_rows<4, true>(p, in, vec, s);
-  }
-  const int64_t items = (int64_t(n) + 15) / 16 * pl.kb;
-  const dim3 grid(static_cast<unsigned>((items + 3) / 4));
-  // (134 MB of x: 36 us non-temporal, 42 through the caches; 24 MB, which they hold: 9.3 against 8.0)
-  const bool nt = int64_t(n) * weights->k_in * 2 > linear::kCachedBytes;
-  auto quant = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, x, ldx, n, weights->k_in, q, sx, pl.kb, pl.a_rows);
-  };
-  if (vec && nt)
-    quant(linear::quant_kernel<true, true>);
-  else if (vec)
-    quant(linear::quant_kernel<true, false>);
-  else
-    quant(linear::quant_kernel<false, false>);
-  AFD_CHECK_LAUNCH();
-  // up to 64 rows the weights are read once; above, tiles (4096 x 4096: 64 rows 12.8 against 13.5 us, 128
-  // rows 14.7 against 13.9)
-  if (n <= 16) return linear::launch_rows<1, false>(p, in, vec, s);
-  if (n <= 32) return linear::launch_rows<2, false>(p, in, vec, s);
-  if (n <= 48) return linear::launch_rows<3, false>(p, in, vec, s);
-  if (n <= 64) return linear::launch_rows<4, false>(p, in, vec, s);
-  switch (linear::best_shape(n, p.n_out, device_cu_count())) {
-    case linear::kT64: return linear::launch_tiles<linear::T64>(p, s);
-    case linear::kT64x128: return linear::launch_tiles<linear::T64x128>(p, s);
-    case linear::kT128: return linear::launch_tiles<linear::T128>(p, s);
-    case linear::kT192x256: return linear::launch_tiles<linear::T192x256>(p, s);
-    case linear::kT256x128: return linear::launch_tiles<linear::T256x128>(p, s);
-    default: return linear::launch_tiles<linear::T256>(p, s);
-  }
+  return linear::run(weights, x, ldx, n, false, ws, ws_bytes, y, ldy, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int afd_linear_silu_mul(const afd_linear_weights* weights, const uint16_t* gate_up, int64_t ld, int32_t n,
+                                   void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream) {
+  return linear::run(weights, gate_up, ld, n, true, ws, ws_bytes, y, ldy, static_cast<hipStream_t>(stream));
 }

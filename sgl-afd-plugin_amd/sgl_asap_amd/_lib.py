@@ -72,6 +72,7 @@ EXPORTED = (
     "afd_linear_pack",
     "afd_linear_workspace",
     "afd_linear",
+    "afd_linear_silu_mul",
     "afd_topk",
     "afd_balance_workspace",
     "afd_expert_counts",
@@ -295,6 +296,7 @@ _SIGS = {
     "afd_linear_pack": ([_P, _I64, _I32, _I32, _P, _P], _I32),
     "afd_linear_workspace": ([_I32, _I32, ctypes.POINTER(_U64)], _I32),
     "afd_linear": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
+    "afd_linear_silu_mul": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
     "afd_topk": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _P], _I32),
     "afd_balance_workspace": ([_I32, _I32, _I32, ctypes.POINTER(_U64)], _I32),
     "afd_expert_counts": ([_P, _I32, _I32, _I32, _P, _P, _I32, _P, _P, _U64, _P], _I32),

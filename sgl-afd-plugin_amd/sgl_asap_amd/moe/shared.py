@@ -15,7 +15,8 @@ The add itself is fused into the combine kernel (``afd_combine``'s ``shared`` ar
 
 ``Fp8SharedExpertMLP`` is the same MLP on the block-FP8 weights that FP8 checkpoints hold
 (``Fp8BlockLinear``): half the weight bytes, which is what a decode step waits for, and the FP8
-matrix rate in prefill.
+matrix rate in prefill. Its activation is taken in the down product's quantization (hidden 4096, intermediate
+1536: 1 token 9.1 us against 20.8 for the bf16 MLP, 300 29.0 against 32.4, 16384 349 against 447).
 """
 
 from __future__ import annotations
@@ -84,7 +85,7 @@ class Fp8SharedExpertMLP(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden_size:
             raise TypeError(f"expected bf16 [n, {self.hidden_size}], got {x.dtype} {tuple(x.shape)}")
-        return self.down(silu_mul(self.gate_up(x)))
+        return self.down.silu_mul(self.gate_up(x))
 
 
 def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:

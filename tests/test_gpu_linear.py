@@ -300,3 +300,67 @@ def test_out_that_shares_elements_with_x_is_refused():
         out = buf[:n, at : at + k]
         assert layer(rows, out=out) is out and torch.equal(out, want)
     assert torch.equal(buf[:n, :k].cpu(), x.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("n,inter,n_out", [(1, 256, 64), (3, 1536, 384), (20, 200, 100), (47, 131, 65), (64, 384, 260), (130, 128, 48),
+                                           (700, 640, 513), (2600, 1536, 512), (9000, 2048, 40)])
+def test_silu_mul_in_the_quantization(n, inter, n_out):
+    """The same bits as the activation and the layer one after the other, from rows with a stride and into them."""
+    g = torch.Generator().manual_seed(n + inter)
+    w, s = e4m3(torch.randn(n_out, inter, generator=g) * 50), torch.rand(ceil(n_out, 128), ceil(inter, 128), generator=g) * 2e-3
+    gu = (torch.randn(n, 2 * inter, generator=g) * 3).to(torch.bfloat16)
+    gu[0, :5] = 100.0
+    if n > 2:
+        gu[1], gu[2, 7], gu[n - 1, inter] = 0.0, float("inf"), float("nan")
+    layer = Fp8BlockLinear(w.to(dev()), s.to(dev()))
+    say(f"silu n={n} inter={inter} n_out={n_out}")
+    gu = gu.to(dev())
+    want = layer(silu_mul_any(gu))
+    got = layer.silu_mul(gu)
+    assert np.array_equal(bits16(got), bits16(want))
+    if n > 2:
+        assert torch.isnan(got[2]).all() and torch.isnan(got[n - 1]).all() and torch.isfinite(got[0]).all()
+    buf = torch.full((n, 2 * inter + 24), 7.0, dtype=torch.bfloat16, device=dev())
+    buf[:, 8 : 8 + 2 * inter] = gu
+    out = torch.full((n, n_out + 9), 5.0, dtype=torch.bfloat16, device=dev())
+    layer.silu_mul(buf[:, 8 : 8 + 2 * inter], out=out[:, :n_out])
+    assert np.array_equal(bits16(out[:, :n_out]), bits16(want)) and (out[:, n_out:] == 5).all()
+    assert np.array_equal(bits16(layer.silu_mul(gu.view(1, n, 2 * inter))[0]), bits16(want))
+
+
+def silu_mul_any(gate_up):
+    """silu_mul of any number of columns: its kernel's rows padded to a multiple of 8."""
+    n, inter = gate_up.shape[0], gate_up.shape[1] // 2
+    pad = (inter + 7) // 8 * 8
+    wide = torch.zeros(n, 2, pad, dtype=torch.bfloat16, device=gate_up.device)
+    wide[:, :, :inter] = gate_up.view(n, 2, inter)
+    return silu_mul(wide.view(n, 2 * pad))[:, :inter].contiguous()
+
+
+def test_silu_mul_refusals_and_capture():
+    g = torch.Generator().manual_seed(1)
+    w, s = e4m3(torch.randn(96, 256, generator=g) * 50), torch.rand(1, 2, generator=g) * 2e-3
+    layer = Fp8BlockLinear(w.to(dev()), s.to(dev()))
+    gu = torch.randn(30, 512, generator=g).to(torch.bfloat16).to(dev())
+    say("silu refusals, capture")
+    with pytest.raises(TypeError):
+        layer.silu_mul(gu[:, :256])
+    with pytest.raises(TypeError):
+        layer.silu_mul(gu.float())
+    with pytest.raises(ValueError):
+        layer.silu_mul(gu, out=gu[:, :96])
+    with pytest.raises(NotImplementedError):
+        layer.silu_mul(gu.clone().requires_grad_())
+    assert layer.silu_mul(gu[:0]).shape == (0, 96)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.silu_mul(gu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer.silu_mul(gu)
+    for _ in range(3):
+        gu.copy_(torch.randn(30, 512, generator=g).to(torch.bfloat16).to(dev()))
+        graph.replay()
+        assert torch.equal(y, layer(silu_mul(gu)))

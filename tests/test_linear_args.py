@@ -99,3 +99,17 @@ def test_overlap():
         assert _overlap(x[: y.shape[0]], y) and _overlap(y, x[: y.shape[0]])
     one = buf[3:4, :16]
     assert not _overlap(one, buf[3:4, 16:40]) and _overlap(one, buf[3:4, 15:40])
+
+
+def test_silu_mul_calls():
+    L = _lib.lib()
+
+    def call(n=4, ld=400, x=16, ws=16, size=1 << 30, y=16, ldy=100, image=16):
+        w = _lib.AfdLinearWeights(100, 200, image, 16)
+        return L.afd_linear_silu_mul(ctypes.byref(w), x, ld, n, ws, size, y, ldy, None)
+
+    assert call(n=0) == OK and call(n=0, x=None, y=None, ws=None) == OK
+    assert L.afd_linear_silu_mul(None, 16, 400, 4, 16, 1 << 30, 16, 100, None) == ARG
+    assert call(n=-1) == ARG and call(x=None) == ARG and call(y=None) == ARG and call(ws=None) == ARG and call(image=None) == ARG
+    assert call(ld=399) == SHAPE and call(ldy=99) == SHAPE and call(image=24) == SHAPE
+    assert call(ws=24) == WS and call(size=100) == WS

@@ -172,6 +172,7 @@ __device__ __forceinline__ uint64_t key64(double v) {
 
 // ---------------------------------------------------------------- scores
 constexpr float kLowest = -__builtin_huge_valf();
+constexpr float kLeast = 0x1p-126f;  // sums below it count as 0: their reciprocal may leave the floats
 __device__ __forceinline__ float logit_f32(const float* p) { return *p; }
 __device__ __forceinline__ float logit_f32(const uint16_t* p) { return bf16_to_f32(*p); }
 __device__ __forceinline__ float canon(float v) {
@@ -714,7 +715,7 @@ __device__ __forceinline__ int choose(const Args& a, const Row<T, W, V>& row, in
     // that hold the place take 6. Three such bits take 14 (2^-19 then), four 30, a softmax's sum over 16 values a
     // lane and 6 butterflies 24: 2^-18 there. A score below 2^-126 may count as 0. Two values stand apart if
     // they differ by twice the row's largest such bound.
-    const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
+    const float inv = a.scoring == AFD_SCORE_SOFTMAX ? (sum >= kLeast ? __builtin_amdgcn_rcpf(sum) : 0.0f) : 1.0f;
     float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -823,12 +824,12 @@ __device__ __forceinline__ float weigh(const Args& a, const Row<T, W, V>& row, f
       for (int j = 0; j < V; ++j) sum += exp_fast(row.l[j] - at);
     }
     sum = sum_f32<W>(sum);
-    return sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
+    return sum >= kLeast ? s * __builtin_amdgcn_rcpf(sum) * a.scale : 0.0f;
   }
   s = BIAS ? fmaxf(l, 0.0f) : score_f32<true>(l, a.scoring);
   if (a.renorm) {
     const float sum = sum_f32<W>(s);
-    s = sum > 0.0f ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
+    s = sum >= kLeast ? s * __builtin_amdgcn_rcpf(sum) : 0.0f;
   }
   return s * a.scale;
 }
@@ -1072,7 +1073,7 @@ __device__ __forceinline__ void balance_rows(const Args& a, int32_t at, const Pi
         if (id >= 0 && id < a.experts) atomicAdd(&cnt[id], 1);
       }
     }
-    const float inv = live && sum > 0.0f ? __builtin_amdgcn_rcpf(sum) : 0.0f;
+    const float inv = live && sum >= kLeast ? __builtin_amdgcn_rcpf(sum) : 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) p[j] += s[j] * inv;
     mine += live ? 1 : 0;
@@ -1234,7 +1235,7 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
       row.set(a, now.raw, li);
       float s[V], d[V];
       const float total = row.template scores<false>(a, s);
-      const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
+      const float inv = total >= kLeast ? __builtin_amdgcn_rcpf(total) : 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) d[j] = 0.0f;
       if (balanced) {
@@ -1270,7 +1271,7 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
         }
         const float chosen = sum_f32<W>(share);
         if (a.renorm)
-          share = chosen > 0.0f ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
+          share = chosen >= kLeast ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
         else if (a.scoring == AFD_SCORE_SOFTMAX)
           share *= inv;
         // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something. Renormalized ones

@@ -614,3 +614,22 @@ def test_bias_that_bars_or_forces_experts(n, experts, top_k, groups, keep, scori
         say(f"bias of {kinds} n={n} E={experts} groups={groups}/{keep} {scoring}")
         out = select(logits, top_k, b, scoring=scoring, groups=groups, keep=keep)
         check_choice(logits, top_k, out, scoring, b, groups=groups, keep=keep)
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "sqrtsoftplus"])
+def test_one_pick_at_the_floats_lower_end(scoring):
+    """One score around 2^-126: its renormalized weight is the scale or, where fp32 does not hold the score, 0."""
+    n, experts, scale = 400, 64, 1.5
+    low = (-2.0 if scoring == "sqrtsoftplus" else -1.0) * torch.linspace(85, 90, n)
+    logits = torch.full((n, experts), -math.inf)
+    logits[:, 9] = low
+    for b in (None, torch.zeros(experts)):
+        say(f"one pick, lower end {scoring} bias={b is not None}")
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, _ = B.select_and_balance(leaf, 1, alpha=1.0, scoring=scoring, routed_scaling_factor=scale,
+                                            correction_bias=None if b is None else b.to(dev()))
+        (grad,) = torch.autograd.grad((out.topk_weights.sum(), loss), (leaf,))
+        w = out.topk_weights.detach().cpu()[:, 0]
+        assert (out.topk_ids == 9).all() and torch.isfinite(grad).all() and torch.isfinite(loss.detach())
+        assert (((w - scale).abs() <= 2.0**-20) | (w == 0)).all()
+        assert (w[low > -86.5 * (2 if scoring == "sqrtsoftplus" else 1)] > 0).all()

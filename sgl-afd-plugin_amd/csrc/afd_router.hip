@@ -314,17 +314,14 @@ struct Row {
   }
 };
 
-// The lanes of this row in a ballot
-template <int W>
-__device__ __forceinline__ uint64_t row_bits(uint64_t ballot, int lane) {
-  if constexpr (W == 64) return ballot;
-  return (ballot >> (lane & ~(W - 1))) & ((uint64_t(1) << W) - 1);
-}
-
 // The lane of this row that holds the first of the set bits
 template <int W>
 __device__ __forceinline__ int first_lane(bool bit, int lane) {
-  return __builtin_ctzll(row_bits<W>(__ballot(bit), lane));
+  const uint64_t all = __ballot(bit);
+  if constexpr (W == 64) return __builtin_ctzll(all);
+  const uint32_t half = lane & 32 ? static_cast<uint32_t>(all >> 32) : static_cast<uint32_t>(all);
+  if constexpr (W == 32) return __builtin_ctz(half);
+  return __builtin_ctz(half >> (lane & 16));  // the other row's bits lie above this one's, of which one is set
 }
 
 // The row's keys, taken largest first (lowest index of equals). A lane sorts its own keys once and only

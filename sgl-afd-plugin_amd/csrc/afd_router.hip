@@ -20,7 +20,7 @@
 // and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
 // else 64 lanes with V = 4, 8 or 16; a choice of many rows takes 16 or 32 lanes up to 256 experts. A
 // lane sorts its values once; a pick is then a max butterfly (DPP and permlane swaps) over the lanes' heads.
-// What bounds it is instructions, not bytes: 16384 x 256 with a bias and 4 of 8 groups takes 17 to 20 us (825 VALU
+// What bounds it is instructions, not bytes: 16384 x 256 with a bias and 4 of 8 groups takes 17 to 20 us (830 VALU
 // instructions for two rows, 11 us of issue; its 18 MB 3.7 us), by the logits alone 9.0; few rows a launch (8 x 256 4.3).
 //
 // Sums over rows: a workgroup takes R consecutive rows, cut where sequences begin and end; each piece

@@ -18,7 +18,7 @@
 //
 // Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
 // and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
-// else 64 lanes with V = 4, 8 or 16; a choice of many rows takes 16 or 32 lanes up to 256 experts. A
+// else 64 lanes with V = 4, 8 or 16; a choice of many rows takes 16 or 32 lanes up to 512 experts. A
 // lane sorts its values once; a pick is then a max butterfly (DPP and permlane swaps) over the lanes' heads.
 // What bounds it is instructions, not bytes: 16384 x 256 with a bias and 4 of 8 groups takes 17 to 20 us (830 VALU
 // instructions for two rows, 11 us of issue; its 18 MB 3.7 us), by the logits alone 9.0; few rows a launch (8 x 256 4.3).
@@ -1341,14 +1341,16 @@ int with_shape(int experts, int lanes, F&& f) {
 // is shared by the rows of a wavefront. By the logits alone 16 lanes (256 experts: 4096 rows 5.4 us
 // against 5.0 in the shapes above, 8192 6.4 against 7.5, 65536 26.7 against 43.7), with a bias, whose scores
 // cost more than the rounds and whose close rows take longer the more experts a lane has, 32 (8192 rows 11.9
-// against 10.4, 16384 14.5 against 16.4, 65536 41.2 against 50.8; 16 lanes: 16384 rows 19.3).
+// against 10.4, 16384 14.5 against 16.4, 65536 41.2 against 50.8; 16 lanes: 16384 rows 19.3). Up to 512 experts 32
+// lanes by the logits (8192 rows 9.5 against 11.4, 65536 46.6 against 55.9); with a bias as good as 64 up to 16384 rows.
 constexpr int kManyRows = 6144, kManyBiasedRows = 12288;
 template <typename F>
 int with_choice_shape(int experts, int lanes, bool bias, int n, F&& f) {
   using std::integral_constant;
-  if (!bias && n >= kManyRows && lanes <= 16 && experts > 64) {
-    if (experts <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    if (experts <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  if (!bias && n >= kManyRows && experts > 64) {
+    if (experts <= 128 && lanes <= 16) return f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    if (experts <= 256 && lanes <= 16) return f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+    if (experts > 256 && experts <= 512 && lanes <= 32) return f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
   }
   if (bias && n >= kManyBiasedRows && lanes <= 32 && experts > 128 && experts <= 256)
     return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
@@ -1534,9 +1536,9 @@ extern "C" int afd_topk(const afd_router_cfg* cfg, const void* logits, int64_t l
       constexpr int W = decltype(wc)::value, V = decltype(vc)::value, kRows = router::kThreads / W;
       router::set_shape(a, W, V, sizeof(T));
       hipStream_t s = static_cast<hipStream_t>(stream);
-      if constexpr (W == 16 && V > 4)
+      if constexpr ((W == 16 && V > 4) || (W == 32 && V == 16))
         return router::launch_topk<router::topk_kernel<T, W, V, false>>(a, kRows, s);
-      else if constexpr (W == 32 && V > 4)
+      else if constexpr (W == 32 && V == 8)
         return router::launch_topk<router::topk_kernel<T, W, V, true>>(a, kRows, s);
       else
         return bias ? router::launch_topk<router::topk_kernel<T, W, V, true>>(a, kRows, s)

@@ -633,3 +633,24 @@ def test_one_pick_at_the_floats_lower_end(scoring):
         assert (out.topk_ids == 9).all() and torch.isfinite(grad).all() and torch.isfinite(loss.detach())
         assert (((w - scale).abs() <= 2.0**-20) | (w == 0)).all()
         assert (w[low > -86.5 * (2 if scoring == "sqrtsoftplus" else 1)] > 0).all()
+
+
+@pytest.mark.parametrize("experts,top_k,groups,keep", [(257, 8, 0, 0), (300, 32, 0, 0), (384, 8, 12, 5), (480, 6, 32, 9), (512, 8, 8, 4)])
+def test_unbiased_choice_of_many_rows_and_experts(experts, top_k, groups, keep):
+    """32 lanes of 16 experts: ordinary rows, ties, masks, next floats."""
+    g = torch.Generator().manual_seed(experts)
+    n = MANY
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.randn(n, experts, generator=g) * 2
+        logits[::4] = torch.randint(-2, 2, (n, experts), generator=g).float()[::4]
+        half = experts // 2
+        logits[1::4, half : 2 * half] = logits[1::4, :half] * (1 + 2.0**-22)
+        logits[torch.rand(n, experts, generator=g) < 0.01] = -math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.003] = math.inf
+        logits[torch.rand(n, experts, generator=g) < 0.003] = math.nan
+        logits[7, 9:], logits[8], logits[9] = -math.inf, -math.inf, math.nan
+        logits = logits.to(dtype)
+        for scoring, renorm in (("softmax", True), ("softmax", False), ("sqrtsoftplus", True)):
+            say(f"many rows and experts E={experts} k={top_k} groups={groups}/{keep} {scoring} {dtype}")
+            out = select(logits, top_k, scoring=scoring, groups=groups, keep=keep, renormalize=renorm)
+            check_choice(logits, top_k, out, scoring, None, renorm, 1.0, groups, keep)

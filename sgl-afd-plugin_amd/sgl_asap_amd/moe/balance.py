@@ -23,7 +23,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .topk import StandardTopKOutput, choice_cfg, launch, logit_rows, need_gpu, on_device, once, router_cfg, router_grad
+from .topk import StandardTopKOutput, choice_cfg, last, launch, logit_rows, need_gpu, on_device, router_cfg, router_grad
 
 
 @lru_cache(maxsize=1024)
@@ -70,11 +70,11 @@ def expert_counts(topk_ids: torch.Tensor, num_experts: int, cu_seqlens: Optional
 
 
 class _Balance(torch.autograd.Function):
-    """(weights, ids, loss, counts) with ids chosen here, (loss, counts) for given ones."""
+    """(weights, ids, loss, counts) with ids chosen here, (loss, counts) for given ones; logits as ``logit_rows`` gives them:
+    what the backward reads is then the input itself."""
 
     @staticmethod
     def forward(ctx, logits, cfg, top_k, alpha, bias, ids, cu, valid):
-        need_gpu("router_logits", logits)
         logits, ld = logit_rows(logits)
         n, experts = logits.shape
         dev = logits.device
@@ -106,16 +106,12 @@ class _Balance(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        return once(_Balance._backward, ctx, *grads)
-
-    @staticmethod
-    def _backward(ctx, *grads):
         logits, ids, cu, valid, counts, coef = ctx.saved_tensors
         gw, gloss = (grads[0], grads[2]) if ids is not None else (None, grads[0])
         grad = None
         if gw is not None or gloss is not None:
             with_loss = (None,) * 4 if gloss is None else (cu, counts, coef, gloss)
-            grad = router_grad(ctx.cfg, logits, ids, valid, gw, *with_loss)
+            grad = last(router_grad(ctx.cfg, logits, ids, valid, gw, *with_loss), logits, gw, gloss)
         return (grad,) + (None,) * 7
 
 
@@ -130,7 +126,8 @@ def balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor, *, alpha: 
     if ids.device != router_logits.device:
         raise ValueError(f"topk_ids is on {ids.device}, router_logits on {router_logits.device}")
     cfg = router_cfg(router_logits.shape[1], ids.shape[1], scoring, False, 0, 0, 1.0, router_logits.dtype)
-    return _Balance.apply(router_logits, cfg, ids.shape[1], float(alpha), None, ids, cu_seqlens, valid)
+    need_gpu("router_logits", router_logits)
+    return _Balance.apply(logit_rows(router_logits)[0], cfg, ids.shape[1], float(alpha), None, ids, cu_seqlens, valid)
 
 
 def select_and_balance(
@@ -150,6 +147,7 @@ def select_and_balance(
     """``select_experts`` and ``balance_loss`` of what it chose, as one pass over the logits each way:
     (top-k output, loss, counts)."""
     cfg = choice_cfg(router_logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor)
-    weights, ids, loss, counts = _Balance.apply(router_logits, cfg, top_k, float(alpha), correction_bias, None,
+    need_gpu("router_logits", router_logits)
+    weights, ids, loss, counts = _Balance.apply(logit_rows(router_logits)[0], cfg, top_k, float(alpha), correction_bias, None,
                                                 cu_seqlens, valid)
     return StandardTopKOutput(weights, ids, router_logits), loss, counts

@@ -24,7 +24,6 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -153,16 +152,26 @@ def router_grad(cfg, logits, ids, valid, gw, cu=None, counts=None, coef=None, gl
     return out
 
 
-_once_differentiable = once_differentiable(lambda ctx, run, *grads: run(ctx, *grads))
+class _NoDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, *made_from):
+        ctx.mark_dirty(grad)
+        return grad
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the router's gradient has no derivative of its own (no second derivatives)")
 
 
-def once(run, ctx, *grads):
-    """``run(ctx, *grads)``, a backward without a backward of its own. Torch's guard against a second
-    derivative costs as much host time as a launch, so it is put up only where one could be asked for."""
-    return _once_differentiable(ctx, run, *grads) if torch.is_grad_enabled() else run(ctx, *grads)
+def last(grad: torch.Tensor, *made_from: Optional[torch.Tensor]) -> torch.Tensor:
+    """``grad``, which a backward made from ``made_from``. Where a second derivative can be asked for (the backward runs with
+    gradients enabled) it is tied to them, whether or not the incoming gradients need one, by a node that raises."""
+    return _NoDerivative.apply(grad, *made_from) if torch.is_grad_enabled() else grad
 
 
 class _Select(torch.autograd.Function):
+    """logits as ``logit_rows`` gives them: what the backward reads is then the input itself."""
+
     @staticmethod
     def forward(ctx, logits, cfg, top_k, bias, valid):
         rows, ids, weights = choose(cfg, top_k, logits, bias, valid)
@@ -174,14 +183,10 @@ class _Select(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gw, _):
-        return once(_Select._backward, ctx, gw)
-
-    @staticmethod
-    def _backward(ctx, gw):
         if gw is None:
             return None, None, None, None, None
         logits, ids, valid = ctx.saved_tensors
-        return router_grad(ctx.cfg, logits, ids, valid, gw), None, None, None, None
+        return last(router_grad(ctx.cfg, logits, ids, valid, gw), logits, gw), None, None, None, None
 
 
 def select_experts(
@@ -206,7 +211,8 @@ def select_experts(
     weights have a gradient by the logits (zero in invalid rows)."""
     cfg = choice_cfg(router_logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor)
     if torch.is_grad_enabled() and router_logits.requires_grad:
-        weights, ids = _Select.apply(router_logits, cfg, top_k, correction_bias, valid)
+        need_gpu("router_logits", router_logits)
+        weights, ids = _Select.apply(logit_rows(router_logits)[0], cfg, top_k, correction_bias, valid)
     else:
         _, ids, weights = choose(cfg, top_k, router_logits, correction_bias, valid)
     return StandardTopKOutput(weights, ids, router_logits)

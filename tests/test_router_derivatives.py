@@ -1,0 +1,78 @@
+"""Derivatives that the router's operators and the dense FP8 layer do not have end in an error, and the ones that they have
+stay connected. On the CPU, with the launches replaced by the definitions in plain torch."""
+
+import pytest
+import torch
+
+from sgl_asap_amd.moe import balance as B
+from sgl_asap_amd.moe import topk as T
+
+TOP_K = 2
+
+
+def fake_choose(cfg, top_k, logits, bias, valid):
+    rows, _ = T.logit_rows(logits)
+    best = torch.softmax(rows.detach(), 1).topk(top_k, 1)
+    return rows, best.indices.to(torch.int32), best.values.contiguous()
+
+
+def fake_grad(cfg, logits, ids, valid, gw, cu=None, counts=None, coef=None, gloss=None):
+    with torch.no_grad():
+        out = 3.0 * logits * logits  # any function of the logits: what is tested is what is tied to it
+        if gw is not None:
+            out = out + gw.sum(1, keepdim=True)
+        return out.clone()
+
+
+def fake_launch(name, device, *args):
+    pass
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    for m in (T, B):
+        for name, fake in (("need_gpu", lambda *a: None), ("router_grad", fake_grad), ("launch", fake_launch)):
+            monkeypatch.setattr(m, name, fake)
+    monkeypatch.setattr(T, "choose", fake_choose)
+    monkeypatch.setattr(torch, "empty", torch.zeros)  # what a launch would have written
+
+
+def values(which, x):
+    """The differentiable outputs, one scalar whose gradient by them is a constant."""
+    ids = torch.zeros(x.shape[0], TOP_K, dtype=torch.int32)
+    if which == "select":
+        return T.select_experts(x, TOP_K).topk_weights.sum()
+    if which == "balance":
+        return B.balance_loss(x, ids, alpha=1.0)[0]
+    out, loss, _ = B.select_and_balance(x, TOP_K, alpha=1.0)
+    return out.topk_weights.sum() + loss
+
+
+ROWS = {"contiguous": lambda x: x, "strided": lambda x: x[:, 2:8], "columns": lambda x: x[:, ::2], "one row": lambda x: x[:1].expand(5, 10)}
+
+
+@pytest.mark.parametrize("rows", sorted(ROWS))
+@pytest.mark.parametrize("which", ["select", "balance", "both"])
+def test_second_derivative_raises_whatever_it_is_mixed_with(plain, which, rows):
+    leaf = torch.randn(4, 10, generator=torch.Generator().manual_seed(0)).requires_grad_()
+    value = values(which, ROWS[rows](leaf))
+    (g,) = torch.autograd.grad(value, leaf, create_graph=True)
+    assert g.requires_grad
+    # the incoming gradient was a constant, and the penalty comes with a term that has a derivative
+    with pytest.raises(RuntimeError, match="no derivative of its own"):
+        ((leaf ** 2).sum() + (g ** 2).sum()).backward()
+    # the first derivative is the plain one
+    (again,) = torch.autograd.grad(values(which, ROWS[rows](leaf)), leaf)
+    assert not again.requires_grad and torch.equal(again, g.detach())
+
+
+@pytest.mark.parametrize("which", ["select", "balance", "both"])
+def test_a_gradient_made_with_its_graph_accumulates_like_any_other(plain, which):
+    leaf = torch.ones(3, 6).requires_grad_()
+    values(which, leaf).backward(create_graph=True)
+    once = leaf.grad.detach().clone()
+    values(which, leaf).backward(create_graph=True)
+    assert torch.equal(leaf.grad.detach(), 2 * once)
+    with torch.no_grad():
+        leaf.grad.zero_()
+    leaf.grad = None

@@ -23,7 +23,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .topk import StandardTopKOutput, choice_cfg, last, launch, logit_rows, need_gpu, on_device, router_cfg, router_grad
+from .topk import (StandardTopKOutput, choice_cfg, last, launch, logit_rows, need_gpu, no_tangent, on_device, router_cfg,
+                   router_grad)
 
 
 @lru_cache(maxsize=1024)
@@ -127,6 +128,7 @@ def balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor, *, alpha: 
         raise ValueError(f"topk_ids is on {ids.device}, router_logits on {router_logits.device}")
     cfg = router_cfg(router_logits.shape[1], ids.shape[1], scoring, False, 0, 0, 1.0, router_logits.dtype)
     need_gpu("router_logits", router_logits)
+    no_tangent("balance_loss", router_logits)
     return _Balance.apply(logit_rows(router_logits)[0], cfg, ids.shape[1], float(alpha), None, ids, cu_seqlens, valid)
 
 
@@ -148,6 +150,7 @@ def select_and_balance(
     (top-k output, loss, counts)."""
     cfg = choice_cfg(router_logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor)
     need_gpu("router_logits", router_logits)
+    no_tangent("select_and_balance", router_logits)
     weights, ids, loss, counts = _Balance.apply(logit_rows(router_logits)[0], cfg, top_k, float(alpha), correction_bias, None,
                                                 cu_seqlens, valid)
     return StandardTopKOutput(weights, ids, router_logits), loss, counts

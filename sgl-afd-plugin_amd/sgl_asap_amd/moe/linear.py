@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .topk import launch, matrix_rows, need_gpu
+from .topk import launch, matrix_rows, need_gpu, no_tangent
 
 FP8_BLOCK = 128
 
@@ -86,6 +86,7 @@ class Fp8BlockLinear(torch.nn.Module):
             raise ValueError(f"x is on {x.device}, the weights on {self.image.device}")
         if torch.is_grad_enabled() and (x.requires_grad or out is not None and out.requires_grad):
             raise NotImplementedError("Fp8BlockLinear has no gradient: call it under torch.no_grad()")
+        no_tangent("Fp8BlockLinear", x, out)
         rows = x if x.dim() == 2 else x.reshape(-1, columns)
         rows, ldx = matrix_rows(rows)
         n = rows.shape[0]

@@ -24,6 +24,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -100,6 +101,15 @@ def on_device(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: t
 def need_gpu(name: str, t: torch.Tensor) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a GPU, got {t.device}: there is no CPU path")
+
+
+def no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses tensors that carry a tangent, which a launch would drop (one needs no gradient, nor gradients enabled)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open: spares the calls
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _groups(num_expert_group: Optional[int], topk_group: Optional[int]):
@@ -210,6 +220,7 @@ def select_experts(
     -inf alone gets weights 0, and so does one whose chosen scores are all below 2^-126. The
     weights have a gradient by the logits (zero in invalid rows)."""
     cfg = choice_cfg(router_logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor)
+    no_tangent("select_experts", router_logits)
     if torch.is_grad_enabled() and router_logits.requires_grad:
         need_gpu("router_logits", router_logits)
         weights, ids = _Select.apply(logit_rows(router_logits)[0], cfg, top_k, correction_bias, valid)

@@ -3,8 +3,10 @@ stay connected. On the CPU, with the launches replaced by the definitions in pla
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from sgl_asap_amd.moe import balance as B
+from sgl_asap_amd.moe import linear as L
 from sgl_asap_amd.moe import topk as T
 
 TOP_K = 2
@@ -76,3 +78,26 @@ def test_a_gradient_made_with_its_graph_accumulates_like_any_other(plain, which)
     with torch.no_grad():
         leaf.grad.zero_()
     leaf.grad = None
+
+
+def test_tangents_are_refused(plain, monkeypatch):
+    """A dual tensor does not require a gradient, so nothing else would notice that its tangent is dropped."""
+    x = torch.ones(3, 6)
+    layer = object.__new__(L.Fp8BlockLinear)
+    torch.nn.Module.__init__(layer)
+    layer.image, layer.in_features, layer.out_features = torch.zeros(1), 6, 4
+    h = torch.ones(3, 6, dtype=torch.bfloat16)
+    with fw.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for t in (fw.make_dual(x, x), fw.make_dual(x, x)[:, :5], fw.make_dual(x, x)[:, ::2]):
+                    for which in ("select", "balance", "both"):
+                        with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                            values(which, t)
+                for args in ((fw.make_dual(h, h),), (h, fw.make_dual(h[:, :4].clone(), h[:, :4].clone()))):
+                    with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                        layer(*args)
+                with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                    layer.silu_mul(fw.make_dual(torch.cat([h, h], 1), torch.cat([h, h], 1)))
+        # no tangent, no refusal, also while a level is open
+        values("select", x), values("balance", x), values("both", x)

@@ -25,6 +25,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from .. import _lib
 
@@ -48,6 +49,8 @@ LOGITS_FORMATS = {torch.float32: _lib.AFD_LOGITS_F32, torch.bfloat16: _lib.AFD_L
 
 def launch(name: str, device: torch.device, *args) -> None:
     """``_lib.call`` on ``device``'s current stream, with ``device`` current."""
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise NotImplementedError(f"{name} cannot be traced: the graph would hold the results' memory, not what writes it")
     # (the plain bindings: torch.cuda's wrappers of these two cost a microsecond each)
     index = device.index
     if index == torch._C._cuda_getDevice():

@@ -1,9 +1,13 @@
 """Derivatives that the router's operators and the dense FP8 layer do not have end in an error, and the ones that they have
 stay connected. On the CPU, with the launches replaced by the definitions in plain torch."""
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 from sgl_asap_amd.moe import balance as B
 from sgl_asap_amd.moe import linear as L
@@ -101,3 +105,66 @@ def test_tangents_are_refused(plain, monkeypatch):
                     layer.silu_mul(fw.make_dual(torch.cat([h, h], 1), torch.cat([h, h], 1)))
         # no tangent, no refusal, also while a level is open
         values("select", x), values("balance", x), values("both", x)
+
+
+def traced(how, f, x):
+    if how == "jit":
+        return torch.jit.trace(f, (x,), check_trace=False)
+    return make_fx(f, tracing_mode="real", pre_dispatch=how == "pre_dispatch")(x)
+
+
+@pytest.mark.parametrize("how", ["fx", "pre_dispatch", "jit"])
+def test_tracing_is_refused(monkeypatch, how):
+    """A trace would hold the allocation of the results and not the launch that writes them."""
+    done, call = [], T._lib.call
+    monkeypatch.setattr(T._lib, "call", lambda name, *args: call(name, *args) if "workspace" in name else done.append(name))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0)
+    for m in (T, B):
+        monkeypatch.setattr(m, "need_gpu", lambda *a: None)
+    layer = object.__new__(L.Fp8BlockLinear)
+    torch.nn.Module.__init__(layer)
+    layer.image, layer.in_features, layer.out_features, layer._weights_ref = torch.zeros(1), 6, 4, None
+    x = torch.ones(3, 6)
+    ids = torch.zeros(3, TOP_K, dtype=torch.int32)
+    calls = [lambda x: T.select_experts(x, TOP_K).topk_weights, lambda x: values("balance", x), lambda x: values("both", x),
+             lambda x: B.expert_counts(ids, 6), lambda x: layer(x.to(torch.bfloat16))]
+    for f in calls:
+        done.clear()
+        f(x)
+        assert len(done) == 1
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            traced(how, f, x)
+        # a mode that records nothing (here one that counts operations) is no trace
+        with FlopCounterMode(display=False):
+            f(x)
+        assert len(done) == 2
+
+
+def test_compiled_functions_run_the_launch_each_time(monkeypatch):
+    """torch.compile breaks its graph at the call, which then runs as it is, on each call's own memory."""
+    calls = []
+
+    class Lib:
+        def afd_topk(self, cfg, logits, ld, bias, valid, n, ids, w, stream):
+            calls.append(n)
+            ctypes.memset(ids, 0, n * TOP_K * 4)
+            (ctypes.c_float * (n * TOP_K)).from_address(w)[:] = [float(len(calls))] * (n * TOP_K)
+            return 0
+
+    fake = Lib()
+    monkeypatch.setattr(T._lib, "lib", lambda: fake)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0)
+    monkeypatch.setattr(T, "need_gpu", lambda *a: None)
+
+    def f(x):
+        out = T.select_experts(x * 2, TOP_K)
+        return out.topk_weights + 1, out.topk_ids
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend="eager")
+    for i in range(3):
+        w, ids = compiled(torch.randn(3, 6))
+        assert len(calls) == i + 1 and (w == i + 2).all() and (ids == 0).all()
+    torch._dynamo.reset()

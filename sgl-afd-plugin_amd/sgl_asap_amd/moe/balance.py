@@ -23,12 +23,13 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .topk import (StandardTopKOutput, choice_cfg, last, launch, logit_rows, need_gpu, no_tangent, on_device, router_cfg,
-                   router_grad)
+from .topk import (StandardTopKOutput, choice_cfg, fit_ints, last, launch, logit_rows, need_gpu, no_tangent, on_device,
+                   router_cfg, router_grad)
 
 
 @lru_cache(maxsize=1024)
 def _workspace_bytes(n: int, experts: int, seqs: int) -> int:
+    fit_ints(n, experts, seqs)
     out = ctypes.c_uint64()
     _lib.call("afd_balance_workspace", n, experts, seqs, ctypes.byref(out))
     return out.value
@@ -50,6 +51,8 @@ def _sequences(cu: Optional[torch.Tensor], device) -> Tuple[int, int]:
 def _check_ids(ids: torch.Tensor) -> torch.Tensor:
     if ids.dtype != torch.int32 or ids.dim() != 2:
         raise TypeError(f"topk_ids must be int32 [n, k], got {ids.dtype} {tuple(ids.shape)}")
+    if ids.shape[1] > 0x7FFFFFFF:
+        fit_ints(ids.shape[1])
     return ids.contiguous()
 
 

@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .topk import launch, matrix_rows, need_gpu, no_tangent
+from .topk import fit_ints, launch, matrix_rows, need_gpu, no_tangent
 
 FP8_BLOCK = 128
 
@@ -56,6 +56,7 @@ class Fp8BlockLinear(torch.nn.Module):
         if scales.dtype != torch.float32 or tuple(scales.shape) != blocks:
             raise ValueError(f"scales must be float32 {blocks} for weights {n_out} x {k_in}, got {scales.dtype} "
                              f"{tuple(scales.shape)}")
+        fit_ints(n_out, k_in)
         size = ctypes.c_uint64()
         _lib.call("afd_linear_layout", n_out, k_in, ctypes.byref(size))
         device = torch.device(device) if device is not None else weight.device

@@ -59,6 +59,12 @@ def launch(name: str, device: torch.device, *args) -> None:
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def fit_ints(*sizes: int) -> None:
+    """Refuses sizes that a C int of the entry points would cut to its 32 bits."""
+    if max(sizes) > 0x7FFFFFFF or min(sizes) < -0x80000000:
+        raise ValueError(f"sizes must fit 32 bits, got {sizes}")
+
+
 @lru_cache(maxsize=256)
 def router_cfg(num_experts: int, top_k: int, scoring: str, renormalize: bool, groups: int, keep: int, scale: float,
                dtype: torch.dtype):
@@ -67,6 +73,7 @@ def router_cfg(num_experts: int, top_k: int, scoring: str, renormalize: bool, gr
         raise NotImplementedError(f"scoring {scoring!r} (supported: {sorted(SCORINGS)})")
     if dtype not in LOGITS_FORMATS:
         raise TypeError(f"router logits must be float32 or bfloat16, got {dtype}")
+    fit_ints(num_experts, top_k, groups, keep)
     cfg = _lib.AfdRouterCfg(num_experts, top_k, SCORINGS[scoring], groups, keep, int(renormalize), scale,
                             LOGITS_FORMATS[dtype])
     return ctypes.pointer(cfg)
@@ -74,10 +81,12 @@ def router_cfg(num_experts: int, top_k: int, scoring: str, renormalize: bool, gr
 
 def matrix_rows(t: torch.Tensor):
     """(t [n, columns] with contiguous rows, their stride in elements)."""
-    columns = t.shape[1]
+    n, columns = t.shape
+    if n > 0x7FFFFFFF:
+        fit_ints(n)
     if t.is_contiguous():
         return t, columns
-    if t.shape[0] == 1 or t.stride(1) != 1 or t.stride(0) < columns:
+    if n == 1 or t.stride(1) != 1 or t.stride(0) < columns:
         return t.contiguous(), columns
     return t, t.stride(0)
 

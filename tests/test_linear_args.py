@@ -113,3 +113,25 @@ def test_silu_mul_calls():
     assert call(n=-1) == ARG and call(x=None) == ARG and call(y=None) == ARG and call(ws=None) == ARG and call(image=None) == ARG
     assert call(ld=399) == SHAPE and call(ldy=99) == SHAPE and call(image=24) == SHAPE
     assert call(ws=24) == WS and call(size=100) == WS
+
+
+def test_sizes_past_32_bits_are_refused(monkeypatch):
+    """Sizes are C ints at the entry points: one past their range must not come out as another, smaller one."""
+    from sgl_asap_amd.moe import linear as M
+
+    called, big = [], (1 << 32) + 8
+    monkeypatch.setattr(M, "need_gpu", lambda *a: None)
+    monkeypatch.setattr(M, "launch", lambda *a: called.append(a))
+    for n_out, k in ((big, 1), (1, big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            Fp8BlockLinear(torch.empty(n_out, k, dtype=torch.uint8, device="meta"),
+                           torch.empty(-(-n_out // 128), -(-k // 128), device="meta"))
+    layer = Fp8BlockLinear(torch.zeros(4, 2, dtype=torch.uint8), torch.zeros(1, 1))
+    layer.image = layer.image.to("meta")
+    called.clear()
+    for x in (torch.empty(big, 2, dtype=torch.bfloat16, device="meta"), torch.empty(2, big // 2, 2, dtype=torch.bfloat16, device="meta")):
+        with pytest.raises(ValueError, match="32 bits"):
+            layer(x)
+    with pytest.raises(ValueError, match="32 bits"):
+        layer.silu_mul(torch.empty(big, 4, dtype=torch.bfloat16, device="meta"))
+    assert not called

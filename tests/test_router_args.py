@@ -160,3 +160,31 @@ def test_logits_of_other_dimensions():
             B.select_and_balance(torch.zeros(shape), 2, alpha=1.0)
         with pytest.raises(ValueError):
             B.balance_loss(torch.zeros(shape), torch.zeros(shape[0], 2, dtype=torch.int32), alpha=1.0)
+
+
+BIG = (1 << 32) + 8  # the entry points' 32-bit counts hold 8 of it
+
+
+def test_sizes_past_32_bits_are_refused(monkeypatch):
+    """Sizes are C ints at the entry points: one past their range must not come out as another, smaller one."""
+    called = []
+    for m in (T, B):
+        monkeypatch.setattr(m, "need_gpu", lambda *a: None)
+        monkeypatch.setattr(m, "launch", lambda *a: called.append(a))
+    meta = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="meta")
+    ids = lambda *shape: meta(*shape, dtype=torch.int32)
+    for call in (
+        lambda: T.select_experts(meta(BIG, 4), 2), lambda: T.select_experts(meta(2, BIG), 2),
+        lambda: T.select_experts(meta(BIG, 9)[:, 2:6], 2), lambda: T.select_experts(meta(BIG, 4, dtype=torch.bfloat16), 2),
+        lambda: T.select_experts(meta(2, 4), BIG), lambda: T.select_experts(meta(2, 4), 2 - (1 << 32)),
+        lambda: T.select_experts(meta(2, 16), 2, num_expert_group=BIG, topk_group=4),
+        lambda: T.select_experts(meta(2, 16), 2, num_expert_group=8, topk_group=BIG),
+        lambda: B.select_and_balance(meta(BIG, 4), 2, alpha=1.0), lambda: B.select_and_balance(meta(2, 4), BIG, alpha=1.0),
+        lambda: B.balance_loss(meta(BIG, 4), ids(BIG, 2), alpha=1.0), lambda: B.balance_loss(meta(2, 4), ids(2, BIG), alpha=1.0),
+        lambda: B.balance_loss(meta(2, 4), ids(2, 2), alpha=1.0, cu_seqlens=ids(BIG)),
+        lambda: B.expert_counts(ids(BIG, 2), 4), lambda: B.expert_counts(ids(2, BIG), 4), lambda: B.expert_counts(ids(2, 2), BIG),
+        lambda: B.expert_counts(ids(2, 2), 4, cu_seqlens=ids(BIG)),
+    ):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    assert not called

@@ -99,7 +99,10 @@ class _Balance(torch.autograd.Function):
         else:
             launch("afd_balance", dev, cfg, logits.data_ptr(), ld, ids.data_ptr(), valid_ptr, cu_ptr, seqs, n, alpha,
                    counts.data_ptr(), coef.data_ptr(), loss.data_ptr(), ws.data_ptr(), ws.numel())
-        ctx.save_for_backward(logits, ids if chosen else None, cu, valid, counts, coef)
+        # counts of the backward's own: the caller's may be added up over ranks before it, by collectives that
+        # autograd does not see
+        own = counts.clone() if ctx.needs_input_grad[0] else None
+        ctx.save_for_backward(logits, ids if chosen else None, cu, valid, own, coef)
         ctx.cfg = cfg
         ctx.set_materialize_grads(False)
         if chosen:

@@ -168,3 +168,25 @@ def test_compiled_functions_run_the_launch_each_time(monkeypatch):
         w, ids = compiled(torch.randn(3, 6))
         assert len(calls) == i + 1 and (w == i + 2).all() and (ids == 0).all()
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("which", ["balance", "both"])
+def test_counts_belong_to_the_caller(plain, monkeypatch, which):
+    """What a caller does to the counts before the backward (adds them up over ranks, say: collectives write without
+    autograd's notice) does not reach the gradient."""
+    seen = []
+
+    def grad(cfg, logits, ids, valid, gw, cu=None, counts=None, coef=None, gloss=None):
+        seen.append(counts.clone())
+        return fake_grad(cfg, logits, ids, valid, gw)
+
+    monkeypatch.setattr(B, "router_grad", grad)
+    for change in (lambda c: c.data.fill_(7), lambda c: c.add_(7)):
+        leaf = torch.ones(3, 6).requires_grad_()
+        if which == "both":
+            _, loss, counts = B.select_and_balance(leaf, TOP_K, alpha=1.0)
+        else:
+            loss, counts = B.balance_loss(leaf, torch.zeros(3, TOP_K, dtype=torch.int32), alpha=1.0)
+        change(counts)
+        loss.backward()
+        assert (counts == 7).all() and (seen.pop() == 0).all()

@@ -14,7 +14,9 @@
 // Balance loss of a sequence with T rows: L_s = E / (k T) sum_e cnt_e P_e, P_e = 1/T sum_t s'_te,
 // s' = s / sum_e s; L = alpha times the mean of L_s over the sequences that have rows.
 //   dL/dl_te = s'_te r(l_te) (c_e - sum_j c_j s'_tj),  c_e = gloss coef cnt_e,
-//   coef = alpha E / (S' k T^2),  r = 1, 1 - sigmoid(l), sigmoid(l) / (2 softplus(l)).
+//   coef = alpha E / (S' k T^2),  r = 1, 1 - sigmoid(l), sigmoid(l) / (2 softplus(l)),
+// with c counted from the row's largest share's, as whole numbers (16384 x 256 with the weights' gradient 16.7 us, 16.2
+// without that step).
 //
 // Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
 // and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
@@ -27,7 +29,7 @@
 // writes its sums and counts to a slot of its own (slot = workgroup + sequence: from one piece to the
 // next one of the two grows), and a second launch adds a sequence's slots in their order. No sum
 // depends on which workgroup ends first. With the choice 16384 x 256 takes 22 us and 9.6 for the second launch (of
-// which 3.6 are any launch's), the gradient, again one pass, 16 (34 MB); given ids, 8192 x 64 6.6, 9.2 and 7.1.
+// which 3.6 are any launch's), the gradient, again one pass, 16.7 (34 MB); given ids, 8192 x 64 6.7, 9.2 and 8.0.
 #include "afd_common.h"
 #include "afd_internal.h"
 
@@ -324,6 +326,13 @@ __device__ __forceinline__ int first_lane(bool bit, int lane) {
   return __builtin_ctz(half >> (lane & 16));  // the other row's bits lie above this one's, of which one is set
 }
 
+// A lane's value in all lanes of its row
+template <int W>
+__device__ __forceinline__ int from_lane(int v, int lane) {
+  if constexpr (W == 64) return __builtin_amdgcn_readlane(v, lane);
+  return __shfl(v, lane, W);
+}
+
 // The row's keys, taken largest first (lowest index of equals). A lane sorts its own keys once and only
 // its head takes part in a round. Low bits of a key say which expert it is:
 // kIndexed (bf16 logits, 16 spare bits): kMaxExperts - 1 - e, so that no two are equal, the winning key
@@ -410,9 +419,7 @@ struct Keys {
     for (int j = 0; j + 1 < V; ++j) key[j] = mine ? key[j + 1] : key[j];
     key[V - 1] = mine ? 0u : key[V - 1];
     if constexpr (KIND == kBare) {
-      // read by all lanes: the winner's e is made in them
-      if constexpr (W == 64) return __builtin_amdgcn_readlane(e, win);
-      return __shfl(e, win, W);
+      return from_lane<W>(e, win);  // the winner's e
     }
     return e;
   }
@@ -1193,15 +1200,13 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
     Piece piece = {r1, -1};
     if (a.coef != nullptr) piece = next_piece(a, at, r1);
     const bool balanced = piece.seq >= 0;
-    float c[V] = {};
+    float f = 0.0f;
+    int32_t cnt[V] = {};
     if (balanced) {
-      const float f = gloss * a.coef[piece.seq];
-      int32_t cnt[V];
+      f = gloss * a.coef[piece.seq];
 #pragma unroll
       for (int j = 0; j < V; ++j)
         cnt[j] = a.counts[int64_t(piece.seq) * a.experts + min(li * V + j, a.experts - 1)];
-#pragma unroll
-      for (int j = 0; j < V; ++j) c[j] = f * cnt[j];
     }
     using R = Row<T, W, V>;
     auto clamp_row = [&](int32_t r) { return min(r, piece.end - 1); };
@@ -1235,50 +1240,80 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
       const float inv = total >= kLeast ? __builtin_amdgcn_rcpf(total) : 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) d[j] = 0.0f;
+      // Both sums are of the form p_e (v_e - sum_j p_j v_j) with shares p that add up to one. v counts from the largest
+      // share's value: a share close to one then leaves no difference of two close numbers, and equal v leave 0.
+      const bool all_shares = a.gw != nullptr && !a.renorm && a.scoring == AFD_SCORE_SOFTMAX;
+      int top = 0;
+      int32_t top_cnt = 0;
+      if (balanced || all_shares) {
+        float most = row.l[0];
+        top = row.e0;
+        top_cnt = cnt[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) {
+          const bool up = row.l[j] > most;
+          most = fmaxf(most, row.l[j]);
+          top = up ? row.e0 + j : top;
+          top_cnt = up ? cnt[j] : top_cnt;
+        }
+        const int win = first_lane<W>(most == max_f32<W>(most), lane);
+        top = from_lane<W>(top, win);
+        top_cnt = from_lane<W>(top_cnt, win);
+      }
       if (balanced) {
         float dot = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) dot += c[j] * (s[j] * inv);
+        for (int j = 0; j < V; ++j) dot += static_cast<float>(cnt[j] - top_cnt) * (s[j] * inv);
         dot = sum_f32<W>(dot);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = s[j] * inv * (c[j] - dot);
+        for (int j = 0; j < V; ++j) d[j] = s[j] * inv * (f * (static_cast<float>(cnt[j] - top_cnt) - dot));
       }
-      if (a.gw != nullptr) {
-        // lane kk < topk: the kk-th chosen expert's share of the weights' scores, and its gradient
+      float* mine = spread + sub * (W * V);
+      if (all_shares) {
+        // every expert's share has a value: its weight's gradient, 0 where it was not chosen (an id that comes twice is
+        // added up)
+        const int id = li < a.topk && static_cast<uint32_t>(now.id) < static_cast<uint32_t>(a.experts) ? now.id : -1;
+#pragma unroll
+        for (int j = 0; j < V; ++j) mine[row.e0 + j] = 0.0f;
+        lds_fence();
+        if (id >= 0) atomicAdd(mine + id, now.gw);
+        lds_fence();
+        const float top_g = mine[top];
+        float g[V], mean = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          g[j] = mine[row.e0 + j] - top_g;
+          mean += g[j] * (s[j] * inv);
+        }
+        lds_fence();
+        mean = sum_f32<W>(mean);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] += s[j] * inv * (a.scale * (g[j] - mean));
+      } else if (a.gw != nullptr) {
+        // lane kk < topk: the kk-th chosen expert's share of the chosen scores (renormalized) or its score, and its gradient
         const int id = li < a.topk && static_cast<uint32_t>(now.id) < static_cast<uint32_t>(a.experts) ? now.id : -1;
         float g = id >= 0 ? now.gw : 0.0f;
-        float* mine = spread + sub * (W * V);
 #pragma unroll
         for (int j = 0; j < V; ++j) mine[row.e0 + j] = row.l[j];
         lds_fence();
         const float l = id >= 0 ? mine[id] : kLowest;
         lds_fence();
-        // share: of the chosen (renormalized) or of all (softmax), or the score itself
         float share;
         if (a.scoring == AFD_SCORE_SOFTMAX) {
-          float m = l;
-          if (!a.renorm) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) m = fmaxf(m, row.l[j]);
-          }
-          m = max_f32<W>(m);
+          const float m = max_f32<W>(l);
           share = id >= 0 ? exp_f32(l - (m == kLowest ? 0.0f : m)) : 0.0f;
         } else {
           share = id >= 0 ? score_f32<true>(l, a.scoring) : 0.0f;
         }
-        const float chosen = sum_f32<W>(share);
-        if (a.renorm)
-          share = chosen >= kLeast ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
-        else if (a.scoring == AFD_SCORE_SOFTMAX)
-          share *= inv;
-        // dw_i = share_i (g_i - sum_j g_j share_j) where the shares add up to one over something. Renormalized ones
-        // add up to one themselves, so g counts from the largest share's: one that holds nearly all (or all, of one
-        // pick) leaves no difference of two close numbers.
         float mean = 0.0f;
-        if (a.renorm) g -= __shfl(g, first_lane<W>(share == max_f32<W>(share), lane), W);
+        if (a.renorm) {
+          const float chosen = sum_f32<W>(share);
+          share = chosen >= kLeast ? share * __builtin_amdgcn_rcpf(chosen) : 0.0f;
+          g -= __shfl(g, first_lane<W>(share == max_f32<W>(share), lane), W);
+        }
         g *= a.scale;
-        if (a.renorm || a.scoring == AFD_SCORE_SOFTMAX) mean = sum_f32<W>(g * share);
-        const float u = share * (g - (a.renorm ? mean : 0.0f));
+        if (a.renorm) mean = sum_f32<W>(g * share);
+        const float u = share * (g - mean);
         // to the lanes that hold the experts, through LDS (an id that comes twice is added up)
 #pragma unroll
         for (int j = 0; j < V; ++j) mine[row.e0 + j] = 0.0f;
@@ -1288,10 +1323,6 @@ __device__ __forceinline__ void grad_rows(const Args& a, float* spread) {
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] += mine[row.e0 + j];
         lds_fence();
-        if (!a.renorm && a.scoring == AFD_SCORE_SOFTMAX) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) d[j] -= s[j] * inv * mean;
-        }
       }
       if (in) {
         T* out = static_cast<T*>(a.dlogits) + int64_t(r) * a.experts + row.e0;

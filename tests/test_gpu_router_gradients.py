@@ -1,4 +1,4 @@
-"""GPU: the router's gradients where one share is close to one, each entry against its own size, in 64 bits.
+"""GPU: every entry of the router's gradients against its own size, in 64 bits.
 
 Reference. With p the shares of all experts (s over their sum), q the shares of the chosen ones, r the slope ds/dl over s:
 
@@ -92,8 +92,66 @@ def check(got, want, bound, dtype=torch.float32):
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol.clamp_min(1e-300)).max())
 
 
+def telling(want, bound):
+    """Nearly every entry is far above its tolerance, so a gradient of zeros, or of another size, fails."""
+    some = bound > 0
+    assert some.any() and float((want.abs() > 16 * REL * bound)[some].double().mean()) > 0.9
+
+
 def on(x, dtype=None):
     return None if x is None else torch.tensor(x, dtype=torch.int32, device=dev()) if isinstance(x, list) else x.to(dev())
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("n,experts,top_k,bias,cu", [
+    (7, 6, 1, False, None), (37, 60, 4, True, [2, 12, 12, 35]), (37, 128, 17, False, [0, 30, 37]), (50, 256, 8, True, None),
+    (37, 500, 8, False, [0, 37]), (37, 900, 32, True, [5, 6, 30]), (6151, 60, 4, False, [2, 12, 1500, 1500, 4000]),
+    (6151, 256, 8, True, [0, 700, 5000, 6151]), (3000, 160, 6, True, None)])
+def test_every_entry(n, experts, top_k, bias, cu, renorm, scoring):
+    scale, alpha, gl = 1.5, 0.02, 2.0
+    for dtype in (torch.float32, torch.bfloat16):
+        g = torch.Generator().manual_seed(n + experts)
+        # popular and unpopular experts, as a router has them: counts that differ
+        logits = (torch.randn(n, experts, generator=g) * 2 + torch.randn(experts, generator=g)).to(dtype)
+        b = torch.randn(experts, generator=g) * 0.05 if bias else None
+        gw = torch.randn(n, top_k, generator=g)
+        valid = torch.rand(n, generator=g) < 0.8
+        say(f"every entry n={n} E={experts} k={top_k} {scoring} renorm={renorm} {dtype}")
+        leaf = logits.to(dev()).requires_grad_()
+        out, loss, cnt = B.select_and_balance(leaf, top_k, alpha=alpha, scoring=scoring, renormalize=renorm, correction_bias=on(b),
+                                              routed_scaling_factor=scale, cu_seqlens=on(cu), valid=on(valid))
+        z, ids = R.canon(logits), out.topk_ids.cpu().long().clamp_min(0)
+        parts = [weights_grad(z, ids, scoring, renorm, scale, gw, valid),
+                 loss_grad(z, cnt.cpu().view(-1, experts), top_k, scoring, gl, alpha, cu, valid)]
+        for take in ((0,), (1,), (0, 1)):
+            outs = [(out.topk_weights, loss)[i] for i in take]
+            gs = [(on(gw), torch.tensor(gl, device=dev()))[i] for i in take]
+            (got,) = torch.autograd.grad(outs, (leaf,), gs, retain_graph=True)
+            want, bound = sum(parts[i][0] for i in take), sum(parts[i][1] for i in take)
+            # (one pick's renormalized weight is the scale: its gradient is 0)
+            if take != (0,) or not renorm or top_k > 1:
+                telling(want, bound)
+            check(got, want, bound, dtype)
+
+
+@pytest.mark.parametrize("scoring", R.SCORINGS)
+@pytest.mark.parametrize("spans", [None, [0, 900, 900, 5000]])
+def test_every_entry_for_given_ids(spans, scoring):
+    """Sequences over many workgroups; ids that repeat, that are no expert's, and rows without any."""
+    n, experts, top_k, alpha = 5000, 256, 8, 1.0
+    g = torch.Generator().manual_seed(4)
+    logits = torch.randn(n, experts, generator=g) * 2
+    ids = (torch.rand(n, top_k, generator=g) ** 2 * (experts + 2)).to(torch.int32) - 1
+    say(f"given ids {scoring} {spans}")
+    leaf = logits.to(dev()).requires_grad_()
+    loss, cnt = B.balance_loss(leaf, ids.to(dev()), alpha=alpha, scoring=scoring, cu_seqlens=on(spans))
+    (got,) = torch.autograd.grad(loss, leaf)
+    want_cnt = R.counts(ids, experts, spans)
+    assert torch.equal(cnt.cpu().long().view(-1, experts), want_cnt)
+    want, bound = loss_grad(R.canon(logits), want_cnt, top_k, scoring, 1.0, alpha, spans)
+    telling(want, bound)
+    check(got, want, bound)
 
 
 def peaked(n, experts, scoring, seed):

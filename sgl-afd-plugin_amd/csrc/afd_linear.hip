@@ -11,8 +11,9 @@
 // rows of a chunk are 256 bytes, all banks once. Which K a lane's bytes stand for does not matter as
 // long as both operands agree. Padding codes are 0; padding rows are never stored.
 //
-// Every block's MFMA sum starts from 0 and is folded into the result with its scale by one fp32
-// fused multiply-add, so scales may be 0, tiny or huge. A row of x with an infinity or a NaN in a block gets
+// Every block's MFMA sum starts from 0 and is folded into the result with its scale sx sw by one fp32
+// fused multiply-add. Scales may be 0, tiny or huge: where a product of two scales is no normal float, the results that it
+// belongs to are made again in 64 bits (see odd_scale). A row of x with an infinity or a NaN in a block gets
 // the scale NaN, which makes that row of y NaN and no other.
 #include "afd_common.h"
 #include "afd_gemm_dev.h"
@@ -153,6 +154,50 @@ __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__
   if (lane < 16) s[int64_t(b) * a_rows + r16 * 16 + lane] = sc;
 }
 
+// ---------------------------------------------------------------- scales whose product leaves the floats
+// sx is between 1e-10 / 448 > 2^-43 and the largest bf16 / 448 < 2^120, so sx sw is a normal float for every x if sw is 0 or
+// within 2^-83 .. 2^8. The kernels look at their weight scales, which are scalars, as they pass (a few scalar instructions a
+// K block: 48 x 2048 x 4096 6.4 -> 6.6 us, 300 x 2000 x 1111 8.9 -> 9.2, 2900 x 4096 x 4096 46.6 -> 47.4, one row and 16384
+// within the noise); where one lies outside, they look at the products themselves, and where one of those
+// is no normal float the results are folded again in 64 bits: every sum and product is then in range.
+__device__ __forceinline__ bool odd_scale(float s) {
+  const uint32_t u = __float_as_uint(s) & 0x7fffffffu;
+  constexpr uint32_t kLow = (127u - 83u) << 23, kHigh = (127u + 8u) << 23, kInf = 0x7f800000u;
+  // other than 0 and below infinity (which, as NaN, stays itself in any arithmetic), and not within the two; no branches
+  return (u - 1 < kInf - 1) & (u - kLow > kHigh - kLow);
+}
+// Whether sx sw, of numbers other than 0, is no normal float
+__device__ __forceinline__ bool odd_product(float sx, float sw) {
+  const float s = fabsf(sx * sw);
+  return odd_scale(sw) && sx == sx && !(s >= 0x1p-126f && s < __builtin_huge_valf());
+}
+// 16 outputs of 16 rows, as the MFMA gives them. fetch(b, q): K block b's activation fragment and (returned) its scale
+template <typename F>
+__device__ __forceinline__ v4f fold_f64(const Args& p, int64_t o16, int lane, F fetch) {
+  const uint8_t* bw = p.b + o16 * (2 * p.kb) * kPiece + lane * 16;
+  const float* sw = p.bs + o16 / 8 * p.kb;
+  double acc[4] = {};
+#pragma unroll 1
+  for (int b = 0; b < p.kb; ++b) {
+    v8i q;
+    const float sx = fetch(b, q);
+    const v8i fw = join(*reinterpret_cast<const v4i*>(bw + int64_t(2 * b) * kPiece),
+                        *reinterpret_cast<const v4i*>(bw + int64_t(2 * b + 1) * kPiece));
+    const v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, q, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0 /*e4m3*/,
+                                                                     0 /*e4m3*/, 0, 0, 0, 0);
+    const double s = double(sx) * sw[b];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += sum[i] * s;
+  }
+  return v4f{static_cast<float>(acc[0]), static_cast<float>(acc[1]), static_cast<float>(acc[2]), static_cast<float>(acc[3])};
+}
+// K block b of row group r16 from the image
+__device__ __forceinline__ float image_fragment(const Args& p, int64_t r16, int b, int lane, v8i& q) {
+  const uint8_t* ax = p.a + (r16 * (2 * p.kb) + 2 * b) * kPiece + lane * 16;
+  q = join(*reinterpret_cast<const v4i*>(ax), *reinterpret_cast<const v4i*>(ax + kPiece));
+  return p.as[int64_t(b) * p.a_rows + r16 * 16 + (lane & 15)];
+}
+
 // ---------------------------------------------------------------- weights (load time)
 __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ w, int64_t ld, int n_out, int k_in,
                                                    int kb, uint8_t* __restrict__ out, int64_t pieces) {
@@ -197,6 +242,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
   constexpr int kCodes = FUSED ? kFusedBytes : 0;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kCodes > kPart ? kCodes : kPart];
   __shared__ float scales[FUSED ? kFusedBytes / 128 : 1];
+  __shared__ bool odd_waves[kRowWaves];
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int o16 = blockIdx.x, g0 = blockIdx.y * MT;
@@ -265,12 +311,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
     }
     __syncthreads();
   }
+  bool odd = false;
   for (int b0 = w; b0 <= last; b0 += kDepth * kRowWaves) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       const int b = b0 + d * kRowWaves;
       if (b > last) break;
       const Block k = ring[d];
+      odd |= odd_scale(k.s_w);
       ring[d] = fetch(b + kDepth * kRowWaves);
       const v8i fw = join(k.w[0], k.w[1]);
 #pragma unroll
@@ -299,11 +347,34 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
   v4f* part = reinterpret_cast<v4f*>(lds);
 #pragma unroll
   for (int m = 0; m < MT; ++m) part[(w * MT + m) * 64 + lane] = acc[m];
+  odd_waves[w] = odd;
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) odd |= odd_waves[i];
   // lane l: row l % 16 of x, outputs 4 (l / 16) .. + 3
   for (int m = w; m < MT; m += kRowWaves) {
     v4f y = part[m * 64 + lane];
     for (int i = 1; i < kRowWaves; ++i) y += part[(i * MT + m) * 64 + lane];
+    if (odd) {
+      const int r = min(m * 16 + (lane & 15), p.n - 1), r16 = min(g0 + m, r16_last);
+      bool again = false;
+      for (int b = 0; b <= last; ++b)
+        again = again || odd_product(FUSED ? scales[b * p.n + r] : p.as[int64_t(b) * p.a_rows + r16 * 16 + (lane & 15)], sw[b]);
+      if (__ballot(again))
+        y = fold_f64(p, o16, lane, [&](int b, v8i& q) {
+          if constexpr (FUSED) {  // the sums have taken the codes' place
+            const uint16_t* x = in.x + r * in.ldx;
+            Raw raw = load_raw<VEC>(x, in.k_in, b, lane >> 4);
+            if constexpr (SILU) raw = silu_mul(raw, load_raw<VEC>(x + in.k_in, in.k_in, b, lane >> 4));
+            v4i code[2];
+            const float sc = quantize(raw, code);
+            q = join(code[0], code[1]);
+            return sc;
+          } else {
+            return image_fragment(p, r16, b, lane, q);
+          }
+        });
+    }
     const int64_t row = int64_t(g0 + m) * 16 + (lane & 15);
     const int o = o16 * 16 + 4 * (lane >> 4);
     if (row >= p.n) continue;
@@ -443,6 +514,7 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   const int sw_row = min((n0 + wn * (T::BN / T::WN)) / 128, (p.n_out - 1) / 128);
   const float* sw = p.bs + int64_t(sw_row) * p.kb;
   float s_w = load_uniform(sw);  // of the stage; the next one's is read where no LDS read is in flight
+  bool odd = odd_scale(s_w);
   const uint8_t* a_lds = lds + wm * TI * 2 * kPiece + lane * 16;
   const uint8_t* b_lds = lds + T::kBOff + wn * TJ * 2 * kPiece + lane * 16;
   const uint8_t* s_lds = lds + T::kSOff + (wm * TI * 16 + (lane & 15)) * 4;
@@ -515,9 +587,31 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
       __builtin_amdgcn_sched_barrier(0);
     });
     s_w = s_w_next;
+    odd |= odd_scale(s_w);
   }
   static_for<kLate>([&](auto c) { fold(std::integral_constant<int, kSteps - kLate + decltype(c)::value>{}); });
   wait_vmcnt<0>();
+
+  if (odd) {
+    bool again = false;
+    for (int b = 0; b <= last; ++b)
+#pragma unroll 1
+      for (int i = 0; i < TI; ++i)
+        again = again || odd_product(p.as[int64_t(b) * p.a_rows + min(m0 + (wm * TI + i) * 16 + (lane & 15), p.n - 1)], sw[b]);
+    if (__ballot(again)) {
+#pragma unroll 1
+      for (int ij = 0; ij < TI * TJ; ++ij) {
+        const int r16 = m0 / 16 + wm * TI + ij / TJ, o16 = n0 / 16 + wn * TJ + ij % TJ;
+        if (r16 > r16_last || o16 > o16_last) continue;
+        const v4f y = fold_f64(p, o16, lane, [&](int b, v8i& q) { return image_fragment(p, r16, b, lane, q); });
+        const int64_t row = int64_t(r16) * 16 + (lane & 15);
+        for (int q = 0; q < 4; ++q)
+          if (row < p.n && o16 * 16 + 4 * (lane >> 4) + q < p.n_out)
+            p.y[row * p.ldy + o16 * 16 + 4 * (lane >> 4) + q] = f32_to_bf16(y[q]);
+      }
+      return;
+    }
+  }
 
   // lane l holds, of row l % 16 of an activation tile, outputs 4 (l / 16) .. + 3 of each weight tile. Two
   // neighbouring weight tiles trade halves so that a lane holds 8 outputs: lane groups 0 and 2 those of tile

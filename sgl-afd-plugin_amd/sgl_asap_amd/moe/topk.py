@@ -242,7 +242,8 @@ def select_experts(
 
 
 class TopK(torch.nn.Module):
-    """``select_experts`` with a layer's settings."""
+    """``select_experts`` with a layer's settings. ``correction_bias`` is a buffer that moves with the module and stays in its
+    fp32 when the module is cast."""
 
     def __init__(
         self,
@@ -267,6 +268,13 @@ class TopK(torch.nn.Module):
                              num_expert_group=num_expert_group if use_grouped_topk else None,
                              topk_group=topk_group if use_grouped_topk else None,
                              routed_scaling_factor=routed_scaling_factor)
+
+    def _apply(self, fn, recurse=True):
+        bias = self.correction_bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.correction_bias.dtype != bias.dtype:
+            self.correction_bias = bias.to(self.correction_bias.device)
+        return self
 
     def forward(self, router_logits: torch.Tensor, valid: Optional[torch.Tensor] = None) -> StandardTopKOutput:
         return select_experts(router_logits, self.top_k, correction_bias=self.correction_bias, valid=valid,

@@ -45,7 +45,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 class Fp8BlockLinear(torch.nn.Module):
     """``weight``: e4m3 codes [n_out, k_in] (float8_e4m3fn, or their bytes); ``scales``: fp32
     [ceil(n_out / 128), ceil(k_in / 128)], the weight being code x scale. Laid out once for the kernels, on ``device``
-    (default: the codes')."""
+    (default: the codes'), where the layer stays: moves and casts of a module leave it, and like the bf16 MLP's weights its own
+    are not in ``state_dict()`` (they come from the checkpoint). It can be copied and pickled."""
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, device=None):
         super().__init__()
@@ -66,9 +67,19 @@ class Fp8BlockLinear(torch.nn.Module):
         self.image = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
         self.scales = scales.to(codes.device, copy=True).contiguous()
         launch("afd_linear_pack", codes.device, codes.data_ptr(), k_in, n_out, k_in, self.image.data_ptr())
+        self._point()
+
+    def _point(self) -> None:
         # _weights holds addresses: the tensors stay attributes, not buffers that a module move would replace
-        self._weights = _lib.AfdLinearWeights(n_out, k_in, self.image.data_ptr(), self.scales.data_ptr())
+        self._weights = _lib.AfdLinearWeights(self.out_features, self.in_features, self.image.data_ptr(), self.scales.data_ptr())
         self._weights_ref = ctypes.byref(self._weights)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_weights", "_weights_ref")}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._point()
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """bf16 [..., k_in] -> bf16 [..., n_out] on the device's current stream, into ``out`` if given ([n,

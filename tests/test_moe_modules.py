@@ -1,11 +1,12 @@
 """The MoE modules as parts of a model: casts, copies and hooks (on the CPU, with the launches left out)."""
 
 import copy
-import pickle
+import io
 
 import pytest
 import torch
 
+from sgl_asap_amd.moe import linear as L
 from sgl_asap_amd.moe import topk as T
 
 
@@ -27,3 +28,36 @@ def test_the_correction_bias_moves_with_the_model():
     for move in (lambda m: m.to("meta"), lambda m: m.to("meta", torch.bfloat16)):
         there = move(copy.deepcopy(topk)).correction_bias
         assert there.device.type == "meta" and there.dtype == torch.float32
+
+
+@pytest.fixture
+def no_launches(monkeypatch):
+    monkeypatch.setattr(L, "need_gpu", lambda *a: None)
+    monkeypatch.setattr(L, "launch", lambda *a: None)
+
+
+def addresses(layer):
+    w = layer._weights_ref._obj
+    return w.n_out, w.k_in, w.image, w.scales
+
+
+def copies(layer):
+    """A deep copy, and one through a file."""
+    file = io.BytesIO()
+    torch.save(layer, file)
+    file.seek(0)
+    return copy.deepcopy(layer), torch.load(file, weights_only=False)
+
+
+def test_copies_of_a_layer_hold_weights_of_their_own(no_launches):
+    layer = L.Fp8BlockLinear(torch.zeros(20, 130, dtype=torch.uint8), torch.rand(1, 2))
+    layer.image.random_(0, 255)
+    before = addresses(layer)
+    for other in copies(layer):
+        assert addresses(other) == (20, 130, other.image.data_ptr(), other.scales.data_ptr())
+        assert other.image.data_ptr() != layer.image.data_ptr() and other.scales.data_ptr() != layer.scales.data_ptr()
+        assert torch.equal(other.image, layer.image) and torch.equal(other.scales, layer.scales)
+        assert (other.out_features, other.in_features) == (20, 130)
+    assert addresses(layer) == before == (20, 130, layer.image.data_ptr(), layer.scales.data_ptr())
+    model = copy.deepcopy(torch.nn.Sequential(layer))
+    assert addresses(model[0])[2] == model[0].image.data_ptr()

@@ -66,8 +66,9 @@ class SharedExpertMLP(torch.nn.Module):
 
 class Fp8SharedExpertMLP(torch.nn.Module):
     """The shared expert on block-FP8 weights: e4m3 codes ``w_gate_up`` [2I, H] = [gate; up] rows and
-    ``w_down`` [H, I], each with its fp32 scales per 128x128 block. x and the activation (rounded
-    to bf16, as the bf16 MLP rounds it) are quantized per 1x128 before their products."""
+    ``w_down`` [H, I], each with its fp32 scales per 128x128 block, any H and I. x and the activation (rounded
+    to bf16, as the bf16 MLP rounds it) are quantized per 1x128 before their products. ``down`` is called with the gate and
+    up rows and takes the activation itself (``Fp8BlockLinear.silu_mul``)."""
 
     def __init__(self, w_gate_up: torch.Tensor, s_gate_up: torch.Tensor, w_down: torch.Tensor, s_down: torch.Tensor,
                  device=None):
@@ -76,8 +77,6 @@ class Fp8SharedExpertMLP(torch.nn.Module):
         if two_i % 2 or tuple(w_down.shape) != (hidden, two_i // 2):
             raise ValueError(f"w_gate_up {tuple(w_gate_up.shape)} and w_down {tuple(w_down.shape)} "
                              "do not form one SwiGLU MLP")
-        if two_i % 16:
-            raise ValueError(f"the intermediate size must be a multiple of 8, got {two_i // 2}")
         self.hidden_size, self.intermediate_size = hidden, two_i // 2
         self.gate_up = Fp8BlockLinear(w_gate_up, s_gate_up, device)
         self.down = Fp8BlockLinear(w_down, s_down, device)

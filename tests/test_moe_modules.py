@@ -1,4 +1,5 @@
-"""The MoE modules as parts of a model: casts, copies and hooks (on the CPU, with the launches left out)."""
+"""The MoE modules as parts of a model: casts, copies and hooks (on the CPU, with the launches left out; on the GPU their
+results)."""
 
 import copy
 import io
@@ -8,6 +9,7 @@ import torch
 
 from sgl_asap_amd.moe import linear as L
 from sgl_asap_amd.moe import topk as T
+from sgl_asap_amd.moe.shared import Fp8SharedExpertMLP
 
 
 @pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.bfloat16(),
@@ -61,3 +63,32 @@ def test_copies_of_a_layer_hold_weights_of_their_own(no_launches):
     assert addresses(layer) == before == (20, 130, layer.image.data_ptr(), layer.scales.data_ptr())
     model = copy.deepcopy(torch.nn.Sequential(layer))
     assert addresses(model[0])[2] == model[0].image.data_ptr()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,inter", [(384, 131), (130, 12), (256, 1)])
+def test_odd_mlps_and_their_copies_give_the_same_bits(hidden, inter):
+    """An intermediate size that the activation's own kernel does not take, against the layers padded to one that it does."""
+    from gpu_util import dev, say
+    from sgl_asap_amd.moe.shared import silu_mul
+
+    g = torch.Generator().manual_seed(inter)
+    ceil = lambda a: -(-a // 128)
+    e4m3 = lambda *shape: (torch.randn(*shape, generator=g) * 50).clamp(-448, 448).to(torch.float8_e4m3fn)
+    w_gu, w_d = e4m3(2 * inter, hidden), e4m3(hidden, inter)
+    s_gu = torch.rand(ceil(2 * inter), ceil(hidden), generator=g) * 2e-3
+    s_d = torch.rand(ceil(hidden), ceil(inter), generator=g) * 2e-3
+    mlp = Fp8SharedExpertMLP(*(t.to(dev()) for t in (w_gu, s_gu, w_d, s_d)))
+    pad = -(-inter // 8) * 8
+    others = (*copies(mlp), Fp8SharedExpertMLP(w_gu, s_gu, w_d, s_d, device=dev()))
+    for n in (1, 7, 40, 150):
+        say(f"odd MLP n={n} hidden={hidden} inter={inter}")
+        x = torch.randn(n, hidden, generator=g).to(torch.bfloat16).to(dev())
+        gate_up = L.Fp8BlockLinear(w_gu.to(dev()), s_gu.to(dev()))(x)
+        wide = torch.zeros(n, 2, pad, dtype=torch.bfloat16, device=dev())
+        wide[:, :, :inter] = gate_up.view(n, 2, inter)
+        h = silu_mul(wide.view(n, 2 * pad))[:, :inter]
+        want = L.Fp8BlockLinear(w_d.to(dev()), s_d.to(dev()))(h)
+        assert torch.isfinite(want).all() and (want != 0).any()
+        for m in (mlp, *others):
+            assert torch.equal(m(x), want)

@@ -81,15 +81,17 @@ class Fp8BlockLinear(torch.nn.Module):
         super().__setstate__(state)
         self._point()
 
-    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, *, silu_mul: bool = False) -> torch.Tensor:
         """bf16 [..., k_in] -> bf16 [..., n_out] on the device's current stream, into ``out`` if given ([n,
-        n_out] with contiguous rows that share no element with x, x two-dimensional)."""
+        n_out] with contiguous rows that share no element with x, x two-dimensional). ``silu_mul``: as the method."""
+        if silu_mul:
+            return self._product("afd_linear_silu_mul", x, 2 * self.in_features, out)
         return self._product("afd_linear", x, self.in_features, out)
 
     def silu_mul(self, gate_up: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer of ``silu_mul(gate_up)``, bf16 [..., 2 k_in] of [gate | up] rows, bit for bit, in a launch less and
-        without the activation in memory."""
-        return self._product("afd_linear_silu_mul", gate_up, 2 * self.in_features, out)
+        without the activation in memory. A call of the module: its hooks run, and see gate_up as what goes in."""
+        return self(gate_up, out, silu_mul=True)
 
     def _product(self, name, x, columns, out):
         if x.dtype != torch.bfloat16 or x.dim() < 1 or x.shape[-1] != columns:

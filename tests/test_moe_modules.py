@@ -65,6 +65,25 @@ def test_copies_of_a_layer_hold_weights_of_their_own(no_launches):
     assert addresses(model[0])[2] == model[0].image.data_ptr()
 
 
+@pytest.mark.parametrize("inter", [1, 12, 131])
+def test_an_mlp_of_any_intermediate_size_is_its_two_layers(no_launches, monkeypatch, inter):
+    """As wide as its layers are, and calls them as modules, so that hooks on either run."""
+    calls, seen = [], []
+    monkeypatch.setattr(L, "launch", lambda name, *a: calls.append(name))
+    ceil = lambda a: -(-a // 128)
+    codes = lambda *shape: torch.zeros(*shape, dtype=torch.uint8)
+    mlp = Fp8SharedExpertMLP(codes(2 * inter, 40), torch.zeros(ceil(2 * inter), 1), codes(40, inter), torch.zeros(1, ceil(inter)))
+    calls.clear()
+    for name, layer in mlp.named_children():
+        layer.register_forward_pre_hook(lambda m, args, name=name: seen.append((name, tuple(args[0].shape))))
+        layer.register_forward_hook(lambda m, args, y, name=name: seen.append((name, tuple(y.shape))))
+    assert mlp(torch.zeros(3, 40, dtype=torch.bfloat16)).shape == (3, 40)
+    assert calls == ["afd_linear", "afd_linear_silu_mul"]
+    assert seen == [("gate_up", (3, 40)), ("gate_up", (3, 2 * inter)), ("down", (3, 2 * inter)), ("down", (3, 40))]
+    with pytest.raises(TypeError):
+        mlp.down(torch.zeros(3, 2 * inter, dtype=torch.bfloat16))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("hidden,inter", [(384, 131), (130, 12), (256, 1)])
 def test_odd_mlps_and_their_copies_give_the_same_bits(hidden, inter):

@@ -11,6 +11,10 @@
 // rows of a chunk are 256 bytes, all banks once. Which K a lane's bytes stand for does not matter as
 // long as both operands agree. Padding codes are 0; padding rows are never stored.
 //
+// The MFMA of e4m3 codes adds the products of 8 columns at a time, each cut towards zero at 2^-13 of the largest one's
+// power of two, and these sums in fp32 (measured with single products beside a pair that cancels). Over N(0, 1) rows and
+// weights 1.2% of the bf16 results are a neighbour of the exact result's rounding, where fp32 products leave 0.1%; the
+// distance to 64 bits is the same (1.66e-3 root mean square, all of it bf16's).
 // Every block's MFMA sum starts from 0 and is folded into the result with its scale sx sw by one fp32
 // fused multiply-add. Scales may be 0, tiny or huge: where a product of two scales is no normal float, the results that it
 // belongs to are made again in 64 bits (see odd_scale). A row of x with an infinity or a NaN in a block gets
@@ -159,7 +163,8 @@ __global__ __launch_bounds__(256) void quant_kernel(const uint16_t* __restrict__
 // within 2^-83 .. 2^8. The kernels look at their weight scales, which are scalars, as they pass (a few scalar instructions a
 // K block: 48 x 2048 x 4096 6.4 -> 6.6 us, 300 x 2000 x 1111 8.9 -> 9.2, 2900 x 4096 x 4096 46.6 -> 47.4, one row and 16384
 // within the noise); where one lies outside, they look at the products themselves, and where one of those
-// is no normal float the results are folded again in 64 bits: every sum and product is then in range.
+// is no normal float the results are folded again in 64 bits: every sum and product is then in range (all of 16384 x 4096 x
+// 4096 so: 1.6 ms for 0.27).
 __device__ __forceinline__ bool odd_scale(float s) {
   const uint32_t u = __float_as_uint(s) & 0x7fffffffu;
   constexpr uint32_t kLow = (127u - 83u) << 23, kHigh = (127u + 8u) << 23, kInf = 0x7f800000u;
@@ -221,8 +226,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ w
 // the whole K and 16 MT rows, its wavefronts every kRowWaves-th K block each: the weights straight into registers
 // (non-temporal, DEPTH blocks ahead), the activations from the image likewise; the wavefronts' sums
 // meet in LDS, in their order. 16 outputs a workgroup because 4096 of them then are one workgroup a CU with all
-// of its weights on their way at once: 1 x 4096 x 4096 takes 5.9 to 6.5 us (16.8 MB), of which a launch that does
-// nothing is 3.6; 48 x 2048 x 4096 5.5 to 6.5 us after 3.2 of quantization.
+// of its weights on their way at once: 1 x 4096 x 4096 takes 5.8 us in a graph (16.8 MB), where a launch that does
+// nothing takes 1.6; 48 x 2048 x 4096 8.8 us with its quantization (traced 6.6 and 3.3).
 // FUSED: no launch before it. The workgroup quantizes its rows into LDS while its first weights are on
 // their way (16 rows' K blocks a wavefront at a time, whichever rows they are of): n K elements, which every
 // workgroup does again, so only where they are few and fit kFusedBytes. SILU: as the quantization's.
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 // next stage is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the last two
 // weight fragments run while the next stage's first fragments are read.
 //
-// 16384 x 4096 x 4096 takes 232 to 280 us (1.96 to 2.37 PFLOP/s; the library's product without block scales 230), at
+// 16384 x 4096 x 4096 takes 227 to 281 us (1.96 to 2.42 PFLOP/s; the library's product without block scales 230), at
 // a clock of 1.4 to 1.7 GHz: power first, and within the cycles (MFMA busy in 65% of them) LDS, whose bytes for a
 // 256 x 256 tile take as long as its MFMAs, and the folds' 4 FMAs an MFMA. 128 x 128 a wavefront would read
 // a quarter less, but its 256 sums a lane leave no vector registers to fold with.
@@ -699,7 +704,8 @@ static int launch_fused_rows(const Args& p, const RowsIn& in, bool vec, hipStrea
 // The shape whose rounds over the CUs take least: rounds x the measured time of one K block (T64 .. T256
 // above). At 4096 x 4096, measured best and chosen: 512 rows T64x128 (20.7 us, T128 25.6), 1024 T128 (28.9, T256x128
 // 40), 1500 T256x128 (43, T128 46), 2900 T192x256 (57.8, T256 60.3, T256x128 72), 5800 T192x256 (106, T256 114),
-// 8192 T256 (136, T192x256 152).
+// 8192 T256 (136, T192x256 152). Measured at 32 K blocks alone: at one to four a tile's first copies and its epilogue are
+// most of its time, which the rule does not know.
 enum { kT64, kT64x128, kT128, kT256x128, kT192x256, kT256, kShapes };
 static int best_shape(int64_t n, int64_t n_out, int cus) {
   static const int bm[kShapes] = {64, 64, 128, 256, 192, 256}, bn[kShapes] = {64, 128, 128, 128, 256, 256};

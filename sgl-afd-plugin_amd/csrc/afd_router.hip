@@ -15,21 +15,23 @@
 // s' = s / sum_e s; L = alpha times the mean of L_s over the sequences that have rows.
 //   dL/dl_te = s'_te r(l_te) (c_e - sum_j c_j s'_tj),  c_e = gloss coef cnt_e,
 //   coef = alpha E / (S' k T^2),  r = 1, 1 - sigmoid(l), sigmoid(l) / (2 softplus(l)),
-// with c counted from the row's largest share's, as whole numbers (16384 x 256 with the weights' gradient 16.7 us, 16.2
-// without that step).
+// with c counted from the row's largest share's, as whole numbers (16384 x 256 with the weights' gradient 15.5 us without
+// that step, 16.2 with it, in turn).
 //
 // Layout: W lanes hold one row, lane i experts [V i, V i + V), so the lanes' order is the experts'
 // and a lane's V logits are wide loads: 16 lanes (4 rows a wavefront) up to 64 experts, 32 up to 128,
 // else 64 lanes with V = 4, 8 or 16; a choice of many rows takes 16 or 32 lanes up to 512 experts. A
 // lane sorts its values once; a pick is then a max butterfly (DPP and permlane swaps) over the lanes' heads.
-// What bounds it is instructions, not bytes: 16384 x 256 with a bias and 4 of 8 groups takes 17 to 20 us (830 VALU
-// instructions for two rows, 11 us of issue; its 18 MB 3.7 us), by the logits alone 9.0; few rows a launch (8 x 256 4.3).
+// What is counted of its time is instructions, not bytes: 16384 x 256 with a bias and 4 of 8 groups takes 17 to 20 us (830
+// VALU instructions for two rows, 11 us of issue, the rest not accounted for; its 18 MB 3.7 us), by the logits alone 9.7;
+// few rows a launch and its latency (8 x 256 4.4, where a launch that does nothing takes 1.4 to 1.6).
 //
 // Sums over rows: a workgroup takes R consecutive rows, cut where sequences begin and end; each piece
 // writes its sums and counts to a slot of its own (slot = workgroup + sequence: from one piece to the
 // next one of the two grows), and a second launch adds a sequence's slots in their order. No sum
-// depends on which workgroup ends first. With the choice 16384 x 256 takes 22 us and 9.6 for the second launch (of
-// which 3.6 are any launch's), the gradient, again one pass, 16.7 (34 MB); given ids, 8192 x 64 6.7, 9.2 and 8.0.
+// depends on which workgroup ends first. With the choice 16384 x 256 takes 22.4 us and 9.6 for the second launch (of
+// which 1.5 are any launch's, the rest dependent reads: slots, ticket, parts), the gradient, again one pass, 16.2 (34
+// MB); given ids, 8192 x 64 6.7, 9.0 and 7.7 (traced medians; in a graph, forward and gradient, 47.1 and 24.6 in all).
 #include "afd_common.h"
 #include "afd_internal.h"
 
@@ -181,7 +183,7 @@ __device__ __forceinline__ float canon(float v) {
   return v != v ? kLowest : fminf(v, 3.402823466e38f);
 }
 // e^x from the hardware's 2^x: the product x log2(e) in two parts, the small one to first order, which
-// keeps the relative error at two ulps for every x (0 below 2^-126)
+// keeps the relative error at two ulps for |x| <= 87.3; past that, where it is left out, 20 (0 below 2^-126)
 __device__ __forceinline__ float exp_f32(float x) {
   constexpr float kLog2e = 1.44269502f, kLog2eLo = 1.92596299e-8f, kLn2 = 0.693147182f;
   const float t = x * kLog2e;
@@ -191,7 +193,8 @@ __device__ __forceinline__ float exp_f32(float x) {
   // no correction where t has left the floats
   return fabsf(t) < 126.0f ? __builtin_fmaf(y, rest * kLn2, y) : y;
 }
-// e^x to |x| 2^-24 relative: for terms of a row's sum and shares, of which the large ones have a small x
+// e^x to (|x| + 2) 2^-24 relative, an instruction instead of four: for terms of a row's sum and shares, of which the large
+// ones have a small x. A gradient's entry carries the error of its own share and of its slope: 2^-18 where |x| is 40.
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 // log(1 + e) for e in [0, 1]: 2 atanh(z), z = e / (2 + e) <= 1/3, by its series up to z^15 (the
 // first term left out is (1/9)^8 / 17 of the sum, below 2^-29)

@@ -8,7 +8,8 @@ pairs that chose expert e and s' the row's scores divided by their sum (``select
 ``expert_counts`` counts alone (what a serving rank keeps to place its experts), ``balance_loss``
 takes ids that were chosen elsewhere, ``select_and_balance`` chooses them in the same pass over the
 logits; its backward writes the gradient of the weights and of the loss in one pass too. Sums run
-in a fixed order: the same call gives the same bits.
+in a fixed order: the same call gives the same bits. The counts are the caller's, to add up over ranks before
+the backward too (it keeps its own); the loss and its gradient are those of this call's rows.
 
 ``cu_seqlens`` int32 [S + 1] (not decreasing) cuts the rows into sequences; rows outside them
 belong to none. Without it all rows are one sequence. ``valid`` bool [n]: rows of False are not counted.

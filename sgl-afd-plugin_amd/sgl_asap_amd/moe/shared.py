@@ -16,7 +16,7 @@ The add itself is fused into the combine kernel (``afd_combine``'s ``shared`` ar
 ``Fp8SharedExpertMLP`` is the same MLP on the block-FP8 weights that FP8 checkpoints hold
 (``Fp8BlockLinear``): half the weight bytes, which is what a decode step waits for, and the FP8
 matrix rate in prefill. Its activation is taken in the down product's quantization (hidden 4096, intermediate
-1536: 1 token 9.1 us against 20.8 for the bf16 MLP, 300 29.0 against 32.4, 16384 349 against 447).
+1536, in a graph: 1 token 8.7 us against 20.4 for the bf16 MLP, 300 28.9 against 31.7, 16384 346 against 452).
 """
 
 from __future__ import annotations

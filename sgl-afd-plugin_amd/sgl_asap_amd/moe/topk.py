@@ -229,8 +229,9 @@ def select_experts(
     ``correction_bias`` f32 [num_experts] takes part in the choice, not in the weights, and has no
     gradient. ``valid`` bool [n]: rows of False (a padded batch) get ids -1, which the expert call
     skips, and weights 0. A NaN logit counts as -inf, +inf as the largest float; a row of
-    -inf alone gets weights 0, and so does one whose chosen scores are all below 2^-126. The
-    weights have a gradient by the logits (zero in invalid rows)."""
+    -inf alone gets weights 0, and so does one whose chosen scores are all below 2^-126 (not with ``renormalize`` and
+    softmax, whose weights are ratios to the largest chosen score). The weights have a gradient by the logits (zero in
+    invalid rows), once: second, forward-mode and traced derivatives are refused."""
     cfg = choice_cfg(router_logits, top_k, scoring, renormalize, num_expert_group, topk_group, routed_scaling_factor)
     no_tangent("select_experts", router_logits)
     if torch.is_grad_enabled() and router_logits.requires_grad:

@@ -273,7 +273,7 @@ class TopK(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         bias = self.correction_bias
         super()._apply(fn, recurse)
-        if bias is not None and self.correction_bias.dtype != bias.dtype:
+        if bias is not None and bias.dtype == torch.float32 != self.correction_bias.dtype:
             self.correction_bias = bias.to(self.correction_bias.device)
         return self
 

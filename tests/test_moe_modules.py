@@ -32,6 +32,12 @@ def test_the_correction_bias_moves_with_the_model():
         assert there.device.type == "meta" and there.dtype == torch.float32
 
 
+def test_a_correction_bias_of_another_type_can_be_cast_to_the_one_it_needs():
+    topk = T.TopK(2, correction_bias=torch.ones(16, dtype=torch.bfloat16))
+    assert topk.float().correction_bias.dtype == torch.float32
+    assert topk.bfloat16().correction_bias.dtype == torch.float32
+
+
 @pytest.fixture
 def no_launches(monkeypatch):
     monkeypatch.setattr(L, "need_gpu", lambda *a: None)

@@ -410,8 +410,8 @@ int afd_silu_mul(const uint16_t* gate_up, int64_t n, int32_t inter, uint16_t* ou
  * block may be shorter); a row of x that holds an infinity or a NaN gives a row of NaN. Any n_out
  * and k_in up to 65536, n <= 2^22. Scales may have any size: where a product of two is no normal
  * float, the results that it belongs to are folded in 64 bits, slowly. afd_linear_pack lays
- * checkpoint codes e4m3 [n_out][ld] out once (image: afd_linear_layout's bytes, 16-byte aligned); scales f32 [ceil(n_out / 128)][ceil(k_in / 128)] are used
- * as they are. x: rows of ldx >= k_in elements, y: rows of ldy >= n_out, none of them x's; the
+ * checkpoint codes e4m3 [n_out][ld] out once (image: afd_linear_layout's bytes, 16-byte aligned);
+ * scales f32 [ceil(n_out / 128)][ceil(k_in / 128)] are used as they are. x: rows of ldx >= k_in elements, y: rows of ldy >= n_out, none of them x's; the
  * elements between rows stay as they are. The workspace (16-byte aligned) holds the quantized rows of one call. */
 typedef struct afd_linear_weights {
   int32_t n_out;

@@ -40,7 +40,8 @@
  *                                take)
  *   afd_linear / ............... the block-FP8 linear layers of the shared expert, the engine's in
  *   afd_linear_pack /            the reference (the MLP called at P/srt/batch_overlap/
- *   afd_linear_silu_mul          operations_strategy.py:94, 255)
+ *   afd_linear_silu_mul          operations_strategy.py:94, 255); int8 checkpoints': afd_linear_i8,
+ *                                afd_linear_i8_silu_mul
  *   afd_expert_counts / ........ no counterpart: where the tokens go, the balance loss of a
  *   afd_balance / ..............  router in training, and the gradient of both by its logits
  *   afd_topk_balance /
@@ -431,6 +432,19 @@ int afd_linear(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
 int afd_linear_silu_mul(const afd_linear_weights* weights, const uint16_t* gate_up, int64_t ld,
                         int32_t n, void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy,
                         afd_stream_t stream);
+
+/* ---- dense int8 product -----------------------------------------------------------------------
+ * y[t, o] = bf16(sx[t] * scales[o] * sum of qx[t] * codes[o]), with x bf16 quantized per token: sx = max(amax, 1e-10) /
+ * 127, qx = rint(x / sx) (quotients in fp32); a row of x that holds an infinity or a NaN gives a row of NaN. The sum
+ * is exact. weights: int8 codes laid out by afd_linear_pack (afd_linear_layout's bytes), scales f32 [n_out] of any
+ * size. Sizes, rows, and the workspace's alignment as afd_linear's. */
+int afd_linear_i8_workspace(int32_t n, int32_t k_in, uint64_t* bytes);
+int afd_linear_i8(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx, int32_t n,
+                  void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy, afd_stream_t stream);
+/* afd_silu_mul's result of gate_up bf16 [n][ld >= 2 k_in] as afd_linear_i8's x, bit for bit, which never is in memory. */
+int afd_linear_i8_silu_mul(const afd_linear_weights* weights, const uint16_t* gate_up, int64_t ld,
+                           int32_t n, void* ws, uint64_t ws_bytes, uint16_t* y, int64_t ldy,
+                           afd_stream_t stream);
 
 /* ---- the router ---------------------------------------------------------------------------
  * Scores of a row of logits l: softmax(l), sigmoid(l) or sqrt(softplus(l)). A NaN logit counts

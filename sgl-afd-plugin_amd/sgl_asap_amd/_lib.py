@@ -73,6 +73,9 @@ EXPORTED = (
     "afd_linear_workspace",
     "afd_linear",
     "afd_linear_silu_mul",
+    "afd_linear_i8_workspace",
+    "afd_linear_i8",
+    "afd_linear_i8_silu_mul",
     "afd_topk",
     "afd_balance_workspace",
     "afd_expert_counts",
@@ -127,7 +130,7 @@ class AfdExpertWeights(ctypes.Structure):
 
 
 class AfdLinearWeights(ctypes.Structure):
-    """afd_linear_weights: a dense layer's FP8 block weights (afd_linear)."""
+    """afd_linear_weights: a dense layer's 8-bit weights (afd_linear, afd_linear_i8)."""
 
     _fields_ = [
         ("n_out", ctypes.c_int32),
@@ -297,6 +300,9 @@ _SIGS = {
     "afd_linear_workspace": ([_I32, _I32, ctypes.POINTER(_U64)], _I32),
     "afd_linear": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
     "afd_linear_silu_mul": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
+    "afd_linear_i8_workspace": ([_I32, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_linear_i8": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
+    "afd_linear_i8_silu_mul": ([ctypes.POINTER(AfdLinearWeights), _P, _I64, _I32, _P, _U64, _P, _I64, _P], _I32),
     "afd_topk": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _P], _I32),
     "afd_balance_workspace": ([_I32, _I32, _I32, ctypes.POINTER(_U64)], _I32),
     "afd_expert_counts": ([_P, _I32, _I32, _I32, _P, _P, _I32, _P, _P, _U64, _P], _I32),

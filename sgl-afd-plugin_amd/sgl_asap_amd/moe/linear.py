@@ -1,9 +1,17 @@
-"""A dense layer with block-FP8 weights: ``y = bf16(q(x) W^T)``, W in e4m3 with one fp32 scale per 128x128 block, x
-quantized in the call to e4m3 with one fp32 scale per 1x128 (``afd_linear``).
+"""Dense layers with 8-bit weights, quantizing their bf16 input in the call; any sizes, one token to prefill.
 
-The format is the experts' (FP8 checkpoints hold their dense layers in it too, the
-shared expert's among them); the reference leaves these layers to the serving engine. Any sizes, one token to prefill.
-For serving: the product has no gradient.
+``Fp8BlockLinear`` (``afd_linear``): ``y = bf16(q(x) W^T)``, W in e4m3 with one fp32 scale per 128x128 block, x
+quantized to e4m3 with one fp32 scale per 1x128. The format is the experts' (FP8 checkpoints hold their dense
+layers in it too, the shared expert's among them).
+
+``Int8Linear`` (``afd_linear_i8``): W in int8 with one fp32 scale per output channel, x quantized to int8 with one fp32
+scale per token (the format of W8A8 checkpoints)::
+
+    sx[t] = max(amax |x[t]|, 1e-10) / 127,  q = rint(x / sx),  y[t, o] = bf16(sx[t] scales[o] sum_k q[t, k] W[o, k])
+
+with the sum exact, so that a row's result does not depend on the rows beside it.
+
+The reference leaves these layers to the serving engine. For serving: the products have no gradient.
 """
 
 from __future__ import annotations
@@ -21,9 +29,9 @@ FP8_BLOCK = 128
 
 
 @lru_cache(maxsize=1024)
-def _workspace_bytes(n: int, k_in: int) -> int:
+def _workspace_bytes(name: str, n: int, k_in: int) -> int:
     out = ctypes.c_uint64()
-    _lib.call("afd_linear_workspace", n, k_in, ctypes.byref(out))
+    _lib.call(name, n, k_in, ctypes.byref(out))
     return out.value
 
 
@@ -42,21 +50,15 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-class Fp8BlockLinear(torch.nn.Module):
-    """``weight``: e4m3 codes [n_out, k_in] (float8_e4m3fn, or their bytes); ``scales``: fp32
-    [ceil(n_out / 128), ceil(k_in / 128)], the weight being code x scale. Laid out once for the kernels, on ``device``
-    (default: the codes'), where the layer stays: moves and casts of a module leave it, and like the bf16 MLP's weights its own
+class _PackedLinear(torch.nn.Module):
+    """What the layers share: codes [n_out, k_in] of a byte each, laid out once for the kernels, on ``device`` (default: the
+    codes'), where the layer stays: moves and casts of a module leave it, and like the bf16 MLP's weights its own
     are not in ``state_dict()`` (they come from the checkpoint). It can be copied and pickled."""
 
-    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, device=None):
-        super().__init__()
-        if weight.dim() != 2 or weight.dtype not in (torch.float8_e4m3fn, torch.uint8, torch.int8):
-            raise TypeError(f"expected e4m3 codes [n_out, k_in], got {weight.dtype} {tuple(weight.shape)}")
+    ENTRY = ""  # the C entry point; ENTRY + "_silu_mul" and ENTRY + "_workspace" stand beside it
+
+    def _pack(self, weight: torch.Tensor, scales: torch.Tensor, device) -> None:
         n_out, k_in = weight.shape
-        blocks = (-(-n_out // FP8_BLOCK), -(-k_in // FP8_BLOCK))
-        if scales.dtype != torch.float32 or tuple(scales.shape) != blocks:
-            raise ValueError(f"scales must be float32 {blocks} for weights {n_out} x {k_in}, got {scales.dtype} "
-                             f"{tuple(scales.shape)}")
         fit_ints(n_out, k_in)
         size = ctypes.c_uint64()
         _lib.call("afd_linear_layout", n_out, k_in, ctypes.byref(size))
@@ -85,8 +87,8 @@ class Fp8BlockLinear(torch.nn.Module):
         """bf16 [..., k_in] -> bf16 [..., n_out] on the device's current stream, into ``out`` if given ([n,
         n_out] with contiguous rows that share no element with x, x two-dimensional). ``silu_mul``: as the method."""
         if silu_mul:
-            return self._product("afd_linear_silu_mul", x, 2 * self.in_features, out)
-        return self._product("afd_linear", x, self.in_features, out)
+            return self._product(self.ENTRY + "_silu_mul", x, 2 * self.in_features, out)
+        return self._product(self.ENTRY, x, self.in_features, out)
 
     def silu_mul(self, gate_up: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer of ``silu_mul(gate_up)``, bf16 [..., 2 k_in] of [gate | up] rows, bit for bit, in a launch less and
@@ -99,8 +101,8 @@ class Fp8BlockLinear(torch.nn.Module):
         if x.device != self.image.device:
             raise ValueError(f"x is on {x.device}, the weights on {self.image.device}")
         if torch.is_grad_enabled() and (x.requires_grad or out is not None and out.requires_grad):
-            raise NotImplementedError("Fp8BlockLinear has no gradient: call it under torch.no_grad()")
-        no_tangent("Fp8BlockLinear", x, out)
+            raise NotImplementedError(f"{type(self).__name__} has no gradient: call it under torch.no_grad()")
+        no_tangent(type(self).__name__, x, out)
         rows = x if x.dim() == 2 else x.reshape(-1, columns)
         rows, ldx = matrix_rows(rows)
         n = rows.shape[0]
@@ -115,9 +117,43 @@ class Fp8BlockLinear(torch.nn.Module):
                 raise ValueError("out must have contiguous rows of its own on x's device")
             if _overlap(rows, y):
                 raise ValueError("out shares elements with x")
-        size = _workspace_bytes(n, self.in_features)
+        size = _workspace_bytes(self.ENTRY + "_workspace", n, self.in_features)
         # a call's own: calls on other streams and captured graphs each have theirs
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         launch(name, x.device, self._weights_ref, rows.data_ptr(), ldx, n,
                ws.data_ptr(), size, y.data_ptr(), y.stride(0) if n > 1 else self.out_features)
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)
+
+
+class Fp8BlockLinear(_PackedLinear):
+    """``weight``: e4m3 codes [n_out, k_in] (float8_e4m3fn, or their bytes); ``scales``: fp32
+    [ceil(n_out / 128), ceil(k_in / 128)], the weight being code x scale."""
+
+    ENTRY = "afd_linear"
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, device=None):
+        super().__init__()
+        if weight.dim() != 2 or weight.dtype not in (torch.float8_e4m3fn, torch.uint8, torch.int8):
+            raise TypeError(f"expected e4m3 codes [n_out, k_in], got {weight.dtype} {tuple(weight.shape)}")
+        n_out, k_in = weight.shape
+        blocks = (-(-n_out // FP8_BLOCK), -(-k_in // FP8_BLOCK))
+        if scales.dtype != torch.float32 or tuple(scales.shape) != blocks:
+            raise ValueError(f"scales must be float32 {blocks} for weights {n_out} x {k_in}, got {scales.dtype} "
+                             f"{tuple(scales.shape)}")
+        self._pack(weight, scales, device)
+
+
+class Int8Linear(_PackedLinear):
+    """``weight``: int8 codes [n_out, k_in]; ``scales``: fp32 [n_out] or [n_out, 1], the weight being code x scale. A row of
+    x with an infinity or a NaN gives a row of NaN."""
+
+    ENTRY = "afd_linear_i8"
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, device=None):
+        super().__init__()
+        if weight.dim() != 2 or weight.dtype != torch.int8:
+            raise TypeError(f"expected int8 codes [n_out, k_in], got {weight.dtype} {tuple(weight.shape)}")
+        n_out = weight.shape[0]
+        if scales.dtype != torch.float32 or tuple(scales.shape) not in ((n_out,), (n_out, 1)):
+            raise ValueError(f"scales must be float32 [{n_out}] or [{n_out}, 1], got {scales.dtype} {tuple(scales.shape)}")
+        self._pack(weight, scales.reshape(n_out), device)

@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import torch
 
-from .linear import Fp8BlockLinear
+from .linear import Fp8BlockLinear, Int8Linear
 from .topk import launch, need_gpu
 
 
@@ -64,11 +64,11 @@ class SharedExpertMLP(torch.nn.Module):
         return torch.mm(silu_mul(gate_up), self.w_down.t())
 
 
-class Fp8SharedExpertMLP(torch.nn.Module):
-    """The shared expert on block-FP8 weights: e4m3 codes ``w_gate_up`` [2I, H] = [gate; up] rows and
-    ``w_down`` [H, I], each with its fp32 scales per 128x128 block, any H and I. x and the activation (rounded
-    to bf16, as the bf16 MLP rounds it) are quantized per 1x128 before their products. ``down`` is called with the gate and
-    up rows and takes the activation itself (``Fp8BlockLinear.silu_mul``)."""
+class _QuantizedSharedExpertMLP(torch.nn.Module):
+    """Two layers of ``LINEAR``: ``w_gate_up`` [2I, H] = [gate; up] rows and ``w_down`` [H, I]. ``down`` is called with the
+    gate and up rows and takes the activation itself (rounded to bf16, as the bf16 MLP rounds it)."""
+
+    LINEAR = None
 
     def __init__(self, w_gate_up: torch.Tensor, s_gate_up: torch.Tensor, w_down: torch.Tensor, s_down: torch.Tensor,
                  device=None):
@@ -78,13 +78,27 @@ class Fp8SharedExpertMLP(torch.nn.Module):
             raise ValueError(f"w_gate_up {tuple(w_gate_up.shape)} and w_down {tuple(w_down.shape)} "
                              "do not form one SwiGLU MLP")
         self.hidden_size, self.intermediate_size = hidden, two_i // 2
-        self.gate_up = Fp8BlockLinear(w_gate_up, s_gate_up, device)
-        self.down = Fp8BlockLinear(w_down, s_down, device)
+        self.gate_up = self.LINEAR(w_gate_up, s_gate_up, device)
+        self.down = self.LINEAR(w_down, s_down, device)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden_size:
             raise TypeError(f"expected bf16 [n, {self.hidden_size}], got {x.dtype} {tuple(x.shape)}")
         return self.down.silu_mul(self.gate_up(x))
+
+
+class Fp8SharedExpertMLP(_QuantizedSharedExpertMLP):
+    """The shared expert on block-FP8 weights: e4m3 codes, each matrix with its fp32 scales per 128x128 block, any H and I.
+    x and the activation are quantized per 1x128 before their products (``Fp8BlockLinear.silu_mul``)."""
+
+    LINEAR = Fp8BlockLinear
+
+
+class Int8SharedExpertMLP(_QuantizedSharedExpertMLP):
+    """The shared expert on int8 weights: int8 codes, each matrix with one fp32 scale per output channel, any H and I. x and
+    the activation are quantized per token before their products (``Int8Linear.silu_mul``)."""
+
+    LINEAR = Int8Linear
 
 
 def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:

@@ -46,6 +46,11 @@
  *   afd_balance / ..............  router in training, and the gradient of both by its logits
  *   afd_topk_balance /
  *   afd_router_grad
+ *   afd_sort_tokens / .......... no counterpart: the permutation that the engine's expert call does inside
+ *   afd_unsort_tokens /          (afd_route, afd_finalize here), for experts that run elsewhere and
+ *   afd_unsort_grad              in training
+ *   afd_residual_norm / ........ the engine's norms before and after a decoder layer's MoE block, which the
+ *   afd_residual_norm_grad       reference calls through it
  *   afd_pack_mxfp4 / _fp8_block  the quant methods' weight repack at load time
  *                                (FlashInfer layout, mxfp4_flashinfer_trtllm_moe.py:11-13)
  *   afd_repack_mxfp4 / ......... the checkpoint expert load (P/srt/model_loader/weight_utils.py
@@ -504,6 +509,71 @@ int afd_router_grad(const afd_router_cfg* cfg, const void* logits, int64_t ld, c
                     const uint8_t* valid, int32_t n, const float* gw, const int32_t* cu_seqlens,
                     int32_t num_seqs, const int32_t* counts, const float* coef, const float* gloss,
                     void* dlogits, afd_stream_t stream);
+
+/* ---- tokens sorted by expert and back ----------------------------------------------------------
+ * Formats of rows that are moved, added up or normed. */
+enum afd_value_fmt { AFD_V_F32 = 0, AFD_V_BF16 = 1, AFD_V_F16 = 2 };
+
+/* Pair t topk + j sends token t to expert ids[t][j]; it is here if expert_lo <= id < expert_lo + num_experts. Pairs
+ * here are sorted by expert, equal ones in their order: positions i32 [n][topk] is a pair's place (-1: not
+ * here), and x's row t is copied to rows[place] for each. counts i32 [num_experts], offsets i32 [num_experts + 1]: the
+ * experts' pairs and where they begin; offsets[num_experts] is the number of rows. rows: n topk of ld >= columns elements;
+ * those past the last are zeroed with zero_behind, else left as they are. Limits: n <= 2^26, topk <= 32, n topk < 2^31,
+ * num_experts <= 1024, columns <= 65536. The workspace (4-byte aligned) is one call's. */
+int afd_sort_workspace(int32_t n, int32_t topk, int32_t num_experts, uint64_t* bytes);
+int afd_sort_tokens(int32_t fmt, const int32_t* ids, int32_t n, int32_t topk, int32_t expert_lo,
+                    int32_t num_experts, const void* x, int64_t ldx, int32_t columns, void* rows,
+                    int64_t ld, int32_t zero_behind, int32_t* positions, int32_t* counts,
+                    int32_t* offsets, void* ws, uint64_t ws_bytes, afd_stream_t stream);
+
+/* out [n][columns]: the sum over j of w[t][j] (f32; NULL: 1) rows[positions[t][j]], in fp32 in that order, rounded once;
+ * positions outside [0, num_rows) are skipped. With NULL weights this is also the gradient of afd_sort_tokens by x. */
+int afd_unsort_tokens(int32_t fmt, const void* rows, int64_t ld, int64_t num_rows,
+                      const int32_t* positions, const float* w, int32_t n, int32_t topk,
+                      int32_t columns, void* out, afd_stream_t stream);
+/* Its gradient from g [n][columns], that of out: d_rows [num_rows][columns] (NULL: not wanted), rows from *total on 0, and
+ * d_w f32 [n][topk] (NULL: not wanted), 0 where the position is skipped. */
+int afd_unsort_grad(int32_t fmt, const void* g, const void* rows, int64_t ld, int64_t num_rows,
+                    const int32_t* positions, const int32_t* total, const float* w, int32_t n,
+                    int32_t topk, int32_t columns, void* d_rows, float* d_w, afd_stream_t stream);
+
+/* ---- the norms before and after a block ---------------------------------------------------------
+ * rms(v) = v / sqrt(mean(v^2) + eps) over a token's row, the mean of squares in fp32;
+ *   h = residual + scale * gate * (rms(y) * w_post, or y without w_post),  normed = rms(h) * w_next
+ * y, residual, h, normed in fmt; w_post, gate and w_next in fmt or in fp32. columns <= 16384, n <= 2^26, eps > 0. */
+enum afd_gate_kind {
+  AFD_GATE_NONE = 0,
+  AFD_GATE_CHANNEL = 1, /* [columns] */
+  AFD_GATE_TOKEN = 2,   /* [n] */
+  AFD_GATE_ELEMENT = 3  /* [n][columns] */
+};
+typedef struct afd_norm_cfg {
+  int32_t columns;
+  int32_t fmt;       /* enum afd_value_fmt */
+  int32_t gate_kind; /* enum afd_gate_kind */
+  int32_t post_f32;  /* w_post is held in fp32 */
+  int32_t gate_f32;
+  int32_t next_f32;
+  float scale;
+  float eps;
+} afd_norm_cfg;
+
+/* y NULL: h is the residual itself (and not written), normed the norm before a block. normed or h NULL: not wanted.
+ * y, residual: rows of ldy, ldr >= columns elements; h, normed [n][columns]. rstd f32 [2][n] (NULL: not wanted): one
+ * over the root of y and of h, which the gradient takes. */
+int afd_residual_norm(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* residual,
+                      int64_t ldr, const void* w_post, const void* gate, const void* w_next, int32_t n,
+                      void* h, void* normed, float* rstd, afd_stream_t stream);
+/* The gradient from dh and dn (that of h and of normed, [n][columns]; one may be NULL: 0). h: rows of ldh elements (without
+ * y: the residual). y may be NULL where there is neither w_post nor d_gate. Outputs that are NULL are not wanted: d_residual,
+ * d_y [n][columns] in fmt, d_gate, d_post, d_next as the parameters are held (n 0: not written). Sums over tokens have one
+ * order. */
+int afd_residual_norm_workspace(const afd_norm_cfg* cfg, int32_t n, uint64_t* bytes);
+int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* h,
+                           int64_t ldh, const void* w_post, const void* gate, const void* w_next,
+                           const float* rstd, int32_t n, const void* dh, const void* dn,
+                           void* d_residual, void* d_y, void* d_gate, void* d_post, void* d_next,
+                           void* ws, uint64_t ws_bytes, afd_stream_t stream);
 
 /* ---- transport (one GPU: producer and consumer streams) ---------------------------------
  * Done flags are 64-bit message counters that only grow (a message's counter is the count of

@@ -1,0 +1,442 @@
+// The norms before and after a block, its gate and the residual's scale in one pass over a token's row, on gfx950:
+//
+//   rms(v) = v / sqrt(mean(v^2) + eps)
+//   h = residual + scale gate (rms(y) w_post, or y)          normed = rms(h) w_next
+//
+// y: the block's output; gate: none, one value per channel, per token or per element. Without y, h is the residual itself and
+// normed the norm before a block. A row's values stay in registers in fp32 from its one read to what is written, each
+// result rounded once (normed is that of h before h is rounded).
+//
+// The gradient, from that of h (dh) and of normed (dn), with u = rms(h), v = rms(y):
+//
+//   d = dh + r_h (g - u mean(g u)),  g = dn w_next            d residual = d
+//   d w_next = sum_t dn u
+//   d y = r_y (q - v mean(q v)),  q = scale gate w_post d     (without the norm: scale gate d)
+//   d w_post = sum_t scale gate d v,  d gate = scale d v w_post, summed over what shares the gate's value
+//
+// Sums over tokens have one order: a workgroup adds up its own tokens in registers, and a second launch the workgroups'.
+#include "afd_common.h"
+#include "afd_internal.h"
+#include "afd_rows_dev.h"
+
+namespace afd {
+namespace norm {
+
+using namespace rows;
+
+constexpr int kMaxTokens = 1 << 26;
+
+struct Args {
+  const void *y, *residual;
+  int64_t ldy, ldr;
+  const void *w_post, *gate, *w_next;
+  bool wide_post, wide_gate, wide_next;  // held in fp32
+  int32_t gate_kind;
+  bool post;
+  float scale, eps;
+  int32_t n, columns;
+  void *h, *normed;
+  float* rstd;  // [2][n]: of y, of h
+  // the gradient's (residual: h)
+  const void *dh, *dn;
+  void *d_res, *d_y, *d_gate;
+  float* sums;  // [slots][3][columns]: of w_next, w_post, the channels' gate
+  bool sum_next, sum_post, sum_gate;
+  bool block;  // anything that belongs to y is wanted
+};
+
+// a lane's chunk of a parameter's row, which is held in T or in fp32. VEC only where both are aligned
+template <typename T, int L, bool VEC>
+__device__ __forceinline__ void load_param(const void* p, bool wide, int64_t offset, int columns, int lane, int c, float (&v)[8]) {
+  if (wide)
+    Row<F32, L, VEC>::load(static_cast<const float*>(p) + offset, columns, lane, c, v);
+  else
+    Row<T, L, VEC>::load(static_cast<const typename T::Held*>(p) + offset, columns, lane, c, v);
+}
+template <typename T>
+__device__ __forceinline__ float load_one(const void* p, bool wide, int64_t at) {
+  return wide ? static_cast<const float*>(p)[at] : T::wide(static_cast<const typename T::Held*>(p)[at]);
+}
+
+// A row by L lanes of NC chunks each
+template <typename T, int L, int NC, bool VEC>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void forward_kernel(Args p) {
+  using R = Row<T, L, VEC>;
+  using Held = typename T::Held;
+  __shared__ float part[2][L / 64];
+  constexpr int kRows = L < 256 ? 256 / L : 1;
+  const int64_t t = int64_t(blockIdx.x) * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  if (t >= p.n) return;  // (a whole wavefront, and with one row a workgroup none)
+  const int lane = threadIdx.x & (L - 1), columns = p.columns;
+  const float inv = 1.0f / static_cast<float>(columns);
+  float h[NC][8];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c, h[c]);
+  if (p.y) {
+    float y[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c, y[c]);
+    if (p.post) {
+      float ss[1] = {0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss[0] = __builtin_fmaf(y[c][j], y[c][j], ss[0]);
+      row_sum<L>(ss, part[0], lane);
+      const float r = 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, p.eps));
+      if (p.rstd && lane == 0) p.rstd[t] = r;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float w[8];
+        load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[c][j] = y[c][j] * r * w[j];
+      }
+    }
+    const float s = p.gate_kind == AFD_GATE_TOKEN ? p.scale * load_one<T>(p.gate, p.wide_gate, t) : p.scale;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (p.gate_kind == AFD_GATE_CHANNEL || p.gate_kind == AFD_GATE_ELEMENT) {
+        float g[8];
+        load_param<T, L, VEC>(p.gate, p.wide_gate, p.gate_kind == AFD_GATE_ELEMENT ? t * columns : 0, columns, lane, c, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[c][j] = __builtin_fmaf(g[j] * s, y[c][j], h[c][j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[c][j] = __builtin_fmaf(s, y[c][j], h[c][j]);
+      }
+    }
+    if (p.h)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) R::store(static_cast<Held*>(p.h) + t * columns, columns, lane, c, h[c]);
+  }
+  if (p.normed) {
+    float ss[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss[0] = __builtin_fmaf(h[c][j], h[c][j], ss[0]);
+    row_sum<L>(ss, part[1], lane);
+    const float r = 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, p.eps));
+    if (p.rstd && lane == 0) p.rstd[int64_t(p.n) + t] = r;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float w[8];
+      load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[c][j] = h[c][j] * r * w[j];
+      R::store(static_cast<Held*>(p.normed) + t * columns, columns, lane, c, h[c]);
+    }
+  }
+}
+
+// Slot s (of gridDim.x kRows) takes every slots-th row
+template <typename T, int L, int NC, bool VEC>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void backward_kernel(Args p) {
+  using R = Row<T, L, VEC>;
+  using Held = typename T::Held;
+  __shared__ float part[2][2 * (L / 64)];
+  constexpr int kRows = L < 256 ? 256 / L : 1;
+  const int64_t slot = int64_t(blockIdx.x) * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const int64_t slots = int64_t(gridDim.x) * kRows;
+  const int lane = threadIdx.x & (L - 1), columns = p.columns;
+  const float inv = 1.0f / static_cast<float>(columns);
+  float sum_next[NC][8] = {}, sum_post[NC][8] = {}, sum_gate[NC][8] = {};
+  int turn = 0;  // of the LDS that a row's sums meet in
+  const bool element = p.gate_kind == AFD_GATE_ELEMENT, channel = p.gate_kind == AFD_GATE_CHANNEL;
+  for (int64_t t = slot; t < p.n; t += slots) {
+    float d[NC][8] = {};
+    if (p.dh)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.dh) + t * columns, columns, lane, c, d[c]);
+    if (p.dn) {
+      float u[NC][8], g[NC][8], dot[1] = {0.0f};
+      const float r = p.rstd[int64_t(p.n) + t];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float w[8];
+        R::load(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c, u[c]);
+        R::load(static_cast<const Held*>(p.dn) + t * columns, columns, lane, c, g[c]);
+        load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[c][j] *= r;
+          sum_next[c][j] = __builtin_fmaf(g[c][j], u[c][j], sum_next[c][j]);
+          g[c][j] *= w[j];
+          dot[0] = __builtin_fmaf(g[c][j], u[c][j], dot[0]);
+        }
+      }
+      row_sum<L>(dot, part[turn ^= 1], lane);
+      const float mean = dot[0] * inv;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[c][j] = __builtin_fmaf(r, __builtin_fmaf(-mean, u[c][j], g[c][j]), d[c][j]);
+    }
+    if (p.d_res)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) R::store(static_cast<Held*>(p.d_res) + t * columns, columns, lane, c, d[c]);
+    if (!p.block) continue;
+    const float s = p.gate_kind == AFD_GATE_TOKEN ? p.scale * load_one<T>(p.gate, p.wide_gate, t) : p.scale;
+    const float r = p.post ? p.rstd[t] : 1.0f;
+    // v: rms(y), or y; d becomes q. dots: of q and v, of d and the normed y (the token's gate)
+    float v[NC][8], dots[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float w[8], g[8];
+      // (without its norm, y matters to the gate's gradient alone)
+      if (p.y) {
+        R::load(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c, v[c]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
+      }
+      if (p.post) load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w);
+      if (element || channel) load_param<T, L, VEC>(p.gate, p.wide_gate, element ? t * columns : 0, columns, lane, c, g);
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] *= r;
+        const float f = p.post ? v[c][j] * w[j] : v[c][j];
+        e[j] = p.scale * d[c][j] * f;
+        dots[1] = __builtin_fmaf(d[c][j], f, dots[1]);
+        sum_gate[c][j] += e[j];
+        d[c][j] *= element || channel ? g[j] * s : s;
+        sum_post[c][j] = __builtin_fmaf(d[c][j], v[c][j], sum_post[c][j]);
+        if (p.post) d[c][j] *= w[j];
+        dots[0] = __builtin_fmaf(d[c][j], v[c][j], dots[0]);
+      }
+      if (element && p.d_gate) {
+        if (p.wide_gate)
+          Row<F32, L, VEC>::store(static_cast<float*>(p.d_gate) + t * columns, columns, lane, c, e);
+        else
+          R::store(static_cast<Held*>(p.d_gate) + t * columns, columns, lane, c, e);
+      }
+    }
+    const bool token = p.gate_kind == AFD_GATE_TOKEN && p.d_gate;
+    if (p.post || token) row_sum<L>(dots, part[turn ^= 1], lane);
+    if (token && lane == 0) {
+      const float e = p.scale * dots[1];
+      if (p.wide_gate)
+        static_cast<float*>(p.d_gate)[t] = e;
+      else
+        static_cast<Held*>(p.d_gate)[t] = T::held(e);
+    }
+    if (p.d_y) {
+      const float mean = dots[0] * inv;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (p.post)  // (without, an infinite y leaves its gradient as it is)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[c][j] = r * __builtin_fmaf(-mean, v[c][j], d[c][j]);
+        R::store(static_cast<Held*>(p.d_y) + t * columns, columns, lane, c, d[c]);
+      }
+    }
+  }
+  float* sums = p.sums + slot * 3 * columns;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (p.sum_next) Row<F32, L, VEC>::store(sums, columns, lane, c, sum_next[c]);
+    if (p.sum_post) Row<F32, L, VEC>::store(sums + columns, columns, lane, c, sum_post[c]);
+    if (p.sum_gate) Row<F32, L, VEC>::store(sums + 2 * columns, columns, lane, c, sum_gate[c]);
+  }
+}
+
+// The slots' sums, 64 columns a workgroup
+struct Finish {
+  const float* sums;
+  int32_t slots, columns;
+  void* out[3];
+  bool wide[3];
+};
+constexpr int kFinishWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(64 * kFinishWaves) void finish_kernel(Finish p) {
+  __shared__ float part[kFinishWaves][64];
+  const int which = blockIdx.y;
+  if (!p.out[which]) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+  float sum = 0.0f;
+  if (col < p.columns)
+    for (int s = w; s < p.slots; s += kFinishWaves) sum += p.sums[(int64_t(s) * 3 + which) * p.columns + col];
+  part[w][lane] = sum;
+  __syncthreads();
+  if (w == 0 && col < p.columns) {
+    for (int i = 1; i < kFinishWaves; ++i) sum += part[i][lane];
+    if (p.wide[which])
+      static_cast<float*>(p.out[which])[col] = sum;
+    else
+      static_cast<typename T::Held*>(p.out[which])[col] = T::held(sum);
+  }
+}
+
+// ---------------------------------------------------------------- host
+static int check(const afd_norm_cfg* cfg, int32_t n) {
+  if (!cfg || n < 0 || n > kMaxTokens) return AFD_ERR_ARG;
+  if (cfg->columns < 1 || cfg->columns > kMaxHidden) return AFD_ERR_SHAPE;
+  if (!known_fmt(cfg->fmt) || cfg->gate_kind < AFD_GATE_NONE || cfg->gate_kind > AFD_GATE_ELEMENT) return AFD_ERR_UNSUPPORTED;
+  if (!(cfg->eps > 0.0f)) return AFD_ERR_ARG;
+  return AFD_OK;
+}
+
+// f(lanes, chunks): the lanes that share a row and the chunks of 8 values each of them holds
+template <typename F>
+static void with_lanes(int columns, F f) {
+  auto go = [&](auto l, auto nc) { f(l, nc); };
+  using std::integral_constant;
+  if (columns <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (columns <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (columns <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  if (columns <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  return go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+// workgroups of the gradient's launch
+static int grid_of(int32_t n, int32_t columns) {
+  const int rows = columns <= 512 ? 4 : 1;
+  const int64_t need = (int64_t(n) + rows - 1) / rows, most = 2 * 256;
+  return static_cast<int>(need < most ? need : most);
+}
+static int slots_of(int32_t n, int32_t columns) { return grid_of(n, columns) * (columns <= 512 ? 4 : 1); }
+
+static bool aligned_params(const Args& p, int fmt) {
+  auto fine = [&](const void* v) { return reinterpret_cast<uintptr_t>(v) % 16 == 0; };
+  return p.columns % 8 == 0 && fine(p.w_post) && fine(p.w_next) && (p.gate_kind == AFD_GATE_TOKEN || fine(p.gate)) &&
+         aligned_rows(p.y, p.ldy, fmt) && aligned_rows(p.residual, p.ldr, fmt);
+}
+
+}  // namespace norm
+}  // namespace afd
+
+using namespace afd;
+
+extern "C" int afd_residual_norm(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* residual, int64_t ldr,
+                                 const void* w_post, const void* gate, const void* w_next, int32_t n, void* h, void* normed,
+                                 float* rstd, afd_stream_t stream) {
+  const int st = norm::check(cfg, n);
+  if (st != AFD_OK) return st;
+  if ((y && ldy < cfg->columns) || ldr < cfg->columns) return AFD_ERR_SHAPE;
+  if (n == 0) return AFD_OK;
+  if (!residual || (!h && !normed) || (!y && h) || (normed && !w_next) || (y && cfg->gate_kind != AFD_GATE_NONE && !gate))
+    return AFD_ERR_ARG;
+  norm::Args p = {};
+  p.y = y;
+  p.residual = residual;
+  p.ldy = ldy;
+  p.ldr = ldr;
+  p.w_post = w_post;
+  p.gate = gate;
+  p.w_next = w_next;
+  p.wide_post = cfg->post_f32;
+  p.wide_gate = cfg->gate_f32;
+  p.wide_next = cfg->next_f32;
+  p.gate_kind = cfg->gate_kind;
+  p.post = w_post != nullptr;
+  p.scale = cfg->scale;
+  p.eps = cfg->eps;
+  p.n = n;
+  p.columns = cfg->columns;
+  p.h = h;
+  p.normed = normed;
+  p.rstd = rstd;
+  const bool vec = norm::aligned_params(p, cfg->fmt) && rows::aligned_rows(h, p.columns, cfg->fmt) &&
+                   rows::aligned_rows(normed, p.columns, cfg->fmt);
+  return rows::with_fmt(cfg->fmt, [&](auto type) -> int {
+    norm::with_lanes(p.columns, [&](auto l, auto nc) {
+      using T = decltype(type);
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, kThreads = L < 256 ? 256 : L;
+      const dim3 grid(static_cast<unsigned>((int64_t(n) * L + kThreads - 1) / kThreads));
+      if (vec)
+        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+      else
+        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+    });
+    AFD_CHECK_LAUNCH();
+    return AFD_OK;
+  });
+}
+
+extern "C" int afd_residual_norm_workspace(const afd_norm_cfg* cfg, int32_t n, uint64_t* bytes) {
+  const int st = norm::check(cfg, n);
+  if (st != AFD_OK) return st;
+  if (!bytes) return AFD_ERR_ARG;
+  *bytes = uint64_t(norm::slots_of(n, cfg->columns)) * 3 * cfg->columns * 4;
+  return AFD_OK;
+}
+
+extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* h, int64_t ldh,
+                                      const void* w_post, const void* gate, const void* w_next, const float* rstd, int32_t n,
+                                      const void* dh, const void* dn, void* d_residual, void* d_y, void* d_gate, void* d_post,
+                                      void* d_next, void* ws, uint64_t ws_bytes, afd_stream_t stream) {
+  uint64_t need;
+  const int st = afd_residual_norm_workspace(cfg, n, &need);
+  if (st != AFD_OK) return st;
+  if ((y && ldy < cfg->columns) || (dn && ldh < cfg->columns)) return AFD_ERR_SHAPE;
+  const int kind = y || d_y ? cfg->gate_kind : AFD_GATE_NONE;
+  const bool sums = d_next || d_post || (kind == AFD_GATE_CHANNEL && d_gate);
+  if (n == 0) return AFD_OK;
+  if ((!dh && !dn) || (dn && (!h || !w_next || !rstd)) || (kind != AFD_GATE_NONE && !gate) || (y && w_post && !rstd) ||
+      (d_next && !dn) || (d_post && !(y && w_post)) || (d_gate && (!y || kind == AFD_GATE_NONE)) || (d_y && !y && w_post))
+    return AFD_ERR_ARG;
+  if (sums && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)) return AFD_ERR_WORKSPACE;
+  norm::Args p = {};
+  p.y = y;
+  p.residual = h;
+  p.ldy = ldy;
+  p.ldr = ldh;
+  p.w_post = w_post;
+  p.gate = gate;
+  p.w_next = w_next;
+  p.wide_post = cfg->post_f32;
+  p.wide_gate = cfg->gate_f32;
+  p.wide_next = cfg->next_f32;
+  p.gate_kind = kind;
+  p.post = y && w_post;
+  p.scale = cfg->scale;
+  p.eps = cfg->eps;
+  p.n = n;
+  p.columns = cfg->columns;
+  p.rstd = const_cast<float*>(rstd);
+  p.dh = dh;
+  p.dn = dn;
+  p.d_res = d_residual;
+  p.d_y = d_y;
+  p.d_gate = kind == AFD_GATE_CHANNEL ? nullptr : d_gate;
+  p.sums = static_cast<float*>(ws);
+  p.sum_next = d_next != nullptr;
+  p.sum_post = d_post != nullptr;
+  p.sum_gate = kind == AFD_GATE_CHANNEL && d_gate;
+  p.block = d_y || d_post || d_gate;
+  const int fmt = cfg->fmt;
+  bool vec = norm::aligned_params(p, fmt);
+  for (const void* v : {dh, dn, static_cast<const void*>(d_residual), static_cast<const void*>(d_y)})
+    vec = vec && rows::aligned_rows(v, p.columns, fmt);
+  if (kind == AFD_GATE_ELEMENT) vec = vec && reinterpret_cast<uintptr_t>(d_gate) % 16 == 0;
+  return rows::with_fmt(fmt, [&](auto type) -> int {
+    using T = decltype(type);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    norm::with_lanes(p.columns, [&](auto l, auto nc) {
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, kThreads = L < 256 ? 256 : L;
+      const dim3 grid(static_cast<unsigned>(norm::grid_of(n, p.columns)));
+      if (vec)
+        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, true>), grid, dim3(kThreads), 0, s, p);
+      else
+        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, false>), grid, dim3(kThreads), 0, s, p);
+    });
+    AFD_CHECK_LAUNCH();
+    if (sums) {
+      norm::Finish f = {};
+      f.sums = p.sums;
+      f.slots = norm::slots_of(n, p.columns);
+      f.columns = p.columns;
+      f.out[0] = d_next;
+      f.out[1] = d_post;
+      f.out[2] = kind == AFD_GATE_CHANNEL ? d_gate : nullptr;
+      f.wide[0] = cfg->next_f32;
+      f.wide[1] = cfg->post_f32;
+      f.wide[2] = cfg->gate_f32;
+      hipLaunchKernelGGL(norm::finish_kernel<T>, dim3((p.columns + 63) / 64, 3), dim3(64 * norm::kFinishWaves), 0, s, f);
+      AFD_CHECK_LAUNCH();
+    }
+    return AFD_OK;
+  });
+}

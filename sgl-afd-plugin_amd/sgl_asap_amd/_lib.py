@@ -34,6 +34,9 @@ AFD_ACT_SWIGLU_LIMIT = 2
 AFD_SCORE_SOFTMAX, AFD_SCORE_SIGMOID, AFD_SCORE_SQRTSOFTPLUS = 0, 1, 2
 AFD_LOGITS_F32, AFD_LOGITS_BF16 = 0, 1
 
+AFD_V_F32, AFD_V_BF16, AFD_V_F16 = 0, 1, 2
+AFD_GATE_NONE, AFD_GATE_CHANNEL, AFD_GATE_TOKEN, AFD_GATE_ELEMENT = 0, 1, 2, 3
+
 AFD_WAIT_GEQ, AFD_WAIT_EQ, AFD_WAIT_AND, AFD_WAIT_NOR = 0, 1, 2, 3
 
 AFD_WALK_STATIC, AFD_WALK_DYNAMIC = 0, 1
@@ -82,6 +85,13 @@ EXPORTED = (
     "afd_balance",
     "afd_topk_balance",
     "afd_router_grad",
+    "afd_sort_workspace",
+    "afd_sort_tokens",
+    "afd_unsort_tokens",
+    "afd_unsort_grad",
+    "afd_residual_norm",
+    "afd_residual_norm_workspace",
+    "afd_residual_norm_grad",
     "afd_host_alloc",
     "afd_host_free",
     "afd_copy_async",
@@ -152,6 +162,21 @@ class AfdRouterCfg(ctypes.Structure):
         ("renormalize", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("logits_fmt", ctypes.c_int32),
+    ]
+
+
+class AfdNormCfg(ctypes.Structure):
+    """afd_norm_cfg: the norms before and after a block (afd_residual_norm)."""
+
+    _fields_ = [
+        ("columns", ctypes.c_int32),
+        ("fmt", ctypes.c_int32),
+        ("gate_kind", ctypes.c_int32),
+        ("post_f32", ctypes.c_int32),
+        ("gate_f32", ctypes.c_int32),
+        ("next_f32", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
     ]
 
 
@@ -249,6 +274,7 @@ class AfdReplyDesc(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I32, _I64, _U64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
+_NORM = ctypes.POINTER(AfdNormCfg)
 _ROUTER, _F32 = ctypes.POINTER(AfdRouterCfg), ctypes.c_float
 _SIGS = {
     "afd_abi_version": ([], _I32),
@@ -312,6 +338,19 @@ _SIGS = {
         _I32,
     ),
     "afd_router_grad": ([_ROUTER, _P, _I64, _P, _P, _I32, _P, _P, _I32, _P, _P, _P, _P, _P], _I32),
+    "afd_sort_workspace": ([_I32, _I32, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_sort_tokens": (
+        [_I32, _P, _I32, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _P, _U64, _P],
+        _I32,
+    ),
+    "afd_unsort_tokens": ([_I32, _P, _I64, _I64, _P, _P, _I32, _I32, _I32, _P, _P], _I32),
+    "afd_unsort_grad": ([_I32, _P, _P, _I64, _I64, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P], _I32),
+    "afd_residual_norm": ([_NORM, _P, _I64, _P, _I64, _P, _P, _P, _I32, _P, _P, _P, _P], _I32),
+    "afd_residual_norm_workspace": ([_NORM, _I32, ctypes.POINTER(_U64)], _I32),
+    "afd_residual_norm_grad": (
+        [_NORM, _P, _I64, _P, _I64, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _U64, _P],
+        _I32,
+    ),
     "afd_host_alloc": ([ctypes.POINTER(ctypes.c_void_p), _U64], _I32),
     "afd_host_free": ([_P], _I32),
     "afd_copy_async": ([_P, _P, _U64, _P], _I32),

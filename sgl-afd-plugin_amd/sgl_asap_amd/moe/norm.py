@@ -1,0 +1,244 @@
+"""The norms before and after a block, fused with its gate and the residual's scale (``afd_residual_norm``; the serving
+engine's in the reference).
+
+    rms(v) = v / sqrt(mean(v^2) + eps)                                  over the last dimension
+    rms_norm:       rms(x) * weight                                     before a block
+    residual_norm:  hidden = residual + scale * gate * (rms(y) * post_weight, or y)
+                    normed = rms(hidden) * next_weight                  before the block behind it
+
+y is the block's output. Activations are fp32, bf16 or fp16, the weights and the gate of the same type or fp32; everything is
+computed in fp32 and rounded once (``normed`` is that of ``hidden`` before it is rounded; a mean of squares past fp32
+gives rows of 0). The gradients, by every tensor, are one pass over the rows too; sums over tokens run in a fixed order: the
+same call gives the same bits.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _lib
+from .sort import value_format
+from .topk import fit_ints, last, launch, matrix_rows, need_gpu, no_tangent
+
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_ELEMENT = (_lib.AFD_GATE_NONE, _lib.AFD_GATE_CHANNEL, _lib.AFD_GATE_TOKEN,
+                                                     _lib.AFD_GATE_ELEMENT)
+
+
+class ResidualNorm(NamedTuple):
+    hidden: torch.Tensor  # the residual stream behind the block
+    normed: Optional[torch.Tensor]  # the next block's input, if next_weight was given
+
+
+@lru_cache(maxsize=256)
+def _cfg(columns: int, fmt: int, kind: int, post: bool, gate: bool, nxt: bool, scale: float, eps: float):
+    return ctypes.pointer(_lib.AfdNormCfg(columns, fmt, kind, post, gate, nxt, scale, eps))
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(columns: int, n: int) -> int:
+    out = ctypes.c_uint64()
+    _lib.call("afd_residual_norm_workspace", _cfg(columns, 0, 0, False, False, False, 1.0, 1.0), n, ctypes.byref(out))
+    return out.value
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _wide(t: Optional[torch.Tensor]) -> bool:
+    return t is not None and t.dtype == torch.float32
+
+
+def _forward(cfg, y, residual, w_post, gate, w_next, rstd):
+    """(hidden or None, normed or None) of two-dimensional tensors."""
+    residual, ldr = matrix_rows(residual)
+    ldy = 0
+    if y is not None:
+        y, ldy = matrix_rows(y)
+    n, columns = residual.shape
+    hidden = None if y is None else torch.empty(n, columns, dtype=residual.dtype, device=residual.device)
+    normed = None if w_next is None else torch.empty(n, columns, dtype=residual.dtype, device=residual.device)
+    launch("afd_residual_norm", residual.device, cfg, _ptr(y), ldy, residual.data_ptr(), ldr, _ptr(w_post), _ptr(gate),
+           _ptr(w_next), n, _ptr(hidden), _ptr(normed), _ptr(rstd))
+    return hidden, normed
+
+
+class _Norm(torch.autograd.Function):
+    """y and residual two-dimensional, as ``matrix_rows`` gives them; without y the norm before a block alone."""
+
+    @staticmethod
+    def forward(ctx, y, residual, w_post, gate, w_next, cfg, kind):
+        n = residual.shape[0]
+        rstd = None
+        if w_post is not None or w_next is not None:
+            rstd = torch.empty(2, n, dtype=torch.float32, device=residual.device)
+        hidden, normed = _forward(cfg, y, residual, w_post, gate, w_next, rstd)
+        h = (residual if y is None else hidden) if w_next is not None else None
+        # y itself is read for its norm's gradient and the gate's
+        held = y if w_post is not None or gate is not None and ctx.needs_input_grad[3] else None
+        ctx.save_for_backward(held, h, w_post, gate, w_next, rstd)
+        ctx.cfg, ctx.kind, ctx.shape, ctx.has_y = cfg, kind, tuple(residual.shape), y is not None
+        ctx.set_materialize_grads(False)
+        if y is None:
+            return normed
+        return (hidden, normed) if normed is not None else hidden
+
+    @staticmethod
+    def backward(ctx, *grads):
+        y, h, w_post, gate, w_next, rstd = ctx.saved_tensors
+        dh, dn = (grads + (None,))[:2] if ctx.has_y else (None, grads[0])
+        none = (None,) * 7
+        if dh is None and dn is None:
+            return none
+        made_from = (dh, dn, y, h, w_post, gate, w_next)
+        g = dh if dh is not None else dn
+        (n, columns), dev = ctx.shape, g.device
+        dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
+        need_y, need_res, need_post, need_gate, need_next = ctx.needs_input_grad[:5]
+        need_next = need_next and dn is not None
+        d_res = torch.empty(n, columns, dtype=g.dtype, device=dev) if need_res else None
+        d_y = torch.empty(n, columns, dtype=g.dtype, device=dev) if need_y and ctx.has_y else None
+        # (without tokens no launch writes the parameters' gradients)
+        like = torch.empty_like if n else torch.zeros_like
+        d_post, d_gate, d_next = (like(t) if need else None
+                                  for t, need in ((w_post, need_post), (gate, need_gate), (w_next, need_next)))
+        if n:
+            y, ldy = (None, 0) if y is None else matrix_rows(y)
+            h, ldh = (None, 0) if h is None else matrix_rows(h)
+            sums = d_post is not None or d_next is not None or d_gate is not None and ctx.kind == GATE_CHANNEL
+            size = _workspace_bytes(columns, n) if sums else 0
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            launch("afd_residual_norm_grad", dev, ctx.cfg, _ptr(y), ldy, _ptr(h), ldh, _ptr(w_post), _ptr(gate), _ptr(w_next),
+                   _ptr(rstd), n, _ptr(dh), _ptr(dn), _ptr(d_res), _ptr(d_y), _ptr(d_gate), _ptr(d_post), _ptr(d_next),
+                   ws.data_ptr(), size)
+        out = (d_y, d_res, d_post, d_gate, d_next)
+        return tuple(None if t is None else last(t, *made_from) for t in out) + (None, None)
+
+
+def _activations(name: str, t: torch.Tensor) -> int:
+    fmt = value_format(name, t)
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be [..., hidden] with hidden >= 1, got {tuple(t.shape)}")
+    fit_ints(t.shape[-1])
+    return fmt
+
+
+def _param(name: str, t: Optional[torch.Tensor], like: torch.Tensor, shape: tuple) -> None:
+    if t is None:
+        return
+    if t.dtype not in (like.dtype, torch.float32):
+        raise TypeError(f"{name} must be {like.dtype} or float32, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+
+
+def _eps(eps: float) -> float:
+    eps = float(eps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError(f"eps must be positive, got {eps}")
+    return eps
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _call(y, residual, w_post, gate, w_next, cfg, kind):
+    """(hidden or None, normed or None) of two-dimensional activations."""
+    given = [t for t in (y, residual, w_post, gate, w_next) if t is not None]
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
+        return _forward(cfg, y, residual, w_post, gate, w_next, None)
+    y = None if y is None else matrix_rows(y)[0]
+    out = _Norm.apply(y, matrix_rows(residual)[0], w_post, gate, w_next, cfg, kind)
+    if y is None:
+        return None, out
+    return out if w_next is not None else (out, None)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6) -> torch.Tensor:
+    """``rms(x) * weight`` of ``x`` [..., hidden] (fp32, bf16 or fp16), in x's type, on the device's current stream. ``weight``
+    [hidden] of x's type or fp32. Gradients by both, once: second, forward-mode and traced derivatives are refused."""
+    fmt = _activations("x", x)
+    columns = x.shape[-1]
+    _param("weight", weight, x, (columns,))
+    need_gpu("x", x)
+    no_tangent("rms_norm", x, weight)
+    cfg = _cfg(columns, fmt, GATE_NONE, False, False, _wide(weight), 1.0, _eps(eps))
+    return _call(None, _rows(x), None, None, weight.contiguous(), cfg, GATE_NONE)[1].view(x.shape)
+
+
+def residual_norm(
+    y: torch.Tensor,
+    residual: torch.Tensor,
+    *,
+    post_weight: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+    scale: float = 1.0,
+    next_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+) -> ResidualNorm:
+    """(hidden, normed) of a block's output ``y`` and the ``residual`` it is added to, both [..., hidden] in one type (fp32,
+    bf16 or fp16), on the device's current stream.
+
+    ``post_weight`` [hidden]: the norm after the block (None: none). ``gate``: [hidden], one value per channel, [..., 1], per
+    token, or [..., hidden], per element. ``scale``: a number. ``next_weight`` [hidden]: the norm before the block behind it
+    (None: ``normed`` is None). Weights and gate are of y's type or fp32. Gradients by every tensor, once: second, forward-mode and
+    traced derivatives are refused."""
+    fmt = _activations("y", y)
+    if residual.dtype != y.dtype or residual.shape != y.shape:
+        raise ValueError(f"y is {y.dtype} {tuple(y.shape)}, residual {residual.dtype} {tuple(residual.shape)}")
+    if residual.device != y.device:
+        raise ValueError(f"residual is on {residual.device}, y on {y.device}")
+    columns = y.shape[-1]
+    _param("post_weight", post_weight, y, (columns,))
+    _param("next_weight", next_weight, y, (columns,))
+    kind, gate_rows = GATE_NONE, gate
+    if gate is not None:
+        if gate.dim() == 1:
+            kind, shape = GATE_CHANNEL, (columns,)
+        elif tuple(gate.shape) == tuple(y.shape) and columns > 1:
+            kind, shape = GATE_ELEMENT, tuple(y.shape)
+            gate_rows = gate.reshape(-1, columns)
+        else:
+            kind, shape = GATE_TOKEN, tuple(y.shape[:-1]) + (1,)
+            gate_rows = gate.reshape(-1)
+        _param("gate", gate, y, shape)
+        gate_rows = gate_rows.contiguous()
+    need_gpu("y", y)
+    no_tangent("residual_norm", y, residual, post_weight, gate, next_weight)
+    scale = float(scale)
+    cfg = _cfg(columns, fmt, kind, _wide(post_weight), _wide(gate), _wide(next_weight), scale, _eps(eps))
+    post_weight, next_weight = (None if t is None else t.contiguous() for t in (post_weight, next_weight))
+    hidden, normed = _call(_rows(y), _rows(residual), post_weight, gate_rows, next_weight, cfg, kind)
+    return ResidualNorm(hidden.view(y.shape), None if normed is None else normed.view(y.shape))
+
+
+class BlockNorms(torch.nn.Module):
+    """A block's norms, gate and residual scale as a module: ``hidden = residual + scale * gate * rms(y) * post_weight``.
+
+    ``input_weight`` [hidden]: the norm before the block (``before``); ``post_weight``: after it (None: none); ``gate``
+    [hidden]: learned per channel (None: none). They are parameters."""
+
+    def __init__(self, input_weight: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
+                 gate: Optional[torch.Tensor] = None, scale: float = 1.0, eps: float = 1e-6):
+        super().__init__()
+        for name, t in (("input_weight", input_weight), ("post_weight", post_weight), ("gate", gate)):
+            if t is not None and (t.dim() != 1 or t.shape != input_weight.shape):
+                raise ValueError(f"{name} must be {tuple(input_weight.shape)}, got {tuple(t.shape)}")
+            self.register_parameter(name, None if t is None else torch.nn.Parameter(t))
+        self.scale, self.eps = float(scale), _eps(eps)
+
+    def before(self, x: torch.Tensor) -> torch.Tensor:
+        return rms_norm(x, self.input_weight, eps=self.eps)
+
+    def after(self, y: torch.Tensor, residual: torch.Tensor, gate: Optional[torch.Tensor] = None,
+              next_weight: Optional[torch.Tensor] = None) -> ResidualNorm:
+        """``gate``: in place of the learned one (per token or per element, from the tokens)."""
+        return residual_norm(y, residual, post_weight=self.post_weight, gate=self.gate if gate is None else gate,
+                             scale=self.scale, next_weight=next_weight, eps=self.eps)

@@ -564,13 +564,13 @@ typedef struct afd_norm_cfg {
 int afd_residual_norm(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* residual,
                       int64_t ldr, const void* w_post, const void* gate, const void* w_next, int32_t n,
                       void* h, void* normed, float* rstd, afd_stream_t stream);
-/* The gradient from dh and dn (that of h and of normed, [n][columns]; one may be NULL: 0). h: rows of ldh elements (without
- * y: the residual). y may be NULL where there is neither w_post nor d_gate. Outputs that are NULL are not wanted: d_residual,
- * d_y [n][columns] in fmt, d_gate, d_post, d_next as the parameters are held (n 0: not written). Sums over tokens have one
- * order. */
+/* The gradient from dh and dn (that of h and of normed, [n][columns]; one may be NULL: 0). residual is read with dn, y with
+ * dn, w_post or d_gate (y NULL else; without a block at all, both y and d_y NULL). Outputs that are NULL are not
+ * wanted: d_residual, d_y [n][columns] in fmt, d_gate, d_post, d_next as the parameters are held (n 0: not written). Sums over
+ * tokens have one order. */
 int afd_residual_norm_workspace(const afd_norm_cfg* cfg, int32_t n, uint64_t* bytes);
-int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* h,
-                           int64_t ldh, const void* w_post, const void* gate, const void* w_next,
+int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy,
+                           const void* residual, int64_t ldr, const void* w_post, const void* gate, const void* w_next,
                            const float* rstd, int32_t n, const void* dh, const void* dn,
                            void* d_residual, void* d_y, void* d_gate, void* d_post, void* d_next,
                            void* ws, uint64_t ws_bytes, afd_stream_t stream);

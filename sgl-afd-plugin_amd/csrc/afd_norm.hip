@@ -11,6 +11,7 @@
 //
 //   d = dh + r_h (g - u mean(g u)),  g = dn w_next            d residual = d
 //   d w_next = sum_t dn u
+//   (h is made again from y and the residual: in fp32, as normed saw it)
 //   d y = r_y (q - v mean(q v)),  q = scale gate w_post d     (without the norm: scale gate d)
 //   d w_post = sum_t scale gate d v,  d gate = scale d v w_post, summed over what shares the gate's value
 //
@@ -37,7 +38,7 @@ struct Args {
   int32_t n, columns;
   void *h, *normed;
   float* rstd;  // [2][n]: of y, of h
-  // the gradient's (residual: h)
+  // the gradient's
   const void *dh, *dn;
   void *d_res, *d_y, *d_gate;
   float* sums;  // [slots][3][columns]: of w_next, w_post, the channels' gate
@@ -58,24 +59,43 @@ __device__ __forceinline__ float load_one(const void* p, bool wide, int64_t at) 
   return wide ? static_cast<const float*>(p)[at] : T::wide(static_cast<const typename T::Held*>(p)[at]);
 }
 
-// A row by L lanes of NC chunks each
+// A row is L lanes' of NC chunks each. With L 64 a workgroup has four, a wavefront each, and no barrier.
+template <int L>
+constexpr int kThreads = L == 64 ? 256 : L;
+template <int L>
+constexpr int kRows = kThreads<L> / L;
+template <int L>
+__device__ __forceinline__ int64_t first_row() {
+  return int64_t(blockIdx.x) * kRows<L> + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+}
+
 template <typename T, int L, int NC, bool VEC>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void forward_kernel(Args p) {
+__global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
   __shared__ float part[2][L / 64];
-  constexpr int kRows = L < 256 ? 256 / L : 1;
-  const int64_t t = int64_t(blockIdx.x) * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const int64_t t = first_row<L>();
   if (t >= p.n) return;  // (a whole wavefront, and with one row a workgroup none)
   const int lane = threadIdx.x & (L - 1), columns = p.columns;
   const float inv = 1.0f / static_cast<float>(columns);
-  float h[NC][8];
+  const bool vector = p.gate_kind == AFD_GATE_CHANNEL || p.gate_kind == AFD_GATE_ELEMENT;
+  typename R::Raw h_raw[NC], y_raw[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c, h[c]);
+  for (int c = 0; c < NC; ++c) h_raw[c] = R::fetch(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c);
+  float h[NC][8], w_next[NC][8];
   if (p.y) {
-    float y[NC][8];
+    float y[NC][8], w[NC][8], g[NC][8];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c, y[c]);
+    for (int c = 0; c < NC; ++c) {
+      y_raw[c] = R::fetch(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c);
+      if (p.post) load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w[c]);
+      if (vector)
+        load_param<T, L, VEC>(p.gate, p.wide_gate, p.gate_kind == AFD_GATE_ELEMENT ? t * columns : 0, columns, lane, c, g[c]);
+      if (p.normed) load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w_next[c]);
+    }
+    const float s = p.gate_kind == AFD_GATE_TOKEN ? p.scale * load_one<T>(p.gate, p.wide_gate, t) : p.scale;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) y_raw[c].widen(y[c]);
     if (p.post) {
       float ss[1] = {0.0f};
 #pragma unroll
@@ -86,29 +106,25 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void forward_kernel(Args p) {
       const float r = 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, p.eps));
       if (p.rstd && lane == 0) p.rstd[t] = r;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float w[8];
-        load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[c][j] = y[c][j] * r * w[j];
-      }
+        for (int j = 0; j < 8; ++j) y[c][j] = y[c][j] * r * w[c][j];
     }
-    const float s = p.gate_kind == AFD_GATE_TOKEN ? p.scale * load_one<T>(p.gate, p.wide_gate, t) : p.scale;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (p.gate_kind == AFD_GATE_CHANNEL || p.gate_kind == AFD_GATE_ELEMENT) {
-        float g[8];
-        load_param<T, L, VEC>(p.gate, p.wide_gate, p.gate_kind == AFD_GATE_ELEMENT ? t * columns : 0, columns, lane, c, g);
+      h_raw[c].widen(h[c]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[c][j] = __builtin_fmaf(g[j] * s, y[c][j], h[c][j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[c][j] = __builtin_fmaf(s, y[c][j], h[c][j]);
-      }
+      for (int j = 0; j < 8; ++j) h[c][j] = __builtin_fmaf(vector ? g[c][j] * s : s, y[c][j], h[c][j]);
     }
     if (p.h)
 #pragma unroll
       for (int c = 0; c < NC; ++c) R::store(static_cast<Held*>(p.h) + t * columns, columns, lane, c, h[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (p.normed) load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w_next[c]);
+      h_raw[c].widen(h[c]);
+    }
   }
   if (p.normed) {
     float ss[1] = {0.0f};
@@ -121,48 +137,85 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void forward_kernel(Args p) {
     if (p.rstd && lane == 0) p.rstd[int64_t(p.n) + t] = r;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float w[8];
-      load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[c][j] = h[c][j] * r * w[j];
+      for (int j = 0; j < 8; ++j) h[c][j] = h[c][j] * r * w_next[c][j];
       R::store(static_cast<Held*>(p.normed) + t * columns, columns, lane, c, h[c]);
     }
   }
 }
 
-// Slot s (of gridDim.x kRows) takes every slots-th row
+// Slot s (of gridDim.x kRows) takes every slots-th row, the next one's values on their way while it works on one. The
+// parameters stay in registers, and so do the slot's sums over its rows.
 template <typename T, int L, int NC, bool VEC>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void backward_kernel(Args p) {
+__global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
   __shared__ float part[2][2 * (L / 64)];
-  constexpr int kRows = L < 256 ? 256 / L : 1;
-  const int64_t slot = int64_t(blockIdx.x) * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-  const int64_t slots = int64_t(gridDim.x) * kRows;
+  const int64_t slot = first_row<L>(), slots = int64_t(gridDim.x) * kRows<L>;
   const int lane = threadIdx.x & (L - 1), columns = p.columns;
   const float inv = 1.0f / static_cast<float>(columns);
-  float sum_next[NC][8] = {}, sum_post[NC][8] = {}, sum_gate[NC][8] = {};
   int turn = 0;  // of the LDS that a row's sums meet in
   const bool element = p.gate_kind == AFD_GATE_ELEMENT, channel = p.gate_kind == AFD_GATE_CHANNEL;
-  for (int64_t t = slot; t < p.n; t += slots) {
-    float d[NC][8] = {};
-    if (p.dh)
+  const bool token = p.gate_kind == AFD_GATE_TOKEN;
+  float sum_next[NC][8] = {}, sum_post[NC][8] = {}, sum_gate[NC][8] = {};
+  float w_next[NC][8], w_post[NC][8], gate[NC][8];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) R::load(static_cast<const Held*>(p.dh) + t * columns, columns, lane, c, d[c]);
+  for (int c = 0; c < NC; ++c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w_next[c][j] = w_post[c][j] = gate[c][j] = 1.0f;
+    if (p.dn) load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w_next[c]);
+    if (p.post) load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w_post[c]);
+    if (channel) load_param<T, L, VEC>(p.gate, p.wide_gate, 0, columns, lane, c, gate[c]);
+  }
+  // what a row needs
+  struct In {
+    typename R::Raw dh[NC], dn[NC], res[NC], y[NC];
+    float gate, r_y, r_h;
+  };
+  auto fetch = [&](int64_t t) {
+    In in = {};
+    if (t >= p.n) return in;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (p.dh) in.dh[c] = R::fetch(static_cast<const Held*>(p.dh) + t * columns, columns, lane, c);
+      if (p.dn) in.dn[c] = R::fetch(static_cast<const Held*>(p.dn) + t * columns, columns, lane, c);
+      if (p.dn) in.res[c] = R::fetch(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c);
+      if (p.y) in.y[c] = R::fetch(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c);
+    }
+    in.gate = token ? load_one<T>(p.gate, p.wide_gate, t) : 1.0f;
+    in.r_y = p.post ? p.rstd[t] : 1.0f;
+    in.r_h = p.dn ? p.rstd[int64_t(p.n) + t] : 0.0f;
+    return in;
+  };
+  In next = fetch(slot);
+  for (int64_t t = slot; t < p.n; t += slots) {
+    const In in = next;
+    next = fetch(t + slots);
+    const float s = p.scale * in.gate;
+    if (element)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) load_param<T, L, VEC>(p.gate, p.wide_gate, t * columns, columns, lane, c, gate[c]);
+    // v: rms(y), or y (0 where it is not needed)
+    float d[NC][8], v[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      in.dh[c].widen(d[c]);
+      in.y[c].widen(v[c]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[c][j] *= in.r_y;
+    }
     if (p.dn) {
       float u[NC][8], g[NC][8], dot[1] = {0.0f};
-      const float r = p.rstd[int64_t(p.n) + t];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        float w[8];
-        R::load(static_cast<const Held*>(p.residual) + t * p.ldr, columns, lane, c, u[c]);
-        R::load(static_cast<const Held*>(p.dn) + t * columns, columns, lane, c, g[c]);
-        load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w);
+        in.res[c].widen(u[c]);
+        in.dn[c].widen(g[c]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          u[c][j] *= r;
+          if (p.y) u[c][j] = __builtin_fmaf(element || channel ? gate[c][j] * s : s, v[c][j] * w_post[c][j], u[c][j]);
+          u[c][j] *= in.r_h;
           sum_next[c][j] = __builtin_fmaf(g[c][j], u[c][j], sum_next[c][j]);
-          g[c][j] *= w[j];
+          g[c][j] *= w_next[c][j];
           dot[0] = __builtin_fmaf(g[c][j], u[c][j], dot[0]);
         }
       }
@@ -171,39 +224,26 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void backward_kernel(Args p) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[c][j] = __builtin_fmaf(r, __builtin_fmaf(-mean, u[c][j], g[c][j]), d[c][j]);
+        for (int j = 0; j < 8; ++j) d[c][j] = __builtin_fmaf(in.r_h, __builtin_fmaf(-mean, u[c][j], g[c][j]), d[c][j]);
     }
     if (p.d_res)
 #pragma unroll
       for (int c = 0; c < NC; ++c) R::store(static_cast<Held*>(p.d_res) + t * columns, columns, lane, c, d[c]);
     if (!p.block) continue;
-    const float s = p.gate_kind == AFD_GATE_TOKEN ? p.scale * load_one<T>(p.gate, p.wide_gate, t) : p.scale;
-    const float r = p.post ? p.rstd[t] : 1.0f;
-    // v: rms(y), or y; d becomes q. dots: of q and v, of d and the normed y (the token's gate)
-    float v[NC][8], dots[2] = {0.0f, 0.0f};
+    // d becomes q. dots: of q and v, of d and the normed y (the token's gate)
+    float dots[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float w[8], g[8];
-      // (without its norm, y matters to the gate's gradient alone)
-      if (p.y) {
-        R::load(static_cast<const Held*>(p.y) + t * p.ldy, columns, lane, c, v[c]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
-      }
-      if (p.post) load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w);
-      if (element || channel) load_param<T, L, VEC>(p.gate, p.wide_gate, element ? t * columns : 0, columns, lane, c, g);
       float e[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[c][j] *= r;
-        const float f = p.post ? v[c][j] * w[j] : v[c][j];
+        const float f = v[c][j] * w_post[c][j];
         e[j] = p.scale * d[c][j] * f;
         dots[1] = __builtin_fmaf(d[c][j], f, dots[1]);
         sum_gate[c][j] += e[j];
-        d[c][j] *= element || channel ? g[j] * s : s;
+        d[c][j] *= element || channel ? gate[c][j] * s : s;
         sum_post[c][j] = __builtin_fmaf(d[c][j], v[c][j], sum_post[c][j]);
-        if (p.post) d[c][j] *= w[j];
+        d[c][j] *= w_post[c][j];
         dots[0] = __builtin_fmaf(d[c][j], v[c][j], dots[0]);
       }
       if (element && p.d_gate) {
@@ -213,9 +253,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void backward_kernel(Args p) {
           R::store(static_cast<Held*>(p.d_gate) + t * columns, columns, lane, c, e);
       }
     }
-    const bool token = p.gate_kind == AFD_GATE_TOKEN && p.d_gate;
-    if (p.post || token) row_sum<L>(dots, part[turn ^= 1], lane);
-    if (token && lane == 0) {
+    if (p.post || (token && p.d_gate)) row_sum<L>(dots, part[turn ^= 1], lane);
+    if (token && p.d_gate && lane == 0) {
       const float e = p.scale * dots[1];
       if (p.wide_gate)
         static_cast<float*>(p.d_gate)[t] = e;
@@ -228,7 +267,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void backward_kernel(Args p) {
       for (int c = 0; c < NC; ++c) {
         if (p.post)  // (without, an infinite y leaves its gradient as it is)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[c][j] = r * __builtin_fmaf(-mean, v[c][j], d[c][j]);
+          for (int j = 0; j < 8; ++j) d[c][j] = in.r_y * __builtin_fmaf(-mean, v[c][j], d[c][j]);
         R::store(static_cast<Held*>(p.d_y) + t * columns, columns, lane, c, d[c]);
       }
     }
@@ -258,6 +297,7 @@ __global__ __launch_bounds__(64 * kFinishWaves) void finish_kernel(Finish p) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   float sum = 0.0f;
   if (col < p.columns)
+#pragma unroll 8
     for (int s = w; s < p.slots; s += kFinishWaves) sum += p.sums[(int64_t(s) * 3 + which) * p.columns + col];
   part[w][lane] = sum;
   __syncthreads();
@@ -282,13 +322,13 @@ static int check(const afd_norm_cfg* cfg, int32_t n) {
 // f(lanes, chunks): the lanes that share a row and the chunks of 8 values each of them holds
 template <typename F>
 static void with_lanes(int columns, F f) {
-  auto go = [&](auto l, auto nc) { f(l, nc); };
   using std::integral_constant;
-  if (columns <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  if (columns <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  if (columns <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  if (columns <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
-  return go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+  if (columns <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (columns <= 1024) return f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  if (columns <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (columns <= 4096) return f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+  if (columns <= 8192) return f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
 // workgroups of the gradient's launch
 static int grid_of(int32_t n, int32_t columns) {
@@ -343,12 +383,12 @@ extern "C" int afd_residual_norm(const afd_norm_cfg* cfg, const void* y, int64_t
   return rows::with_fmt(cfg->fmt, [&](auto type) -> int {
     norm::with_lanes(p.columns, [&](auto l, auto nc) {
       using T = decltype(type);
-      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, kThreads = L < 256 ? 256 : L;
-      const dim3 grid(static_cast<unsigned>((int64_t(n) * L + kThreads - 1) / kThreads));
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value;
+      const dim3 grid((n + norm::kRows<L> - 1) / norm::kRows<L>);
       if (vec)
-        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, true>), grid, dim3(norm::kThreads<L>), 0, static_cast<hipStream_t>(stream), p);
       else
-        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
+        hipLaunchKernelGGL((norm::forward_kernel<T, L, NC, false>), grid, dim3(norm::kThreads<L>), 0, static_cast<hipStream_t>(stream), p);
     });
     AFD_CHECK_LAUNCH();
     return AFD_OK;
@@ -363,26 +403,26 @@ extern "C" int afd_residual_norm_workspace(const afd_norm_cfg* cfg, int32_t n, u
   return AFD_OK;
 }
 
-extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* h, int64_t ldh,
+extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, int64_t ldy, const void* residual, int64_t ldr,
                                       const void* w_post, const void* gate, const void* w_next, const float* rstd, int32_t n,
                                       const void* dh, const void* dn, void* d_residual, void* d_y, void* d_gate, void* d_post,
                                       void* d_next, void* ws, uint64_t ws_bytes, afd_stream_t stream) {
   uint64_t need;
   const int st = afd_residual_norm_workspace(cfg, n, &need);
   if (st != AFD_OK) return st;
-  if ((y && ldy < cfg->columns) || (dn && ldh < cfg->columns)) return AFD_ERR_SHAPE;
+  if ((y && ldy < cfg->columns) || (dn && ldr < cfg->columns)) return AFD_ERR_SHAPE;
   const int kind = y || d_y ? cfg->gate_kind : AFD_GATE_NONE;
   const bool sums = d_next || d_post || (kind == AFD_GATE_CHANNEL && d_gate);
   if (n == 0) return AFD_OK;
-  if ((!dh && !dn) || (dn && (!h || !w_next || !rstd)) || (kind != AFD_GATE_NONE && !gate) || (y && w_post && !rstd) ||
-      (d_next && !dn) || (d_post && !(y && w_post)) || (d_gate && (!y || kind == AFD_GATE_NONE)) || (d_y && !y && w_post))
+  if ((!dh && !dn) || (dn && (!residual || !w_next || !rstd)) || (kind != AFD_GATE_NONE && !gate) || ((y || d_y) && w_post && !rstd) ||
+      (d_next && !dn) || (d_post && !(y && w_post)) || (d_gate && (!y || kind == AFD_GATE_NONE)) || (d_y && !y && (w_post || dn)))
     return AFD_ERR_ARG;
   if (sums && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16)) return AFD_ERR_WORKSPACE;
   norm::Args p = {};
   p.y = y;
-  p.residual = h;
+  p.residual = residual;
   p.ldy = ldy;
-  p.ldr = ldh;
+  p.ldr = ldr;
   p.w_post = w_post;
   p.gate = gate;
   p.w_next = w_next;
@@ -415,12 +455,12 @@ extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, in
     using T = decltype(type);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     norm::with_lanes(p.columns, [&](auto l, auto nc) {
-      constexpr int L = decltype(l)::value, NC = decltype(nc)::value, kThreads = L < 256 ? 256 : L;
+      constexpr int L = decltype(l)::value, NC = decltype(nc)::value;
       const dim3 grid(static_cast<unsigned>(norm::grid_of(n, p.columns)));
       if (vec)
-        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, true>), grid, dim3(kThreads), 0, s, p);
+        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, true>), grid, dim3(norm::kThreads<L>), 0, s, p);
       else
-        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, false>), grid, dim3(kThreads), 0, s, p);
+        hipLaunchKernelGGL((norm::backward_kernel<T, L, NC, false>), grid, dim3(norm::kThreads<L>), 0, s, p);
     });
     AFD_CHECK_LAUNCH();
     if (sums) {

@@ -25,79 +25,86 @@ struct F16 {
   static __device__ __forceinline__ _Float16 held(float v) { return static_cast<_Float16>(v); }
 };
 
-// Eight values at p, 16-byte aligned
+// Eight values as they are held, and in fp32
 template <typename T>
-__device__ __forceinline__ void load8(const typename T::Held* p, float (&v)[8]) {
-  if constexpr (sizeof(typename T::Held) == 4) {
-    const v4f lo = reinterpret_cast<const v4f*>(p)[0], hi = reinterpret_cast<const v4f*>(p)[1];
+struct Raw8 {
+  static constexpr int kWords = 8 * sizeof(typename T::Held) / 16;
+  v4i w[kWords];
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+    if constexpr (sizeof(typename T::Held) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = lo[i];
-      v[4 + i] = hi[i];
-    }
-  } else {
-    const v4i raw = *reinterpret_cast<const v4i*>(p);
-    if constexpr (std::is_same<T, Bf16>::value) {
+      for (int i = 0; i < 8; ++i) v[i] = __int_as_float(w[i / 4][i % 4]);
+    } else if constexpr (std::is_same<T, Bf16>::value) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(static_cast<uint32_t>(raw[i]) << 16);
-        v[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(raw[i]) & 0xffff0000u);
+        v[2 * i] = __uint_as_float(static_cast<uint32_t>(w[0][i]) << 16);
+        v[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(w[0][i]) & 0xffff0000u);
       }
     } else {
-      const v8h h = __builtin_bit_cast(v8h, raw);
+      const v8h h = __builtin_bit_cast(v8h, w[0]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(h[i]);
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(typename T::Held* p, const float (&v)[8]) {
-  if constexpr (sizeof(typename T::Held) == 4) {
-    reinterpret_cast<v4f*>(p)[0] = v4f{v[0], v[1], v[2], v[3]};
-    reinterpret_cast<v4f*>(p)[1] = v4f{v[4], v[5], v[6], v[7]};
-  } else if constexpr (std::is_same<T, Bf16>::value) {
-    v4i raw;
+  __device__ __forceinline__ void narrow(const float (&v)[8]) {
+    if constexpr (sizeof(typename T::Held) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = static_cast<int>(pk_bf16(v[2 * i], v[2 * i + 1]));
-    *reinterpret_cast<v4i*>(p) = raw;
-  } else {
-    v8h h;
+      for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = __float_as_int(v[i]);
+    } else if constexpr (std::is_same<T, Bf16>::value) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = static_cast<_Float16>(v[i]);
-    *reinterpret_cast<v4i*>(p) = __builtin_bit_cast(v4i, h);
+      for (int i = 0; i < 4; ++i) w[0][i] = static_cast<int>(pk_bf16(v[2 * i], v[2 * i + 1]));
+    } else {
+      v8h h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = static_cast<_Float16>(v[i]);
+      w[0] = __builtin_bit_cast(v4i, h);
+    }
   }
-}
+};
 
 // A row of `columns` values shared by LANES lanes, lane l's chunk c (of 8 values). VEC: neighbouring values in 16-byte
 // loads (the row is 16-byte aligned, its length a multiple of 8); else values LANES apart, so that a wavefront's lanes still
-// touch neighbouring values. What lies past the end reads as 0 and is not written.
+// touch neighbouring values. What lies past the end reads as 0 and is not written. NT: past the caches.
 template <typename T, int LANES, bool VEC>
 struct Row {
   using Held = typename T::Held;
+  using Raw = Raw8<T>;
   static __device__ __forceinline__ int column(int lane, int c, int j) {
     return VEC ? (c * LANES + lane) * 8 + j : (c * 8 + j) * LANES + lane;
   }
-  static __device__ __forceinline__ void load(const Held* p, int columns, int lane, int c, float (&v)[8]) {
+  template <bool NT = false>
+  static __device__ __forceinline__ Raw fetch(const Held* p, int columns, int lane, int c) {
+    Raw r = {};
     if constexpr (VEC) {
       const int at = column(lane, c, 0);
       if (at < columns) {
-        load8<T>(p + at, v);
-      } else {
+        const v4i* src = reinterpret_cast<const v4i*>(p + at);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        for (int i = 0; i < Raw::kWords; ++i) r.w[i] = NT ? __builtin_nontemporal_load(src + i) : src[i];
       }
     } else {
+      typedef Held v8x __attribute__((ext_vector_type(8)));
+      v8x h = {};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int at = column(lane, c, j);
-        v[j] = at < columns ? T::wide(p[at]) : 0.0f;
+        if (at < columns) h[j] = p[at];
       }
+      r = __builtin_bit_cast(Raw, h);
     }
+    return r;
+  }
+  static __device__ __forceinline__ void load(const Held* p, int columns, int lane, int c, float (&v)[8]) {
+    fetch(p, columns, lane, c).widen(v);
   }
   static __device__ __forceinline__ void store(Held* p, int columns, int lane, int c, const float (&v)[8]) {
     if constexpr (VEC) {
       const int at = column(lane, c, 0);
-      if (at < columns) store8<T>(p + at, v);
+      Raw r;
+      r.narrow(v);
+      if (at < columns)
+#pragma unroll
+        for (int i = 0; i < Raw::kWords; ++i) reinterpret_cast<v4i*>(p + at)[i] = r.w[i];
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -111,10 +118,25 @@ struct Row {
 // The sums of v over the wavefront, in every lane; one order of additions
 template <int N>
 __device__ __forceinline__ void wave_sum(float (&v)[N]) {
+  // within a row of 16 lanes by cross-lane operands, then across rows and halves by swaps
+  auto dpp = [&](auto ctrl) {
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1)
+    for (int i = 0; i < N; ++i)
+      v[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[i]), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  dpp(std::integral_constant<int, 0xb1>{});   // lanes 1 0 3 2 of four
+  dpp(std::integral_constant<int, 0x4e>{});   // lanes 2 3 0 1 of four
+  dpp(std::integral_constant<int, 0x141>{});  // the half row reversed
+  dpp(std::integral_constant<int, 0x140>{});  // the row reversed
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d);
+  for (int i = 0; i < N; ++i) {
+    const uint32_t u = __float_as_uint(v[i]);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float s = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const uint32_t t = __float_as_uint(s);
+    const auto q = __builtin_amdgcn_permlane32_swap(t, t, false, false);
+    v[i] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+  }
 }
 // The sums of v over LANES lanes that share a row. part: LDS of LANES / 64 x N floats, not used again before a barrier
 // (callers alternate between two).

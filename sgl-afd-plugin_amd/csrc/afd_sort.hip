@@ -285,7 +285,9 @@ __device__ __forceinline__ int64_t position_of(const Back& p, int64_t i) {
   return at < p.num_rows ? at : -1;
 }
 
-// A wavefront (L 64) or a workgroup (L 256) a token
+// A wavefront (L 64) or a workgroup (L 256) a token, kBatch of its rows on their way at once. Rows are read once: past the
+// caches.
+constexpr int kBatch = 8;
 template <typename T, int L, bool VEC>
 __global__ __launch_bounds__(256) void back_kernel(Back p) {
   using R = Row<T, L, VEC>;
@@ -296,26 +298,35 @@ __global__ __launch_bounds__(256) void back_kernel(Back p) {
   const Held* rows = static_cast<const Held*>(p.rows);
   for (int c = 0; c * L * 8 < p.columns; ++c) {
     float acc[8] = {};
-#pragma unroll 4
-    for (int j = 0; j < p.topk; ++j) {
-      const int64_t at = position_of(p, t * p.topk + j);
-      if (at < 0) continue;
-      const float w = p.w ? p.w[t * p.topk + j] : 1.0f;
-      float v[8];
-      R::load(rows + at * p.ld, p.columns, lane, c, v);
+    for (int j0 = 0; j0 < p.topk; j0 += kBatch) {
+      typename R::Raw raw[kBatch];
+      float w[kBatch];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+      for (int j = 0; j < kBatch; ++j) {
+        const int64_t i = t * p.topk + min(j0 + j, p.topk - 1), at = j0 + j < p.topk ? position_of(p, i) : -1;
+        w[j] = at < 0 ? 0.0f : p.w ? p.w[i] : 1.0f;
+        raw[j] = {};
+        if (at >= 0) raw[j] = R::template fetch<true>(rows + at * p.ld, p.columns, lane, c);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        float v[8];
+        raw[j].widen(v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = __builtin_fmaf(w[j], v[q], acc[q]);
+      }
     }
     R::store(static_cast<Held*>(p.out) + t * p.columns, p.columns, lane, c, acc);
   }
 }
 
-// The gradient of the rows and the weights, a token at a time
+// The gradient of the rows and the weights, a token at a time: its row of g is read for each batch of its pairs (once where
+// there are no more), the pairs' rows once
 template <typename T, int L, bool VEC>
 __global__ __launch_bounds__(256) void back_grad_kernel(Back p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
-  __shared__ float part[2][4];
+  __shared__ float part[2][4 * kBatch];
   const int64_t t = int64_t(blockIdx.x) * (256 / L) + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
   if (t >= p.n) return;
   const int lane = threadIdx.x & (L - 1);
@@ -323,31 +334,47 @@ __global__ __launch_bounds__(256) void back_grad_kernel(Back p) {
   const Held* g = static_cast<const Held*>(p.g) + t * p.columns;
   Held* d_rows = static_cast<Held*>(p.d_rows);
   int turn = 0;  // of the LDS that the sums meet in
-  for (int j = 0; j < p.topk; ++j) {
-    const int64_t i = t * p.topk + j, at = position_of(p, i);
-    if (at < 0) {
-      if (p.d_w && lane == 0) p.d_w[i] = 0.0f;
-      continue;
+  for (int j0 = 0; j0 < p.topk; j0 += kBatch) {
+    int64_t at[kBatch];
+    float w[kBatch], dot[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t i = t * p.topk + min(j0 + j, p.topk - 1);
+      at[j] = j0 + j < p.topk ? position_of(p, i) : -1;
+      w[j] = p.w ? p.w[i] : 1.0f;
+      dot[j] = 0.0f;
     }
-    const float w = p.w ? p.w[i] : 1.0f;
-    float dot[1] = {0.0f};
     for (int c = 0; c * L * 8 < p.columns; ++c) {
-      float go[8], v[8];
-      R::load(g, p.columns, lane, c, go);
-      if (p.d_w) {
-        R::load(rows + at * p.ld, p.columns, lane, c, v);
+      float go[8];
+      typename R::Raw raw[kBatch];
+      const typename R::Raw g_raw = R::fetch(g, p.columns, lane, c);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) dot[0] = __builtin_fmaf(go[q], v[q], dot[0]);
+      for (int j = 0; j < kBatch; ++j) {
+        raw[j] = {};
+        if (p.d_w && at[j] >= 0) raw[j] = R::template fetch<true>(rows + at[j] * p.ld, p.columns, lane, c);
       }
-      if (p.d_rows) {
+      g_raw.widen(go);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = w * go[q];
-        R::store(d_rows + at * p.columns, p.columns, lane, c, v);
+      for (int j = 0; j < kBatch; ++j) {
+        if (at[j] < 0) continue;
+        float v[8];
+        if (p.d_w) {
+          raw[j].widen(v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) dot[j] = __builtin_fmaf(go[q], v[q], dot[j]);
+        }
+        if (p.d_rows) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = w[j] * go[q];
+          R::store(d_rows + at[j] * p.columns, p.columns, lane, c, v);
+        }
       }
     }
     if (p.d_w) {
       row_sum<L>(dot, part[turn ^= 1], lane);
-      if (lane == 0) p.d_w[i] = dot[0];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (lane == 0 && j0 + j < p.topk) p.d_w[t * p.topk + j0 + j] = at[j] < 0 ? 0.0f : dot[j];
     }
   }
   // rows that no pair has

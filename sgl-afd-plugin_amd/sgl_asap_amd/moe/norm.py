@@ -77,10 +77,9 @@ class _Norm(torch.autograd.Function):
         if w_post is not None or w_next is not None:
             rstd = torch.empty(2, n, dtype=torch.float32, device=residual.device)
         hidden, normed = _forward(cfg, y, residual, w_post, gate, w_next, rstd)
-        h = (residual if y is None else hidden) if w_next is not None else None
-        # y itself is read for its norm's gradient and the gate's
-        held = y if w_post is not None or gate is not None and ctx.needs_input_grad[3] else None
-        ctx.save_for_backward(held, h, w_post, gate, w_next, rstd)
+        # the residual and y are read to make hidden again, y for its norm's gradient and the gate's too
+        held = y if w_next is not None or w_post is not None or gate is not None and ctx.needs_input_grad[3] else None
+        ctx.save_for_backward(held, residual if w_next is not None else None, w_post, gate, w_next, rstd)
         ctx.cfg, ctx.kind, ctx.shape, ctx.has_y = cfg, kind, tuple(residual.shape), y is not None
         ctx.set_materialize_grads(False)
         if y is None:
@@ -89,12 +88,12 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        y, h, w_post, gate, w_next, rstd = ctx.saved_tensors
+        y, residual, w_post, gate, w_next, rstd = ctx.saved_tensors
         dh, dn = (grads + (None,))[:2] if ctx.has_y else (None, grads[0])
         none = (None,) * 7
         if dh is None and dn is None:
             return none
-        made_from = (dh, dn, y, h, w_post, gate, w_next)
+        made_from = (dh, dn, y, residual, w_post, gate, w_next)
         g = dh if dh is not None else dn
         (n, columns), dev = ctx.shape, g.device
         dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
@@ -108,11 +107,11 @@ class _Norm(torch.autograd.Function):
                                   for t, need in ((w_post, need_post), (gate, need_gate), (w_next, need_next)))
         if n:
             y, ldy = (None, 0) if y is None else matrix_rows(y)
-            h, ldh = (None, 0) if h is None else matrix_rows(h)
+            residual, ldr = (None, 0) if residual is None else matrix_rows(residual)
             sums = d_post is not None or d_next is not None or d_gate is not None and ctx.kind == GATE_CHANNEL
             size = _workspace_bytes(columns, n) if sums else 0
             ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            launch("afd_residual_norm_grad", dev, ctx.cfg, _ptr(y), ldy, _ptr(h), ldh, _ptr(w_post), _ptr(gate), _ptr(w_next),
+            launch("afd_residual_norm_grad", dev, ctx.cfg, _ptr(y), ldy, _ptr(residual), ldr, _ptr(w_post), _ptr(gate), _ptr(w_next),
                    _ptr(rstd), n, _ptr(dh), _ptr(dn), _ptr(d_res), _ptr(d_y), _ptr(d_gate), _ptr(d_post), _ptr(d_next),
                    ws.data_ptr(), size)
         out = (d_y, d_res, d_post, d_gate, d_next)

@@ -53,13 +53,13 @@ def forward(d, post, nxt, scale):
 
 
 def backward(d, post, nxt, scale, dh=True, dn=True):
-    """{name: gradient with bounds}; h is read as it was rounded."""
+    """{name: gradient with bounds}; h as it is before it is rounded."""
     dtype, out = d["y"].dtype, {}
-    h, held, _ = forward(d, post, nxt, scale)
+    h = forward(d, post, nxt, scale)[0]
     g = Bounded(torch.zeros_like(d["y"])) if not dh else Bounded(d["dh"])
     if nxt and dn:
         r = unit(h)[1]
-        u = held * r
+        u = h * r
         q = Bounded(d["dn"]) * Bounded(d["next"])
         out["next"] = (Bounded(d["dn"]) * u).sum(0).held(d["next"].dtype)
         g = g + r * (q - u * (q * u).mean())
@@ -302,8 +302,12 @@ def test_derivatives_that_are_refused():
             with pytest.raises(NotImplementedError):
                 call()
     out = residual_norm(y, res, next_weight=w_next)
+    out.hidden.detach().add_(1.0)  # (not what the backward reads)
+    (before,) = torch.autograd.grad(out.normed, y, y.detach(), retain_graph=True)
+    (after,) = torch.autograd.grad(residual_norm(y, res, next_weight=w_next).normed, y, y.detach())
+    assert torch.equal(before, after)
     with torch.no_grad():
-        out.hidden.add_(1.0)  # what the backward reads
+        res.add_(1.0)
     with pytest.raises(RuntimeError, match="inplace"):
         out.normed.sum().backward()
 

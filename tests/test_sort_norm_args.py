@@ -95,7 +95,7 @@ def test_norm_calls():
     assert grad(dh=None, dn=None, d_next=None) == ARG and grad(h=None) == ARG and grad(nxt=None) == ARG and grad(rstd=None) == ARG
     assert grad(dn=None) == ARG  # d_next without dn
     assert grad(d_post=16) == ARG and grad(d_gate=16) == ARG and grad(cfg(kind=1)) == ARG
-    assert grad(y=None, post=16) == ARG and grad(cfg(kind=1), y=None, gate=16, d_gate=16) == ARG
+    assert grad(y=None, post=16) == ARG and grad(y=None) == ARG and grad(cfg(kind=1), y=None, gate=16, d_gate=16) == ARG
     assert grad(ldy=63) == SHAPE and grad(ldh=63) == SHAPE
     assert grad(ws=None) == WS and grad(size=16) == WS and grad(ws=24) == WS
 

@@ -41,8 +41,8 @@ struct Args {
   // the gradient's
   const void *dh, *dn;
   void *d_res, *d_y, *d_gate;
-  float* sums;  // [slots][3][columns]: of w_next, w_post, the channels' gate
-  bool sum_next, sum_post, sum_gate;
+  float* sums;  // [slots][2][columns]: of w_next, of w_post and the channels' gate
+  bool sum_next, sum_block;
   bool block;  // anything that belongs to y is wanted
 };
 
@@ -145,27 +145,42 @@ __global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
 }
 
 // Slot s (of gridDim.x kRows) takes every slots-th row, the next one's values on their way while it works on one. The
-// parameters stay in registers, and so do the slot's sums over its rows.
+// slot's sums over its rows stay in registers, and so do the parameters: w_next and k = scale w_post (the channels' gate).
+// With g the row's or the element's gate (1 without) everything of the block goes through k and one sum,
+//
+//   h = residual + g k v,   q = g k d,   a = sum_t g d v
+//   d w_post = scale (the channels' gate) a,   the channels' d gate = scale w_post a,   others': k d v, or its sum over the row
+//
+// 18 operations a value and 16 registers of sums for 8 columns, so that 16 wavefronts fit a CU.
 template <typename T, int L, int NC, bool VEC>
-__global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
+__global__ __launch_bounds__(kThreads<L>) __attribute__((amdgpu_waves_per_eu(sizeof(typename T::Held) == 2 && VEC ? 4 : 2))) void
+backward_kernel(Args p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
-  __shared__ float part[2][2 * (L / 64)];
+  __shared__ float part[2][L / 64];
   const int64_t slot = first_row<L>(), slots = int64_t(gridDim.x) * kRows<L>;
   const int lane = threadIdx.x & (L - 1), columns = p.columns;
   const float inv = 1.0f / static_cast<float>(columns);
   int turn = 0;  // of the LDS that a row's sums meet in
-  const bool element = p.gate_kind == AFD_GATE_ELEMENT, channel = p.gate_kind == AFD_GATE_CHANNEL;
-  const bool token = p.gate_kind == AFD_GATE_TOKEN;
-  float sum_next[NC][8] = {}, sum_post[NC][8] = {}, sum_gate[NC][8] = {};
-  float w_next[NC][8], w_post[NC][8], gate[NC][8];
+  const bool element = p.gate_kind == AFD_GATE_ELEMENT, token = p.gate_kind == AFD_GATE_TOKEN;
+  float sum_next[NC][8] = {}, sum_block[NC][8] = {};
+  float w_next[NC][8], k[NC][8];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w_next[c][j] = w_post[c][j] = gate[c][j] = 1.0f;
     if (p.dn) load_param<T, L, VEC>(p.w_next, p.wide_next, 0, columns, lane, c, w_next[c]);
-    if (p.post) load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w_post[c]);
-    if (channel) load_param<T, L, VEC>(p.gate, p.wide_gate, 0, columns, lane, c, gate[c]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[c][j] = p.scale;
+    float w[8];
+    if (p.post) {
+      load_param<T, L, VEC>(p.w_post, p.wide_post, 0, columns, lane, c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[c][j] *= w[j];
+    }
+    if (p.gate_kind == AFD_GATE_CHANNEL) {
+      load_param<T, L, VEC>(p.gate, p.wide_gate, 0, columns, lane, c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[c][j] *= w[j];
+    }
   }
   // what a row needs
   struct In {
@@ -187,14 +202,22 @@ __global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
     in.r_h = p.dn ? p.rstd[int64_t(p.n) + t] : 0.0f;
     return in;
   };
-  In next = fetch(slot);
+  constexpr bool kAhead = NC == 1;  // (two chunks a lane leave no registers for another row)
+  In next = {};
+  if constexpr (kAhead) next = fetch(slot);
   for (int64_t t = slot; t < p.n; t += slots) {
-    const In in = next;
-    next = fetch(t + slots);
-    const float s = p.scale * in.gate;
-    if (element)
+    const In in = kAhead ? next : fetch(t);
+    if constexpr (kAhead) next = fetch(t + slots);
+    float g[NC][8];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) load_param<T, L, VEC>(p.gate, p.wide_gate, t * columns, columns, lane, c, gate[c]);
+    for (int c = 0; c < NC; ++c) {
+      if (element) {
+        load_param<T, L, VEC>(p.gate, p.wide_gate, t * columns, columns, lane, c, g[c]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[c][j] = in.gate;
+      }
+    }
     // v: rms(y), or y (0 where it is not needed)
     float d[NC][8], v[NC][8];
 #pragma unroll
@@ -205,18 +228,18 @@ __global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
       for (int j = 0; j < 8; ++j) v[c][j] *= in.r_y;
     }
     if (p.dn) {
-      float u[NC][8], g[NC][8], dot[1] = {0.0f};
+      float u[NC][8], e[NC][8], dot[1] = {0.0f};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         in.res[c].widen(u[c]);
-        in.dn[c].widen(g[c]);
+        in.dn[c].widen(e[c]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (p.y) u[c][j] = __builtin_fmaf(element || channel ? gate[c][j] * s : s, v[c][j] * w_post[c][j], u[c][j]);
+          if (p.y) u[c][j] = __builtin_fmaf(g[c][j] * k[c][j], v[c][j], u[c][j]);
           u[c][j] *= in.r_h;
-          sum_next[c][j] = __builtin_fmaf(g[c][j], u[c][j], sum_next[c][j]);
-          g[c][j] *= w_next[c][j];
-          dot[0] = __builtin_fmaf(g[c][j], u[c][j], dot[0]);
+          sum_next[c][j] = __builtin_fmaf(e[c][j], u[c][j], sum_next[c][j]);
+          e[c][j] *= w_next[c][j];
+          dot[0] = __builtin_fmaf(e[c][j], u[c][j], dot[0]);
         }
       }
       row_sum<L>(dot, part[turn ^= 1], lane);
@@ -224,45 +247,50 @@ __global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[c][j] = __builtin_fmaf(in.r_h, __builtin_fmaf(-mean, u[c][j], g[c][j]), d[c][j]);
+        for (int j = 0; j < 8; ++j) d[c][j] = __builtin_fmaf(in.r_h, __builtin_fmaf(-mean, u[c][j], e[c][j]), d[c][j]);
     }
     if (p.d_res)
 #pragma unroll
       for (int c = 0; c < NC; ++c) R::store(static_cast<Held*>(p.d_res) + t * columns, columns, lane, c, d[c]);
     if (!p.block) continue;
-    // d becomes q. dots: of q and v, of d and the normed y (the token's gate)
-    float dots[2] = {0.0f, 0.0f};
+    // d becomes q; dot: of q and v (an element's gate), else of k d and v
+    float dot[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float f = v[c][j] * w_post[c][j];
-        e[j] = p.scale * d[c][j] * f;
-        dots[1] = __builtin_fmaf(d[c][j], f, dots[1]);
-        sum_gate[c][j] += e[j];
-        d[c][j] *= element || channel ? gate[c][j] * s : s;
-        sum_post[c][j] = __builtin_fmaf(d[c][j], v[c][j], sum_post[c][j]);
-        d[c][j] *= w_post[c][j];
-        dots[0] = __builtin_fmaf(d[c][j], v[c][j], dots[0]);
-      }
-      if (element && p.d_gate) {
-        if (p.wide_gate)
-          Row<F32, L, VEC>::store(static_cast<float*>(p.d_gate) + t * columns, columns, lane, c, e);
-        else
-          R::store(static_cast<Held*>(p.d_gate) + t * columns, columns, lane, c, e);
+      for (int j = 0; j < 8; ++j) sum_block[c][j] = __builtin_fmaf(element || token ? g[c][j] * d[c][j] : d[c][j], v[c][j], sum_block[c][j]);
+      if (element) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = k[c][j] * d[c][j] * v[c][j];
+          d[c][j] *= k[c][j] * g[c][j];
+          dot[0] = __builtin_fmaf(d[c][j], v[c][j], dot[0]);
+        }
+        if (p.d_gate) {
+          if (p.wide_gate)
+            Row<F32, L, VEC>::store(static_cast<float*>(p.d_gate) + t * columns, columns, lane, c, e);
+          else
+            R::store(static_cast<Held*>(p.d_gate) + t * columns, columns, lane, c, e);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d[c][j] *= k[c][j];
+          dot[0] = __builtin_fmaf(d[c][j], v[c][j], dot[0]);
+          d[c][j] *= in.gate;
+        }
       }
     }
-    if (p.post || (token && p.d_gate)) row_sum<L>(dots, part[turn ^= 1], lane);
+    if (p.post || (token && p.d_gate)) row_sum<L>(dot, part[turn ^= 1], lane);
     if (token && p.d_gate && lane == 0) {
-      const float e = p.scale * dots[1];
       if (p.wide_gate)
-        static_cast<float*>(p.d_gate)[t] = e;
+        static_cast<float*>(p.d_gate)[t] = dot[0];
       else
-        static_cast<Held*>(p.d_gate)[t] = T::held(e);
+        static_cast<Held*>(p.d_gate)[t] = T::held(dot[0]);
     }
     if (p.d_y) {
-      const float mean = dots[0] * inv;
+      const float mean = dot[0] * inv * in.gate;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         if (p.post)  // (without, an infinite y leaves its gradient as it is)
@@ -272,42 +300,48 @@ __global__ __launch_bounds__(kThreads<L>) void backward_kernel(Args p) {
       }
     }
   }
-  float* sums = p.sums + slot * 3 * columns;
+  float* sums = p.sums + slot * 2 * columns;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     if (p.sum_next) Row<F32, L, VEC>::store(sums, columns, lane, c, sum_next[c]);
-    if (p.sum_post) Row<F32, L, VEC>::store(sums + columns, columns, lane, c, sum_post[c]);
-    if (p.sum_gate) Row<F32, L, VEC>::store(sums + 2 * columns, columns, lane, c, sum_gate[c]);
+    if (p.sum_block) Row<F32, L, VEC>::store(sums + columns, columns, lane, c, sum_block[c]);
   }
 }
 
-// The slots' sums, 64 columns a workgroup
+// The slots' sums, 64 columns a workgroup: d w_next, and d w_post and the channels' d gate from one sum
 struct Finish {
   const float* sums;
   int32_t slots, columns;
-  void* out[3];
-  bool wide[3];
+  float scale;
+  const void *w_post, *gate;  // null: 1
+  bool wide_next, wide_post, wide_gate;
+  void *d_next, *d_post, *d_gate;
 };
 constexpr int kFinishWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(64 * kFinishWaves) void finish_kernel(Finish p) {
   __shared__ float part[kFinishWaves][64];
-  const int which = blockIdx.y;
-  if (!p.out[which]) return;
+  const bool block = blockIdx.y == 1;
+  if (block ? !p.d_post && !p.d_gate : !p.d_next) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
   float sum = 0.0f;
   if (col < p.columns)
 #pragma unroll 8
-    for (int s = w; s < p.slots; s += kFinishWaves) sum += p.sums[(int64_t(s) * 3 + which) * p.columns + col];
+    for (int s = w; s < p.slots; s += kFinishWaves) sum += p.sums[(int64_t(s) * 2 + block) * p.columns + col];
   part[w][lane] = sum;
   __syncthreads();
-  if (w == 0 && col < p.columns) {
-    for (int i = 1; i < kFinishWaves; ++i) sum += part[i][lane];
-    if (p.wide[which])
-      static_cast<float*>(p.out[which])[col] = sum;
+  if (w != 0 || col >= p.columns) return;
+  for (int i = 1; i < kFinishWaves; ++i) sum += part[i][lane];
+  auto store = [&](void* to, bool wide, float v) {
+    if (wide)
+      static_cast<float*>(to)[col] = v;
     else
-      static_cast<typename T::Held*>(p.out[which])[col] = T::held(sum);
-  }
+      static_cast<typename T::Held*>(to)[col] = T::held(v);
+  };
+  if (!block) return store(p.d_next, p.wide_next, sum);
+  sum *= p.scale;
+  if (p.d_post) store(p.d_post, p.wide_post, p.gate ? sum * load_one<T>(p.gate, p.wide_gate, col) : sum);
+  if (p.d_gate) store(p.d_gate, p.wide_gate, p.w_post ? sum * load_one<T>(p.w_post, p.wide_post, col) : sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -399,7 +433,7 @@ extern "C" int afd_residual_norm_workspace(const afd_norm_cfg* cfg, int32_t n, u
   const int st = norm::check(cfg, n);
   if (st != AFD_OK) return st;
   if (!bytes) return AFD_ERR_ARG;
-  *bytes = uint64_t(norm::slots_of(n, cfg->columns)) * 3 * cfg->columns * 4;
+  *bytes = uint64_t(norm::slots_of(n, cfg->columns)) * 2 * cfg->columns * 4;
   return AFD_OK;
 }
 
@@ -443,8 +477,7 @@ extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, in
   p.d_gate = kind == AFD_GATE_CHANNEL ? nullptr : d_gate;
   p.sums = static_cast<float*>(ws);
   p.sum_next = d_next != nullptr;
-  p.sum_post = d_post != nullptr;
-  p.sum_gate = kind == AFD_GATE_CHANNEL && d_gate;
+  p.sum_block = d_post || (kind == AFD_GATE_CHANNEL && d_gate);
   p.block = d_y || d_post || d_gate;
   const int fmt = cfg->fmt;
   bool vec = norm::aligned_params(p, fmt);
@@ -468,13 +501,16 @@ extern "C" int afd_residual_norm_grad(const afd_norm_cfg* cfg, const void* y, in
       f.sums = p.sums;
       f.slots = norm::slots_of(n, p.columns);
       f.columns = p.columns;
-      f.out[0] = d_next;
-      f.out[1] = d_post;
-      f.out[2] = kind == AFD_GATE_CHANNEL ? d_gate : nullptr;
-      f.wide[0] = cfg->next_f32;
-      f.wide[1] = cfg->post_f32;
-      f.wide[2] = cfg->gate_f32;
-      hipLaunchKernelGGL(norm::finish_kernel<T>, dim3((p.columns + 63) / 64, 3), dim3(64 * norm::kFinishWaves), 0, s, f);
+      f.scale = p.scale;
+      f.w_post = w_post;
+      f.gate = kind == AFD_GATE_CHANNEL ? gate : nullptr;
+      f.wide_next = p.wide_next;
+      f.wide_post = p.wide_post;
+      f.wide_gate = p.wide_gate;
+      f.d_next = d_next;
+      f.d_post = d_post;
+      f.d_gate = kind == AFD_GATE_CHANNEL ? d_gate : nullptr;
+      hipLaunchKernelGGL(norm::finish_kernel<T>, dim3((p.columns + 63) / 64, 2), dim3(64 * norm::kFinishWaves), 0, s, f);
       AFD_CHECK_LAUNCH();
     }
     return AFD_OK;

@@ -285,39 +285,38 @@ __device__ __forceinline__ int64_t position_of(const Back& p, int64_t i) {
   return at < p.num_rows ? at : -1;
 }
 
-// A wavefront (L 64) or a workgroup (L 256) a token, kBatch of its rows on their way at once. Rows are read once: past the
-// caches.
+// A wavefront a token's 512 columns, kBatch of its rows on their way at once; rows are read once: past the caches. No
+// loop over the columns, so that many short wavefronts keep loads on their way whatever share of the pairs is here.
 constexpr int kBatch = 8;
-template <typename T, int L, bool VEC>
-__global__ __launch_bounds__(256) void back_kernel(Back p) {
-  using R = Row<T, L, VEC>;
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void back_kernel(Back p, uint32_t chunks) {
+  using R = Row<T, 64, VEC>;
   using Held = typename T::Held;
-  const int64_t t = int64_t(blockIdx.x) * (256 / L) + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const uint64_t item = uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = static_cast<int64_t>(item / chunks);
   if (t >= p.n) return;
-  const int lane = threadIdx.x & (L - 1);
+  const int c = static_cast<int>(item % chunks), lane = threadIdx.x & 63;
   const Held* rows = static_cast<const Held*>(p.rows);
-  for (int c = 0; c * L * 8 < p.columns; ++c) {
-    float acc[8] = {};
-    for (int j0 = 0; j0 < p.topk; j0 += kBatch) {
-      typename R::Raw raw[kBatch];
-      float w[kBatch];
+  float acc[8] = {};
+  for (int j0 = 0; j0 < p.topk; j0 += kBatch) {
+    typename R::Raw raw[kBatch];
+    float w[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int64_t i = t * p.topk + min(j0 + j, p.topk - 1), at = j0 + j < p.topk ? position_of(p, i) : -1;
-        w[j] = at < 0 ? 0.0f : p.w ? p.w[i] : 1.0f;
-        raw[j] = {};
-        if (at >= 0) raw[j] = R::template fetch<true>(rows + at * p.ld, p.columns, lane, c);
-      }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        float v[8];
-        raw[j].widen(v);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] = __builtin_fmaf(w[j], v[q], acc[q]);
-      }
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t i = t * p.topk + min(j0 + j, p.topk - 1), at = j0 + j < p.topk ? position_of(p, i) : -1;
+      w[j] = at < 0 ? 0.0f : p.w ? p.w[i] : 1.0f;
+      raw[j] = {};
+      if (at >= 0) raw[j] = R::template fetch<true>(rows + at * p.ld, p.columns, lane, c);
     }
-    R::store(static_cast<Held*>(p.out) + t * p.columns, p.columns, lane, c, acc);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      float v[8];
+      raw[j].widen(v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] = __builtin_fmaf(w[j], v[q], acc[q]);
+    }
   }
+  R::store(static_cast<Held*>(p.out) + t * p.columns, p.columns, lane, c, acc);
 }
 
 // The gradient of the rows and the weights, a token at a time: its row of g is read for each batch of its pairs (once where
@@ -504,9 +503,18 @@ extern "C" int afd_unsort_tokens(int32_t fmt, const void* rows, int64_t ld, int6
   p.num_rows = num_rows;
   p.out = out;
   const bool vec = rows::aligned_rows(rows, ld, fmt) && rows::aligned_rows(out, columns, fmt) && columns % 8 == 0;
-  return sorting::with_shape(p, fmt, vec, [&](auto type, auto lanes, auto v, dim3 grid) {
-    hipLaunchKernelGGL((sorting::back_kernel<decltype(type), decltype(lanes)::value, decltype(v)::value>), grid, dim3(256), 0,
-                       static_cast<hipStream_t>(stream), p);
+  const uint32_t chunks = (columns + 511) / 512;
+  const int64_t grid = (int64_t(n) * chunks + 3) / 4;
+  if (grid > 0xffffff) return AFD_ERR_SHAPE;  // (out alone would be 34 GB of a type of two bytes)
+  return rows::with_fmt(fmt, [&](auto type) -> int {
+    using T = decltype(type);
+    const dim3 blocks(static_cast<unsigned>(grid));
+    if (vec)
+      hipLaunchKernelGGL((sorting::back_kernel<T, true>), blocks, dim3(256), 0, static_cast<hipStream_t>(stream), p, chunks);
+    else
+      hipLaunchKernelGGL((sorting::back_kernel<T, false>), blocks, dim3(256), 0, static_cast<hipStream_t>(stream), p, chunks);
+    AFD_CHECK_LAUNCH();
+    return AFD_OK;
   });
 }
 

@@ -22,7 +22,7 @@ inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; 
 struct Raw {
   uint32_t u[2][8];
 };
-// VEC: rows take 16-byte loads and k_in is a multiple of 16 (then a chunk is whole or missing). p: the
+// VEC: rows are 16-byte aligned and k_in is a multiple of 16 (then a chunk is whole or missing). p: the
 // row; c: the lane's chunk. What lies past k_in reads as 0.
 template <bool VEC, bool NT = false>
 __device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int c) {
@@ -37,6 +37,13 @@ __device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int 
       for (int i = 0; i < 4; ++i) {
         r.u[h][i] = k0 < k_in ? lo[i] : 0;
         r.u[h][4 + i] = k0 < k_in ? hi[i] : 0;
+      }
+    } else if (k0 + 16 <= k_in) {
+      const v4i lo = load_words<false>(p + k0), hi = load_words<false>(p + k0 + 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r.u[h][i] = lo[i];
+        r.u[h][4 + i] = hi[i];
       }
     } else {
 #pragma unroll

@@ -62,34 +62,28 @@ struct Raw8 {
   }
 };
 
-// A row of `columns` values shared by LANES lanes, lane l's chunk c (of 8 values). VEC: neighbouring values in 16-byte
-// loads (the row is 16-byte aligned, its length a multiple of 8); else values LANES apart, so that a wavefront's lanes still
-// touch neighbouring values. What lies past the end reads as 0 and is not written. NT: past the caches.
+// A row of `columns` values shared by LANES lanes, lane l's chunk c: eight neighbouring values from (c LANES + l) 8 on. VEC: the
+// row is 16-byte aligned and its length a multiple of 8; else its whole chunks are read and written at the alignment they
+// have, and the last one value by value. Either way a lane holds the same values, so results do not depend on
+// it. What lies past the end reads as 0 and is not written. NT: past the caches.
 template <typename T, int LANES, bool VEC>
 struct Row {
   using Held = typename T::Held;
   using Raw = Raw8<T>;
-  static __device__ __forceinline__ int column(int lane, int c, int j) {
-    return VEC ? (c * LANES + lane) * 8 + j : (c * 8 + j) * LANES + lane;
-  }
+  static __device__ __forceinline__ int column(int lane, int c) { return (c * LANES + lane) * 8; }
   template <bool NT = false>
   static __device__ __forceinline__ Raw fetch(const Held* p, int columns, int lane, int c) {
     Raw r = {};
-    if constexpr (VEC) {
-      const int at = column(lane, c, 0);
-      if (at < columns) {
-        const v4i* src = reinterpret_cast<const v4i*>(p + at);
+    const int at = column(lane, c);
+    if (VEC ? at < columns : at + 8 <= columns) {
 #pragma unroll
-        for (int i = 0; i < Raw::kWords; ++i) r.w[i] = NT ? __builtin_nontemporal_load(src + i) : src[i];
-      }
-    } else {
+      for (int i = 0; i < Raw::kWords; ++i) r.w[i] = load_words<VEC, NT>(reinterpret_cast<const char*>(p + at) + 16 * i);
+    } else if (!VEC && at < columns) {
       typedef Held v8x __attribute__((ext_vector_type(8)));
       v8x h = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = column(lane, c, j);
-        if (at < columns) h[j] = p[at];
-      }
+      for (int j = 0; j < 7; ++j)
+        if (at + j < columns) h[j] = p[at + j];
       r = __builtin_bit_cast(Raw, h);
     }
     return r;
@@ -98,19 +92,16 @@ struct Row {
     fetch(p, columns, lane, c).widen(v);
   }
   static __device__ __forceinline__ void store(Held* p, int columns, int lane, int c, const float (&v)[8]) {
-    if constexpr (VEC) {
-      const int at = column(lane, c, 0);
+    const int at = column(lane, c);
+    if (VEC ? at < columns : at + 8 <= columns) {
       Raw r;
       r.narrow(v);
-      if (at < columns)
 #pragma unroll
-        for (int i = 0; i < Raw::kWords; ++i) reinterpret_cast<v4i*>(p + at)[i] = r.w[i];
-    } else {
+      for (int i = 0; i < Raw::kWords; ++i) store_words<VEC>(reinterpret_cast<char*>(p + at) + 16 * i, r.w[i]);
+    } else if (!VEC && at < columns) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = column(lane, c, j);
-        if (at < columns) p[at] = T::held(v[j]);
-      }
+      for (int j = 0; j < 7; ++j)
+        if (at + j < columns) p[at + j] = T::held(v[j]);
     }
   }
 };

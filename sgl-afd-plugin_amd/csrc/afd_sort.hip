@@ -52,37 +52,51 @@ __device__ __forceinline__ int scan(int v, int* waves, int* total) {
 }
 
 // ---------------------------------------------------------------- moving
-// x's row t to each of its positions. Rows are moved as Units of 16, 4 or 2 bytes. A token is L lanes' work.
+// x's row t to each of its positions, 16 bytes at a time. VEC: rows are aligned and made of whole ones; else at the
+// alignment they have, with up to seven pieces of 2 bytes behind the last. A token is L lanes' work.
 struct Move {
-  const void* x;
-  void* rows;
-  int64_t ldx, ld;  // in Units
-  int32_t units, n, topk;
+  const char* x;
+  char* rows;
+  int64_t ldx, ld;  // in bytes
+  int32_t bytes, n, topk;
   int32_t behind;  // whether rows past the last pair's, up to n topk, are zeroed
 };
-template <typename Unit, int L>
+template <bool VEC, int L>
 __device__ __forceinline__ void move_token(const Move& m, int64_t t, const int* at, int lane) {
-  const Unit* from = static_cast<const Unit*>(m.x) + t * m.ldx;
-  Unit* rows = static_cast<Unit*>(m.rows);
-  for (int u = lane; u < m.units; u += L) {
-    const Unit v = from[u];
+  const char* from = m.x + t * m.ldx;
+  const int words = m.bytes / 16;
+  for (int u = lane; u < words; u += L) {
+    const v4i v = load_words<VEC>(from + 16 * u);
     for (int j = 0; j < m.topk; ++j)
-      if (at[j] >= 0) rows[at[j] * m.ld + u] = v;
+      if (at[j] >= 0) store_words<VEC>(m.rows + at[j] * m.ld + 16 * u, v);
+  }
+  if constexpr (!VEC) {
+    const int left = words * 8 + lane;  // (pieces of 2 bytes)
+    if (left < m.bytes / 2) {
+      const uint16_t v = reinterpret_cast<const uint16_t*>(from)[left];
+      for (int j = 0; j < m.topk; ++j)
+        if (at[j] >= 0) reinterpret_cast<uint16_t*>(m.rows + at[j] * m.ld)[left] = v;
+    }
   }
 }
-template <typename Unit, int L>
+template <bool VEC, int L>
 __device__ __forceinline__ void zero_behind(const Move& m, int64_t t, int total, int lane) {
   if (!m.behind) return;
-  const Unit zero = {};
-  for (int64_t r = int64_t(total) + t; r < int64_t(m.n) * m.topk; r += m.n)
-    for (int u = lane; u < m.units; u += L) static_cast<Unit*>(m.rows)[r * m.ld + u] = zero;
+  for (int64_t r = int64_t(total) + t; r < int64_t(m.n) * m.topk; r += m.n) {
+    char* row = m.rows + r * m.ld;
+    for (int u = lane; u < m.bytes / 16; u += L) store_words<VEC>(row + 16 * u, v4i{0, 0, 0, 0});
+    if constexpr (!VEC) {
+      const int left = m.bytes / 16 * 8 + lane;
+      if (left < m.bytes / 2) reinterpret_cast<uint16_t*>(row)[left] = 0;
+    }
+  }
 }
 
 // Few pairs: one launch. A workgroup for each token and one more: each reads all pairs' ids (at most 16 a lane) and
 // counts the pairs before its own: a pair's key is (expert, pair), and its position the number of smaller keys. The one more writes
 // the tables.
 constexpr int kFewThreads = 256, kFewEach = 16, kFewPairs = kFewThreads * kFewEach;
-template <typename Unit>
+template <bool VEC>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(Pairs p, Move m) {
   constexpr int kWaves = kFewThreads / 64;
   __shared__ int part[kWaves][kMaxTopk + 1];
@@ -148,8 +162,8 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(Pairs p, Move m) {
   int total = 0;
   for (int i = 0; i < kWaves; ++i) total += part[i][m.topk];
   __syncthreads();
-  move_token<Unit, kFewThreads>(m, token, at, t);
-  zero_behind<Unit, kFewThreads>(m, token, total, t);
+  move_token<VEC, kFewThreads>(m, token, at, t);
+  zero_behind<VEC, kFewThreads>(m, token, total, t);
 }
 
 // Many pairs: chunks of a multiple of 1024, at most kMaxChunks. Each chunk's counts by expert, then each chunk's
@@ -254,14 +268,14 @@ __global__ __launch_bounds__(kChunk) void place_kernel(Pairs p, int chunk, const
 }
 
 // A wavefront a token
-template <typename Unit>
+template <bool VEC>
 __global__ __launch_bounds__(256) void move_kernel(Move m, const int32_t* __restrict__ positions,
                                                    const int32_t* __restrict__ total) {
   const int64_t t = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= m.n) return;
   const int lane = threadIdx.x & 63;
-  move_token<Unit, 64>(m, t, positions + t * m.topk, lane);
-  if (m.behind) zero_behind<Unit, 64>(m, t, *total, lane);
+  move_token<VEC, 64>(m, t, positions + t * m.topk, lane);
+  if (m.behind) zero_behind<VEC, 64>(m, t, *total, lane);
 }
 
 // ---------------------------------------------------------------- back
@@ -391,42 +405,22 @@ static int check(int32_t n, int32_t topk, int32_t fmt, int32_t columns) {
   return known_fmt(fmt) ? AFD_OK : AFD_ERR_UNSUPPORTED;
 }
 
-// f(Unit{}, units in a value): the widest unit that x and the rows are made of
-template <typename F>
-static int with_unit(const void* x, int64_t ldx, const void* rows, int64_t ld, int32_t columns, int32_t fmt, F f) {
-  const int size = value_size(fmt);
-  auto fits = [&](int bytes) {
-    return (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) % bytes == 0 && ldx * size % bytes == 0 &&
-           ld * size % bytes == 0 && int64_t(columns) * size % bytes == 0;
-  };
-  if (fits(16)) return f(v4i{}, 16);
-  if (fits(4)) return f(uint32_t{}, 4);
-  return f(uint16_t{}, 2);
-}
-
-static int sort(const Pairs& p, const Move& m0, int32_t fmt, int32_t columns, int32_t* hist, hipStream_t s) {
-  return with_unit(m0.x, m0.ldx, m0.rows, m0.ld, columns, fmt, [&](auto unit, int bytes) -> int {
-    using Unit = decltype(unit);
-    const int size = value_size(fmt);
-    Move m = m0;
-    m.ldx = m.ldx * size / bytes;
-    m.ld = m.ld * size / bytes;
-    m.units = static_cast<int32_t>(int64_t(columns) * size / bytes);
-    if (p.pairs <= kFewPairs) {
-      hipLaunchKernelGGL(few_kernel<Unit>, dim3(m.n + 1), dim3(kFewThreads), 0, s, p, m);
-      AFD_CHECK_LAUNCH();
-      return AFD_OK;
-    }
-    const int chunk = chunk_of(p.pairs);
-    const dim3 chunks(static_cast<unsigned>((int64_t(p.pairs) + chunk - 1) / chunk));
-    hipLaunchKernelGGL(count_kernel, chunks, dim3(kChunk), 0, s, p, chunk, hist);
-    AFD_CHECK_LAUNCH();
-    hipLaunchKernelGGL(place_kernel, chunks, dim3(kChunk), 0, s, p, chunk, hist);
-    AFD_CHECK_LAUNCH();
-    hipLaunchKernelGGL(move_kernel<Unit>, dim3((m.n + 3) / 4), dim3(256), 0, s, m, p.positions, p.offsets + p.experts);
+template <bool VEC>
+static int launch_sort(const Pairs& p, const Move& m, int32_t* hist, hipStream_t s) {
+  if (p.pairs <= kFewPairs) {
+    hipLaunchKernelGGL(few_kernel<VEC>, dim3(m.n + 1), dim3(kFewThreads), 0, s, p, m);
     AFD_CHECK_LAUNCH();
     return AFD_OK;
-  });
+  }
+  const int chunk = chunk_of(p.pairs);
+  const dim3 chunks(static_cast<unsigned>((int64_t(p.pairs) + chunk - 1) / chunk));
+  hipLaunchKernelGGL(count_kernel, chunks, dim3(kChunk), 0, s, p, chunk, hist);
+  AFD_CHECK_LAUNCH();
+  hipLaunchKernelGGL(place_kernel, chunks, dim3(kChunk), 0, s, p, chunk, hist);
+  AFD_CHECK_LAUNCH();
+  hipLaunchKernelGGL(move_kernel<VEC>, dim3((m.n + 3) / 4), dim3(256), 0, s, m, p.positions, p.offsets + p.experts);
+  AFD_CHECK_LAUNCH();
+  return AFD_OK;
 }
 
 // tokens of fewer are a workgroup's work each, of more a wavefront's
@@ -481,8 +475,13 @@ extern "C" int afd_sort_tokens(int32_t fmt, const int32_t* ids, int32_t n, int32
   if (!counts || !offsets || (n > 0 && (!ids || !x || !rows || !positions))) return AFD_ERR_ARG;
   if (need > 0 && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 4)) return AFD_ERR_WORKSPACE;
   const sorting::Pairs p = {ids, n * topk, expert_lo, num_experts, positions, counts, offsets};
-  const sorting::Move m = {x, rows, ldx, ld, 0, n, topk, zero_behind};
-  return sorting::sort(p, m, fmt, columns, static_cast<int32_t*>(ws), static_cast<hipStream_t>(stream));
+  const int size = rows::value_size(fmt);
+  const sorting::Move m = {static_cast<const char*>(x), static_cast<char*>(rows), ldx * size, ld * size, columns * size,
+                           n, topk, zero_behind};
+  int32_t* hist = static_cast<int32_t*>(ws);
+  const bool vec = rows::aligned_rows(x, ldx, fmt) && rows::aligned_rows(rows, ld, fmt) && m.bytes % 16 == 0;
+  return vec ? sorting::launch_sort<true>(p, m, hist, static_cast<hipStream_t>(stream))
+             : sorting::launch_sort<false>(p, m, hist, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int afd_unsort_tokens(int32_t fmt, const void* rows, int64_t ld, int64_t num_rows, const int32_t* positions,

@@ -49,21 +49,24 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _wide(t: Optional[torch.Tensor]) -> bool:
-    return t is not None and t.dtype == torch.float32
+def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _forward(cfg, y, residual, w_post, gate, w_next, rstd):
     """(hidden or None, normed or None) of two-dimensional tensors."""
     residual, ldr = matrix_rows(residual)
+    hidden = normed = y_ptr = h_ptr = n_ptr = next_ptr = None
     ldy = 0
     if y is not None:
         y, ldy = matrix_rows(y)
-    n, columns = residual.shape
-    hidden = None if y is None else torch.empty(n, columns, dtype=residual.dtype, device=residual.device)
-    normed = None if w_next is None else torch.empty(n, columns, dtype=residual.dtype, device=residual.device)
-    launch("afd_residual_norm", residual.device, cfg, _ptr(y), ldy, residual.data_ptr(), ldr, _ptr(w_post), _ptr(gate),
-           _ptr(w_next), n, _ptr(hidden), _ptr(normed), _ptr(rstd))
+        hidden = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        y_ptr, h_ptr = y.data_ptr(), hidden.data_ptr()
+    if w_next is not None:
+        normed = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        n_ptr, next_ptr = normed.data_ptr(), w_next.data_ptr()
+    launch("afd_residual_norm", residual.device, cfg, y_ptr, ldy, residual.data_ptr(), ldr, _ptr(w_post), _ptr(gate), next_ptr,
+           residual.shape[0], h_ptr, n_ptr, _ptr(rstd))
     return hidden, normed
 
 
@@ -126,15 +129,16 @@ def _activations(name: str, t: torch.Tensor) -> int:
     return fmt
 
 
-def _param(name: str, t: Optional[torch.Tensor], like: torch.Tensor, shape: tuple) -> None:
-    if t is None:
-        return
-    if t.dtype not in (like.dtype, torch.float32):
+def _param(name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> bool:
+    """Whether the parameter is held in fp32."""
+    wide = t.dtype == torch.float32
+    if not wide and t.dtype != like.dtype:
         raise TypeError(f"{name} must be {like.dtype} or float32, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+    return wide
 
 
 def _eps(eps: float) -> float:
@@ -148,16 +152,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
-def _call(y, residual, w_post, gate, w_next, cfg, kind):
-    """(hidden or None, normed or None) of two-dimensional activations."""
-    given = [t for t in (y, residual, w_post, gate, w_next) if t is not None]
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
-        return _forward(cfg, y, residual, w_post, gate, w_next, None)
-    y = None if y is None else matrix_rows(y)[0]
-    out = _Norm.apply(y, matrix_rows(residual)[0], w_post, gate, w_next, cfg, kind)
-    if y is None:
-        return None, out
-    return out if w_next is not None else (out, None)
+def _needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6) -> torch.Tensor:
@@ -165,11 +161,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6) -> tor
     [hidden] of x's type or fp32. Gradients by both, once: second, forward-mode and traced derivatives are refused."""
     fmt = _activations("x", x)
     columns = x.shape[-1]
-    _param("weight", weight, x, (columns,))
+    wide = _param("weight", weight, x, (columns,))
     need_gpu("x", x)
     no_tangent("rms_norm", x, weight)
-    cfg = _cfg(columns, fmt, GATE_NONE, False, False, _wide(weight), 1.0, _eps(eps))
-    return _call(None, _rows(x), None, None, weight.contiguous(), cfg, GATE_NONE)[1].view(x.shape)
+    cfg = _cfg(columns, fmt, GATE_NONE, False, False, wide, 1.0, _eps(eps))
+    weight, rows = _whole(weight), _rows(x)
+    if _needs_grad(x, weight):
+        out = _Norm.apply(None, matrix_rows(rows)[0], None, None, weight, cfg, GATE_NONE)
+    else:
+        out = _forward(cfg, None, rows, None, None, weight, None)[1]
+    return out if rows is x else out.view(x.shape)
 
 
 def residual_norm(
@@ -194,28 +195,36 @@ def residual_norm(
         raise ValueError(f"y is {y.dtype} {tuple(y.shape)}, residual {residual.dtype} {tuple(residual.shape)}")
     if residual.device != y.device:
         raise ValueError(f"residual is on {residual.device}, y on {y.device}")
-    columns = y.shape[-1]
-    _param("post_weight", post_weight, y, (columns,))
-    _param("next_weight", next_weight, y, (columns,))
-    kind, gate_rows = GATE_NONE, gate
+    columns, kind = y.shape[-1], GATE_NONE
+    wide_post = wide_gate = wide_next = False
+    if post_weight is not None:
+        wide_post = _param("post_weight", post_weight, y, (columns,))
+        post_weight = _whole(post_weight)
+    if next_weight is not None:
+        wide_next = _param("next_weight", next_weight, y, (columns,))
+        next_weight = _whole(next_weight)
     if gate is not None:
         if gate.dim() == 1:
-            kind, shape = GATE_CHANNEL, (columns,)
-        elif tuple(gate.shape) == tuple(y.shape) and columns > 1:
-            kind, shape = GATE_ELEMENT, tuple(y.shape)
-            gate_rows = gate.reshape(-1, columns)
+            kind, wide_gate = GATE_CHANNEL, _param("gate", gate, y, (columns,))
+        elif gate.shape == y.shape and columns > 1:
+            kind, wide_gate = GATE_ELEMENT, _param("gate", gate, y, tuple(y.shape))
+            gate = _rows(gate)
         else:
-            kind, shape = GATE_TOKEN, tuple(y.shape[:-1]) + (1,)
-            gate_rows = gate.reshape(-1)
-        _param("gate", gate, y, shape)
-        gate_rows = gate_rows.contiguous()
+            kind, wide_gate = GATE_TOKEN, _param("gate", gate, y, tuple(y.shape[:-1]) + (1,))
+            gate = gate.reshape(-1)
+        gate = _whole(gate)
     need_gpu("y", y)
     no_tangent("residual_norm", y, residual, post_weight, gate, next_weight)
-    scale = float(scale)
-    cfg = _cfg(columns, fmt, kind, _wide(post_weight), _wide(gate), _wide(next_weight), scale, _eps(eps))
-    post_weight, next_weight = (None if t is None else t.contiguous() for t in (post_weight, next_weight))
-    hidden, normed = _call(_rows(y), _rows(residual), post_weight, gate_rows, next_weight, cfg, kind)
-    return ResidualNorm(hidden.view(y.shape), None if normed is None else normed.view(y.shape))
+    cfg = _cfg(columns, fmt, kind, wide_post, wide_gate, wide_next, float(scale), _eps(eps))
+    rows = _rows(y)
+    if _needs_grad(y, residual, post_weight, gate, next_weight):
+        out = _Norm.apply(matrix_rows(rows)[0], matrix_rows(_rows(residual))[0], post_weight, gate, next_weight, cfg, kind)
+        hidden, normed = out if next_weight is not None else (out, None)
+    else:
+        hidden, normed = _forward(cfg, rows, _rows(residual), post_weight, gate, next_weight, None)
+    if rows is not y:
+        hidden, normed = hidden.view(y.shape), None if normed is None else normed.view(y.shape)
+    return ResidualNorm(hidden, normed)
 
 
 class BlockNorms(torch.nn.Module):

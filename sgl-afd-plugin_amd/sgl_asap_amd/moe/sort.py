@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from .topk import fit_ints, last, launch, matrix_rows, need_gpu, no_tangent, on_device
+from .topk import fit_ints, last, launch, matrix_rows, need_gpu, no_tangent
 
 VALUE_FORMATS = {torch.float32: _lib.AFD_V_F32, torch.bfloat16: _lib.AFD_V_BF16, torch.float16: _lib.AFD_V_F16}
 
@@ -60,10 +60,11 @@ def _sort(x, ids, num_experts, expert_lo, out):
     counts = torch.empty(num_experts, dtype=torch.int32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     # a call's own: calls on other streams and captured graphs each have theirs
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     ld = rows.stride(0) if rows.shape[0] > 1 else hidden
     launch("afd_sort_tokens", dev, VALUE_FORMATS[x.dtype], ids.data_ptr(), n, k, expert_lo, num_experts, x.data_ptr(), ldx, hidden,
-           rows.data_ptr(), ld, out is None, positions.data_ptr(), counts.data_ptr(), offsets.data_ptr(), ws.data_ptr(), size)
+           rows.data_ptr(), ld, out is None, positions.data_ptr(), counts.data_ptr(), offsets.data_ptr(),
+           None if ws is None else ws.data_ptr(), size)
     return rows, TokenOrder(positions, counts, offsets)
 
 
@@ -135,7 +136,8 @@ class _Unsort(torch.autograd.Function):
 def _matrix(name: str, t: torch.Tensor) -> None:
     if t.dim() != 2 or t.shape[1] < 1:
         raise ValueError(f"{name} must be [rows, hidden] with hidden >= 1, got {tuple(t.shape)}")
-    fit_ints(t.shape[1])
+    if t.shape[1] > 0x7FFFFFFF:
+        fit_ints(t.shape[1])
     value_format(name, t)
 
 
@@ -159,7 +161,7 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, ex
     if topk_ids.device != x.device:
         raise ValueError(f"topk_ids is on {topk_ids.device}, x on {x.device}")
     no_tangent("sort_tokens", x, out)
-    ids = topk_ids.contiguous()
+    ids = topk_ids if topk_ids.is_contiguous() else topk_ids.contiguous()
     if out is None:
         if torch.is_grad_enabled() and x.requires_grad:
             rows, *order = _Sort.apply(x, ids, num_experts, expert_lo)
@@ -194,20 +196,23 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, topk_weights: Optional[
     if positions.dtype != torch.int32 or positions.dim() != 2 or offsets.dtype != torch.int32 or offsets.dim() != 1:
         raise TypeError("order must hold int32 positions [n, k] and offsets [num_experts + 1]")
     n, k = positions.shape
-    fit_ints(n, k)
+    if n > 0x7FFFFFFF or k > 0x7FFFFFFF:
+        fit_ints(n, k)
     need_gpu("rows", rows)
     dev = rows.device
-    on_device("positions", positions, torch.int32, (n, k), dev)
-    on_device("offsets", offsets, torch.int32, (offsets.shape[0],), dev)
+    if positions.device != dev or offsets.device != dev or not positions.is_contiguous() or not offsets.is_contiguous():
+        raise ValueError(f"positions and offsets must be contiguous on {dev}, got {positions.device} strides {positions.stride()} "
+                         f"and {offsets.device} strides {offsets.stride()}")
     if offsets.shape[0] < 1:
         raise ValueError("offsets must hold the number of rows")
     no_tangent("unsort_tokens", rows, topk_weights)
     if topk_weights is not None:
-        if tuple(topk_weights.shape) != (n, k) or not topk_weights.is_floating_point():
+        if topk_weights.shape != positions.shape or not topk_weights.is_floating_point():
             raise ValueError(f"topk_weights must be [{n}, {k}], got {topk_weights.dtype} {tuple(topk_weights.shape)}")
         if topk_weights.device != dev:
             raise ValueError(f"topk_weights is on {topk_weights.device}, rows on {dev}")
-        topk_weights = topk_weights.to(torch.float32).contiguous()
+        if topk_weights.dtype != torch.float32 or not topk_weights.is_contiguous():
+            topk_weights = topk_weights.to(torch.float32).contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or topk_weights is not None and topk_weights.requires_grad):
         return _Unsort.apply(matrix_rows(rows)[0], topk_weights, positions, offsets)
     return _unsort(rows, positions, topk_weights)

@@ -56,7 +56,7 @@ __device__ __forceinline__ float quantize(const Raw& r, v4i (&q)[2]) {
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, r.u[h][i] & 0x7fff7fffu));
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, r.h[h].u[i] & 0x7fff7fffu));
   uint32_t top = uint32_t(max(most[0], most[1])) << 16;
   const auto r0 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
   top = max(r0[0], r0[1]);
@@ -72,7 +72,7 @@ __device__ __forceinline__ float quantize(const Raw& r, v4i (&q)[2]) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t w = finite ? r.u[h][2 * i + j] : 0u;
+        const uint32_t w = finite ? r.h[h].u[2 * i + j] : 0u;
         v[2 * j] = div_by(__uint_as_float(w << 16), sc, rsc);
         v[2 * j + 1] = div_by(__uint_as_float(w & 0xffff0000u), sc, rsc);
       }

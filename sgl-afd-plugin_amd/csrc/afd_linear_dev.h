@@ -17,58 +17,64 @@ constexpr int64_t kCachedBytes = int64_t(64) << 20;
 
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// A wavefront's share of an activation image: 16 rows x one K block, lane l chunks l / 16 of both
-// 64-column pieces of row l % 16. Raw: those 2 x 16 bf16 values, two a word.
-struct Raw {
-  uint32_t u[2][8];
+// 16 bf16 values of a row from column k0 (a multiple of 16) on, two a word. VEC: rows are 16-byte aligned and k_in is a
+// multiple of 16 (then the 16 are whole or missing). What lies past k_in reads as 0.
+struct Half {
+  uint32_t u[8];
 };
-// VEC: rows are 16-byte aligned and k_in is a multiple of 16 (then a chunk is whole or missing). p: the
-// row; c: the lane's chunk. What lies past k_in reads as 0.
 template <bool VEC, bool NT = false>
-__device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int c) {
-  Raw r;
+__device__ __forceinline__ Half load_half(const uint16_t* p, int k_in, int k0) {
+  Half r;
+  if constexpr (VEC) {
+    const uint16_t* src = p + min(k0, k_in - 16);
+    const v4i lo = load_words<true, NT>(src), hi = load_words<true, NT>(src + 8);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int k0 = b * 128 + h * 64 + c * 16;
-    if constexpr (VEC) {
-      const v4i* src = reinterpret_cast<const v4i*>(p + min(k0, k_in - 16));
-      const v4i lo = NT ? __builtin_nontemporal_load(src) : src[0], hi = NT ? __builtin_nontemporal_load(src + 1) : src[1];
+    for (int i = 0; i < 4; ++i) {
+      r.u[i] = k0 < k_in ? lo[i] : 0;
+      r.u[4 + i] = k0 < k_in ? hi[i] : 0;
+    }
+  } else if (k0 + 16 <= k_in) {
+    const v4i lo = load_words<false>(p + k0), hi = load_words<false>(p + k0 + 8);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r.u[h][i] = k0 < k_in ? lo[i] : 0;
-        r.u[h][4 + i] = k0 < k_in ? hi[i] : 0;
-      }
-    } else if (k0 + 16 <= k_in) {
-      const v4i lo = load_words<false>(p + k0), hi = load_words<false>(p + k0 + 8);
+    for (int i = 0; i < 4; ++i) {
+      r.u[i] = lo[i];
+      r.u[4 + i] = hi[i];
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r.u[h][i] = lo[i];
-        r.u[h][4 + i] = hi[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = k0 + 2 * i;
-        const uint32_t lo = p[min(k, k_in - 1)], hi = p[min(k + 1, k_in - 1)];
-        r.u[h][i] = (k < k_in ? lo : 0u) | (k + 1 < k_in ? hi << 16 : 0u);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + 2 * i;
+      const uint32_t lo = p[min(k, k_in - 1)], hi = p[min(k + 1, k_in - 1)];
+      r.u[i] = (k < k_in ? lo : 0u) | (k + 1 < k_in ? hi << 16 : 0u);
     }
   }
   return r;
 }
-
-// bf16(silu(g) u) of a lane's gate and up values
-__device__ __forceinline__ Raw silu_mul(const Raw& g, const Raw& u) {
+// A wavefront's share of an activation image: 16 rows x one K block, lane l chunks l / 16 of both
+// 64-column pieces of row l % 16. p: the row; c: the lane's chunk.
+struct Raw {
+  Half h[2];
+};
+template <bool VEC, bool NT = false>
+__device__ __forceinline__ Raw load_raw(const uint16_t* p, int k_in, int b, int c) {
   Raw r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t a = g.u[h][i], b = u.u[h][i];
-      r.u[h][i] = pk_bf16(act_swiglu(__uint_as_float(a << 16), __uint_as_float(b << 16)),
-                          act_swiglu(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)));
-    }
+  for (int h = 0; h < 2; ++h) r.h[h] = load_half<VEC, NT>(p, k_in, b * 128 + h * 64 + c * 16);
   return r;
+}
+// bf16(silu(g) u) of a lane's gate and up values
+__device__ __forceinline__ Half silu_mul(const Half& g, const Half& u) {
+  Half r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = g.u[i], b = u.u[i];
+    r.u[i] = pk_bf16(act_swiglu(__uint_as_float(a << 16), __uint_as_float(b << 16)),
+                     act_swiglu(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)));
+  }
+  return r;
+}
+__device__ __forceinline__ Raw silu_mul(const Raw& g, const Raw& u) {
+  return {{silu_mul(g.h[0], u.h[0]), silu_mul(g.h[1], u.h[1])}};
 }
 
 // ---------------------------------------------------------------- tiles

@@ -33,25 +33,26 @@ struct Args {
   uint16_t* y;
   int64_t ldy;
   int32_t n, n_out, kb;  // kb: K blocks of 128
-  bool wide;             // rows of y take 16-byte stores
 };
 
 __device__ __forceinline__ v4i mfma(v4i w, v4i x, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------- activations
 // The largest magnitude's bits of a lane's values (infinities and NaN above every number)
-__device__ __forceinline__ uint32_t largest(const Raw& r) {
+__device__ __forceinline__ uint32_t largest(const Half& r) {
   typedef uint16_t v2u __attribute__((ext_vector_type(2)));
   v2u most = {0, 0};
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, r.u[h][i] & 0x7fff7fffu));
+  for (int i = 0; i < 8; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, r.u[i] & 0x7fff7fffu));
   return uint32_t(max(most[0], most[1])) << 16;
 }
-// The largest of a row's four lanes (lanes l with the same l % 16)
+// The largest of a row's lanes: those l with the same l % ROWS
+template <int ROWS>
 __device__ __forceinline__ uint32_t largest_of_row(uint32_t top) {
+  if constexpr (ROWS <= 4)
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x124 /*row_ror:4*/, 0xf, 0xf, false)));
+  if constexpr (ROWS <= 8)
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x128 /*row_ror:8*/, 0xf, 0xf, false)));
   const auto r0 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
   top = max(r0[0], r0[1]);
   const auto r1 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
@@ -69,74 +70,75 @@ struct RowScale {
 };
 // the code of v in the low byte: 1.5 2^23 + v rounds v to the nearest integer, ties to even, in two's complement
 __device__ __forceinline__ uint32_t code_of(float v) { return __float_as_uint(v + 12582912.0f); }
-// int8 codes of a lane's two chunks; quotients of a row stay below 127 (1 + 2^-23)
-__device__ __forceinline__ void quantize(const Raw& r, const RowScale& sc, v4i (&q)[2]) {
+// int8 codes of 16 values; quotients of a row stay below 127 (1 + 2^-23)
+__device__ __forceinline__ v4i quantize(const Half& r, const RowScale& sc) {
+  v4i q;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int i = 0; i < 4; ++i) {
+    uint32_t pair[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t pair[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t w = sc.finite ? r.u[h][2 * i + j] : 0u;
-        const uint32_t lo = code_of(div_by(__uint_as_float(w << 16), sc.s, sc.inv));
-        const uint32_t hi = code_of(div_by(__uint_as_float(w & 0xffff0000u), sc.s, sc.inv));
-        pair[j] = __builtin_amdgcn_perm(hi, lo, 0x0c0c0400u);
-      }
-      q[h][i] = static_cast<int>(__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u));
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t w = sc.finite ? r.u[2 * i + j] : 0u;
+      const uint32_t lo = code_of(div_by(__uint_as_float(w << 16), sc.s, sc.inv));
+      const uint32_t hi = code_of(div_by(__uint_as_float(w & 0xffff0000u), sc.s, sc.inv));
+      pair[j] = __builtin_amdgcn_perm(hi, lo, 0x0c0c0400u);
     }
+    q[i] = static_cast<int>(__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u));
+  }
+  return q;
 }
 
-// A workgroup of WAVES wavefronts takes 16 rows, a wavefront every WAVES-th K block of them. D: the K blocks that a
-// wavefront holds in registers between the rows' maximum and the codes (x is read once); 0: x is read
-// again for the codes, any K. NT: non-temporal reads, for an x that no cache holds anyway.
+// A workgroup of WAVES wavefronts takes ROWS rows. A wavefront's unit is 16 columns a lane, 1024 / ROWS of its rows', and it
+// takes every WAVES-th. D: the units that it holds in registers between the rows' maximum and the codes (x is read once);
+// 0: x is read again for the codes, any K. NT: non-temporal reads, for an x that no cache holds anyway.
 // SILU: x's rows are [gate | up] of 2 k_in columns and what is quantized is bf16(silu(gate) up).
-template <int WAVES, int D, bool VEC, bool NT, bool SILU>
+template <int ROWS, int WAVES, int D, bool VEC, bool NT, bool SILU>
 __global__ __launch_bounds__(64 * WAVES) void quant_kernel(const uint16_t* __restrict__ x, int64_t ldx, int n, int k_in,
                                                            uint8_t* __restrict__ q, float* __restrict__ s, int kb) {
-  __shared__ uint32_t tops[WAVES][16];
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = blockIdx.x;
-  const int row = min(r16 * 16 + (lane & 15), n - 1);  // past the end: the last again
-  const uint16_t* p = x + row * ldx;
-  auto fetch = [&](int b) {
-    Raw raw = load_raw<VEC, NT>(p, k_in, b, lane >> 4);
-    if constexpr (SILU) raw = silu_mul(raw, load_raw<VEC, NT>(p + k_in, k_in, b, lane >> 4));
+  __shared__ uint32_t tops[WAVES][ROWS];
+  constexpr int kLanes = 64 / ROWS;  // of a row
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int chunks = 8 * kb, units = (chunks + kLanes - 1) / kLanes;
+  const int at = blockIdx.x * ROWS + lane % ROWS;
+  const uint16_t* p = x + int64_t(min(at, n - 1)) * ldx;  // past the end: the last row again
+  auto fetch = [&](int unit) {
+    const int k0 = (unit * kLanes + lane / ROWS) * 16;
+    Half raw = load_half<VEC, NT>(p, k_in, k0);
+    if constexpr (SILU) raw = silu_mul(raw, load_half<VEC, NT>(p + k_in, k_in, k0));
     return raw;
   };
   constexpr int kHeld = D > 0 ? D : 1;
-  Raw raw[kHeld];
+  Half raw[kHeld];
   uint32_t top = 0;
   if constexpr (D > 0) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) raw[d] = fetch(min(w + d * WAVES, kb - 1));
+    for (int d = 0; d < D; ++d) raw[d] = fetch(min(w + d * WAVES, units - 1));
 #pragma unroll
     for (int d = 0; d < D; ++d) top = max(top, largest(raw[d]));
   } else {
-#pragma unroll 2
-    for (int b = w; b < kb; b += WAVES) top = max(top, largest(fetch(b)));
+    for (int u = w; u < units; u += WAVES) top = max(top, largest(fetch(u)));
   }
-  top = largest_of_row(top);
-  if (lane < 16) tops[w][lane] = top;
+  top = largest_of_row<ROWS>(top);
+  if (lane < ROWS) tops[w][lane] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) top = max(top, tops[i][lane & 15]);
+  for (int i = 0; i < WAVES; ++i) top = max(top, tops[i][lane % ROWS]);
   const RowScale sc(top);
-  uint8_t* out = q + int64_t(r16) * (2 * kb) * kPiece + lane * 16;
-  auto store = [&](int b, const Raw& v) {
-    v4i code[2];
-    quantize(v, sc, code);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) *reinterpret_cast<v4i*>(out + int64_t(2 * b + h) * kPiece) = code[h];
+  // chunk c of a row lies in piece c / 4, at its row's place
+  uint8_t* out = q + int64_t(at / 16) * (2 * kb) * kPiece + at % 16 * 16;
+  auto store = [&](int unit, const Half& v) {
+    const int c = unit * kLanes + lane / ROWS;
+    const v4i code = quantize(v, sc);
+    if (c < chunks) *reinterpret_cast<v4i*>(out + int64_t(c / 4) * kPiece + c % 4 * 256) = code;
   };
   if constexpr (D > 0) {
 #pragma unroll
     for (int d = 0; d < D; ++d)
-      if (w + d * WAVES < kb) store(w + d * WAVES, raw[d]);
+      if (w + d * WAVES < units) store(w + d * WAVES, raw[d]);
   } else {
-#pragma unroll 2
-    for (int b = w; b < kb; b += WAVES) store(b, fetch(b));
+    for (int u = w; u < units; u += WAVES) store(u, fetch(u));
   }
-  if (w == 0 && lane < 16) s[r16 * 16 + lane] = sc.held();
+  if (w == 0 && lane < ROWS) s[at] = sc.held();
 }
 
 // ---------------------------------------------------------------- results
@@ -237,17 +239,16 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 #pragma unroll
     for (int u = 0; u < kUp; ++u) {
       if ((w + u * kRowWaves) * 16 >= items) continue;
-      atomicMax(&tops[r[u]], largest_of_row(largest(raw[u])));
+      atomicMax(&tops[r[u]], largest_of_row<16>(max(largest(raw[u].h[0]), largest(raw[u].h[1]))));
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < kUp; ++u) {
       if ((w + u * kRowWaves) * 16 >= items) continue;
-      v4i q[2];
-      quantize(raw[u], RowScale(tops[r[u]]), q);
+      const RowScale sc(tops[r[u]]);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<v4i*>(lds + (((2 * b[u] + h) * 4 + c) * p.n + r[u]) * 16) = q[h];
+        *reinterpret_cast<v4i*>(lds + (((2 * b[u] + h) * 4 + c) * p.n + r[u]) * 16) = quantize(raw[u].h[h], sc);
     }
     __syncthreads();
 #pragma unroll
@@ -292,8 +293,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 #pragma unroll
     for (int q = 0; q < 4; ++q) y[q] = scaled(sum[q], sx[m], sw[q], odd_scale(sw[q]));
     uint16_t* out = p.y + row * p.ldy + o;
-    if (p.wide && o + 4 <= p.n_out) {
-      *reinterpret_cast<uint2*>(out) = uint2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+    if (o + 4 <= p.n_out) {
+      typedef int v2i_any __attribute__((ext_vector_type(2), aligned(2)));
+      *reinterpret_cast<v2i_any*>(out) = v2i_any{static_cast<int>(pk_bf16(y[0], y[1])), static_cast<int>(pk_bf16(y[2], y[3]))};
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
@@ -303,71 +305,70 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 }
 
 // ---------------------------------------------------------------- tiles
-// BM rows of x by BN outputs, WM x WN wavefronts of TI x TJ MFMA tiles of 16x16 each. A stage is one K block (128) of
-// both operands, copied HBM -> LDS in 1 KiB pieces into S slots.
+// BM rows of x by BN outputs, WM x WN x WK wavefronts of TI x TJ MFMA tiles of 16x16 each; the WK groups share the tile and
+// take K in turns, their sums meet in LDS at the end. A stage is 64 columns of both operands for each group, copied
+// HBM -> LDS in 1 KiB pieces into S slots.
 //
 // A wavefront holds its TI activation fragments of a stage in registers and walks the TJ weight fragments, read two
 // ahead, in an order kept as written. When the last two are in registers (all of its reads of the
 // stage done) it waits for its copies of the next stage and meets the others at the stage's one barrier: the
 // next stage is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the last two
 // weight fragments run while the next stage's first fragments are read.
-template <int BM_, int BN_, int WM_, int WN_, int S_>
+template <int BM_, int BN_, int WM_, int WN_, int WK_, int S_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_;
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WK = WK_, S = S_;
+  static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
   static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
-  static constexpr int kAPieces = BM / 16 * 2, kBPieces = BN / 16 * 2;
-  static constexpr int kAQ = kAPieces / kWaves, kBQ = kBPieces / kWaves;
-  static constexpr int kBOff = kAPieces * kPiece;
-  static constexpr int kStage = kBOff + kBPieces * kPiece;
-  static constexpr int kLds = S * kStage;
-  static constexpr int kCopies = kAQ + kBQ;  // a wavefront's copies of a stage
-  static_assert(TI * 16 * WM == BM && TJ * 16 * WN == BN && kAQ * kWaves == kAPieces && kBQ * kWaves == kBPieces, "tile");
-  static_assert(TJ % 4 == 0 && kLds <= 160 * 1024, "fragments by their number mod 4; LDS");
-  static_assert((S & (S - 1)) == 0 && S >= 2 && (S - 1) * kCopies < 64, "slots by a mask; vmcnt is a 6-bit counter");
+  static constexpr int kAPieces = BM / 16, kBPieces = BN / 16, kGroup = kAPieces + kBPieces, kPieces = WK * kGroup;
+  static constexpr int kStage = kPieces * kPiece;
+  static constexpr int kRing = S * kStage, kSums = (WK - 1) * WM * WN * TI * TJ * 1024;
+  static constexpr int kLds = kRing > kSums ? kRing : kSums;
+  static constexpr int kCopies = (kPieces + kWaves - 1) / kWaves;  // a wavefront's copies of a stage
+  static_assert(TI * 16 * WM == BM && TJ * 16 * WN == BN, "tile");
+  static constexpr int kRingB = TJ % 4 == 0 ? 4 : 3;  // weight fragments in registers
+  static_assert(TJ % kRingB == 0 && TJ % 2 == 0 && kLds <= 160 * 1024, "fragments by their number; pairs of results; LDS");
+  static_assert(S >= 2 && (S - 1) * kCopies < 64, "vmcnt is a 6-bit counter");
 };
 
-template <typename T>
-__global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
-  constexpr int TI = T::TI, TJ = T::TJ;
+// NT: results are stored past the caches, for rows whose 64-byte pieces are aligned (through L2 the 134 MB of 16384 x 4096 x
+// 4096 cost 23 us more: 227 us, with no stores at all 198, so 204; 6000 x 2048 x 3584 57.1 against 54.0; where pieces lie
+// across lines it is the other way: 6000 x 2048 x 3500 59.5 against 78.4).
+template <typename T, bool NT>
+__global__ __launch_bounds__(T::kThreads) __attribute__((amdgpu_waves_per_eu(2))) void tile_kernel(Args p) {
+  constexpr int TI = T::TI, TJ = T::TJ, WK = T::WK, kCopies = T::kCopies, S = T::S, kRingB = T::kRingB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wm = w / T::WN, wn = w % T::WN;
+  const int wk = w / (T::WM * T::WN), wm = w / T::WN % T::WM, wn = w % T::WN;
   const int mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
   const TileAt at = tile_at(blockIdx.x, mts, nts);
   if (at.mt < 0) return;
   // (the divisions run in vector registers; what follows from the tile is scalar)
   const int mt = __builtin_amdgcn_readfirstlane(at.mt), nt = __builtin_amdgcn_readfirstlane(at.nt);
-  const int kt = 2 * p.kb, last = p.kb - 1;
+  const int kt = 2 * p.kb, last = (kt + WK - 1) / WK - 1;
   const int m0 = mt * T::BM, n0 = nt * T::BN;
   const int r16_last = (p.n + 15) / 16 - 1, o16_last = (p.n_out + 15) / 16 - 1;
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_offset(lds));
   const uint32_t voff = static_cast<uint32_t>(lane) * 16;
 
-  // this wavefront's pieces of a stage: piece q of an operand is row group q / 2, 64-column half q % 2.
-  // Row groups past the end re-read the last one; their results are not stored.
-  const uint8_t* a_src[T::kAQ];
-  const uint8_t* b_src[T::kBQ];
+  // this wavefront's pieces of a stage: every kWaves-th, of group q / kGroup its activations' row groups, then its
+  // weights'. Past the last piece the last again (the same bytes), past the last row group the last one, whose
+  // results are not stored.
+  const uint8_t* src[kCopies];
+  int ks[kCopies], dst[kCopies];
 #pragma unroll
-  for (int i = 0; i < T::kAQ; ++i) {
-    const int q = w * T::kAQ + i;
-    a_src[i] = p.a + (int64_t(min(m0 / 16 + q / 2, r16_last)) * kt + q % 2) * kPiece;
+  for (int c = 0; c < kCopies; ++c) {
+    const int q = min(c * T::kWaves + w, T::kPieces - 1), r = q % T::kGroup;
+    src[c] = r < T::kAPieces ? p.a + int64_t(min(m0 / 16 + r, r16_last)) * kt * kPiece
+                             : p.b + int64_t(min(n0 / 16 + r - T::kAPieces, o16_last)) * kt * kPiece;
+    ks[c] = q / T::kGroup;
+    dst[c] = q * kPiece;
   }
-#pragma unroll
-  for (int i = 0; i < T::kBQ; ++i) {
-    const int q = w * T::kBQ + i;
-    b_src[i] = p.b + (int64_t(min(n0 / 16 + q / 2, o16_last)) * kt + q % 2) * kPiece;
-  }
-  constexpr int kCopies = T::kCopies, S = T::S;
-  auto copy = [&](int b, auto c_c) {
+  // copy c of stage b into a slot; past the end of K the last piece (a group that has none left adds nothing)
+  auto copy = [&](int b, int slot, auto c_c) {
     constexpr int c = decltype(c_c)::value;
-    const uint32_t st = lds_base + static_cast<uint32_t>((b & (S - 1)) * T::kStage);
-    const uint32_t off = voff + static_cast<uint32_t>(b) * (2 * kPiece);
-    if constexpr (c < T::kAQ)
-      lds_dma16(st + (w * T::kAQ + c) * kPiece, a_src[c], off);
-    else
-      lds_dma16(st + T::kBOff + (w * T::kBQ + c - T::kAQ) * kPiece, b_src[c - T::kAQ], off);
+    const int k = WK == 1 ? b : min(b * WK + ks[c], kt - 1);
+    lds_dma16(lds_base + static_cast<uint32_t>(slot * T::kStage + dst[c]), src[c], voff + static_cast<uint32_t>(k) * kPiece);
   };
 
   v4i acc[TI][TJ];
@@ -376,22 +377,14 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 #pragma unroll
     for (int j = 0; j < TJ; ++j) acc[i][j] = v4i{0, 0, 0, 0};
 
-  const uint8_t* a_lds = lds + wm * TI * 2 * kPiece + lane * 16;
-  const uint8_t* b_lds = lds + T::kBOff + wn * TJ * 2 * kPiece + lane * 16;
-  v4i fa[TI][2], fb[4][2];
-  auto read_a = [&](int b, int i) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      fa[i][h] = *reinterpret_cast<const v4i*>(a_lds + (b & (S - 1)) * T::kStage + (2 * i + h) * kPiece);
-  };
-  auto read_b = [&](int b, int j, int to) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      fb[to][h] = *reinterpret_cast<const v4i*>(b_lds + (b & (S - 1)) * T::kStage + (2 * j + h) * kPiece);
-  };
+  const uint8_t* a_lds = lds + (wk * T::kGroup + wm * TI) * kPiece + lane * 16;
+  const uint8_t* b_lds = lds + (wk * T::kGroup + T::kAPieces + wn * TJ) * kPiece + lane * 16;
+  v4i fa[TI], fb[kRingB];
+  auto read_a = [&](int slot, int i) { fa[i] = *reinterpret_cast<const v4i*>(a_lds + slot * T::kStage + i * kPiece); };
+  auto read_b = [&](int slot, int j, int to) { fb[to] = *reinterpret_cast<const v4i*>(b_lds + slot * T::kStage + j * kPiece); };
 
   static_for<S>([&](auto s) {
-    static_for<kCopies>([&](auto c) { copy(min(static_cast<int>(decltype(s)::value), last), c); });
+    static_for<kCopies>([&](auto c) { copy(min(static_cast<int>(decltype(s)::value), last), decltype(s)::value, c); });
   });
   wait_vmcnt<(S - 1) * kCopies>();
   __syncthreads();
@@ -399,33 +392,60 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
   for (int i = 0; i < TI; ++i) read_a(0, i);
   read_b(0, 0, 0);
   read_b(0, 1, 1);
-  constexpr int kSteps = 2 * TI * TJ;
+  constexpr int kSteps = TI * TJ;
+  int slot = 0;
+  // (kt is even: only with more than two groups can some have nothing in the last stage)
+  const int mine = WK > 2 && last * WK + wk >= kt ? last - 1 : last;
   for (int b = 0; b <= last; ++b) {
     const int ahead = min(b + S, last);  // past the end: the last stage over itself, the same bytes
+    const int slot1 = slot + 1 == S ? 0 : slot + 1;
+    if constexpr (WK > 2)
+      if (b > mine) {
+#pragma unroll
+        for (int i = 0; i < TI; ++i) fa[i] = v4i{0, 0, 0, 0};
+      }
     static_for<kSteps>([&](auto mc) {
-      constexpr int m = decltype(mc)::value, i = m % TI, h = m / TI % 2, j = m / (2 * TI);
-      constexpr int kFree = (TJ - 2) * TI * 2;  // the first step at which the stage's slot is free
+      constexpr int m = decltype(mc)::value, i = m % TI, j = m / TI;
+      constexpr int kFree = (TJ - 2) * TI;  // the first step at which the stage's slot is free
       if constexpr (m == kFree) {
         wait_vmcnt_lds<(S - 2) * kCopies>();  // copies land in the order they were issued in
         __syncthreads();
       }
-      if constexpr (i == 0 && h == 0) {
+      if constexpr (i == 0) {
         if constexpr (j < TJ - 2)
-          read_b(b, j + 2, (j + 2) % 4);
+          read_b(slot, j + 2, (j + 2) % kRingB);
         else
-          read_b(b + 1, j + 2 - TJ, (j + 2) % 4);
+          read_b(slot1, j + 2 - TJ, (j + 2) % kRingB);
       }
-      acc[i][j] = mfma(fb[j % 4][h], fa[i][h], acc[i][j]);
-      if constexpr (m >= kFree) {  // the copies of the stage after next, dealt to the steps that are left
+      acc[i][j] = mfma(fb[j % kRingB], fa[i], acc[i][j]);
+      if constexpr (m >= kFree) {  // the copies of the stage that takes this one's slot, dealt to the steps that are left
         constexpr int kLeft = kSteps - kFree, at = m - kFree;
         constexpr int c0 = kCopies * at / kLeft, c1 = kCopies * (at + 1) / kLeft;
-        static_for<c1 - c0>([&](auto c) { copy(ahead, std::integral_constant<int, c0 + decltype(c)::value>{}); });
+        static_for<c1 - c0>([&](auto c) { copy(ahead, slot, std::integral_constant<int, c0 + decltype(c)::value>{}); });
       }
-      if constexpr (j == TJ - 1 && h == 1) read_a(b + 1, i);
+      if constexpr (j == TJ - 1) read_a(slot1, i);
       __builtin_amdgcn_sched_barrier(0);
     });
+    slot = slot1;
   }
   wait_vmcnt<0>();
+
+  if constexpr (WK > 1) {
+    __syncthreads();  // the last copies have landed: the sums take the ring's place
+    v4i* part = reinterpret_cast<v4i*>(lds);
+    const int u = w % (T::WM * T::WN);
+    if (wk > 0) {
+#pragma unroll
+      for (int ij = 0; ij < TI * TJ; ++ij)
+        part[(((wk - 1) * T::WM * T::WN + u) * TI * TJ + ij) * 64 + lane] = acc[ij / TJ][ij % TJ];
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int g = 0; g < WK - 1; ++g)
+#pragma unroll
+      for (int ij = 0; ij < TI * TJ; ++ij) acc[ij / TJ][ij % TJ] += part[((g * T::WM * T::WN + u) * TI * TJ + ij) * 64 + lane];
+  }
 
   // lane l holds, of row l % 16 of an activation tile, outputs 4 (l / 16) .. + 3 of each weight tile. Two
   // neighbouring weight tiles trade halves so that a lane holds 8 outputs: lane groups 0 and 2 those of tile
@@ -460,8 +480,11 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
       const int o = n0 + (wn * TJ + j + (lg & 1)) * 16 + (lg >> 1) * 8;
       if (row >= p.n) continue;
       uint16_t* out = p.y + row * p.ldy + o;
-      if (p.wide && o + 8 <= p.n_out) {
-        *reinterpret_cast<v4i*>(out) = chunk;
+      if (o + 8 <= p.n_out) {
+        if constexpr (NT)
+          __builtin_nontemporal_store(chunk, reinterpret_cast<v4i*>(out));
+        else
+          *reinterpret_cast<v4i_any*>(out) = chunk;
       } else {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
@@ -473,12 +496,26 @@ __global__ __launch_bounds__(T::kThreads) void tile_kernel(Args p) {
 }
 
 // ---------------------------------------------------------------- host
-using T64 = Shape<64, 64, 4, 1, 4>;
-using T64x128 = Shape<64, 128, 2, 2, 4>;
-using T128 = Shape<128, 128, 2, 2, 4>;
-using T256x128 = Shape<256, 128, 4, 2, 2>;
-using T192x256 = Shape<192, 256, 2, 4, 2>;
-using T256 = Shape<256, 256, 4, 2, 2>;
+// Tile shapes. A tile's time is a fixed part (its first copies, its results) and one for each K block, measured
+// with every CU at work (in 10 ns): the larger the tile, the less of its time goes into moving operands, and the fewer of them
+// there are to fill the CUs. Small tiles have few MFMAs a stage, so that its barrier and its copies' latency are what takes time:
+// their wavefronts split K, and a stage is two or four groups' 64 columns (300 x 2000 x 1111, 64 x 64: one group 7.7 us, two 7.6
+// with half the LDS; 32 x 64 with four 6.7).
+using T32x64 = Shape<32, 64, 2, 1, 4, 4>;
+using T64 = Shape<64, 64, 4, 1, 2, 4>;
+using T64x128 = Shape<64, 128, 2, 2, 2, 4>;
+using T128 = Shape<128, 128, 4, 2, 1, 4>;
+using T256x128 = Shape<256, 128, 4, 2, 1, 4>;
+using T192x128 = Shape<192, 128, 4, 2, 1, 4>;
+using T192 = Shape<192, 192, 4, 2, 1, 3>;
+using T192x256 = Shape<192, 256, 2, 4, 1, 3>;
+using T256 = Shape<256, 256, 2, 4, 1, 3>;
+struct ShapeCost {
+  int bm, bn, fixed, block;
+};
+constexpr ShapeCost kCosts[] = {{32, 64, 240, 15},    {64, 64, 220, 20},   {64, 128, 310, 30},  {128, 128, 270, 40}, {192, 128, 350, 55},
+                                {256, 128, 420, 74}, {192, 192, 450, 84}, {192, 256, 500, 94}, {256, 256, 800, 130}};
+enum { kT32x64, kT64, kT64x128, kT128, kT192x128, kT256x128, kT192, kT192x256, kT256, kShapes };
 
 struct Plan {
   int kb;
@@ -495,7 +532,11 @@ static Plan plan(int32_t n, int32_t k_in) {
 template <typename T>
 static int launch_tiles(const Args& p, hipStream_t s) {
   const int64_t mts = (p.n + T::BM - 1) / T::BM, nts = (p.n_out + T::BN - 1) / T::BN;
-  hipLaunchKernelGGL(tile_kernel<T>, dim3(static_cast<unsigned>(tile_grid(mts, nts))), dim3(T::kThreads), 0, s, p);
+  const dim3 grid(static_cast<unsigned>(tile_grid(mts, nts)));
+  if (reinterpret_cast<uintptr_t>(p.y) % 64 == 0 && p.ldy % 32 == 0)
+    hipLaunchKernelGGL((tile_kernel<T, true>), grid, dim3(T::kThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((tile_kernel<T, false>), grid, dim3(T::kThreads), 0, s, p);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
@@ -515,36 +556,34 @@ static int launch_fused_rows(const Args& p, const RowsIn& in, bool vec, hipStrea
   if (p.n <= 32) return launch_rows<2, true, SILU>(p, in, vec, s);
   return launch_rows<4, true, SILU>(p, in, vec, s);
 }
-template <bool VEC, bool NT, bool SILU>
+template <int ROWS, bool VEC, bool NT, bool SILU>
 static int launch_quant(const Args& p, const RowsIn& in, uint8_t* q, float* sx, hipStream_t s) {
-  const dim3 grid((p.n + 15) / 16);
+  const dim3 grid((p.n + ROWS - 1) / ROWS);
   auto go = [&](auto kernel, int waves) {
     hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, in.x, in.ldx, p.n, in.k_in, q, sx, p.kb);
   };
-  if (p.kb <= 4)
-    go(quant_kernel<4, 1, VEC, NT, SILU>, 4);
-  else if (p.kb <= 16)
-    go(quant_kernel<8, 2, VEC, NT, SILU>, 8);
-  else if (p.kb <= 32)
-    go(quant_kernel<16, 2, VEC, NT, SILU>, 16);
-  else if (p.kb <= 64)
-    go(quant_kernel<16, 4, VEC, NT, SILU>, 16);
+  // units: 8 kb chunks of 64 / ROWS lanes
+  const int units = (8 * p.kb * ROWS + 63) / 64;
+  if (units <= 8)
+    go(quant_kernel<ROWS, 4, 2, VEC, NT, SILU>, 4);
+  else if (units <= 32)
+    go(quant_kernel<ROWS, 8, 4, VEC, NT, SILU>, 8);
+  else if (units <= 64)
+    go(quant_kernel<ROWS, 16, 4, VEC, NT, SILU>, 16);
   else
-    go(quant_kernel<16, 0, VEC, NT, SILU>, 16);
+    go(quant_kernel<ROWS, 16, 0, VEC, NT, SILU>, 16);
   AFD_CHECK_LAUNCH();
   return AFD_OK;
 }
 
-// The shape whose rounds over the CUs take least: rounds x the time of one K block.
-enum { kT64, kT64x128, kT128, kT256x128, kT192x256, kT256, kShapes };
-static int best_shape(int64_t n, int64_t n_out, int cus) {
-  static const int bm[kShapes] = {64, 64, 128, 256, 192, 256}, bn[kShapes] = {64, 128, 128, 128, 256, 256};
-  static const int cost[kShapes] = {35, 49, 72, 116, 148, 186};
+// The shape whose rounds over the CUs take least
+static int best_shape(int64_t n, int64_t n_out, int kb, int cus) {
   int best = 0;
   int64_t least = 0;
   for (int i = 0; i < kShapes; ++i) {
-    const int64_t tiles = ((n + bm[i] - 1) / bm[i]) * ((n_out + bn[i] - 1) / bn[i]);
-    const int64_t time = (tiles + cus - 1) / cus * cost[i];
+    const ShapeCost& c = kCosts[i];
+    const int64_t tiles = ((n + c.bm - 1) / c.bm) * ((n_out + c.bn - 1) / c.bn);
+    const int64_t time = (tiles + cus - 1) / cus * (c.fixed + int64_t(kb) * c.block);
     if (i == 0 || time < least) {
       best = i;
       least = time;
@@ -578,7 +617,6 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   p.n = n;
   p.n_out = weights->n_out;
   p.kb = pl.kb;
-  p.wide = reinterpret_cast<uintptr_t>(y) % 16 == 0 && ldy % 8 == 0;
   const RowsIn in = {x, ldx, weights->k_in};
   const int64_t elements = int64_t(n) * pl.kb * 128;
   if (n <= kFusedRows && elements <= (vec ? kFusedBytes : kFusedBytes / 3))
@@ -586,9 +624,18 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   const bool nt = int64_t(n) * weights->k_in * (silu ? 4 : 2) > kCachedBytes;
   auto quant = [&](auto silu_c) {
     constexpr bool kSilu = decltype(silu_c)::value;
-    if (vec && nt) return launch_quant<true, true, kSilu>(p, in, q, sx, s);
-    if (vec) return launch_quant<true, false, kSilu>(p, in, q, sx, s);
-    return launch_quant<false, false, kSilu>(p, in, q, sx, s);
+    // as few rows a workgroup as give no more than one to each CU (4 / 8 / 16 rows: 1000 x 2048 13.2 / 16.7 / 17.1 us with the
+    // product, 16384 x 4096 268 / 243 / 244)
+    const int cus = device_cu_count();
+    auto rows = [&](auto rows_c) {
+      constexpr int R = decltype(rows_c)::value;
+      if (vec && nt) return launch_quant<R, true, true, kSilu>(p, in, q, sx, s);
+      if (vec) return launch_quant<R, true, false, kSilu>(p, in, q, sx, s);
+      return launch_quant<R, false, false, kSilu>(p, in, q, sx, s);
+    };
+    if (n <= 4 * cus) return rows(std::integral_constant<int, 4>{});
+    if (n <= 8 * cus) return rows(std::integral_constant<int, 8>{});
+    return rows(std::integral_constant<int, 16>{});
   };
   st = silu ? quant(std::true_type{}) : quant(std::false_type{});
   if (st != AFD_OK) return st;
@@ -596,10 +643,13 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   if (n <= 32) return launch_rows<2, false, false>(p, in, vec, s);
   if (n <= 48) return launch_rows<3, false, false>(p, in, vec, s);
   if (n <= 64) return launch_rows<4, false, false>(p, in, vec, s);
-  switch (best_shape(n, p.n_out, device_cu_count())) {
+  switch (best_shape(n, p.n_out, p.kb, device_cu_count())) {
+    case kT32x64: return launch_tiles<T32x64>(p, s);
     case kT64: return launch_tiles<T64>(p, s);
     case kT64x128: return launch_tiles<T64x128>(p, s);
     case kT128: return launch_tiles<T128>(p, s);
+    case kT192x128: return launch_tiles<T192x128>(p, s);
+    case kT192: return launch_tiles<T192>(p, s);
     case kT192x256: return launch_tiles<T192x256>(p, s);
     case kT256x128: return launch_tiles<T256x128>(p, s);
     default: return launch_tiles<T256>(p, s);

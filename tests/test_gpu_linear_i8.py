@@ -74,7 +74,8 @@ def test_bits(n, k, n_out):
 
 
 @pytest.mark.parametrize("n,n_out", [(65, 4096), (500, 4100), (1000, 4000), (1500, 4096), (2900, 4096), (70, 65000), (5000, 300),
-                                     (5800, 4096), (2885, 4091), (3900, 3100), (8200, 2048), (4096, 4096)])
+                                     (5800, 4096), (2885, 4091), (3900, 3100), (8200, 2048), (4096, 4096), (100, 130), (300, 1111),
+                                     (1500, 1536), (2900, 1600), (3800, 2048), (2900, 4352), (66, 200), (300, 3000)])
 def test_bits_of_every_tile_shape(n, n_out):
     """Calls that take each of the tile shapes, with rows and outputs that end inside a tile."""
     k = 700

@@ -83,7 +83,7 @@ class _Norm(torch.autograd.Function):
         # the residual and y are read to make hidden again, y for its norm's gradient and the gate's too
         held = y if w_next is not None or w_post is not None or gate is not None and ctx.needs_input_grad[3] else None
         ctx.save_for_backward(held, residual if w_next is not None else None, w_post, gate, w_next, rstd)
-        ctx.cfg, ctx.kind, ctx.shape, ctx.has_y = cfg, kind, tuple(residual.shape), y is not None
+        ctx.cfg, ctx.kind, ctx.shape, ctx.has_y, ctx.needs_next = cfg, kind, residual.shape, y is not None, w_next is not None
         ctx.set_materialize_grads(False)
         if y is None:
             return normed
@@ -91,34 +91,50 @@ class _Norm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        y, residual, w_post, gate, w_next, rstd = ctx.saved_tensors
-        dh, dn = (grads + (None,))[:2] if ctx.has_y else (None, grads[0])
-        none = (None,) * 7
+        dn = grads[-1] if ctx.needs_next else None
+        dh = grads[0] if ctx.has_y else None
         if dh is None and dn is None:
-            return none
+            return (None,) * 7
+        y, residual, w_post, gate, w_next, rstd = ctx.saved_tensors
         made_from = (dh, dn, y, residual, w_post, gate, w_next)
-        g = dh if dh is not None else dn
-        (n, columns), dev = ctx.shape, g.device
-        dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
-        need_y, need_res, need_post, need_gate, need_next = ctx.needs_input_grad[:5]
-        need_next = need_next and dn is not None
-        d_res = torch.empty(n, columns, dtype=g.dtype, device=dev) if need_res else None
-        d_y = torch.empty(n, columns, dtype=g.dtype, device=dev) if need_y and ctx.has_y else None
+        need_y, need_res, need_post, need_gate, need_next, _, _ = ctx.needs_input_grad
+        n, columns = shape = ctx.shape
+        dh_ptr = dn_ptr = y_ptr = res_ptr = d_y = d_res = d_post = d_gate = d_next = ws = None
+        ldy = ldr = size = 0
+        if dh is not None:
+            g = dh = _whole(dh)
+            dh_ptr = dh.data_ptr()
+        if dn is not None:
+            g = dn = _whole(dn)
+            dn_ptr = dn.data_ptr()
+            residual, ldr = matrix_rows(residual)
+            res_ptr = residual.data_ptr()
+        if y is not None:
+            y, ldy = matrix_rows(y)
+            y_ptr = y.data_ptr()
+        dtype, dev = g.dtype, g.device
         # (without tokens no launch writes the parameters' gradients)
         like = torch.empty_like if n else torch.zeros_like
-        d_post, d_gate, d_next = (like(t) if need else None
-                                  for t, need in ((w_post, need_post), (gate, need_gate), (w_next, need_next)))
+        if need_y:
+            d_y = torch.empty(shape, dtype=dtype, device=dev)
+        if need_res:
+            d_res = torch.empty(shape, dtype=dtype, device=dev)
+        if need_post:
+            d_post = like(w_post)
+        if need_gate:
+            d_gate = like(gate)
+        if need_next and dn is not None:
+            d_next = like(w_next)
         if n:
-            y, ldy = (None, 0) if y is None else matrix_rows(y)
-            residual, ldr = (None, 0) if residual is None else matrix_rows(residual)
-            sums = d_post is not None or d_next is not None or d_gate is not None and ctx.kind == GATE_CHANNEL
-            size = _workspace_bytes(columns, n) if sums else 0
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            launch("afd_residual_norm_grad", dev, ctx.cfg, _ptr(y), ldy, _ptr(residual), ldr, _ptr(w_post), _ptr(gate), _ptr(w_next),
-                   _ptr(rstd), n, _ptr(dh), _ptr(dn), _ptr(d_res), _ptr(d_y), _ptr(d_gate), _ptr(d_post), _ptr(d_next),
-                   ws.data_ptr(), size)
-        out = (d_y, d_res, d_post, d_gate, d_next)
-        return tuple(None if t is None else last(t, *made_from) for t in out) + (None, None)
+            if d_post is not None or d_next is not None or d_gate is not None and ctx.kind == GATE_CHANNEL:
+                size = _workspace_bytes(columns, n)
+                ws = torch.empty(size, dtype=torch.uint8, device=dev)
+            launch("afd_residual_norm_grad", dev, ctx.cfg, y_ptr, ldy, res_ptr, ldr, _ptr(w_post), _ptr(gate), _ptr(w_next),
+                   _ptr(rstd), n, dh_ptr, dn_ptr, _ptr(d_res), _ptr(d_y), _ptr(d_gate), _ptr(d_post), _ptr(d_next), _ptr(ws), size)
+        if torch.is_grad_enabled():
+            d_y, d_res, d_post, d_gate, d_next = (None if t is None else last(t, *made_from)
+                                                  for t in (d_y, d_res, d_post, d_gate, d_next))
+        return d_y, d_res, d_post, d_gate, d_next, None, None
 
 
 def _activations(name: str, t: torch.Tensor) -> int:

@@ -113,7 +113,7 @@ class _Unsort(torch.autograd.Function):
         rows, weights, positions, offsets = ctx.saved_tensors
         (n, k), dev, (num_rows, hidden) = positions.shape, g.device, ctx.rows
         made_from = (g, rows, weights)
-        g = g.contiguous()
+        g = g if g.is_contiguous() else g.contiguous()
         d_rows = d_w = None
         if ctx.needs_input_grad[0]:
             # (without tokens no launch writes the rows)
@@ -127,9 +127,8 @@ class _Unsort(torch.autograd.Function):
                positions.data_ptr(), offsets.data_ptr() + 4 * (offsets.shape[0] - 1),
                None if weights is None else weights.data_ptr(), n, k, hidden,
                None if d_rows is None else d_rows.data_ptr(), None if d_w is None else d_w.data_ptr())
-        # (one node that refuses a second derivative for both)
-        d_rows = None if d_rows is None else last(d_rows, *made_from)
-        d_w = None if d_w is None else last(d_w, *made_from)
+        if torch.is_grad_enabled():
+            d_rows, d_w = (None if t is None else last(t, *made_from) for t in (d_rows, d_w))
         return d_rows, d_w, None, None
 
 

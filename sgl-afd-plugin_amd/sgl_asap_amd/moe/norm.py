@@ -53,6 +53,10 @@ def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _forward(cfg, y, residual, w_post, gate, w_next, rstd):
     """(hidden or None, normed or None) of two-dimensional tensors."""
     residual, ldr = matrix_rows(residual)
@@ -60,10 +64,10 @@ def _forward(cfg, y, residual, w_post, gate, w_next, rstd):
     ldy = 0
     if y is not None:
         y, ldy = matrix_rows(y)
-        hidden = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        hidden = _like(residual)
         y_ptr, h_ptr = y.data_ptr(), hidden.data_ptr()
     if w_next is not None:
-        normed = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        normed = _like(residual)
         n_ptr, next_ptr = normed.data_ptr(), w_next.data_ptr()
     launch("afd_residual_norm", residual.device, cfg, y_ptr, ldy, residual.data_ptr(), ldr, _ptr(w_post), _ptr(gate), next_ptr,
            residual.shape[0], h_ptr, n_ptr, _ptr(rstd))
@@ -98,7 +102,7 @@ class _Norm(torch.autograd.Function):
         y, residual, w_post, gate, w_next, rstd = ctx.saved_tensors
         made_from = (dh, dn, y, residual, w_post, gate, w_next)
         need_y, need_res, need_post, need_gate, need_next, _, _ = ctx.needs_input_grad
-        n, columns = shape = ctx.shape
+        n, columns = ctx.shape
         dh_ptr = dn_ptr = y_ptr = res_ptr = d_y = d_res = d_post = d_gate = d_next = ws = None
         ldy = ldr = size = 0
         if dh is not None:
@@ -112,13 +116,13 @@ class _Norm(torch.autograd.Function):
         if y is not None:
             y, ldy = matrix_rows(y)
             y_ptr = y.data_ptr()
-        dtype, dev = g.dtype, g.device
+        dev = g.device
         # (without tokens no launch writes the parameters' gradients)
         like = torch.empty_like if n else torch.zeros_like
         if need_y:
-            d_y = torch.empty(shape, dtype=dtype, device=dev)
+            d_y = torch.empty_like(g)
         if need_res:
-            d_res = torch.empty(shape, dtype=dtype, device=dev)
+            d_res = torch.empty_like(g)
         if need_post:
             d_post = like(w_post)
         if need_gate:

@@ -55,7 +55,7 @@ def _sort(x, ids, num_experts, expert_lo, out):
     x, ldx = matrix_rows(x)
     hidden = x.shape[1]
     rows = torch.empty(n * k, hidden, dtype=x.dtype, device=dev) if out is None else out
-    positions = torch.empty(n, k, dtype=torch.int32, device=dev)
+    positions = torch.empty_like(ids)
     # tensors of their own: what adds up counts over ranks in place leaves the others as the backward saved them
     counts = torch.empty(num_experts, dtype=torch.int32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)

@@ -514,12 +514,12 @@ int afd_router_grad(const afd_router_cfg* cfg, const void* logits, int64_t ld, c
  * Formats of rows that are moved, added up or normed. */
 enum afd_value_fmt { AFD_V_F32 = 0, AFD_V_BF16 = 1, AFD_V_F16 = 2 };
 
-/* Pair t topk + j sends token t to expert ids[t][j]; it is here if expert_lo <= id < expert_lo + num_experts. Pairs
- * here are sorted by expert, equal ones in their order: positions i32 [n][topk] is a pair's place (-1: not
- * here), and x's row t is copied to rows[place] for each. counts i32 [num_experts], offsets i32 [num_experts + 1]: the
- * experts' pairs and where they begin; offsets[num_experts] is the number of rows. rows: n topk of ld >= columns elements;
- * those past the last are zeroed with zero_behind, else left as they are. Limits: n <= 2^26, topk <= 32, n topk < 2^31,
- * num_experts <= 1024, columns <= 65536. The workspace (4-byte aligned) is one call's. */
+/* Pair t topk + j sends token t to expert ids[t][j]; it is here if expert_lo <= id < expert_lo + num_experts
+ * (expert_lo >= 0). Pairs here are sorted by expert, equal ones in their order: positions i32 [n][topk] is a pair's place
+ * (-1: not here), and x's row t is copied to rows[place] for each. counts i32 [num_experts], offsets i32 [num_experts + 1]:
+ * the experts' pairs and where they begin; offsets[num_experts] is the number of rows. rows: n topk of ld >= columns
+ * elements, none of them x's; those past the last are zeroed with zero_behind, else left as they are. Limits: n <= 2^26,
+ * topk <= 32, n topk < 2^31, num_experts <= 1024, columns <= 65536. The workspace (4-byte aligned) is one call's. */
 int afd_sort_workspace(int32_t n, int32_t topk, int32_t num_experts, uint64_t* bytes);
 int afd_sort_tokens(int32_t fmt, const int32_t* ids, int32_t n, int32_t topk, int32_t expert_lo,
                     int32_t num_experts, const void* x, int64_t ldx, int32_t columns, void* rows,

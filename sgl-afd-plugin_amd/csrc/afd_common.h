@@ -15,7 +15,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 // 16 bytes at any address that holds 2-byte values (global memory takes wide loads and stores at any alignment). The
-// typedef's alignment is lost where it is a template's argument: through load_words and store_words.
+// typedef's alignment is lost where it is a template's argument: through load_words and store_words. NT: past the caches.
 typedef v4i v4i_any __attribute__((aligned(2)));
 template <bool ALIGNED, bool NT = false>
 __device__ __forceinline__ v4i load_words(const void* p) {
@@ -27,9 +27,11 @@ __device__ __forceinline__ v4i load_words(const void* p) {
     return NT ? __builtin_nontemporal_load(src) : *src;
   }
 }
-template <bool ALIGNED>
+template <bool ALIGNED, bool NT = false>
 __device__ __forceinline__ void store_words(void* p, v4i v) {
-  if constexpr (ALIGNED)
+  if constexpr (ALIGNED && NT)
+    __builtin_nontemporal_store(v, static_cast<v4i*>(p));
+  else if constexpr (ALIGNED)
     *static_cast<v4i*>(p) = v;
   else
     *static_cast<v4i_any*>(p) = v;

@@ -65,7 +65,7 @@ struct Raw8 {
 // A row of `columns` values shared by LANES lanes, lane l's chunk c: eight neighbouring values from (c LANES + l) 8 on. VEC: the
 // row is 16-byte aligned and its length a multiple of 8; else its whole chunks are read and written at the alignment they
 // have, and the last one value by value. Either way a lane holds the same values, so results do not depend on
-// it. What lies past the end reads as 0 and is not written. NT: past the caches.
+// it. What lies past the end reads as 0 and is not written. NT: past the caches (aligned rows).
 template <typename T, int LANES, bool VEC>
 struct Row {
   using Held = typename T::Held;
@@ -91,13 +91,14 @@ struct Row {
   static __device__ __forceinline__ void load(const Held* p, int columns, int lane, int c, float (&v)[8]) {
     fetch(p, columns, lane, c).widen(v);
   }
+  template <bool NT = false>
   static __device__ __forceinline__ void store(Held* p, int columns, int lane, int c, const float (&v)[8]) {
     const int at = column(lane, c);
     if (VEC ? at < columns : at + 8 <= columns) {
       Raw r;
       r.narrow(v);
 #pragma unroll
-      for (int i = 0; i < Raw::kWords; ++i) store_words<VEC>(reinterpret_cast<char*>(p + at) + 16 * i, r.w[i]);
+      for (int i = 0; i < Raw::kWords; ++i) store_words<VEC, NT>(reinterpret_cast<char*>(p + at) + 16 * i, r.w[i]);
     } else if (!VEC && at < columns) {
 #pragma unroll
       for (int j = 0; j < 7; ++j)
@@ -150,6 +151,8 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* part, int lane) {
   }
 }
 
+// results of more bytes go past the caches (L2 has 32 MB, the memory-side cache 256 for inputs and results)
+constexpr int64_t kPastBytes = int64_t(48) << 20;
 inline int value_size(int fmt) { return fmt == AFD_V_F32 ? 4 : 2; }
 inline bool known_fmt(int fmt) { return fmt == AFD_V_F32 || fmt == AFD_V_BF16 || fmt == AFD_V_F16; }
 // Whether rows at p, `ld` values apart, take 16-byte loads

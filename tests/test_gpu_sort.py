@@ -65,7 +65,7 @@ SIZES = [(1, 1, 1, 1), (1, 8, 4, 2), (3, 33, 1024, 32), (8, 4096, 256, 8), (127,
 def test_order_and_rows(n, hidden, experts, k):
     x, _, _, ids = make(n, hidden, experts, k, torch.bfloat16, n + k)
     say(f"sort n={n} hidden={hidden} experts={experts} k={k}")
-    for lo, here in ((0, experts), (experts // 3, max(1, experts // 2)), (-5, 8)):
+    for lo, here in ((0, experts), (experts // 3, max(1, experts // 2)), (experts - 1, 8)):
         want = order_of(ids, here, lo)
         rows, order = sort_tokens(x.to(dev()), ids.to(dev()), here, expert_lo=lo)
         check_order(order, want)
@@ -316,6 +316,8 @@ def test_refusals_of_calls():
         sort_tokens(x.clone().requires_grad_(), ids, 4, out=buf)
     with pytest.raises(ValueError):
         sort_tokens(x, ids.cpu(), 4)
+    with pytest.raises(ValueError):
+        sort_tokens(x, ids, 4, expert_lo=-1)
     _, order = sort_tokens(x, ids, 4)
     with pytest.raises(ValueError):
         unsort_tokens(rows, order, w.cpu())

@@ -37,7 +37,7 @@ def test_sort_calls():
     for name in ("ids", "x", "rows", "pos", "counts", "offsets"):
         assert sort(**{name: None}) == ARG, name
     assert sort(fmt=3) == FMT and sort(fmt=-1) == FMT
-    assert sort(n=-1) == ARG and sort(k=0) == SHAPE and sort(k=33) == SHAPE and sort(experts=0) == SHAPE
+    assert sort(lo=-1) == ARG and sort(n=-1) == ARG and sort(k=0) == SHAPE and sort(k=33) == SHAPE and sort(experts=0) == SHAPE
     assert sort(experts=1025) == SHAPE and sort(columns=0) == SHAPE and sort(columns=65537, ldx=65537, ld=65537) == SHAPE
     assert sort(ldx=9) == SHAPE and sort(ld=9) == SHAPE
     assert sort(ws=None) == WS and sort(size=5 * 4 * 4 - 1) == WS and sort(ws=18) == WS

@@ -566,6 +566,8 @@ static int launch_quant(const Args& p, const RowsIn& in, uint8_t* q, float* sx, 
   const int units = (8 * p.kb * ROWS + 63) / 64;
   if (units <= 8)
     go(quant_kernel<ROWS, 4, 2, VEC, NT, SILU>, 4);
+  else if (units <= 16)
+    go(quant_kernel<ROWS, 8, 2, VEC, NT, SILU>, 8);
   else if (units <= 32)
     go(quant_kernel<ROWS, 8, 4, VEC, NT, SILU>, 8);
   else if (units <= 64)
@@ -624,18 +626,15 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   const bool nt = int64_t(n) * weights->k_in * (silu ? 4 : 2) > kCachedBytes;
   auto quant = [&](auto silu_c) {
     constexpr bool kSilu = decltype(silu_c)::value;
-    // as few rows a workgroup as give no more than one to each CU (4 / 8 / 16 rows: 1000 x 2048 13.2 / 16.7 / 17.1 us with the
-    // product, 16384 x 4096 268 / 243 / 244)
-    const int cus = device_cu_count();
+    // Four rows a workgroup while those are few for the CUs, eight above (4096 columns in a graph, 4 / 8 / 16 rows: 300 tokens
+    // 3.5 / 4.8 / 7.5 us, 2900 7.8 / 9.0 / 9.5, 8192 22.2 / 20.5 / 21.3, 16384 41.0 / 38.6 / 37.8)
     auto rows = [&](auto rows_c) {
       constexpr int R = decltype(rows_c)::value;
       if (vec && nt) return launch_quant<R, true, true, kSilu>(p, in, q, sx, s);
       if (vec) return launch_quant<R, true, false, kSilu>(p, in, q, sx, s);
       return launch_quant<R, false, false, kSilu>(p, in, q, sx, s);
     };
-    if (n <= 4 * cus) return rows(std::integral_constant<int, 4>{});
-    if (n <= 8 * cus) return rows(std::integral_constant<int, 8>{});
-    return rows(std::integral_constant<int, 16>{});
+    return n <= 16 * device_cu_count() ? rows(std::integral_constant<int, 4>{}) : rows(std::integral_constant<int, 8>{});
   };
   st = silu ? quant(std::true_type{}) : quant(std::false_type{});
   if (st != AFD_OK) return st;

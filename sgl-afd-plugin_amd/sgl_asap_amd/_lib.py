@@ -403,4 +403,6 @@ def check(status: int, name: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(lib(), name)(*args)
+    if status != AFD_OK:
+        check(status, name)

@@ -155,7 +155,8 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, ex
     n, k = topk_ids.shape
     if x.shape[0] != n:
         raise ValueError(f"{n} rows of ids for x {tuple(x.shape)}")
-    fit_ints(n, k, num_experts, expert_lo)
+    if n > 0x7FFFFFFF or k > 0x7FFFFFFF or not 0 <= num_experts <= 0x7FFFFFFF or not 0 <= expert_lo <= 0x7FFFFFFF:
+        fit_ints(n, k, num_experts, expert_lo)
     need_gpu("x", x)
     if topk_ids.device != x.device:
         raise ValueError(f"topk_ids is on {topk_ids.device}, x on {x.device}")

@@ -314,6 +314,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(Args p, RowsIn in)
 // stage done) it waits for its copies of the next stage and meets the others at the stage's one barrier: the
 // next stage is there for all, and this one's slot is free for the copies of stage b + S. The MFMAs of the last two
 // weight fragments run while the next stage's first fragments are read.
+//
+// 16384 x 4096 x 4096 takes 204 to 211 us (2.6 to 2.7 POP/s; a library's product without scales 252): in the loop over K 3.2
+// POP/s, MFMA busy in 64% of all cycles at 1.95 GHz, and 8 to 10 us a round of tiles for its first copies and its results.
+// Operands move at 16 to 18 bytes a cycle and CU, which is what bounds the loop (without copies 196 us for 239, without LDS
+// reads 234; deeper rings, cache hints and workgroups that stay resident and start the next tile's copies early change
+// nothing or lose). Stages of 64 columns free their slots sooner than of 128 (231 for 241), and wavefronts of 128 x 64
+// hold more of what the long side needs than of 64 x 128 (222 for 231).
 template <int BM_, int BN_, int WM_, int WN_, int WK_, int S_>
 struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WK = WK_, S = S_;
@@ -620,8 +627,11 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   p.n_out = weights->n_out;
   p.kb = pl.kb;
   const RowsIn in = {x, ldx, weights->k_in};
+  // the rows kernel's own quantization: a launch less, and up to 32 K elements no slower than two in a graph (4096 x 4096, with
+  // and without: 1 row 6.3 and 8.7 us, 4 rows 7.3 and 9.2, 8 rows 9.4 and 9.5; 64 x 512 7.0 and 6.2), half of that
+  // where rows are not aligned (4 x 4001 7.7 and 9.4, 8 x 4001 11.5 and 9.7)
   const int64_t elements = int64_t(n) * pl.kb * 128;
-  if (n <= kFusedRows && elements <= (vec ? kFusedBytes : kFusedBytes / 3))
+  if (n <= kFusedRows && elements <= (vec ? kFusedBytes : kFusedBytes / 2))
     return silu ? launch_fused_rows<true>(p, in, vec, s) : launch_fused_rows<false>(p, in, vec, s);
   const bool nt = int64_t(n) * weights->k_in * (silu ? 4 : 2) > kCachedBytes;
   auto quant = [&](auto silu_c) {
@@ -638,6 +648,8 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   };
   st = silu ? quant(std::true_type{}) : quant(std::false_type{});
   if (st != AFD_OK) return st;
+  // up to 64 rows the weights are read once; above, tiles (4096 x 4096 without the quantization: 64 rows 8.7 us against 8.6 with
+  // tiles of 32 x 64, 48 x 2048 x 4096 4.8 against 5.9, 100 rows 15.1 against 8.6)
   if (n <= 16) return launch_rows<1, false, false>(p, in, vec, s);
   if (n <= 32) return launch_rows<2, false, false>(p, in, vec, s);
   if (n <= 48) return launch_rows<3, false, false>(p, in, vec, s);

@@ -66,7 +66,7 @@ template <int L>
 constexpr int kRows = kThreads<L> / L;
 template <int L>
 __device__ __forceinline__ int64_t first_row() {
-  return int64_t(blockIdx.x) * kRows<L> + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  return block_of_many() * kRows<L> + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
 }
 
 // NT: results past the caches, where they are more than those hold (16384 x 4096 bf16 96.5 -> 95.2 us; 8192 rows in training 58 ->
@@ -421,7 +421,7 @@ extern "C" int afd_residual_norm(const afd_norm_cfg* cfg, const void* y, int64_t
     norm::with_lanes(p.columns, [&](auto l, auto nc) {
       using T = decltype(type);
       constexpr int L = decltype(l)::value, NC = decltype(nc)::value;
-      const dim3 grid((n + norm::kRows<L> - 1) / norm::kRows<L>);
+      const dim3 grid = rows::grid_of_many((int64_t(n) + norm::kRows<L> - 1) / norm::kRows<L>);
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(norm::kThreads<L>), 0, static_cast<hipStream_t>(stream), p);
       };

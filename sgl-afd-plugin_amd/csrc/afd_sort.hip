@@ -94,7 +94,8 @@ __device__ __forceinline__ void zero_behind(const Move& m, int64_t t, int total,
 
 // Few pairs: one launch. A workgroup for each token and one more: each reads all pairs' ids (at most 16 a lane) and
 // counts the pairs before its own: a pair's key is (expert, pair), and its position the number of smaller keys. The one more writes
-// the tables.
+// the tables. 8 tokens of 4096 to 8 of 256 experts: 6.2 us in a trace, where a launch that does nothing takes 1.4; three
+// launches take 13.7 for 6124 pairs.
 constexpr int kFewThreads = 256, kFewEach = 16, kFewPairs = kFewThreads * kFewEach;
 template <bool VEC>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(Pairs p, Move m) {
@@ -167,7 +168,8 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(Pairs p, Move m) {
 }
 
 // Many pairs: chunks of a multiple of 1024, at most kMaxChunks. Each chunk's counts by expert, then each chunk's
-// positions from the counts of all chunks (which every workgroup adds up), then the rows.
+// positions from the counts of all chunks (which every workgroup adds up), then the rows (131072 pairs of 256 experts: 4.7 and
+// 5.4 us before the rows' 83).
 constexpr int kChunk = 1024, kMaxChunks = 256, kChunkWaves = kChunk / 64;
 
 inline int chunk_of(int64_t pairs) {
@@ -301,7 +303,9 @@ __device__ __forceinline__ int64_t position_of(const Back& p, int64_t i) {
 }
 
 // A wavefront a token's 512 columns, kBatch of its rows on their way at once; rows are read once: past the caches. No
-// loop over the columns, so that many short wavefronts keep loads on their way whatever share of the pairs is here.
+// loop over the columns, so that many short wavefronts keep loads on their way whatever share of the pairs is here (8192 x 2048
+// with 8 rows a token 58 us, 5.2 TB/s, where a wavefront for all of a token's columns took 77; 16384 x 4096 with 2 of 8 here 68
+// for 119; 8 tokens 3.8 for 5.7).
 constexpr int kBatch = 8;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void back_kernel(Back p, uint32_t chunks) {
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(256) void back_kernel(Back p, uint32_t chunks) {
 }
 
 // The gradient of the rows and the weights, a token at a time: its row of g is read for each batch of its pairs (once where
-// there are no more), the pairs' rows once
+// there are no more), the pairs' rows once. 8192 x 2048 with 8 rows a token: 116 us, 4.9 TB/s
 template <typename T, int L, bool VEC>
 __global__ __launch_bounds__(256) void back_grad_kernel(Back p) {
   using R = Row<T, L, VEC>;

@@ -182,7 +182,7 @@ class _NoDerivative(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *_):
-        raise RuntimeError("the router's gradient has no derivative of its own (no second derivatives)")
+        raise RuntimeError("this gradient has no derivative of its own (no second derivatives)")
 
 
 def last(grad: torch.Tensor, *made_from: Optional[torch.Tensor]) -> torch.Tensor:

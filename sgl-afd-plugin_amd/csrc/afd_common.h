@@ -367,6 +367,8 @@ __host__ __device__ __forceinline__ int64_t fp8_image_offset(int64_t mat, int64_
 // Issued through inline assembly so the compiler does not drain every outstanding copy
 // before each LDS read; callers wait with wait_vmcnt<N>() (vector-memory operations
 // complete in issue order for loads) and a barrier before reading what they copied.
+// The compiler puts no wait states into inline assembly: one is needed between the write of M0 and the copy that reads it,
+// five between a vector instruction (a readfirstlane) that writes the base and the copy. The s_mov is one of them, the s_nop four.
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
@@ -381,24 +383,25 @@ __device__ __forceinline__ const void* uniform_ptr(const void* p) {
 }
 
 __device__ __forceinline__ void lds_dma16(uint32_t m0, const void* base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0), "v"(voff),
                "s"(uniform_ptr(base))
                : "memory");
 }
 
 __device__ __forceinline__ void lds_dma4(uint32_t m0, const void* base, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0), "v"(voff),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(m0), "v"(voff),
                "s"(uniform_ptr(base))
                : "memory");
 }
 
 // Global stores through inline assembly: the compiler neither moves, merges nor splits them,
 // so a caller that counts its vector-memory instructions for s_waitcnt knows their number.
-// A store of more than 8 bytes reads its data registers one cycle late, and the compiler
-// does not see that hazard in inline assembly, so the s_nop keeps the next instruction from
-// overwriting them first.
+// A store of more than 8 bytes reads its data registers late, and the compiler does not see that
+// hazard in inline assembly: the s_nop's two wait states keep the next instructions from overwriting
+// them first (with one, the last 4 lanes of each 16 stored the next chunk's values now and then where other
+// kernels ran beside).
 __device__ __forceinline__ void store16(void* p, v4i v) {
-  asm volatile("global_store_dwordx4 %0, %1, off\n\ts_nop 0" ::"v"(p), "v"(v) : "memory");
+  asm volatile("global_store_dwordx4 %0, %1, off\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
 }
 __device__ __forceinline__ void store8(void* p, uint32_t v) {
   asm volatile("global_store_byte %0, %1, off" ::"v"(p), "v"(v) : "memory");

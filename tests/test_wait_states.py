@@ -116,6 +116,7 @@ def test_what_is_found(code, what):
 def test_the_library_has_the_wait_states(tmp_path):
     if not os.path.exists(OBJDUMP):
         pytest.skip("no disassembler")
+    _lib.lib()
     path = shutil.copy(_lib.LIB_PATH, tmp_path / "lib.so")
     subprocess.run([OBJDUMP, "--offloading", path], cwd=tmp_path, check=True, capture_output=True)
     images = sorted(f for f in os.listdir(tmp_path) if f.endswith("gfx950"))

@@ -21,6 +21,7 @@ from functools import lru_cache
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .topk import fit_ints, launch, matrix_rows, need_gpu, no_tangent
@@ -85,7 +86,8 @@ class _PackedLinear(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, *, silu_mul: bool = False) -> torch.Tensor:
         """bf16 [..., k_in] -> bf16 [..., n_out] on the device's current stream, into ``out`` if given ([n,
-        n_out] with contiguous rows that share no element with x, x two-dimensional). ``silu_mul``: as the method."""
+        n_out] with contiguous rows that share no element with x, x two-dimensional; an in-place change to autograd).
+        ``silu_mul``: as the method."""
         if silu_mul:
             return self._product(self.ENTRY + "_silu_mul", x, 2 * self.in_features, out)
         return self._product(self.ENTRY, x, self.in_features, out)
@@ -122,6 +124,8 @@ class _PackedLinear(torch.nn.Module):
         ws = torch.empty(size, dtype=torch.uint8, device=x.device)
         launch(name, x.device, self._weights_ref, rows.data_ptr(), ldx, n,
                ws.data_ptr(), size, y.data_ptr(), y.stride(0) if n > 1 else self.out_features)
+        if out is not None:
+            increment_version(out)  # a backward that saved what it held raises
         return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)
 
 

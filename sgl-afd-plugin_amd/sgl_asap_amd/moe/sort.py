@@ -18,6 +18,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .topk import fit_ints, last, launch, matrix_rows, need_gpu, no_tangent
@@ -147,8 +148,8 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, ex
 
     Rows past the last are 0. With ``out`` ([at least n k, hidden] in x's type, contiguous rows in memory that x's does not
     meet) the rows go there and those past the last stay as they are: what a serving rank that holds few of the experts
-    uses, without a gradient. An expert that a token names twice gets it twice. The rows have a gradient by x, once: second,
-    forward-mode and traced derivatives are refused."""
+    uses, without a gradient; to autograd it is an in-place change of ``out``. An expert that a token names twice gets it twice.
+    The rows have a gradient by x, once: second, forward-mode and traced derivatives are refused."""
     _matrix("x", x)
     if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2:
         raise TypeError(f"topk_ids must be int32 [n, k], got {topk_ids.dtype} {tuple(topk_ids.shape)}")
@@ -175,7 +176,9 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, ex
         raise ValueError("out must have contiguous rows of its own on x's device")
     if _meet(x, out):
         raise ValueError("out meets x in memory")
-    return _sort(x, ids, num_experts, expert_lo, out)
+    result = _sort(x, ids, num_experts, expert_lo, out)
+    increment_version(out)  # a backward that saved what it held raises
+    return result
 
 
 def _meet(x: torch.Tensor, out: torch.Tensor) -> bool:

@@ -22,6 +22,7 @@ from dataclasses import dataclass
 from typing import Dict, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .topk import format_is_standard
@@ -271,6 +272,7 @@ def _quant_act(cfg, act, x, q, s, stream):
     if n > 0:
         _lib.call("afd_quant_act", ctypes.byref(cfg), x.data_ptr(), n, q.data_ptr(), s.data_ptr(),
                   _stream_handle(stream))
+        increment_version((q, s))  # a caller's: a backward that saved what they held raises
     return q, s
 
 
@@ -465,6 +467,7 @@ class AfdExperts(torch.nn.Module):
             out.data_ptr(),
             _stream_handle(),
         )
+        increment_version(out)  # a caller's: a backward that saved what it held raises
         return out
 
     def call_ptrs(self, n: int, x_ptr: int, xs_ptr: int, ids_ptr: int, w_ptr: int, out_ptr: int,
@@ -524,6 +527,7 @@ class AfdExperts(torch.nn.Module):
         ws = self.workspace()
         _lib.call("afd_moe_ffn_batch", ctypes.byref(self.cfg), ctypes.byref(self._wstruct), descs, len(jobs),
                   ws.data_ptr(), ws.numel(), _stream_handle())
+        increment_version(results)
         return results
 
     def call_batch_ptrs(self, rows, stream: int, capacity: Optional[int] = None) -> None:
@@ -635,6 +639,7 @@ class AfdExperts(torch.nn.Module):
             out.data_ptr(),
             _stream_handle(),
         )
+        increment_version(out)  # a caller's: a backward that saved what it held raises
         return out
 
     def layout_for(self, n: int) -> dict:

@@ -29,6 +29,7 @@ import time
 from typing import Dict, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from ..moe.experts import new_job_desc, set_job
@@ -114,4 +115,5 @@ class FfnGraphRunner:
         else:
             set_job(self.desc, x=x[0].contiguous(), ids=ids, w=w, out=out)
         self.graphs[(layer_id, self.buckets[i])].replay()
+        increment_version(out)  # a backward that saved what it held raises
         return out

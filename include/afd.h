@@ -532,7 +532,8 @@ int afd_unsort_tokens(int32_t fmt, const void* rows, int64_t ld, int64_t num_row
                       const int32_t* positions, const float* w, int32_t n, int32_t topk,
                       int32_t columns, void* out, afd_stream_t stream);
 /* Its gradient from g [n][columns], that of out: d_rows [num_rows][columns] (NULL: not wanted), rows from *total on 0, and
- * d_w f32 [n][topk] (NULL: not wanted), 0 where the position is skipped. */
+ * d_w f32 [n][topk] (NULL: not wanted), 0 where the position is skipped. A row is one pair's at most, and no pair's from *total
+ * on. Those before it that no pair has, as of positions that a caller set to -1, are left as they are: clear d_rows first. */
 int afd_unsort_grad(int32_t fmt, const void* g, const void* rows, int64_t ld, int64_t num_rows,
                     const int32_t* positions, const int32_t* total, const float* w, int32_t n,
                     int32_t topk, int32_t columns, void* d_rows, float* d_w, afd_stream_t stream);

@@ -41,6 +41,29 @@ class TokenOrder(NamedTuple):
     offsets: torch.Tensor  # i32 [num_experts + 1]: where they begin; the last: the rows that are used
 
 
+class SortedOrder(TokenOrder):
+    """The order that ``sort_tokens`` returns, every row before offsets[-1] being some pair's. Of what is made of it (a slice,
+    ``_replace``, a copy), and of its tensors once they were changed, that is not known."""
+
+    own = False  # whether sort_tokens made it
+
+    @classmethod
+    def made(cls, *tensors: torch.Tensor) -> "SortedOrder":
+        order = cls(*tensors)
+        order.own = True
+        return order
+
+    @classmethod
+    def _make(cls, fields):
+        return TokenOrder._make(fields)
+
+    def __reduce__(self):
+        return TokenOrder, tuple(self)
+
+    def complete(self) -> bool:
+        return self.own and not any(t.is_inference() or t._version for t in (self.positions, self.offsets))
+
+
 @lru_cache(maxsize=1024)
 def _workspace_bytes(n: int, k: int, experts: int) -> int:
     fit_ints(n, k, experts)
@@ -66,7 +89,7 @@ def _sort(x, ids, num_experts, expert_lo, out):
     launch("afd_sort_tokens", dev, VALUE_FORMATS[x.dtype], ids.data_ptr(), n, k, expert_lo, num_experts, x.data_ptr(), ldx, hidden,
            rows.data_ptr(), ld, out is None, positions.data_ptr(), counts.data_ptr(), offsets.data_ptr(),
            None if ws is None else ws.data_ptr(), size)
-    return rows, TokenOrder(positions, counts, offsets)
+    return rows, SortedOrder.made(positions, counts, offsets)
 
 
 def _unsort(rows, positions, weights):
@@ -97,7 +120,8 @@ class _Sort(torch.autograd.Function):
 
 
 class _Unsort(torch.autograd.Function):
-    """rows as ``matrix_rows`` gives them: what the backward reads is then the input itself."""
+    """rows as ``matrix_rows`` gives them: what the backward reads is then the input itself. offsets: None if there may be
+    rows before the last that no pair has."""
 
     @staticmethod
     def forward(ctx, rows, weights, positions, offsets):
@@ -116,17 +140,21 @@ class _Unsort(torch.autograd.Function):
         made_from = (g, rows, weights)
         g = g if g.is_contiguous() else g.contiguous()
         d_rows = d_w = None
+        total = None
         if ctx.needs_input_grad[0]:
-            # (without tokens no launch writes the rows)
-            d_rows = (torch.empty if n else torch.zeros)(num_rows, hidden, dtype=g.dtype, device=dev)
+            # (without tokens no launch writes the rows; nor, of an order that is not complete, those that no pair has: those
+            # past the last neither then, as positions may go there)
+            d_rows = (torch.empty if n and offsets is not None else torch.zeros)(num_rows, hidden, dtype=g.dtype, device=dev)
+            if offsets is None:
+                offsets = torch.full((1,), 0x7FFFFFFF, dtype=torch.int32, device=dev)
+            total = offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
         if rows is not None:
             d_w = torch.empty(n, k, dtype=torch.float32, device=dev)
             rows, ld = matrix_rows(rows)
         else:
             ld = hidden
         launch("afd_unsort_grad", dev, VALUE_FORMATS[g.dtype], g.data_ptr(), None if rows is None else rows.data_ptr(), ld, num_rows,
-               positions.data_ptr(), offsets.data_ptr() + 4 * (offsets.shape[0] - 1),
-               None if weights is None else weights.data_ptr(), n, k, hidden,
+               positions.data_ptr(), total, None if weights is None else weights.data_ptr(), n, k, hidden,
                None if d_rows is None else d_rows.data_ptr(), None if d_w is None else d_w.data_ptr())
         if torch.is_grad_enabled():
             d_rows, d_w = (None if t is None else last(t, *made_from) for t in (d_rows, d_w))
@@ -166,7 +194,7 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, *, ex
     if out is None:
         if torch.is_grad_enabled() and x.requires_grad:
             rows, *order = _Sort.apply(x, ids, num_experts, expert_lo)
-            return rows, TokenOrder(*order)
+            return rows, SortedOrder.made(*order)
         return _sort(x, ids, num_experts, expert_lo, None)
     if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise NotImplementedError("sort_tokens into out has no gradient: call it under torch.no_grad()")
@@ -192,8 +220,11 @@ def _meet(x: torch.Tensor, out: torch.Tensor) -> bool:
 def unsort_tokens(rows: torch.Tensor, order: TokenOrder, topk_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[n, hidden]: each token's sum of its ``rows`` [at least offsets[-1], hidden] (fp32, bf16 or fp16), with
     ``topk_weights`` [n, k] (fp32, others are cast; None: 1). Pairs that are not here add nothing, whatever their weights; a
-    token without any gets 0. Added up in fp32 in the order of j, rounded once. Gradients by the rows (0 in those past
-    the last) and the weights (0 where the pair is not here), once, as ``sort_tokens``."""
+    token without any gets 0. Added up in fp32 in the order of j, rounded once. Gradients by the rows (0 in those that no pair
+    has) and the weights (0 where the pair is not here), once, as ``sort_tokens``.
+
+    ``order`` may be one that was made of ``sort_tokens``': a part of the tokens' positions, or positions set to -1 to drop pairs
+    (its gradient by the rows clears them first). A row is one pair's at most: two that name it would each write its gradient."""
     _matrix("rows", rows)
     positions, offsets = order.positions, order.offsets
     if positions.dtype != torch.int32 or positions.dim() != 2 or offsets.dtype != torch.int32 or offsets.dim() != 1:
@@ -217,5 +248,6 @@ def unsort_tokens(rows: torch.Tensor, order: TokenOrder, topk_weights: Optional[
         if topk_weights.dtype != torch.float32 or not topk_weights.is_contiguous():
             topk_weights = topk_weights.to(torch.float32).contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or topk_weights is not None and topk_weights.requires_grad):
-        return _Unsort.apply(matrix_rows(rows)[0], topk_weights, positions, offsets)
+        whole = isinstance(order, SortedOrder) and order.complete()
+        return _Unsort.apply(matrix_rows(rows)[0], topk_weights, positions, offsets if whole else None)
     return _unsort(rows, positions, topk_weights)

@@ -464,21 +464,28 @@ __global__ __launch_bounds__(T::kThreads) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
   for (int j = 0; j < TJ; j += 2) {
     float sw[2][4];
-    bool odd = false;
+    uint32_t odd = 0;  // a bit for each of the lane's eight channels: a channel's way does not depend on those beside it
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         sw[u][q] = p.bs[min(n0 + (wn * TJ + j + u) * 16 + 4 * lg + q, p.n_out - 1)];
-        odd |= odd_scale(sw[u][q]);
+        odd |= static_cast<uint32_t>(odd_scale(sw[u][q])) << (4 * u + q);
       }
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       float y[2][4];
+      if (odd) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[u][q] = scaled(acc[i][j + u][q], sx[i], sw[u][q], odd);
+          for (int q = 0; q < 4; ++q) y[u][q] = scaled(acc[i][j + u][q], sx[i], sw[u][q], odd >> (4 * u + q) & 1);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[u][q] = scaled(acc[i][j + u][q], sx[i], sw[u][q], false);
+      }
       const auto d0 = __builtin_amdgcn_permlane16_swap(pk_bf16(y[0][0], y[0][1]), pk_bf16(y[1][0], y[1][1]), false, false);
       const auto d1 = __builtin_amdgcn_permlane16_swap(pk_bf16(y[0][2], y[0][3]), pk_bf16(y[1][2], y[1][3]), false, false);
       const v4i chunk = {static_cast<int>(d0[0]), static_cast<int>(d1[0]), static_cast<int>(d0[1]),

@@ -539,7 +539,7 @@ int afd_unsort_grad(int32_t fmt, const void* g, const void* rows, int64_t ld, in
                     int32_t topk, int32_t columns, void* d_rows, float* d_w, afd_stream_t stream);
 
 /* ---- the norms before and after a block ---------------------------------------------------------
- * rms(v) = v / sqrt(mean(v^2) + eps) over a token's row, the mean of squares in fp32;
+ * rms(v) = v / sqrt(mean(v^2) + eps) over a token's row, in fp32, of any numbers (a row with an infinity: NaN there, else 0);
  *   h = residual + scale * gate * (rms(y) * w_post, or y without w_post),  normed = rms(h) * w_next
  * y, residual, h, normed in fmt; w_post, gate and w_next in fmt or in fp32. columns <= 16384, n <= 2^26, eps > 0. */
 enum afd_gate_kind {

@@ -69,13 +69,35 @@ __device__ __forceinline__ int64_t first_row() {
   return block_of_many() * kRows<L> + (L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
 }
 
+// 1 / sqrt(mean of the squares of a row's values + eps). Where their sum leaves fp32 (ss is the row's, so all of its lanes agree)
+// it is made again of values scaled by a power of two, so any row of numbers has its root; one that holds an infinity
+// gets 0. part: LDS as row_sum's, two of them
+template <int L, int NC>
+__device__ __forceinline__ float inv_root(const float (&v)[NC][8], float inv, float eps, float* part, float* again, int lane) {
+  float ss[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss[0] = __builtin_fmaf(v[c][j], v[c][j], ss[0]);
+  row_sum<L>(ss, part, lane);
+  if (ss[0] != __builtin_inff()) return 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, eps));
+  constexpr float kDown = 0x1p-72f;  // 16384 squares of the largest float are then 2^126
+  float small[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) small[0] = __builtin_fmaf(kDown * v[c][j], kDown * v[c][j], small[0]);
+  row_sum<L>(small, again, lane);
+  return kDown / sqrtf(__builtin_fmaf(small[0], inv, kDown * (kDown * eps)));
+}
+
 // NT: results past the caches, where they are more than those hold (16384 x 4096 bf16 96.5 -> 95.2 us; 8192 rows in training 58 ->
 // 61, and the gradient behind it 83 -> 72)
 template <typename T, int L, int NC, bool VEC, bool NT>
 __global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
   using R = Row<T, L, VEC>;
   using Held = typename T::Held;
-  __shared__ float part[2][L / 64];
+  __shared__ float part[3][L / 64];  // (the third one's two uses have the second's barrier between them)
   const int64_t t = first_row<L>();
   if (t >= p.n) return;  // (a whole wavefront, and with one row a workgroup none)
   const int lane = threadIdx.x & (L - 1), columns = p.columns;
@@ -99,13 +121,7 @@ __global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) y_raw[c].widen(y[c]);
     if (p.post) {
-      float ss[1] = {0.0f};
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss[0] = __builtin_fmaf(y[c][j], y[c][j], ss[0]);
-      row_sum<L>(ss, part[0], lane);
-      const float r = 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, p.eps));
+      const float r = inv_root<L, NC>(y, inv, p.eps, part[0], part[2], lane);
       if (p.rstd && lane == 0) p.rstd[t] = r;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -129,13 +145,7 @@ __global__ __launch_bounds__(kThreads<L>) void forward_kernel(Args p) {
     }
   }
   if (p.normed) {
-    float ss[1] = {0.0f};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss[0] = __builtin_fmaf(h[c][j], h[c][j], ss[0]);
-    row_sum<L>(ss, part[1], lane);
-    const float r = 1.0f / sqrtf(__builtin_fmaf(ss[0], inv, p.eps));
+    const float r = inv_root<L, NC>(h, inv, p.eps, part[1], part[2], lane);
     if (p.rstd && lane == 0) p.rstd[int64_t(p.n) + t] = r;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {

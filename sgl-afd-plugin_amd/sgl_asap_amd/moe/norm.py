@@ -7,8 +7,8 @@ engine's in the reference).
                     normed = rms(hidden) * next_weight                  before the block behind it
 
 y is the block's output. Activations are fp32, bf16 or fp16, the weights and the gate of the same type or fp32; everything is
-computed in fp32 and rounded once (``normed`` is that of ``hidden`` before it is rounded; a mean of squares past fp32
-gives rows of 0). The gradients, by every tensor, are one pass over the rows too; sums over tokens run in a fixed order: the
+computed in fp32 and rounded once (``normed`` is that of ``hidden`` before it is rounded). Values may be any numbers of their
+type: a sum of squares past fp32 is made of scaled ones. The gradients, by every tensor, are one pass over the rows too; sums over tokens run in a fixed order: the
 same call gives the same bits.
 """
 

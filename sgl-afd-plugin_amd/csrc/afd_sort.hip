@@ -26,8 +26,8 @@ struct Pairs {
   int32_t *positions, *counts, *offsets;
 };
 __device__ __forceinline__ int expert_of(const Pairs& p, int i) {
-  const uint32_t e = static_cast<uint32_t>(p.ids[i]) - static_cast<uint32_t>(p.expert_lo);
-  return e < static_cast<uint32_t>(p.experts) ? static_cast<int>(e) : -1;
+  const int32_t id = p.ids[i];
+  return id >= p.expert_lo && id - p.expert_lo < p.experts ? id - p.expert_lo : -1;  // (expert_lo >= 0: no difference wraps)
 }
 
 // Exclusive sums of v over the THREADS threads of a workgroup, and the total. waves: LDS, one a wavefront

@@ -251,7 +251,7 @@ class BlockNorms(torch.nn.Module):
     """A block's norms, gate and residual scale as a module: ``hidden = residual + scale * gate * rms(y) * post_weight``.
 
     ``input_weight`` [hidden]: the norm before the block (``before``); ``post_weight``: after it (None: none); ``gate``
-    [hidden]: learned per channel (None: none). They are parameters."""
+    [hidden]: learned per channel (None: none). They are parameters: those that are given as one are the module's own."""
 
     def __init__(self, input_weight: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
                  gate: Optional[torch.Tensor] = None, scale: float = 1.0, eps: float = 1e-6):
@@ -259,7 +259,7 @@ class BlockNorms(torch.nn.Module):
         for name, t in (("input_weight", input_weight), ("post_weight", post_weight), ("gate", gate)):
             if t is not None and (t.dim() != 1 or t.shape != input_weight.shape):
                 raise ValueError(f"{name} must be {tuple(input_weight.shape)}, got {tuple(t.shape)}")
-            self.register_parameter(name, None if t is None else torch.nn.Parameter(t))
+            self.register_parameter(name, t if t is None or isinstance(t, torch.nn.Parameter) else torch.nn.Parameter(t))
         self.scale, self.eps = float(scale), _eps(eps)
 
     def before(self, x: torch.Tensor) -> torch.Tensor:

@@ -224,7 +224,7 @@ def residual_norm(
         wide_next = _param("next_weight", next_weight, y, (columns,))
         next_weight = _whole(next_weight)
     if gate is not None:
-        if gate.dim() == 1:
+        if gate.dim() == 1 and (y.dim() > 1 or gate.shape[0] == columns):  # ([1] beside one token: its gate)
             kind, wide_gate = GATE_CHANNEL, _param("gate", gate, y, (columns,))
         elif gate.shape == y.shape and columns > 1:
             kind, wide_gate = GATE_ELEMENT, _param("gate", gate, y, tuple(y.shape))

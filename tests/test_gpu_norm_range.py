@@ -1,5 +1,5 @@
 """GPU: a block's norms at the ends of their range: sums of squares past fp32, workgroups past 2^20, rows of any
-alignment."""
+alignment, a gate of one value for a single token."""
 
 import pytest
 import torch
@@ -121,3 +121,19 @@ def test_rows_of_any_alignment_have_the_same_bits(dtype, kind, n, hidden):
         results.append([t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, (dh.to(dev()), dn.to(dev())))))
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@pytest.mark.parametrize("hidden", [1, 7, 64])
+def test_one_token_and_its_gate(hidden):
+    """y [hidden], a gate per token of [1], per channel of [hidden]."""
+    g = torch.Generator().manual_seed(2)
+    y, res, gate = torch.randn(hidden, generator=g), torch.randn(hidden, generator=g), torch.randn(1, generator=g)
+    say(f"one token hidden={hidden}")
+    leaves = [t.to(dev()).requires_grad_() for t in (y, res, gate)]
+    out = residual_norm(leaves[0], leaves[1], gate=leaves[2], scale=0.5)
+    rows = [t.to(dev()).view(1, -1).requires_grad_() for t in (y, res, gate)]
+    want = residual_norm(rows[0], rows[1], gate=rows[2], scale=0.5)
+    assert out.hidden.shape == (hidden,) and torch.equal(out.hidden, want.hidden[0])
+    g_out = torch.randn(hidden, generator=g).to(dev())
+    for got, exp, leaf in zip(torch.autograd.grad(out.hidden, leaves, g_out), torch.autograd.grad(want.hidden, rows, g_out[None]), leaves):
+        assert got.shape == leaf.shape and torch.equal(got.view(-1), exp.view(-1))

@@ -1,8 +1,9 @@
-"""A block's norms as a module, on the host."""
+"""A block's norms as a module, and a single token's gate, on the host."""
 
+import pytest
 import torch
 
-from sgl_asap_amd.moe.norm import BlockNorms
+from sgl_asap_amd.moe.norm import BlockNorms, residual_norm
 
 
 def test_given_parameters_are_the_module_s():
@@ -16,3 +17,14 @@ def test_given_parameters_are_the_module_s():
     plain = BlockNorms(torch.ones(8), torch.ones(8))
     assert all(isinstance(t, torch.nn.Parameter) and t.requires_grad for t in plain.parameters())
     assert plain.gate is None
+
+
+def test_a_gate_of_one_token():
+    """[1] beside y [hidden] is a gate per token: its shape passes."""
+    y = torch.zeros(8)
+    for gate in (torch.ones(1), torch.ones(8)):
+        with pytest.raises(ValueError, match="GPU"):
+            residual_norm(y, y, gate=gate)
+    for gate in (torch.ones(2), torch.ones(0), torch.ones(9)):
+        with pytest.raises(ValueError, match="gate must be"):
+            residual_norm(y, y, gate=gate)

@@ -68,7 +68,7 @@ class _PackedLinear(torch.nn.Module):
         need_gpu("weight", codes)
         self.out_features, self.in_features = n_out, k_in
         self.image = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
-        self.scales = scales.to(codes.device, copy=True).contiguous()
+        self.scales = scales.detach().to(codes.device, copy=True).contiguous()
         launch("afd_linear_pack", codes.device, codes.data_ptr(), k_in, n_out, k_in, self.image.data_ptr())
         self._point()
 

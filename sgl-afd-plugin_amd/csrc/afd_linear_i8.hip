@@ -634,9 +634,9 @@ static int run(const afd_linear_weights* weights, const uint16_t* x, int64_t ldx
   p.n_out = weights->n_out;
   p.kb = pl.kb;
   const RowsIn in = {x, ldx, weights->k_in};
-  // the rows kernel's own quantization: a launch less, and up to 32 K elements no slower than two in a graph (4096 x 4096, with
-  // and without: 1 row 6.3 and 8.7 us, 4 rows 7.3 and 9.2, 8 rows 9.4 and 9.5; 64 x 512 7.0 and 6.2), half of that
-  // where rows are not aligned (4 x 4001 7.7 and 9.4, 8 x 4001 11.5 and 9.7)
+  // the rows kernel's own quantization, up to 32 K elements: a launch less, which a call from Python has 3 us of, and in a graph no
+  // slower than two but for many short rows (4096 x 4096, with and without: 1 row 6.3 and 8.7 us, 4 rows 7.3 and 9.2, 8 rows 9.4
+  // and 9.5; 64 x 512 7.0 and 6.2); half of that where rows are not aligned (4 x 4001 7.7 and 9.4, 8 x 4001 11.5 and 9.7)
   const int64_t elements = int64_t(n) * pl.kb * 128;
   if (n <= kFusedRows && elements <= (vec ? kFusedBytes : kFusedBytes / 2))
     return silu ? launch_fused_rows<true>(p, in, vec, s) : launch_fused_rows<false>(p, in, vec, s);

@@ -151,7 +151,9 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* part, int lane) {
   }
 }
 
-// results of more bytes go past the caches (L2 has 32 MB, the memory-side cache 256 for inputs and results)
+// Results of more bytes go past the caches (L2 has 32 MB, the memory-side cache 256 for inputs and results). Measured for the
+// norms (afd_norm.hip); the sorted rows take the same number, of all pairs' rows, as those that are here are not known on the
+// host (afd_sort.hip)
 constexpr int64_t kPastBytes = int64_t(48) << 20;
 // Workgroups in two dimensions (a dimension's threads are counted in 32 bits), and their number there
 inline dim3 grid_of_many(int64_t blocks) {

@@ -95,7 +95,7 @@ __device__ __forceinline__ void zero_behind(const Move& m, int64_t t, int total,
 // Few pairs: one launch. A workgroup for each token and one more: each reads all pairs' ids (at most 16 a lane) and
 // counts the pairs before its own: a pair's key is (expert, pair), and its position the number of smaller keys. The one more writes
 // the tables. 8 tokens of 4096 to 8 of 256 experts: 6.2 us in a trace, where a launch that does nothing takes 1.4; three
-// launches take 13.7 for 6124 pairs.
+// launches take 13.7 for 6124 pairs. The limit is what 16 keys a lane hold; beside it the two forms have not been compared.
 constexpr int kFewThreads = 256, kFewEach = 16, kFewPairs = kFewThreads * kFewEach;
 template <bool VEC>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(Pairs p, Move m) {
@@ -269,8 +269,10 @@ __global__ __launch_bounds__(kChunk) void place_kernel(Pairs p, int chunk, const
   }
 }
 
-// A wavefront a token. NT: past the caches, where the rows are more than those hold (16384 tokens with a quarter of their
-// 8 experts here 88 -> 83 us, the way back behind it 72 -> 69)
+// A wavefront a token. NT: past the caches, where all pairs' rows would be more than kPastBytes, whichever of them are here. It is
+// even over a pass and not best everywhere: 16384 x 4096 with a quarter of the 8 experts here 83 us for 88 through the caches,
+// and the way back behind it 69 for 72; 8192 x 2048 with all here 78 for 60, the way back 58 for 61 (twice) and its gradient 116
+// for 127, the pass 310 for 309; 2048 x 2048 (67 MB of rows, which the memory-side cache holds) 18.7 for 15.0
 template <bool VEC, bool NT>
 __global__ __launch_bounds__(256) void move_kernel(Move m, const int32_t* __restrict__ positions,
                                                    const int32_t* __restrict__ total) {

@@ -6,10 +6,10 @@ engine's in the reference).
     residual_norm:  hidden = residual + scale * gate * (rms(y) * post_weight, or y)
                     normed = rms(hidden) * next_weight                  before the block behind it
 
-y is the block's output. Activations are fp32, bf16 or fp16, the weights and the gate of the same type or fp32; everything is
-computed in fp32 and rounded once (``normed`` is that of ``hidden`` before it is rounded). Values may be any numbers of their
-type: a sum of squares past fp32 is made of scaled ones. The gradients, by every tensor, are one pass over the rows too; sums over tokens run in a fixed order: the
-same call gives the same bits.
+y is the block's output. Activations are fp32, bf16 or fp16, the weights and the gate of the same type or fp32; everything
+is computed in fp32 and rounded once (``normed`` is that of ``hidden`` before it is rounded). Values may be any numbers of
+their type: a sum of squares past fp32 is made of scaled ones. The gradients, by every tensor, are one pass over the rows
+too; sums over tokens run in a fixed order: the same call gives the same bits.
 """
 
 from __future__ import annotations

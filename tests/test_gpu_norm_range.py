@@ -7,6 +7,7 @@ import torch
 from error_bounds import Bounded
 from gpu_util import dev, say
 from sgl_asap_amd.moe.norm import residual_norm, rms_norm
+from test_gpu_norm import EPS, backward, make
 
 pytestmark = pytest.mark.gpu
 
@@ -63,6 +64,24 @@ def test_large_outputs_and_residuals(dtype, hidden):
         assert want.held(dtype).holds(h)
         assert (unit(want, eps)[0] * Bounded(w_next)).held(dtype).holds(normed)
         assert float(normed[0].abs().max()) > 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+@pytest.mark.parametrize("hidden", [384, 4096, 9000])
+def test_gradients_of_large_outputs_and_residuals(dtype, gate, hidden):
+    n = 5
+    say(f"gradients of large blocks {dtype} {gate} hidden={hidden}")
+    for size_y, size_r in ((1e19, 1e19), (1e19, 1.0), (1.0, 1e19), (1e30, 1e25)):
+        d = make(n, hidden, dtype, True, gate, hidden)
+        d["y"], d["res"] = large(n, hidden, size_y, 1).to(dtype), large(n, hidden, size_r, 2).to(dtype)
+        leaves = {k: d[k].to(dev()).requires_grad_() for k in ("y", "res", "gate", "post", "next") if d[k] is not None}
+        outs = residual_norm(leaves["y"], leaves["res"], post_weight=leaves["post"], gate=leaves.get("gate"), scale=0.5,
+                             next_weight=leaves["next"], eps=EPS)
+        grads = torch.autograd.grad(outs, list(leaves.values()), (d["dh"].to(dev()), d["dn"].to(dev())))
+        want = backward(d, True, True, 0.5)
+        for name, got in zip(leaves, grads):
+            assert want[name].holds(got), (name, size_y, size_r)
 
 
 def test_infinite_rows_stay_as_they_were():
